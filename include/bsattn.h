@@ -217,6 +217,51 @@ int bsattn_prefill(bsattn_cache* cache, const void* q, const int32_t* seq_ids,
                    int32_t n_seqs, int32_t n_query, float scale, void* out,
                    void* stream);
 
+/* Rotary positions.  For a head x[0, 128) of the token at position p, the
+ * pairs (a, b) of its first `dims` dims become
+ *   a' = factor (a cos phi - b sin phi),  b' = factor (a sin phi + b cos phi),
+ * phi = p * theta[i], for pair i = (x[2i], x[2i + 1]) (interleaved: the
+ * reference's `traditional`) or (x[i], x[i + dims / 2]); the other dims stay
+ * as they are.  Context scaling is in theta and factor. */
+typedef struct bsattn_rope {
+  const double* theta;  /* device, [dims / 2]: radians per position */
+  int32_t dims;         /* rotated leading dims of each head: even, 2..128 */
+  int32_t interleaved;  /* 0 or 1 */
+  float factor;         /* on the rotated dims; 1 for plain rotary positions */
+  int32_t reserved;     /* must be 0 */
+} bsattn_rope;
+
+/* Rotates x [n_seqs, heads, n_tokens, D] into out (dense, the same shape, in
+ * the cache's dtype): applyRotaryPosition(rope, to:, cache:)
+ * (Libraries/MLXLMCommon/RoPEApplication.swift:23-27).  strides: elements
+ * between sequences, heads and tokens of x, multiples of 8 (null: dense);
+ * the 128 dims are contiguous, x and out 16-byte aligned.  positions (device,
+ * [n_seqs, n_tokens] int32) may be null: then sequence i's tokens follow
+ * those that the cache holds, at its device-side length (the tokens are
+ * rotated before they are appended; also inside a captured
+ * [rotate, append_step, decode] loop).  out may be x itself when x is dense;
+ * otherwise they must not overlap. */
+int bsattn_rotate(bsattn_cache* cache, const bsattn_rope* rope, const void* x,
+                  const int64_t* strides, int32_t heads, const int32_t* seq_ids,
+                  int32_t n_seqs, int32_t n_tokens, const int32_t* positions,
+                  void* out, void* stream);
+
+/* RMS norms of queries and keys per head, then their rotary positions, in
+ * one pass: y = x * rsqrt(mean(x^2) + eps) * (weight_offset + weight), rotated
+ * as bsattn_rotate does, in fp32 and rounded once.  q / q_out
+ * [n_seqs, Hq, n_tokens, D], k / k_out [n_seqs, Hkv, n_tokens, D], weights
+ * [D] in the cache's dtype.  Strides, positions and aliasing as in
+ * bsattn_rotate: q and k may be views into one fused projection, the outputs
+ * are what bsattn_append and the decodes take.  Replaces the qNorm / kNorm and
+ * rope calls ahead of attentionWithCacheUpdate. */
+int bsattn_norm_rotate(bsattn_cache* cache, const bsattn_rope* rope, const void* q,
+                       const int64_t* q_strides, const void* k,
+                       const int64_t* k_strides, const void* q_weight,
+                       const void* k_weight, float eps, float weight_offset,
+                       const int32_t* seq_ids, int32_t n_seqs, int32_t n_tokens,
+                       const int32_t* positions, void* q_out, void* k_out,
+                       void* stream);
+
 /* Graph-capturable decode loop.  bsattn_reserve takes the pages for
  * n_tokens more tokens of each listed sequence now; bsattn_append_step then
  * appends one token per listed sequence (k / v [n_seqs, Hkv, 1, D]) at the
@@ -285,6 +330,7 @@ int bsattn_export_summaries(const bsattn_cache* cache, int32_t seq, void* out,
 #define BSATTN_KERNEL_APPEND 4  /* token append */
 #define BSATTN_KERNEL_SUMMARY 5 /* retired, always 0: summaries are written by the launch that stores the keys */
 #define BSATTN_KERNEL_PREFILL 6 /* dense causal prefill attention */
+#define BSATTN_KERNEL_ROTATE 7  /* rotary positions, with the norms or alone */
 int bsattn_profile_enable(bsattn_cache* cache, int32_t enable);
 int bsattn_profile_read(bsattn_cache* cache, int32_t kernel, double* total_ms,
                         int64_t* launches);

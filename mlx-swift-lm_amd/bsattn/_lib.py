@@ -42,6 +42,8 @@ EXPORTS = (
     "bsattn_append_decode",
     "bsattn_decode_multi",
     "bsattn_prefill",
+    "bsattn_rotate",
+    "bsattn_norm_rotate",
     "bsattn_reserve",
     "bsattn_append_step",
     "bsattn_sync",
@@ -55,7 +57,8 @@ EXPORTS = (
     "bsattn_profile_read",
 )
 
-KERNEL_SCORE, KERNEL_TOPK, KERNEL_ATTEND, KERNEL_COMBINE, KERNEL_APPEND, KERNEL_SUMMARY, KERNEL_PREFILL = range(7)
+KERNEL_SCORE, KERNEL_TOPK, KERNEL_ATTEND, KERNEL_COMBINE, KERNEL_APPEND, KERNEL_SUMMARY, KERNEL_PREFILL, \
+    KERNEL_ROTATE = range(8)
 
 
 class BsattnError(RuntimeError):
@@ -94,6 +97,16 @@ class Info(ctypes.Structure):
     ]
 
 
+class Rope(ctypes.Structure):
+    _fields_ = [
+        ("theta", ctypes.c_void_p),
+        ("dims", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("factor", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
 _lib = None
 
 
@@ -109,6 +122,7 @@ def lib() -> ctypes.CDLL:
     P = ctypes.c_void_p
     i32 = ctypes.c_int32
     PI32 = ctypes.POINTER(ctypes.c_int32)
+    PI64 = ctypes.POINTER(ctypes.c_int64)
     PP = ctypes.POINTER(ctypes.c_void_p)
     sig = {
         "bsattn_version": (i32, []),
@@ -128,6 +142,9 @@ def lib() -> ctypes.CDLL:
         "bsattn_append_decode": (ctypes.c_int, [P, P, P, P, PI32, i32, ctypes.c_float, P, P, P]),
         "bsattn_decode_multi": (ctypes.c_int, [P, P, PI32, i32, i32, ctypes.c_float, P, P, P]),
         "bsattn_prefill": (ctypes.c_int, [P, P, PI32, i32, i32, ctypes.c_float, P, P]),
+        "bsattn_rotate": (ctypes.c_int, [P, ctypes.POINTER(Rope), P, PI64, i32, PI32, i32, i32, P, P, P]),
+        "bsattn_norm_rotate": (ctypes.c_int, [P, ctypes.POINTER(Rope), P, PI64, P, PI64, P, P, ctypes.c_float,
+                                              ctypes.c_float, PI32, i32, i32, P, P, P, P]),
         "bsattn_reserve": (ctypes.c_int, [P, PI32, i32, i32, P]),
         "bsattn_append_step": (ctypes.c_int, [P, P, P, PI32, i32, P]),
         "bsattn_sync": (ctypes.c_int, [P, P]),

@@ -416,6 +416,61 @@ class BlockSparseKVCache:
                                    scale, _ptr(out), _stream(self.device)))
         return out
 
+    # -- rotary positions ------------------------------------------------------
+    def _check_strided(self, t: torch.Tensor, name: str, heads: int):
+        """Element strides of t [B, heads, L, D] between sequences, heads and
+        tokens; the dims are contiguous and every row 16-byte aligned."""
+        if t.device != self.device or t.dtype != self.dtype:
+            raise ValueError(f"{name} must be a {self.dtype} tensor on {self.device}")
+        if t.dim() != 4 or heads < 1 or t.shape[1] != heads or t.shape[3] != self._dim or 0 in t.shape:
+            raise ValueError(f"{name} must be [B, {heads or 'H'}, L, {self._dim}], got {tuple(t.shape)}")
+        # (torch gives a dimension of one element any stride)
+        st = [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
+        if st[3] != 1 or st[0] % 8 or st[1] % 8 or st[2] % 8 or t.data_ptr() % 16:
+            raise ValueError(f"{name} must have contiguous, 16-byte aligned heads, got strides {t.stride()} at "
+                             f"offset {t.storage_offset()}")
+        return (ctypes.c_int64 * 3)(*st[:3])
+
+    def _check_rope(self, rope) -> None:
+        if rope.device != self.device:
+            raise ValueError(f"the rope is on {rope.device}, the cache on {self.device}")
+
+    def _check_positions(self, positions: Optional[torch.Tensor], B: int, L: int):
+        if positions is None:
+            return None
+        if positions.dtype != torch.int32 or positions.device != self.device or not positions.is_contiguous() \
+                or tuple(positions.shape) != (B, L):
+            raise ValueError(f"positions must be a contiguous int32 tensor ({B}, {L}) on {self.device}, got "
+                             f"{positions.dtype} {tuple(positions.shape)}")
+        return positions.data_ptr()
+
+    def normRotate(self, queries: torch.Tensor, keys: torch.Tensor, qWeight: torch.Tensor, kWeight: torch.Tensor,
+                   eps: float, rope, positions: Optional[torch.Tensor] = None,
+                   seq_ids: Optional[Sequence[int]] = None, weightOffset: float = 0.0):
+        """RMS norms of the heads of queries [B, Hq, L, D] and keys
+        [B, Hkv, L, D], scaled by weightOffset + weight ([D]), then their
+        rotary positions, in one pass.  Views into a fused projection will do;
+        the results are dense.  positions [B, L] int32; by default each
+        sequence's tokens follow those that the cache holds."""
+        qs = self._check_strided(queries, "queries", self._hq)
+        ks = self._check_strided(keys, "keys", self._hkv)
+        B, _, L, _ = queries.shape
+        if keys.shape[0] != B or keys.shape[2] != L:
+            raise ValueError("queries and keys disagree on B or L")
+        for name, w in (("qWeight", qWeight), ("kWeight", kWeight)):
+            if w.dtype != self.dtype or w.device != self.device or tuple(w.shape) != (self._dim,) \
+                    or not w.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous {self.dtype} tensor ({self._dim},) on {self.device}")
+        self._check_rope(rope)
+        pos = self._check_positions(positions, B, L)
+        q = torch.empty(queries.shape, dtype=self.dtype, device=self.device)
+        k = torch.empty(keys.shape, dtype=self.dtype, device=self.device)
+        check(self._lib.bsattn_norm_rotate(self._h, rope._ref, queries.data_ptr(), qs, keys.data_ptr(), ks,
+                                           qWeight.data_ptr(), kWeight.data_ptr(), eps, weightOffset,
+                                           i32_array(seq_ids), B, L, pos, q.data_ptr(), k.data_ptr(),
+                                           _stream(self.device)))
+        return q, k
+
     # -- kernel timing -------------------------------------------------------
     def profile(self, enable: bool = True) -> None:
         """Start (or stop) timing this cache's eager kernel launches; resets sums."""

@@ -115,7 +115,7 @@ struct StepAppend {
 // slot's events are set) and marks the slot used.
 enum ProfKind {
   kProfScore = 0, kProfTopk = 1, kProfAttend = 2, kProfCombine = 3, kProfAppend = 4,
-  kProfSummary = 5, kProfPrefill = 6, kProfKinds = 7
+  kProfSummary = 5, kProfPrefill = 6, kProfRotate = 7, kProfKinds = 8
 };
 struct Timing {
   hipEvent_t start = nullptr, stop = nullptr;
@@ -239,6 +239,25 @@ hipError_t launch_prefill(const Geometry& g, const SeqBatch& b, int L, int nspli
                           void* out, float* ws, hipEvent_t done, hipStream_t s, Timing* prof);
 // parts for a launch of n sequences of up to `tokens` tokens
 int prefill_splits(const Geometry& g, int n, int L, int tokens);
+// Rotary positions of one or two tensors (queries, keys) [n, heads, L, 128]
+// with element strides sb / sh / sl, into dense outputs; w: norm weights of
+// each (null: no norm).  The launch covers entries b0 .. b0 + n - 1 of the
+// call; pos: [entries of the call, L], or null: entry i's tokens follow the
+// ids[i]-th device-side length.
+struct RotateBatch {
+  const uint16_t* x[2];
+  const uint16_t* w[2];
+  uint16_t* out[2];
+  int64_t sb[2], sh[2], sl[2];
+  const double* theta;  // [dims / 2] radians per position
+  const int32_t* pos;
+  int32_t heads[2];
+  int32_t L, b0, dims, interleaved;
+  int32_t share;  // heads per workgroup (launch_rotate sets it)
+  float m, eps, woff;
+  int32_t ids[kMaxBatch];
+};
+hipError_t launch_rotate(const Geometry& g, RotateBatch rb, int n, hipStream_t s, Timing* prof);
 hipError_t launch_export(const Geometry& g, const SeqBatch& b, int T, void* k_out,
                          void* v_out, hipStream_t s);
 hipError_t launch_export_quantized(const Geometry& g, const SeqBatch& b, int T,

@@ -1,0 +1,121 @@
+// bsattn_ops.cpp -- the C ABI's operators around the cache: rotary positions
+// and the norms before them.  Argument checking and kernel sequencing.
+#include <hip/hip_runtime_api.h>
+
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
+#include "bsattn_host.h"
+
+using namespace bsattn;
+
+namespace {
+
+int check_rope(const bsattn_rope& r) {
+  if (!r.theta) return fail(BSATTN_ERR_INVALID, "null rope angles");
+  if (r.dims < 2 || r.dims > kHeadDim || r.dims % 2)
+    return fail(BSATTN_ERR_INVALID, "rope dims %d unsupported (even, 2 to %d)", r.dims, kHeadDim);
+  if (r.interleaved != 0 && r.interleaved != 1)
+    return fail(BSATTN_ERR_INVALID, "rope interleaved must be 0 or 1 (got %d)", r.interleaved);
+  if (!std::isfinite(r.factor)) return fail(BSATTN_ERR_INVALID, "rope factor must be finite");
+  if (r.reserved != 0) return fail(BSATTN_ERR_INVALID, "rope reserved field must be 0");
+  if ((uintptr_t)r.theta % 8) return fail(BSATTN_ERR_INVALID, "rope angles must be 8-byte aligned");
+  return BSATTN_OK;
+}
+
+// tensor i of the batch: x [n, heads, L, D] with its strides, into out
+int set_tensor(RotateBatch& rb, int i, const char* name, const void* x, const int64_t* strides, int heads, int L,
+               void* out) {
+  if (((uintptr_t)x | (uintptr_t)out) % 16)
+    return fail(BSATTN_ERR_INVALID, "%s and its output must be 16-byte aligned", name);
+  const int64_t dense[3] = {(int64_t)heads * L * kHeadDim, (int64_t)L * kHeadDim, kHeadDim};
+  const int64_t* st = strides ? strides : dense;
+  for (int j = 0; j < 3; ++j) {
+    if (st[j] % 8 || st[j] < 0)
+      return fail(BSATTN_ERR_INVALID, "%s strides must be multiples of 8 elements and >= 0 (got %lld)", name,
+                  (long long)st[j]);
+    if (x == out && st[j] != dense[j])
+      return fail(BSATTN_ERR_INVALID, "%s can be rotated in place only when it is dense", name);
+  }
+  rb.x[i] = (const uint16_t*)x;
+  rb.out[i] = (uint16_t*)out;
+  rb.heads[i] = heads;
+  rb.sb[i] = st[0];
+  rb.sh[i] = st[1];
+  rb.sl[i] = st[2];
+  return BSATTN_OK;
+}
+
+int rotate_impl(bsattn_cache* c, const bsattn_rope& rope, RotateBatch& rb, const int32_t* seq_ids, int32_t n_seqs,
+                int32_t n_tokens, const int32_t* positions, hipStream_t s) {
+  std::vector<int32_t> seqs;
+  int rc = seq_list(c, seq_ids, n_seqs, seqs);
+  if (rc) return rc;
+  DeviceGuard dg(c->d.device);
+  if (!dg.ok) return fail(BSATTN_ERR_HIP, "hipSetDevice(%d) failed", c->d.device);
+  if (!positions && (rc = send_unsent(c, s))) return rc;
+  rb.theta = rope.theta;
+  rb.dims = rope.dims;
+  rb.interleaved = rope.interleaved;
+  rb.m = rope.factor;
+  rb.pos = positions;
+  rb.L = n_tokens;
+  for (int i0 = 0; i0 < n_seqs; i0 += kMaxBatch) {
+    const int n = std::min(kMaxBatch, n_seqs - i0);
+    rb.b0 = i0;
+    for (int i = 0; i < n; ++i) rb.ids[i] = seqs[i0 + i];
+    Timing tm[kProfKinds];
+    Timing* prof = prof_slots(c, s, tm);
+    const hipError_t e = launch_rotate(c->geo, rb, n, s, prof);
+    prof_collect(c, prof);
+    if (e != hipSuccess) return hip_fail(e, "rotate launch");
+  }
+  return BSATTN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int bsattn_rotate(bsattn_cache* c, const bsattn_rope* rope, const void* x, const int64_t* strides, int32_t heads,
+                  const int32_t* seq_ids, int32_t n_seqs, int32_t n_tokens, const int32_t* positions, void* out,
+                  void* stream) try {
+  if (!c || !rope || !x || !out) return fail(BSATTN_ERR_INVALID, "null argument");
+  if (int rc = check_rope(*rope)) return rc;
+  if (n_tokens < 1) return fail(BSATTN_ERR_INVALID, "n_tokens must be >= 1 (got %d)", n_tokens);
+  if (heads < 1 || heads > 65535) return fail(BSATTN_ERR_INVALID, "heads %d out of range [1, 65535]", heads);
+  RotateBatch rb{};
+  if (int rc = set_tensor(rb, 0, "x", x, strides, heads, n_tokens, out)) return rc;
+  return rotate_impl(c, *rope, rb, seq_ids, n_seqs, n_tokens, positions, (hipStream_t)stream);
+} catch (...) {
+  return on_exception();
+}
+
+int bsattn_norm_rotate(bsattn_cache* c, const bsattn_rope* rope, const void* q, const int64_t* q_strides,
+                       const void* k, const int64_t* k_strides, const void* q_weight, const void* k_weight, float eps,
+                       float weight_offset, const int32_t* seq_ids, int32_t n_seqs, int32_t n_tokens,
+                       const int32_t* positions, void* q_out, void* k_out, void* stream) try {
+  if (!c || !rope || !q || !k || !q_weight || !k_weight || !q_out || !k_out)
+    return fail(BSATTN_ERR_INVALID, "null argument");
+  if (int rc = check_rope(*rope)) return rc;
+  if (n_tokens < 1) return fail(BSATTN_ERR_INVALID, "n_tokens must be >= 1 (got %d)", n_tokens);
+  if (!(eps >= 0.0f) || !std::isfinite(eps)) return fail(BSATTN_ERR_INVALID, "eps must be finite and >= 0");
+  if (!std::isfinite(weight_offset)) return fail(BSATTN_ERR_INVALID, "weight_offset must be finite");
+  if (((uintptr_t)q_weight | (uintptr_t)k_weight) % 16)
+    return fail(BSATTN_ERR_INVALID, "the norm weights must be 16-byte aligned");
+  if (q_out == k_out || q_out == k || k_out == q)
+    return fail(BSATTN_ERR_INVALID, "queries and keys need outputs of their own");
+  RotateBatch rb{};
+  if (int rc = set_tensor(rb, 0, "queries", q, q_strides, c->geo.hq, n_tokens, q_out)) return rc;
+  if (int rc = set_tensor(rb, 1, "keys", k, k_strides, c->geo.hkv, n_tokens, k_out)) return rc;
+  rb.w[0] = (const uint16_t*)q_weight;
+  rb.w[1] = (const uint16_t*)k_weight;
+  rb.eps = eps;
+  rb.woff = weight_offset;
+  return rotate_impl(c, *rope, rb, seq_ids, n_seqs, n_tokens, positions, (hipStream_t)stream);
+} catch (...) {
+  return on_exception();
+}
+
+}  // extern "C"
