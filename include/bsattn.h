@@ -217,6 +217,23 @@ int bsattn_prefill(bsattn_cache* cache, const void* q, const int32_t* seq_ids,
                    int32_t n_seqs, int32_t n_query, float scale, void* out,
                    void* stream);
 
+/* Dense decode: attention of one new token per sequence over every token of
+ * its cache (16-bit or quantized), or over the last `window` ones (0: all):
+ * softmax(q k^T * scale) v as the dense path of attentionWithCacheUpdate
+ * computes for L = 1 (AttentionUtils.swift:46-52, :68-75; KVCache.swift:
+ * 1533-1621), for the layers and models that take no block selection.  The
+ * token's own key and value have been appended.  q / out [n_seqs, Hq, 1, D];
+ * sinks: [Hq] float logits (device) that join each head's softmax without a
+ * value, or null.  A sequence that holds no token gives zeros.  Like
+ * bsattn_decode it sizes its launches from the held pages and reads the
+ * device-side lengths, so it may follow bsattn_append_step without
+ * bsattn_sync.  Long sequences are split over the GPU and joined through the
+ * workspace that bsattn_prefill describes; when none can be had the call runs
+ * unsplit: slower, and rounded differently. */
+int bsattn_decode_dense(bsattn_cache* cache, const void* q, const int32_t* seq_ids,
+                        int32_t n_seqs, int32_t window, const float* sinks,
+                        float scale, void* out, void* stream);
+
 /* Rotary positions.  For a head x[0, 128) of the token at position p, the
  * pairs (a, b) of its first `dims` dims become
  *   a' = factor (a cos phi - b sin phi),  b' = factor (a sin phi + b cos phi),
@@ -331,6 +348,7 @@ int bsattn_export_summaries(const bsattn_cache* cache, int32_t seq, void* out,
 #define BSATTN_KERNEL_SUMMARY 5 /* retired, always 0: summaries are written by the launch that stores the keys */
 #define BSATTN_KERNEL_PREFILL 6 /* dense causal prefill attention */
 #define BSATTN_KERNEL_ROTATE 7  /* rotary positions, with the norms or alone */
+#define BSATTN_KERNEL_DENSE 8   /* dense decode attention (its join counts as BSATTN_KERNEL_COMBINE) */
 int bsattn_profile_enable(bsattn_cache* cache, int32_t enable);
 int bsattn_profile_read(bsattn_cache* cache, int32_t kernel, double* total_ms,
                         int64_t* launches);

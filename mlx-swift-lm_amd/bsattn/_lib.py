@@ -42,6 +42,7 @@ EXPORTS = (
     "bsattn_append_decode",
     "bsattn_decode_multi",
     "bsattn_prefill",
+    "bsattn_decode_dense",
     "bsattn_rotate",
     "bsattn_norm_rotate",
     "bsattn_reserve",
@@ -58,7 +59,7 @@ EXPORTS = (
 )
 
 KERNEL_SCORE, KERNEL_TOPK, KERNEL_ATTEND, KERNEL_COMBINE, KERNEL_APPEND, KERNEL_SUMMARY, KERNEL_PREFILL, \
-    KERNEL_ROTATE = range(8)
+    KERNEL_ROTATE, KERNEL_DENSE = range(9)
 
 
 class BsattnError(RuntimeError):
@@ -142,6 +143,7 @@ def lib() -> ctypes.CDLL:
         "bsattn_append_decode": (ctypes.c_int, [P, P, P, P, PI32, i32, ctypes.c_float, P, P, P]),
         "bsattn_decode_multi": (ctypes.c_int, [P, P, PI32, i32, i32, ctypes.c_float, P, P, P]),
         "bsattn_prefill": (ctypes.c_int, [P, P, PI32, i32, i32, ctypes.c_float, P, P]),
+        "bsattn_decode_dense": (ctypes.c_int, [P, P, PI32, i32, i32, P, ctypes.c_float, P, P]),
         "bsattn_rotate": (ctypes.c_int, [P, ctypes.POINTER(Rope), P, PI64, i32, PI32, i32, i32, P, P, P]),
         "bsattn_norm_rotate": (ctypes.c_int, [P, ctypes.POINTER(Rope), P, PI64, P, PI64, P, P, ctypes.c_float,
                                               ctypes.c_float, PI32, i32, i32, P, P, P, P]),

@@ -416,6 +416,31 @@ class BlockSparseKVCache:
                                    scale, _ptr(out), _stream(self.device)))
         return out
 
+    # -- dense decode ------------------------------------------------------------
+    def _check_sinks(self, sinks: Optional[torch.Tensor]):
+        if sinks is None:
+            return None
+        if sinks.dtype != torch.float32 or sinks.device != self.device or tuple(sinks.shape) != (self._hq,) \
+                or not sinks.is_contiguous():
+            raise ValueError(f"sinks must be a contiguous float32 tensor ({self._hq},) on {self.device}")
+        return sinks.data_ptr()
+
+    def decodeDense(self, queries: torch.Tensor, scale: float, window: Optional[int] = None,
+                    sinks: Optional[torch.Tensor] = None,
+                    seq_ids: Optional[Sequence[int]] = None) -> torch.Tensor:
+        """Attention of queries [B, Hq, 1, D] over every token that the
+        sequences hold (the new one appended), or over the last `window`: the
+        reference's dense decode, for layers that take no block selection.
+        sinks: [Hq] float32 logits that join each head's softmax without a
+        value.  A sequence without tokens gives zeros."""
+        B = self._check_q(queries)
+        if window is not None and window < 1:
+            raise ValueError(f"window must be at least 1 (got {window})")
+        out = torch.empty_like(queries)
+        check(self._lib.bsattn_decode_dense(self._h, queries.data_ptr(), i32_array(seq_ids), B, window or 0,
+                                            self._check_sinks(sinks), scale, out.data_ptr(), _stream(self.device)))
+        return out
+
     # -- rotary positions ------------------------------------------------------
     def _check_strided(self, t: torch.Tensor, name: str, heads: int):
         """Element strides of t [B, heads, L, D] between sequences, heads and

@@ -115,7 +115,7 @@ struct StepAppend {
 // slot's events are set) and marks the slot used.
 enum ProfKind {
   kProfScore = 0, kProfTopk = 1, kProfAttend = 2, kProfCombine = 3, kProfAppend = 4,
-  kProfSummary = 5, kProfPrefill = 6, kProfRotate = 7, kProfKinds = 8
+  kProfSummary = 5, kProfPrefill = 6, kProfRotate = 7, kProfDense = 8, kProfKinds = 9
 };
 struct Timing {
   hipEvent_t start = nullptr, stop = nullptr;
@@ -258,6 +258,21 @@ struct RotateBatch {
   int32_t ids[kMaxBatch];
 };
 hipError_t launch_rotate(const Geometry& g, RotateBatch rb, int n, hipStream_t s, Timing* prof);
+// Dense decode: entry i is the query of sequence ids[i]; its parts of `cu`
+// units of 32 tokens are the launch's part0[i] and on.  window: the last tokens
+// seen (0: all); sinks: [hq] logits of the heads, or null.
+struct DenseBatch {
+  int32_t n, cu, window;
+  float sl2;
+  const float* sinks;
+  int32_t ids[kMaxBatch];
+  int32_t part0[kMaxBatch];
+};
+int dense_plan(const Geometry& g, const int32_t* units, DenseBatch& db);
+// ws: parts * hq rows of kHeadDim + 2 floats (not needed with one part an
+// entry); the launch that joins them records `done` (may be null)
+hipError_t launch_dense(const Geometry& g, const DenseBatch& db, int parts, const void* q, void* out, float* ws,
+                        hipEvent_t done, hipStream_t s, Timing* prof);
 hipError_t launch_export(const Geometry& g, const SeqBatch& b, int T, void* k_out,
                          void* v_out, hipStream_t s);
 hipError_t launch_export_quantized(const Geometry& g, const SeqBatch& b, int T,

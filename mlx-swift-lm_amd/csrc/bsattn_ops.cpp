@@ -1,8 +1,10 @@
-// bsattn_ops.cpp -- the C ABI's operators around the cache: rotary positions
-// and the norms before them.  Argument checking and kernel sequencing.
+// bsattn_ops.cpp -- the C ABI's operators around the cache: dense decode,
+// rotary positions and the norms before them.  Argument checking and kernel
+// sequencing.
 #include <hip/hip_runtime_api.h>
 
 #include <algorithm>
+#include <climits>
 #include <cmath>
 #include <vector>
 
@@ -74,9 +76,69 @@ int rotate_impl(bsattn_cache* c, const bsattn_rope& rope, RotateBatch& rb, const
   return BSATTN_OK;
 }
 
+// workspace and event for the parts of a call, as for a split prefill
+template <typename F>
+hipError_t with_partials(bsattn_cache* c, int64_t rows, hipStream_t s, F launch) {
+  if (capturing(s)) return launch(graph_workspace(c, rows), nullptr);
+  PrefillSpaces* spaces = PrefillSpaces::of(c->d.device);
+  return spaces ? spaces->with(s, launch) : launch(nullptr, nullptr);
+}
+
 }  // namespace
 
 extern "C" {
+
+int bsattn_decode_dense(bsattn_cache* c, const void* q, const int32_t* seq_ids, int32_t n_seqs, int32_t window,
+                        const float* sinks, float scale, void* out, void* stream) try {
+  if (!c || !q || !out) return fail(BSATTN_ERR_INVALID, "null argument");
+  if (window < 0) return fail(BSATTN_ERR_INVALID, "window must be >= 0 (got %d)", window);
+  if (((uintptr_t)q | (uintptr_t)out) % 16) return fail(BSATTN_ERR_INVALID, "q and out must be 16-byte aligned");
+  if ((uintptr_t)sinks % 4) return fail(BSATTN_ERR_INVALID, "sinks must be 4-byte aligned");
+  std::vector<int32_t> seqs;
+  int rc = seq_list(c, seq_ids, n_seqs, seqs);
+  if (rc) return rc;
+  DeviceGuard dg(c->d.device);
+  if (!dg.ok) return fail(BSATTN_ERR_HIP, "hipSetDevice(%d) failed", c->d.device);
+  hipStream_t s = (hipStream_t)stream;
+  rc = send_unsent(c, s);
+  if (rc) return rc;
+  const Geometry& g = c->geo;
+  for (int i0 = 0; i0 < n_seqs; i0 += kMaxBatch) {
+    DenseBatch db{};
+    db.n = std::min(kMaxBatch, n_seqs - i0);
+    db.window = window;
+    db.sl2 = scale * 1.4426950408889634f;
+    db.sinks = sinks;
+    int32_t units[kMaxBatch];
+    for (int i = 0; i < db.n; ++i) {
+      db.ids[i] = seqs[i0 + i];
+      // (the pages may hold fewer tokens than fit them; a window can begin
+      // and end inside a unit)
+      const int64_t held = (int64_t)c->pages[db.ids[i]].size() * g.tb;
+      units[i] = (int32_t)((held + 31) / 32);
+      if (window > 0) units[i] = (int32_t)std::min<int64_t>(units[i], ((int64_t)window + 62) / 32);
+    }
+    const int parts = dense_plan(g, units, db);
+    const uint16_t* qq = (const uint16_t*)q + (size_t)i0 * g.hq * kHeadDim;
+    uint16_t* oo = (uint16_t*)out + (size_t)i0 * g.hq * kHeadDim;
+    Timing tm[kProfKinds];
+    Timing* prof = prof_slots(c, s, tm);
+    auto run = [&](float* ws, hipEvent_t done) {
+      if (ws) return launch_dense(g, db, parts, qq, oo, ws, done, s, prof);
+      DenseBatch whole = db;  // (without a workspace: one part an entry)
+      whole.cu = INT32_MAX / 32;
+      for (int i = 0; i < db.n; ++i) whole.part0[i] = i;
+      return launch_dense(g, whole, db.n, qq, oo, nullptr, nullptr, s, prof);
+    };
+    const hipError_t e = parts == db.n ? launch_dense(g, db, parts, qq, oo, nullptr, nullptr, s, prof)
+                                       : with_partials(c, (int64_t)parts * g.hq, s, run);
+    prof_collect(c, prof);
+    if (e != hipSuccess) return hip_fail(e, "dense decode launch");
+  }
+  return BSATTN_OK;
+} catch (...) {
+  return on_exception();
+}
 
 int bsattn_rotate(bsattn_cache* c, const bsattn_rope* rope, const void* x, const int64_t* strides, int32_t heads,
                   const int32_t* seq_ids, int32_t n_seqs, int32_t n_tokens, const int32_t* positions, void* out,
