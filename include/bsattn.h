@@ -74,7 +74,7 @@ typedef struct bsattn_info {
   int64_t page_bytes;      /* bytes of one page across all kv heads, incl. summaries */
   int64_t pool_bytes;      /* device bytes of the handle's pages, summaries and metadata
                               (workspaces not counted) */
-  int64_t free_pages;      /* pages not owned by any sequence */
+  int64_t free_pages;      /* pages that no sequence holds */
 } bsattn_info;
 
 int32_t bsattn_version(void);
@@ -267,7 +267,7 @@ int bsattn_rotate(bsattn_cache* cache, const bsattn_rope* rope, const void* x,
  * one pass: y = x * rsqrt(mean(x^2) + eps) * (weight_offset + weight), rotated
  * as bsattn_rotate does, in fp32 and rounded once.  q / q_out
  * [n_seqs, Hq, n_tokens, D], k / k_out [n_seqs, Hkv, n_tokens, D], weights
- * [D] in the cache's dtype.  Strides, positions and aliasing as in
+ * [D] in the cache's dtype (both null: no norm, the positions alone).  Strides, positions and aliasing as in
  * bsattn_rotate: q and k may be views into one fused projection, the outputs
  * are what bsattn_append and the decodes take.  Replaces the qNorm / kNorm and
  * rope calls ahead of attentionWithCacheUpdate. */
@@ -297,6 +297,21 @@ int bsattn_reserve(bsattn_cache* cache, const int32_t* seq_ids,
 int bsattn_append_step(bsattn_cache* cache, const void* k, const void* v,
                        const int32_t* seq_ids, int32_t n_seqs, void* stream);
 int bsattn_sync(bsattn_cache* cache, void* stream);
+
+/* Forks: sequence dst_ids[i] becomes the first n_tokens[i] tokens of sequence
+ * src_ids[i] (n_tokens null: all that it holds), for samples or beams that
+ * continue one prompt, or a prompt that many requests begin with.  A source
+ * may be listed many times; the destinations are distinct, empty (no pages
+ * either) and not among the sources.  The pages of full blocks are shared and
+ * freed when their last holder lets them go (bsattn_trim, bsattn_reset); a
+ * partial last block is copied, for which the pool must have a page.  The
+ * sequences are independent from then on, and decode, trim and export as if
+ * each had been appended by itself.  (A trim that ends inside a block which
+ * others hold copies its page, and needs a free one.)  src_ids, dst_ids and
+ * n_tokens are host arrays.  Not in a capture.  The paged form of copying a
+ * cache (KVCacheSimple.copy, KVCache.swift:429-437). */
+int bsattn_fork(bsattn_cache* cache, const int32_t* src_ids, const int32_t* dst_ids,
+                int32_t n, const int32_t* n_tokens, void* stream);
 
 /* Drops the last n_tokens of each listed sequence (clamped to its length);
  * writes the number trimmed per sequence to trimmed (host, may be NULL).
@@ -349,6 +364,7 @@ int bsattn_export_summaries(const bsattn_cache* cache, int32_t seq, void* out,
 #define BSATTN_KERNEL_PREFILL 6 /* dense causal prefill attention */
 #define BSATTN_KERNEL_ROTATE 7  /* rotary positions, with the norms or alone */
 #define BSATTN_KERNEL_DENSE 8   /* dense decode attention (its join counts as BSATTN_KERNEL_COMBINE) */
+#define BSATTN_KERNEL_FORK 9    /* forks */
 int bsattn_profile_enable(bsattn_cache* cache, int32_t enable);
 int bsattn_profile_read(bsattn_cache* cache, int32_t kernel, double* total_ms,
                         int64_t* launches);

@@ -48,6 +48,7 @@ EXPORTS = (
     "bsattn_reserve",
     "bsattn_append_step",
     "bsattn_sync",
+    "bsattn_fork",
     "bsattn_trim",
     "bsattn_reset",
     "bsattn_copy",
@@ -59,7 +60,7 @@ EXPORTS = (
 )
 
 KERNEL_SCORE, KERNEL_TOPK, KERNEL_ATTEND, KERNEL_COMBINE, KERNEL_APPEND, KERNEL_SUMMARY, KERNEL_PREFILL, \
-    KERNEL_ROTATE, KERNEL_DENSE = range(9)
+    KERNEL_ROTATE, KERNEL_DENSE, KERNEL_FORK = range(10)
 
 
 class BsattnError(RuntimeError):
@@ -150,6 +151,7 @@ def lib() -> ctypes.CDLL:
         "bsattn_reserve": (ctypes.c_int, [P, PI32, i32, i32, P]),
         "bsattn_append_step": (ctypes.c_int, [P, P, P, PI32, i32, P]),
         "bsattn_sync": (ctypes.c_int, [P, P]),
+        "bsattn_fork": (ctypes.c_int, [P, PI32, PI32, i32, PI32, P]),
         "bsattn_trim": (ctypes.c_int, [P, PI32, i32, i32, PI32, P]),
         "bsattn_reset": (ctypes.c_int, [P, PI32, i32, P]),
         "bsattn_copy": (ctypes.c_int, [P, PP, P]),

@@ -425,6 +425,13 @@ class BlockSparseKVCache:
             raise ValueError(f"sinks must be a contiguous float32 tensor ({self._hq},) on {self.device}")
         return sinks.data_ptr()
 
+    def _check_window(self, window: Optional[int]) -> int:
+        if window is None:
+            return 0
+        if window < 1:
+            raise ValueError(f"window must be at least 1 (got {window})")
+        return min(int(window), 2 ** 31 - 1)
+
     def decodeDense(self, queries: torch.Tensor, scale: float, window: Optional[int] = None,
                     sinks: Optional[torch.Tensor] = None,
                     seq_ids: Optional[Sequence[int]] = None) -> torch.Tensor:
@@ -434,11 +441,9 @@ class BlockSparseKVCache:
         sinks: [Hq] float32 logits that join each head's softmax without a
         value.  A sequence without tokens gives zeros."""
         B = self._check_q(queries)
-        if window is not None and window < 1:
-            raise ValueError(f"window must be at least 1 (got {window})")
         out = torch.empty_like(queries)
-        check(self._lib.bsattn_decode_dense(self._h, queries.data_ptr(), i32_array(seq_ids), B, window or 0,
-                                            self._check_sinks(sinks), scale, out.data_ptr(), _stream(self.device)))
+        check(self._lib.bsattn_decode_dense(self._h, queries.data_ptr(), i32_array(seq_ids), B,
+                                            self._check_window(window), self._check_sinks(sinks), scale, out.data_ptr(), _stream(self.device)))
         return out
 
     # -- rotary positions ------------------------------------------------------
@@ -469,20 +474,25 @@ class BlockSparseKVCache:
                              f"{positions.dtype} {tuple(positions.shape)}")
         return positions.data_ptr()
 
-    def normRotate(self, queries: torch.Tensor, keys: torch.Tensor, qWeight: torch.Tensor, kWeight: torch.Tensor,
-                   eps: float, rope, positions: Optional[torch.Tensor] = None,
+    def normRotate(self, queries: torch.Tensor, keys: torch.Tensor, qWeight: Optional[torch.Tensor],
+                   kWeight: Optional[torch.Tensor], eps: float, rope, positions: Optional[torch.Tensor] = None,
                    seq_ids: Optional[Sequence[int]] = None, weightOffset: float = 0.0):
         """RMS norms of the heads of queries [B, Hq, L, D] and keys
         [B, Hkv, L, D], scaled by weightOffset + weight ([D]), then their
         rotary positions, in one pass.  Views into a fused projection will do;
-        the results are dense.  positions [B, L] int32; by default each
-        sequence's tokens follow those that the cache holds."""
+        the results are dense.  Both weights None: the positions alone.
+        positions [B, L] int32; by default each sequence's tokens follow those
+        that the cache holds."""
         qs = self._check_strided(queries, "queries", self._hq)
         ks = self._check_strided(keys, "keys", self._hkv)
         B, _, L, _ = queries.shape
         if keys.shape[0] != B or keys.shape[2] != L:
             raise ValueError("queries and keys disagree on B or L")
+        if (qWeight is None) != (kWeight is None):
+            raise ValueError("give both norm weights or neither")
         for name, w in (("qWeight", qWeight), ("kWeight", kWeight)):
+            if w is None:
+                continue
             if w.dtype != self.dtype or w.device != self.device or tuple(w.shape) != (self._dim,) \
                     or not w.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous {self.dtype} tensor ({self._dim},) on {self.device}")
@@ -491,7 +501,8 @@ class BlockSparseKVCache:
         q = torch.empty(queries.shape, dtype=self.dtype, device=self.device)
         k = torch.empty(keys.shape, dtype=self.dtype, device=self.device)
         check(self._lib.bsattn_norm_rotate(self._h, rope._ref, queries.data_ptr(), qs, keys.data_ptr(), ks,
-                                           qWeight.data_ptr(), kWeight.data_ptr(), eps, weightOffset,
+                                           None if qWeight is None else qWeight.data_ptr(),
+                                           None if kWeight is None else kWeight.data_ptr(), eps, weightOffset,
                                            i32_array(seq_ids), B, L, pos, q.data_ptr(), k.data_ptr(),
                                            _stream(self.device)))
         return q, k
@@ -570,6 +581,16 @@ class BlockSparseKVCache:
         out = (ctypes.c_int32 * len(ids))()
         check(lib().bsattn_trim(self._h, i32_array(ids), len(ids), n, out, _stream(self.device)))
         return int(out[0])
+
+    def fork(self, src: Sequence[int], dst: Sequence[int], n_tokens: Optional[Sequence[int]] = None) -> None:
+        """Sequence dst[i] (empty) becomes the first n_tokens[i] tokens of
+        src[i] (default: all of them): the pages of full blocks are shared, a
+        partial last block is copied.  From then on the sequences are
+        independent; trim and reset free the pages that nobody else holds."""
+        if len(src) != len(dst) or (n_tokens is not None and len(n_tokens) != len(src)):
+            raise ValueError("src, dst and n_tokens must have one entry per fork")
+        check(self._lib.bsattn_fork(self._h, i32_array(src), i32_array(dst), len(src), i32_array(n_tokens),
+                                    _stream(self.device)))
 
     def reset(self, seq_ids: Sequence[int]) -> None:
         check(lib().bsattn_reset(self._h, i32_array(seq_ids), len(seq_ids), _stream(self.device)))

@@ -199,6 +199,7 @@ int bsattn_cache_create(const bsattn_desc* desc, bsattn_cache** out) try {
     c->len.assign(d.max_seqs, 0);
     c->pages.assign(d.max_seqs, {});
     c->free_pages.resize(c->num_pages);
+    c->sharers.assign(c->num_pages, 0);
   } catch (...) {
     delete c;
     throw;
@@ -855,6 +856,57 @@ int bsattn_prefill(bsattn_cache* c, const void* q, const int32_t* seq_ids, int32
   return on_exception();
 }
 
+// Sequences that a trim leaves inside a block which others hold too: each but
+// the last holder gets a copy of the block's page, before any bookkeeping.
+// The copies go to free pages (the first from_free, from the top of the
+// stack), beyond those to pages that the trim itself lets go.
+struct UnsharedTails {
+  struct Tail {
+    int32_t seq, to;
+  };
+  std::vector<Tail> list;
+  size_t from_free = 0;
+};
+
+static int unshare_tails(bsattn_cache* c, const std::vector<int32_t>& seqs, int n_tokens, hipStream_t s,
+                         UnsharedTails& out) {
+  const int tb = c->d.block_size;
+  auto kept = [&](int sq) { return c->len[sq] - std::min(c->len[sq], n_tokens); };
+  std::vector<int32_t> shared;  // the sequences that end inside a shared block
+  for (int sq : seqs)
+    if (kept(sq) % tb && c->sharers[c->pages[sq][kept(sq) / tb]] > 0) shared.push_back(sq);
+  if (shared.empty()) return BSATTN_OK;
+  std::vector<int32_t> dropped(c->num_pages, 0);  // holders that let go of each page
+  for (int sq : seqs)
+    for (size_t b = (size_t)(kept(sq) + tb - 1) / tb; b < c->pages[sq].size(); ++b) ++dropped[c->pages[sq][b]];
+  std::vector<int32_t> from;
+  for (int sq : shared) {
+    const int32_t page = c->pages[sq][kept(sq) / tb];
+    if (dropped[page] >= c->sharers[page]) continue;  // the last holder keeps it
+    ++dropped[page];
+    out.list.push_back({sq, -1});
+    from.push_back(page);
+  }
+  if (out.list.empty()) return BSATTN_OK;
+  if (capturing(s))
+    return fail(BSATTN_ERR_INVALID, "a trim inside a block that other sequences hold cannot be captured");
+  out.from_free = std::min(out.list.size(), c->free_pages.size());
+  std::vector<int32_t> to(c->free_pages.end() - out.from_free, c->free_pages.end());
+  for (int64_t p = 0; p < c->num_pages && to.size() < out.list.size(); ++p)
+    if (dropped[p] > c->sharers[p]) to.push_back((int32_t)p);
+  if (to.size() < out.list.size())
+    return fail(BSATTN_ERR_NO_PAGES, "page pool exhausted: %zu sequences end inside blocks that others hold",
+                out.list.size());
+  const size_t bytes = page_slabs(c->geo);
+  for (size_t i = 0; i < to.size(); ++i) {
+    out.list[i].to = to[i];
+    HIP_TRY(hipMemcpyAsync(c->geo.pool + (size_t)to[i] * bytes, c->geo.pool + (size_t)from[i] * bytes, bytes,
+                           hipMemcpyDeviceToDevice, s),
+            "page copy");
+  }
+  return BSATTN_OK;
+}
+
 int bsattn_trim(bsattn_cache* c, const int32_t* seq_ids, int32_t n_seqs, int32_t n_tokens,
                 int32_t* trimmed, void* stream) try {
   if (!c) return fail(BSATTN_ERR_INVALID, "null argument");
@@ -868,7 +920,11 @@ int bsattn_trim(bsattn_cache* c, const int32_t* seq_ids, int32_t n_seqs, int32_t
   rc = send_unsent(c, (hipStream_t)stream);
   if (rc) return rc;
   Patches patches;
-  patches.reserve(2 * seqs.size());  // the loop below then cannot throw
+  patches.reserve(3 * seqs.size());  // the loops below then cannot throw
+  UnsharedTails tails;
+  rc = unshare_tails(c, seqs, n_tokens, (hipStream_t)stream, tails);
+  if (rc) return rc;
+  c->free_pages.resize(c->free_pages.size() - tails.from_free);
   for (int i = 0; i < n_seqs; ++i) {
     const int sq = seqs[i];
     const int t = std::min(c->len[sq], n_tokens);
@@ -877,6 +933,14 @@ int bsattn_trim(bsattn_cache* c, const int32_t* seq_ids, int32_t n_seqs, int32_t
     release_pages(c, sq, (c->len[sq] + c->d.block_size - 1) / c->d.block_size, patches);
     patches.emplace_back(sq, c->len[sq]);
   }
+  for (const auto& t : tails.list) {
+    int32_t& page = c->pages[t.seq].back();
+    --c->sharers[page];
+    page = t.to;
+    patches.emplace_back(c->geo.bt_off + t.seq * c->d.max_blocks_per_seq + (int)c->pages[t.seq].size() - 1, t.to);
+  }
+  for (size_t i = tails.from_free; i < tails.list.size(); ++i)  // (taken from the pages released here)
+    c->free_pages.erase(std::find(c->free_pages.begin(), c->free_pages.end(), tails.list[i].to));
   return flush_patches(c, patches, (hipStream_t)stream);
 } catch (...) {
   return on_exception();
@@ -915,6 +979,7 @@ int bsattn_copy(const bsattn_cache* src, bsattn_cache** out, void* stream) try {
     c->len = src->len;
     c->pages = src->pages;
     c->free_pages = src->free_pages;
+    c->sharers = src->sharers;
     c->unsent = src->unsent;
   } catch (...) {
     bsattn_cache_destroy(c);

@@ -95,6 +95,11 @@ struct bsattn_cache {
   bool stale = false;
   std::vector<std::vector<int32_t>> pages;
   std::vector<int32_t> free_pages;  // stack; back() is handed out next
+  // holders of each page beyond the first: forks share the full blocks of
+  // their prompt.  A page that a sequence may still write to (its last partial
+  // block and those behind it) is never shared: a fork copies the partial
+  // block, and so does a trim that ends inside a shared one.
+  std::vector<int32_t> sharers;
   // metadata words that a failed launch may have left unset (or set ahead of
   // the host): sent before the next call's own (send_unsent)
   bsattn::Patches unsent;
@@ -318,12 +323,17 @@ inline int release_pages(bsattn_cache* c, int seq, int keep_blocks,
                   Patches& patches) {
   auto& pg = c->pages[seq];
   while ((int)pg.size() > keep_blocks) {
-    c->free_pages.push_back(pg.back());
+    int32_t& others = c->sharers[pg.back()];
+    if (others > 0) --others;
+    else c->free_pages.push_back(pg.back());
     pg.pop_back();
   }
   cap_patch(c, seq, patches);
   return BSATTN_OK;
 }
+
+// bytes of a page's slabs
+inline size_t page_slabs(const Geometry& g) { return (size_t)g.hkv * g.slab_bytes; }
 
 // Profiling slots for one C-ABI call: null unless profiling is on and the
 // stream is not being captured into a graph.

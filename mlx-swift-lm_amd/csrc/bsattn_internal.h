@@ -115,7 +115,8 @@ struct StepAppend {
 // slot's events are set) and marks the slot used.
 enum ProfKind {
   kProfScore = 0, kProfTopk = 1, kProfAttend = 2, kProfCombine = 3, kProfAppend = 4,
-  kProfSummary = 5, kProfPrefill = 6, kProfRotate = 7, kProfDense = 8, kProfKinds = 9
+  kProfSummary = 5, kProfPrefill = 6, kProfRotate = 7, kProfDense = 8, kProfFork = 9,
+  kProfKinds = 10
 };
 struct Timing {
   hipEvent_t start = nullptr, stop = nullptr;
@@ -239,6 +240,13 @@ hipError_t launch_prefill(const Geometry& g, const SeqBatch& b, int L, int nspli
                           void* out, float* ws, hipEvent_t done, hipStream_t s, Timing* prof);
 // parts for a launch of n sequences of up to `tokens` tokens
 int prefill_splits(const Geometry& g, int n, int L, int tokens);
+// Forks: sequence dst[i] becomes the first tokens[i] tokens of src[i]; the page
+// tail_from[i] of its last, partial block is copied to tail_to[i] (-1: none)
+struct ForkBatch {
+  int32_t n;
+  int32_t src[kMaxBatch], dst[kMaxBatch], tokens[kMaxBatch], tail_from[kMaxBatch], tail_to[kMaxBatch];
+};
+hipError_t launch_fork(const Geometry& g, const ForkBatch& fb, hipStream_t s, Timing* prof);
 // Rotary positions of one or two tensors (queries, keys) [n, heads, L, 128]
 // with element strides sb / sh / sl, into dense outputs; w: norm weights of
 // each (null: no norm).  The launch covers entries b0 .. b0 + n - 1 of the

@@ -1,5 +1,5 @@
 // bsattn_ops.cpp -- the C ABI's operators around the cache: dense decode,
-// rotary positions and the norms before them.  Argument checking and kernel
+// forks, rotary positions and the norms before them.  Argument checking and kernel
 // sequencing.
 #include <hip/hip_runtime_api.h>
 
@@ -140,6 +140,83 @@ int bsattn_decode_dense(bsattn_cache* c, const void* q, const int32_t* seq_ids, 
   return on_exception();
 }
 
+int bsattn_fork(bsattn_cache* c, const int32_t* src_ids, const int32_t* dst_ids, int32_t n, const int32_t* n_tokens,
+                void* stream) try {
+  if (!c || !src_ids || !dst_ids) return fail(BSATTN_ERR_INVALID, "null argument");
+  int rc = check_synced(c);
+  if (rc) return rc;
+  std::vector<int32_t> dst;
+  rc = seq_list(c, dst_ids, n, dst);
+  if (rc) return rc;
+  const int tb = c->d.block_size;
+  std::vector<char> is_dst(c->d.max_seqs, 0);
+  for (int sq : dst) {
+    is_dst[sq] = 1;
+    if (c->len[sq] != 0 || !c->pages[sq].empty())
+      return fail(BSATTN_ERR_INVALID, "sequence %d is not empty: a fork needs an empty one (bsattn_reset)", sq);
+  }
+  std::vector<int32_t> tokens(n), tails;  // tails: the pairs with a partial block
+  for (int i = 0; i < n; ++i) {
+    const int sq = src_ids[i];
+    if (sq < 0 || sq >= c->d.max_seqs)
+      return fail(BSATTN_ERR_RANGE, "sequence id %d out of range [0, %d)", sq, c->d.max_seqs);
+    if (is_dst[sq]) return fail(BSATTN_ERR_INVALID, "sequence %d is forked from and to", sq);
+    tokens[i] = n_tokens ? n_tokens[i] : c->len[sq];
+    if (tokens[i] < 0 || tokens[i] > c->len[sq])
+      return fail(BSATTN_ERR_RANGE, "a fork of %d tokens from sequence %d, which holds %d", tokens[i], sq, c->len[sq]);
+    if (tokens[i] % tb) tails.push_back(i);
+  }
+  if (tails.size() > c->free_pages.size())
+    return fail(BSATTN_ERR_NO_PAGES, "page pool exhausted: need %zu pages, %zu free", tails.size(),
+                c->free_pages.size());
+  DeviceGuard dg(c->d.device);
+  if (!dg.ok) return fail(BSATTN_ERR_HIP, "hipSetDevice(%d) failed", c->d.device);
+  hipStream_t s = (hipStream_t)stream;
+  if (capturing(s)) return fail(BSATTN_ERR_INVALID, "a fork cannot be captured");
+  rc = send_unsent(c, s);
+  if (rc) return rc;
+  // every allocation first: the new rows, and what takes a failed launch back
+  std::vector<std::vector<int32_t>> rows(n);
+  Patches undo;
+  for (int i = 0; i < n; ++i) {
+    const auto& pg = c->pages[src_ids[i]];
+    rows[i].reserve((tokens[i] + tb - 1) / tb);
+    rows[i].assign(pg.begin(), pg.begin() + tokens[i] / tb);
+    undo.emplace_back(dst[i], 0);
+    undo.emplace_back(c->geo.cap_off + dst[i], 0);
+  }
+  for (size_t t = 0; t < tails.size(); ++t) rows[tails[t]].push_back(c->free_pages[c->free_pages.size() - 1 - t]);
+  for (int i0 = 0; i0 < n; i0 += kMaxBatch) {
+    ForkBatch fb{};
+    fb.n = std::min(kMaxBatch, n - i0);
+    for (int i = 0; i < fb.n; ++i) {
+      const bool partial = tokens[i0 + i] % tb != 0;
+      fb.src[i] = src_ids[i0 + i];
+      fb.dst[i] = dst[i0 + i];
+      fb.tokens[i] = tokens[i0 + i];
+      fb.tail_from[i] = partial ? c->pages[src_ids[i0 + i]][tokens[i0 + i] / tb] : -1;
+      fb.tail_to[i] = partial ? rows[i0 + i].back() : -1;
+    }
+    Timing tm[kProfKinds];
+    Timing* prof = prof_slots(c, s, tm);
+    const hipError_t e = launch_fork(c->geo, fb, s, prof);
+    prof_collect(c, prof);
+    if (e != hipSuccess) {
+      c->unsent.swap(undo);
+      return hip_fail(e, "fork launch");
+    }
+  }
+  c->free_pages.resize(c->free_pages.size() - tails.size());
+  for (int i = 0; i < n; ++i) {
+    for (int b = 0; b < tokens[i] / tb; ++b) ++c->sharers[rows[i][b]];
+    c->pages[dst[i]].swap(rows[i]);
+    c->len[dst[i]] = tokens[i];
+  }
+  return BSATTN_OK;
+} catch (...) {
+  return on_exception();
+}
+
 int bsattn_rotate(bsattn_cache* c, const bsattn_rope* rope, const void* x, const int64_t* strides, int32_t heads,
                   const int32_t* seq_ids, int32_t n_seqs, int32_t n_tokens, const int32_t* positions, void* out,
                   void* stream) try {
@@ -158,8 +235,8 @@ int bsattn_norm_rotate(bsattn_cache* c, const bsattn_rope* rope, const void* q, 
                        const void* k, const int64_t* k_strides, const void* q_weight, const void* k_weight, float eps,
                        float weight_offset, const int32_t* seq_ids, int32_t n_seqs, int32_t n_tokens,
                        const int32_t* positions, void* q_out, void* k_out, void* stream) try {
-  if (!c || !rope || !q || !k || !q_weight || !k_weight || !q_out || !k_out)
-    return fail(BSATTN_ERR_INVALID, "null argument");
+  if (!c || !rope || !q || !k || !q_out || !k_out) return fail(BSATTN_ERR_INVALID, "null argument");
+  if (!q_weight != !k_weight) return fail(BSATTN_ERR_INVALID, "one norm weight without the other");
   if (int rc = check_rope(*rope)) return rc;
   if (n_tokens < 1) return fail(BSATTN_ERR_INVALID, "n_tokens must be >= 1 (got %d)", n_tokens);
   if (!(eps >= 0.0f) || !std::isfinite(eps)) return fail(BSATTN_ERR_INVALID, "eps must be finite and >= 0");
