@@ -261,7 +261,9 @@ struct RotateBatch {
   const int32_t* pos;
   int32_t heads[2];
   int32_t L, b0, dims, interleaved;
-  int32_t share;  // heads per workgroup (launch_rotate sets it)
+  // set by launch_rotate: heads per workgroup, log2 of the tokens per
+  // workgroup and of the pairs (rounded up)
+  int32_t share, tsh, hsh;
   float m, eps, woff;
   int32_t ids[kMaxBatch];
 };
