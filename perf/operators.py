@@ -243,7 +243,8 @@ def _prepare_own(c, seed):
         config, longest = _scaling_config(c["scaling"], c["rot"])
         rope = bs.initializeRope(c["rot"], c["base"], c["interleaved"], config, longest, device=0)
         q, k = _projected(c, seed)
-        st = {"kind": c["kind"], "rope": rope, "cache": _cache(c, c["B"], 64), "q": q, "pos": _positions(c, seed)}
+        st = {"bs": bs, "kind": c["kind"], "rope": rope, "cache": _cache(c, c["B"], 64), "q": q,
+              "pos": _positions(c, seed)}
         if c["kind"] == "norm":
             st.update(k=k, w=_weights(c, seed), offset=c["offset"])
         return st
@@ -263,7 +264,7 @@ def _prepare_own(c, seed):
                 cache.append(k[None], v[None], seq_ids=[first + b])
             del k, v
     q, k, v = _new(c, seed)
-    st = {"kind": c["kind"], "cache": cache, "q": q}
+    st = {"bs": bs, "kind": c["kind"], "cache": cache, "q": q}
     if fork:
         st.update(k=k, v=v, dst=list(range(c["B"])), src=[first + i // c["branches"] for i in range(c["B"])])
     else:
@@ -316,7 +317,7 @@ def prepare(case, seed):
 # one pass
 # ---------------------------------------------------------------------------
 def _run_own(s):
-    bs, cache = _bsattn(), s["cache"]
+    bs, cache = s["bs"], s["cache"]
     if s["kind"] == "rotary":
         return bs.applyRotaryPosition(s["rope"], s["q"], cache, positions=s["pos"])
     if s["kind"] == "norm":
