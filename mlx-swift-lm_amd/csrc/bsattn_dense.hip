@@ -3,11 +3,19 @@
 //   o = sum_t p_t v_t / (sum_t p_t + exp(sink - m)),  p_t = exp(scale q.k_t - m)
 // for 16-bit and affine caches.
 //
-// Bound by the bytes of K and V: each is read once, by one workgroup.  The
-// tokens of a (sequence, kv head) are cut into parts of `cu` units of 32
-// tokens, one workgroup of four waves each, wave w taking units w, w + 4, ...
-// of the part; the parts are joined by k_dense_join.  A wave works in
-// registers alone, one unit at a time with MFMA 16x16x32:
+// Bound by the bytes of K and V: each is read once, by one workgroup.  8
+// sequences of 32k bf16 tokens, 8 kv heads (1.07 GB): 163 us with the join, 6.6
+// TB/s, where a streaming read of as much takes 154; 4 of 131k int4 tokens (604
+// MB) 99 us, 90 with nothing but the loads; 4 of 262k int8 tokens in 16-head
+// groups (1.14 GB) 179 us, loads alone 170.
+// The tokens of a (sequence, kv head) are cut into parts of `cu` units of 32
+// tokens, one workgroup of four waves each, wave w taking every fourth unit of
+// the part; the parts are joined by k_dense_join.  A wave works in registers
+// alone, one unit at a time with MFMA 16x16x32, and asks for the next unit's K
+// as soon as this one's is used, its V likewise.  Nothing may stand in front of
+// those loads' waits: a block-table entry read as a vector, loads behind a
+// branch, or scales that have to move between registers made every unit wait
+// for all of them (131k int4 tokens: 99 us, 112 before):
 //   S^T[token][head] = K[token][:] . Q^T      (A = K rows, B = Q^T)
 //   O^T[dim][head]  += V^T[dim][token] . P^T  (A = V^T,    B = P^T)
 // In both products a lane (column n, group g) holds head n's share of tokens
@@ -27,6 +35,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "bsattn_append.h"
 #include "bsattn_codes.h"
@@ -65,6 +74,29 @@ __device__ __forceinline__ void split_operand(const float* x, float rest, u32x4&
   }
 }
 
+// The same from weights that are shared out (quantized caches): x holds the
+// lane's tokens, all eight (WIDE) or four of them (odd: the last four).  hi, lo
+// as split_operand's.
+template <bool WIDE, int NT>
+__device__ __forceinline__ void weight_operand(const float (&x)[NT], bool odd, u32x4& hi, u32x4& lo) {
+  uint32_t h[NT / 2], r[NT / 2];
+#pragma unroll
+  for (int j = 0; j < NT / 2; ++j) {
+    h[j] = cvt_pk<0>(x[2 * j], x[2 * j + 1]);
+    r[j] = cvt_pk<0>(x[2 * j] - lo16<0>(h[j]), x[2 * j + 1] - hi16<0>(h[j]));
+  }
+  if constexpr (WIDE) {
+    hi = u32x4{h[0], h[1], h[2], h[3]};
+    lo = u32x4{r[0], r[1], r[2], r[3]};
+  } else {
+    uint32_t got[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      got[j] = __float_as_uint(column8(__uint_as_float(odd ? h[j] : r[j])));
+    hi = u32x4{odd ? got[0] : h[0], odd ? got[1] : h[1], odd ? r[0] : got[0], odd ? r[1] : got[1]};
+  }
+}
+
 // The range of a sequence that the call sees: tokens [lo, len), units of 32
 // from u0 on.
 struct DenseRange {
@@ -79,310 +111,114 @@ __device__ __forceinline__ DenseRange dense_range(const Geometry& geo, const Den
   return r;
 }
 
-// KIND: 0 fp16, 1 bf16, 4 / 8 affine codes (fp16 queries).
-// grid (parts of all entries, Hkv)
-template <int KIND, bool WIDE>
-__global__ __launch_bounds__(256) void k_dense(Geometry geo, DenseBatch db, const uint16_t* __restrict__ q,
-                                               uint16_t* __restrict__ out, float* __restrict__ partials) {
-  constexpr int DT = KIND == 1 ? 1 : 0;
-  constexpr bool Q = KIND >= 4;
-  constexpr int KB = Q ? KIND : 4;
-  constexpr int NK = Q ? 2 * QCode<KB>::KF : 8;   // K fragments of a unit
-  constexpr int NV = Q ? 8 / QCode<KB>::DPF : 8;  // V fragments of a unit
-  constexpr int HC = WIDE ? 16 : 8;               // heads that the workgroup can hold
-  // P's range: fp16 weights are lifted to at most 2^14, so that small ones keep
-  // their bits (bf16 has fp32's range).  In a quantized cache a weight also
-  // meets its token's scale: where one of 2 or more turns up, the weights are
-  // at most 1 from there on (65504 times that still fits).
-  float lift = DT == 0 ? kTop - kSlack : 0.0f;
-  __shared__ float s_m[4][16], s_l[4][16];
-  __shared__ __align__(16) float s_o[4][HC][kHeadDim + 4];
-  const int h = blockIdx.y;
-  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int n = lane & 15, g = lane >> 4;
+// One workgroup's part: units of entry bi, in the order in which its waves
+// take them (wave w the places w, w + 4, ...): `full` units from fa on, whose
+// tokens are all seen, then up to two at the ends of the range that are not.
+struct DensePart {
+  int bi, seq, parts, fa, full, places, head;  // head: the first of the two (or the only one)
+  DenseRange r;
+  __device__ __forceinline__ int unit(int place) const {
+    return place < full ? fa + place : place == full ? head : r.u0 + r.units - 1;
+  }
+};
+__device__ __forceinline__ DensePart dense_part(const Geometry& geo, const DenseBatch& db) {
+  DensePart w;
+  const int lane = threadIdx.x & 63;
   // the entry whose parts hold this workgroup's
-  const int bi = __popcll(__ballot(lane < db.n && db.part0[lane] <= (int)blockIdx.x)) - 1;
-  const int part = (int)blockIdx.x - uniform(db.part0[bi]);
-  const int seq = uniform(db.ids[bi]);
-  const int G = geo.group;
-  const DenseRange r = dense_range(geo, db, seq);
-  const int parts = (r.units + db.cu - 1) / db.cu;
-  if (part >= max(parts, 1)) return;
-  const int ua = r.u0 + part * db.cu, ub = min(ua + db.cu, r.u0 + r.units);
-  u32x4 qf[4];
-  {
-    const uint16_t* src = q + ((size_t)bi * geo.hq + h * G + (n & (G - 1))) * kHeadDim + 8 * g;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) qf[s] = *(const u32x4*)(src + 32 * s);
+  w.bi = __popcll(__ballot(lane < db.n && db.part0[lane] <= (int)blockIdx.x)) - 1;
+  w.seq = uniform(db.ids[w.bi]);
+  w.r = dense_range(geo, db, w.seq);
+  w.parts = (w.r.units + db.cu - 1) / db.cu;
+  const int part = (int)blockIdx.x - uniform(db.part0[w.bi]), end = w.r.u0 + w.r.units;
+  const int ua = w.r.u0 + part * db.cu, ub = min(ua + db.cu, end);
+  const bool first = ua == w.r.u0 && 32 * ua < w.r.lo;
+  const bool last = ub == end && 32 * ub > w.r.len && !(first && ub == ua + 1);
+  w.places = max(ub - ua, 0);
+  w.fa = ua + first;
+  w.full = w.places - first - last;
+  w.head = first ? ua : ub - 1;
+  // (an entry of no tokens has one part, whose output is zeros)
+  if (w.places == 0) w.full = w.parts > 0 || part > 0 ? -1 : 0;
+  return w;
+}
+
+// Slabs of the units that a wave takes: the block table is read through the
+// scalar cache one unit ahead (a vector load here would put its wait in front
+// of the fragments on their way).
+struct DensePages {
+  const int32_t* bt;
+  int sh, unit, page;  // sh: log2 of the units per block; the unit asked for last, and its page
+  __device__ __forceinline__ DensePages(const Geometry& geo, const DensePart& w, int place) {
+    sh = geo.tb == 64 ? 1 : 0;
+    bt = block_table(geo, w.seq);
+    ask(w, place);
   }
-  const int sh = geo.tb == 64 ? 1 : 0;
-  const int32_t* bt = block_table(geo, seq);
-  int pbase = ua >> sh;  // the block whose page lane 0 holds
-  int pages = bt[min(pbase + lane, geo.mbps - 1)];
-  const float rest = n >= 8 ? 1.0f : 0.0f;
-
-  u32x4 kf[NK], vf[NV];
-  u32x4 sb[Q ? 8 : 1];
-  auto slab_of = [&](int u) __attribute__((always_inline)) -> const uint8_t* {
-    int b = (u >> sh) - pbase;
-    if (b >= 64) {
-      pbase += b;
-      pages = bt[min(pbase + lane, geo.mbps - 1)];
-      b = 0;
-    }
-    const int page = __builtin_amdgcn_readlane(pages, b);
-    return geo.pool + ((size_t)page * geo.hkv + h) * geo.slab_bytes;
-  };
-  auto load_k = [&](const uint8_t* slab, int u) __attribute__((always_inline)) {
-    const int sub = u & sh;
-    const u32x4* p = (const u32x4*)(slab + geo.k_off) + sub * (NK * 64) + lane;
-#pragma unroll
-    for (int i = 0; i < NK; ++i) kf[i] = __builtin_nontemporal_load(p + i * 64);
-  };
-  auto load_v = [&](const uint8_t* slab, int u) __attribute__((always_inline)) {
-    const int sub = u & sh;
-    const u32x4* p = (const u32x4*)(slab + geo.v_off) + sub * 64 + lane;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) vf[i] = __builtin_nontemporal_load(p + (i << sh) * 64);
-  };
-  auto load_sb = [&](const uint8_t* slab, int u) __attribute__((always_inline)) {
-    const int sub = u & sh;
-    const u32x4* p = (const u32x4*)(slab + geo.sb_off) + g * (geo.tb >> 2) + 8 * sub;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sb[Q ? e : 0] = p[e];
-  };
-
-  f32x4 o[8], ob0 = f32x4{0.f, 0.f, 0.f, 0.f}, ob1 = ob0;
-#pragma unroll
-  for (int dt = 0; dt < 8; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, base = 0.0f, l = 0.0f;
-
-  // the queries' share of the code offsets (see bsattn_quant.hip): qk is the
-  // QK operand, qs / qb its sum and q's over each 64 dims
-  u32x4 qk[4];
-  float q0 = 0.f, q1 = 0.f, q0c = 0.f, q1c = 0.f;
-  uint32_t code_base = 0;
-  if constexpr (Q) {
-    code_base = f16_pair_1024();
-    const u32x4 ones = u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
-    const f32x4 zero = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      qk[s] = qf[s];
-      if constexpr (KB == 4) {
-        qk[s][1] = f16x2_unit16(qf[s][1]);
-        qk[s][3] = f16x2_unit16(qf[s][3]);
-      }
-    }
-    q0 = mfma_f16(ones, qf[1], mfma_f16(ones, qf[0], zero))[0];
-    q1 = mfma_f16(ones, qf[3], mfma_f16(ones, qf[2], zero))[0];
-    q0c = kDecOff * mfma_f16(ones, qk[1], mfma_f16(ones, qk[0], zero))[0];
-    q1c = kDecOff * mfma_f16(ones, qk[3], mfma_f16(ones, qk[2], zero))[0];
+  // (places past the part's ask for its last one; a sequence without tokens for
+  // its first table entry, which names some page of the pool at all times)
+  __device__ __forceinline__ void ask(const DensePart& w, int place) {
+    unit = w.places > 0 ? w.unit(min(place, w.places - 1)) : 0;
+    page = *((const __attribute__((address_space(4))) int32_t*)(uintptr_t)(bt + (unit >> sh)));
   }
-
-  int u = ua + wave;
-  if (u < ub) {
-    const uint8_t* slab = slab_of(u);
-    load_k(slab, u);
-    if constexpr (Q) load_sb(slab, u);
-    load_v(slab, u);
+  __device__ __forceinline__ const uint8_t* slab(const Geometry& geo) const {
+    return geo.pool + ((size_t)page * geo.hkv + blockIdx.y) * geo.slab_bytes;
   }
-  while (u < ub) {
-    const int next = u + 4;
-    const bool more = next < ub;
-    const uint8_t* slab = more ? slab_of(next) : nullptr;
-    __builtin_amdgcn_sched_barrier(0);
-    // scores of tokens 32 u + 8 g + e, in the log2 domain
-    float pv[8];
-    if constexpr (!Q) {
-      f32x4 acc[2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < 4; ++s) acc[t] = mfma16x16x32<DT>(kf[4 * t + s], qf[s], acc[t]);
-      }
-      if (more) load_k(slab, next);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) pv[e] = acc[e >> 2][e & 3] * db.sl2;
-    } else {
-      f32x4 r0[2], r1[2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const u32x4* kt = kf + t * QCode<KB>::KF;
-        r0[t] = f32x4{-q0c, -q0c, -q0c, -q0c};
-        r1[t] = f32x4{-q1c, -q1c, -q1c, -q1c};
-        r0[t] = mfma_f16(k_operand<KB>(kt, 0, code_base), qk[0], r0[t]);
-        r0[t] = mfma_f16(k_operand<KB>(kt, 1, code_base), qk[1], r0[t]);
-        r1[t] = mfma_f16(k_operand<KB>(kt, 2, code_base), qk[2], r1[t]);
-        r1[t] = mfma_f16(k_operand<KB>(kt, 3, code_base), qk[3], r1[t]);
-      }
-      if (more) load_k(slab, next);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float sc = lo_f(sb[e][0]) * r0[e >> 2][e & 3];
-        sc = __builtin_fmaf(hi_f(sb[e][0]), r1[e >> 2][e & 3], sc);
-        sc = __builtin_fmaf(lo_f(sb[e][1]), q0, sc);
-        sc = __builtin_fmaf(hi_f(sb[e][1]), q1, sc);
-        pv[e] = sc * db.sl2;
-      }
-    }
-    // tokens that the query does not see: no score, and nothing of what lies
-    // there (old pages hold anything) reaches the products
-    const bool edge = 32 * u < r.lo || 32 * u + 32 > r.len;
-    if (edge) {
-      const int t0 = 32 * u + 8 * g;
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (t0 + e < r.lo || t0 + e >= r.len) {
-          pv[e] = -INFINITY;
-          if constexpr (Q) sb[e] = u32x4{0u, 0u, 0u, 0u};
-        }
-    }
-    if constexpr (Q) {
-      uint32_t any = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) any |= sb[e][2];
-      if (lift > 0.0f && __any((any & 0x40004000u) != 0)) {  // exponents of 2 and more
-        const float f = __builtin_amdgcn_exp2f(-kTop);
-        lift -= kTop;
-        base += kTop;
-        l *= f;
-#pragma unroll
-        for (int dt = 0; dt < 8; ++dt) o[dt] *= f;
-        ob0 *= f;
-        ob1 *= f;
-      }
-    }
-    float mx = pv[0];
-#pragma unroll
-    for (int e = 1; e < 8; ++e) mx = fmaxf(mx, pv[e]);
-    if (__any(mx > m + kSlack)) {
-      const float top = fmaxf(m, max_over_groups(mx));
-      const float f = top == m ? 1.0f : __builtin_amdgcn_exp2f(m - top);
-      m = top;
-      base = (top == -INFINITY ? 0.0f : top) - lift;
-      l *= f;
-#pragma unroll
-      for (int dt = 0; dt < 8; ++dt) o[dt] *= f;
-      if constexpr (Q) {
-        ob0 *= f;
-        ob1 *= f;
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      pv[e] = __builtin_amdgcn_exp2f(pv[e] - base);
-      l += pv[e];
-    }
-    u32x4 hi, lo;
-    split_operand<DT, WIDE>(pv, rest, hi, lo);
-    if constexpr (!Q) {
-      if (edge) {
-        const int t0 = 32 * u + 8 * g;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int ta = t0 + 2 * j, tb = ta + 1;
-          const uint32_t keep = (ta >= r.lo && ta < r.len ? 0x0000FFFFu : 0u) | (tb >= r.lo && tb < r.len ? 0xFFFF0000u : 0u);
-#pragma unroll
-          for (int dt = 0; dt < 8; ++dt) vf[dt][j] &= keep;
-        }
-      }
-#pragma unroll
-      for (int dt = 0; dt < 8; ++dt) {
-        o[dt] = mfma16x16x32<DT>(vf[dt], hi, o[dt]);
-        if constexpr (WIDE) o[dt] = mfma16x16x32<DT>(vf[dt], lo, o[dt]);
-      }
-    } else {
-      // sum_t p v_bias per dim group (every row of ob the same), and
-      // P_g = p * v_scale_g against the codes; the codes' offset of 1024 is
-      // taken off with the same P_g, unit by unit
-      u32x4 vb0, vb1;
-      float p0[8], p1[8];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t a = sb[2 * j][3], b = sb[2 * j + 1][3];
-        vb0[j] = __builtin_amdgcn_perm(b, a, 0x05040100u);
-        vb1[j] = __builtin_amdgcn_perm(b, a, 0x07060302u);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = KB == 4 && (e & 2) ? pv[e] * kUnit16 : pv[e];  // int4's unit-16 elements
-        p0[e] = x * lo_f(sb[e][2]);
-        p1[e] = x * hi_f(sb[e][2]);
-      }
-      if (more) load_sb(slab, next);
-      ob0 = mfma_f16(vb0, hi, ob0);
-      ob1 = mfma_f16(vb1, hi, ob1);
-      if constexpr (WIDE) {
-        ob0 = mfma_f16(vb0, lo, ob0);
-        ob1 = mfma_f16(vb1, lo, ob1);
-      }
-      const u32x4 off = u32x4{0xE400E400u, 0xE400E400u, 0xE400E400u, 0xE400E400u};  // -1024
-      u32x4 h0, l0, h1, l1;
-      split_operand<0, WIDE>(p0, rest, h0, l0);
-      split_operand<0, WIDE>(p1, rest, h1, l1);
-#pragma unroll
-      for (int dt = 0; dt < 8; ++dt) {
-        const u32x4 a = v_operand<KB, 1>(vf, dt, 0, code_base);
-        const u32x4& ph = dt < 4 ? h0 : h1;
-        o[dt] = mfma_f16(off, ph, o[dt]);
-        o[dt] = mfma_f16(a, ph, o[dt]);
-        if constexpr (WIDE) {
-          const u32x4& pl = dt < 4 ? l0 : l1;
-          o[dt] = mfma_f16(off, pl, o[dt]);
-          o[dt] = mfma_f16(a, pl, o[dt]);
-        }
-      }
-    }
-    if (more) load_v(slab, next);
-    __builtin_amdgcn_sched_barrier(0);
-    u = next;
-  }
+};
 
-  // the waves' shares, then the part's
+// 16 bytes at a uniform address plus a lane's offset, read once
+__device__ __forceinline__ u32x4 stream16(const uint8_t* base, uint32_t at) {
+  return __builtin_nontemporal_load((const u32x4*)(base + at));
+}
+// a lane's offset, kept in 32 bits up to here (the load then adds it to the
+// uniform address itself)
+__device__ __forceinline__ uint32_t offset32(uint32_t at) {
+  asm volatile("" : "+v"(at));
+  return at;
+}
+
+// The four waves' shares of a part joined: this wave's o (lane (head n, group
+// g), dims 16 dt + 4 g ..), sums l over its own tokens, and their reference
+// (-inf: no token); written as the output (one part) or as a partial
+// (o, reference, l).
+template <int DT, bool WIDE>
+__device__ __forceinline__ void dense_finish(const Geometry& geo, const DenseBatch& db, const DensePart& w,
+                                             const f32x4 (&o)[8], float ref, float l, uint16_t* __restrict__ out,
+                                             float* __restrict__ partials) {
+  __shared__ float s_m[4][16], s_l[4][16];
+  __shared__ __align__(16) float s_o[4][WIDE ? 16 : 8][kHeadDim + 4];
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int n = lane & 15, g = lane >> 4, G = geo.group, h = blockIdx.y;
   l = sum_over_groups(l);
   if (n < G) {
     if (g == 0) {
-      s_m[wave][n] = m == -INFINITY ? m : base;
+      s_m[wave][n] = ref;
       s_l[wave][n] = l;
     }
-  }
 #pragma unroll
-  for (int dt = 0; dt < 8; ++dt) {
-    f32x4 x = o[dt];
-    if constexpr (Q) x += dt < 4 ? ob0 : ob1;
-    if constexpr (!WIDE) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] += column8(x[i]);
-    }
-    if (n < G) *(f32x4*)&s_o[wave][n][16 * dt + 4 * g] = x;
+    for (int dt = 0; dt < 8; ++dt) *(f32x4*)&s_o[wave][n][16 * dt + 4 * g] = o[dt];
   }
   __syncthreads();
   for (int e = threadIdx.x; e < G * kHeadDim; e += 256) {
     const int head = e >> 7, d = e & 127;
     float M = s_m[0][head];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) M = fmaxf(M, s_m[w][head]);
+    for (int v = 1; v < 4; ++v) M = fmaxf(M, s_m[v][head]);
     float L = 0.f, a = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float mw = s_m[w][head];
-      const float f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - M);
-      L += f * s_l[w][head];
-      a += f * s_o[w][head][d];
+    for (int v = 0; v < 4; ++v) {
+      const float mv = s_m[v][head];
+      const float f = mv == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mv - M);
+      L += f * s_l[v][head];
+      a += f * s_o[v][head][d];
     }
     const int hq = h * G + head;
-    if (parts <= 1) {
-      if (db.sinks && r.len > 0) {
+    if (w.parts <= 1) {
+      if (db.sinks && w.r.len > 0) {
         const float sk = db.sinks[hq] * kLog2e, top = fmaxf(M, sk);
         const float f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - top);
         L = L * f + (sk == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sk - top));
         a *= f;
       }
-      out[((size_t)bi * geo.hq + hq) * kHeadDim + d] = from_f32<DT>(L == 0.f ? 0.f : a / L);
+      out[((size_t)w.bi * geo.hq + hq) * kHeadDim + d] = from_f32<DT>(L == 0.f ? 0.f : a / L);
     } else {
       float* pp = partials + ((size_t)blockIdx.x * geo.hq + hq) * (kHeadDim + 2);
       pp[d] = a;
@@ -394,27 +230,429 @@ __global__ __launch_bounds__(256) void k_dense(Geometry geo, DenseBatch db, cons
   }
 }
 
-// The parts of one (entry, query head) joined; grid (Hq, n)
+// 16-bit caches.  grid (parts of all entries, Hkv)
+template <int DT, bool WIDE>
+__global__ __launch_bounds__(256, 3) void k_dense(Geometry geo, DenseBatch db, const uint16_t* __restrict__ q,
+                                               uint16_t* __restrict__ out, float* __restrict__ partials) {
+  // P's range: fp16 weights are lifted to at most 2^14, so that small ones keep
+  // their bits (bf16 has fp32's range)
+  constexpr float kLift = DT == 0 ? kTop - kSlack : 0.0f;
+  const DensePart w = dense_part(geo, db);
+  if (w.full < 0) return;  // nothing here: past the sequence's end
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int n = lane & 15, g = lane >> 4, G = geo.group, h = blockIdx.y;
+  int place = wave;  // of the unit that a step takes
+  DensePages pages(geo, w, place);
+  u32x4 qf[4];
+  {
+    const uint16_t* src = q + ((size_t)w.bi * geo.hq + h * G + (n & (G - 1))) * kHeadDim + 8 * g;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) qf[s] = *(const u32x4*)(src + 32 * s);
+  }
+  const float rest = n >= 8 ? 1.0f : 0.0f;
+  const uint32_t at = (uint32_t)lane * 16;
+  u32x4 kf[8], vf[8];
+  auto load_k = [&](const uint8_t* slab, int u) __attribute__((always_inline)) {
+    const uint8_t* p = slab + geo.k_off + (u & pages.sh) * 8192;
+    const uint32_t x = offset32(at);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) kf[i] = stream16(p + i * 1024, x);
+  };
+  auto load_v = [&](const uint8_t* slab, int u) __attribute__((always_inline)) {
+    const uint8_t* p = slab + geo.v_off + (u & pages.sh) * 1024;
+    const uint32_t x = offset32(at);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) vf[i] = stream16(p + (i << pages.sh) * 1024, x);
+  };
+  f32x4 o[8];
+#pragma unroll
+  for (int dt = 0; dt < 8; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, base = 0.0f, l = 0.0f;
+  // EDGE: some of the unit's tokens are not seen.  MORE: the wave has another
+  // unit, which is asked for (without a branch: behind one the compiler must
+  // wait as if nothing had been)
+  auto step = [&](auto edge, auto m_) __attribute__((always_inline)) {
+    constexpr bool EDGE = decltype(edge)::value, MORE = decltype(m_)::value;
+    const int next = pages.unit;
+    const uint8_t* slab = pages.slab(geo);
+    if constexpr (MORE) pages.ask(w, place + 8);
+    __builtin_amdgcn_sched_barrier(0);
+    // scores of tokens 32 u + 8 g + e, in the log2 domain; the next unit's K
+    // is asked for as soon as this one's is used, its V likewise
+    float pv[8];
+    f32x4 acc[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < 4; ++s) acc[t] = mfma16x16x32<DT>(kf[4 * t + s], qf[s], acc[t]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (MORE) load_k(slab, next);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) pv[e] = acc[e >> 2][e & 3] * db.sl2;
+    // tokens that the query does not see: no score, and nothing of what lies
+    // there (old pages hold anything) reaches the products
+    if constexpr (EDGE) {
+      const int t0 = 32 * w.unit(place) + 8 * g;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool a = t0 + 2 * j >= w.r.lo && t0 + 2 * j < w.r.len;
+        const bool b = t0 + 2 * j + 1 >= w.r.lo && t0 + 2 * j + 1 < w.r.len;
+        if (!a) pv[2 * j] = -INFINITY;
+        if (!b) pv[2 * j + 1] = -INFINITY;
+        const uint32_t keep = (a ? 0x0000FFFFu : 0u) | (b ? 0xFFFF0000u : 0u);
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) vf[dt][j] &= keep;
+      }
+    }
+    float mx = pv[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) mx = fmaxf(mx, pv[e]);
+    if (__any(mx > m + kSlack)) {
+      const float top = fmaxf(m, max_over_groups(mx));
+      const float f = top == m ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+      m = top;
+      base = (top == -INFINITY ? 0.0f : top) - kLift;
+      l *= f;
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt) o[dt] *= f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      pv[e] = __builtin_amdgcn_exp2f(pv[e] - base);
+      l += pv[e];
+    }
+    u32x4 hi, lo;
+    split_operand<DT, WIDE>(pv, rest, hi, lo);
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) {
+      o[dt] = mfma16x16x32<DT>(vf[dt], hi, o[dt]);
+      if constexpr (WIDE) o[dt] = mfma16x16x32<DT>(vf[dt], lo, o[dt]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (MORE) load_v(slab, next);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  {
+    // (a wave without a unit asks for the part's last one, too: behind a branch
+    // the loop would wait for everything under way)
+    const int u = pages.unit;
+    const uint8_t* slab = pages.slab(geo);
+    pages.ask(w, place + 4);
+    load_k(slab, u);
+    load_v(slab, u);
+  }
+  // (a wave's units are all full ones, but for its last)
+  for (; place + 4 < w.places; place += 4) step(std::false_type(), std::true_type());
+  if (place < w.full) step(std::false_type(), std::false_type());
+  else if (place < w.places) step(std::true_type(), std::false_type());
+  if constexpr (!WIDE) {
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[dt][i] += column8(o[dt][i]);
+  }
+  dense_finish<DT, WIDE>(geo, db, w, o, m == -INFINITY ? m : base, l, out, partials);
+}
+
+// Affine caches of KB bits, dequantised inside the products (the codes as fp16
+// operands: bsattn_codes.h).  Per group j of 64 dims and token t,
+//   s_t = sum_j ks_j (sum_d q_d c_d) + kb_j Q_j,   Q_j = sum_d q_d
+//   o_d = sum_t (p_t vs_j) c_td + sum_t p_t vb_j
+// with the codes' offset of 1024 taken off after the first product (K: 1024 sum
+// q') and by a product of the same operand with -1024 (V).  The VALU work for each code and score bounds the kernel, so
+// the two copies of a narrow group's heads share the scores: columns 0-7 take
+// the unit's even QK tile (tokens 8g .. 8g + 3 of lane group g), columns 8-15
+// the odd one (8g + 4 .. 8g + 7), and exchange what PV needs of the other: the
+// rounded weights go to columns 0-7, what the rounding left to 8-15.  sum p vb
+// stays fp32 and per lane until the end.
+// grid (parts of all entries, Hkv)
+template <int KB, bool WIDE>
+__global__ __launch_bounds__(256, 3) void k_dense_q(Geometry geo, DenseBatch db, const uint16_t* __restrict__ q,
+                                                 uint16_t* __restrict__ out, float* __restrict__ partials) {
+  constexpr int NK = 2 * QCode<KB>::KF, NV = 8 / QCode<KB>::DPF;  // K and V fragments of a unit
+  constexpr int NT = WIDE ? 8 : 4;                                // tokens of a unit whose scores a lane holds
+  const DensePart w = dense_part(geo, db);
+  if (w.full < 0) return;  // nothing here: past the sequence's end
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int n = lane & 15, g = lane >> 4, G = geo.group, h = blockIdx.y;
+  const bool odd = !WIDE && n >= 8;
+  const int tok0 = 8 * g + (odd ? 4 : 0);
+  int place = wave;  // of the unit that a step takes
+  DensePages pages(geo, w, place);
+  u32x4 qf[4];
+  {
+    const uint16_t* src = q + ((size_t)w.bi * geo.hq + h * G + (n & (G - 1))) * kHeadDim + 8 * g;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) qf[s] = *(const u32x4*)(src + 32 * s);
+  }
+  const uint32_t code_base = f16_pair_1024();
+  const uint32_t at = (uint32_t)lane * 16;
+  // scales and biases: a lane loads one token's (token lane & 31 of the unit, in
+  // the slab's order), and reads the NT of its scores through LDS
+  __shared__ u32x4 s_sb[4][32];
+  const uint32_t sb_at = 16u * (uint32_t)(((lane >> 3) & 3) * (geo.tb >> 2) + (lane & 7));
+  u32x4 kf[NK], vf[NV], sbx;
+  auto load_k = [&](const uint8_t* slab, int u) __attribute__((always_inline)) {
+    const uint8_t* p = slab + geo.k_off + (u & pages.sh) * (NK * 1024);
+    const uint32_t x = offset32(at);
+#pragma unroll
+    for (int i = 0; i < NK; ++i) kf[i] = stream16(p + i * 1024, x);
+  };
+  auto load_v = [&](const uint8_t* slab, int u) __attribute__((always_inline)) {
+    const uint8_t* p = slab + geo.v_off + (u & pages.sh) * 1024;
+    const uint32_t x = offset32(at);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) vf[i] = stream16(p + (i << pages.sh) * 1024, x);
+  };
+  auto load_sb = [&](const uint8_t* slab, int u) __attribute__((always_inline)) {
+    sbx = stream16(slab + geo.sb_off + (u & pages.sh) * 128, offset32(sb_at));
+  };
+
+  // the queries' sums over each 64 dims: of q, and of the QK operand (int4:
+  // with its unit-16 elements scaled) times 1024
+  u32x4 qk[4];
+  float q0, q1, q0c, q1c;
+  {
+    const u32x4 ones = u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
+    const f32x4 zero = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      qk[s] = qf[s];
+      if constexpr (KB == 4) {
+        qk[s][1] = f16x2_unit16(qf[s][1]);
+        qk[s][3] = f16x2_unit16(qf[s][3]);
+      }
+    }
+    q0c = mfma_f16(ones, qk[1], mfma_f16(ones, qk[0], zero))[0] * kDecOff;
+    q1c = mfma_f16(ones, qk[3], mfma_f16(ones, qk[2], zero))[0] * kDecOff;
+    q0 = mfma_f16(ones, qf[1], mfma_f16(ones, qf[0], zero))[0];
+    q1 = mfma_f16(ones, qf[3], mfma_f16(ones, qf[2], zero))[0];
+  }
+
+  f32x4 o[8];
+#pragma unroll
+  for (int dt = 0; dt < 8; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // P's range: lifted to at most 2^14 as for fp16 caches; a weight also meets
+  // its token's scale, and where one of 2 or more turns up the weights are at
+  // most 1 from there on (65504 times that still fits)
+  float lift = kTop - kSlack;
+  float m = -INFINITY, base = 0.0f, l = 0.0f, ob0 = 0.0f, ob1 = 0.0f;
+  auto rescale = [&](float f) __attribute__((always_inline)) {
+    l *= f;
+    ob0 *= f;
+    ob1 *= f;
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) o[dt] *= f;
+  };
+
+  // EDGE: some of the unit's tokens are not seen.  MORE: the wave has another
+  // unit, which is asked for (without a branch: behind one the compiler must
+  // wait as if nothing had been)
+  auto step = [&](auto edge, auto m_) __attribute__((always_inline)) {
+    constexpr bool EDGE = decltype(edge)::value, MORE = decltype(m_)::value;
+    const int next = pages.unit;
+    const uint8_t* slab = pages.slab(geo);
+    if constexpr (MORE) pages.ask(w, place + 8);
+    __builtin_amdgcn_sched_barrier(0);
+    f32x4 r0[2], r1[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const u32x4* kt = kf + t * QCode<KB>::KF;
+      r0[t] = mfma_f16(k_operand<KB>(kt, 0, code_base), qk[0], f32x4{0.f, 0.f, 0.f, 0.f});
+      r1[t] = mfma_f16(k_operand<KB>(kt, 2, code_base), qk[2], f32x4{0.f, 0.f, 0.f, 0.f});
+      r0[t] = mfma_f16(k_operand<KB>(kt, 1, code_base), qk[1], r0[t]);
+      r1[t] = mfma_f16(k_operand<KB>(kt, 3, code_base), qk[3], r1[t]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (MORE) load_k(slab, next);
+    __builtin_amdgcn_sched_barrier(0);
+    s_sb[wave][lane & 31] = sbx;
+    wave_lds_order();
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (MORE) load_sb(slab, next);
+    __builtin_amdgcn_sched_barrier(0);
+    u32x4 sb[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) sb[i] = s_sb[wave][8 * g + (odd ? 4 : 0) + i];
+    // scores over the reference, in the log2 domain
+    float pv[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const float a = (WIDE ? r0[i >> 2][i & 3] : odd ? r0[1][i] : r0[0][i]) - q0c;
+      const float b = (WIDE ? r1[i >> 2][i & 3] : odd ? r1[1][i] : r1[0][i]) - q1c;
+      float x = lo_f(sb[i][0]) * a;
+      x = __builtin_fmaf(hi_f(sb[i][0]), b, x);
+      x = __builtin_fmaf(lo_f(sb[i][1]), q0, x);
+      x = __builtin_fmaf(hi_f(sb[i][1]), q1, x);
+      pv[i] = __builtin_fmaf(x, db.sl2, -base);
+    }
+    // tokens that the query does not see: no score, and nothing of what lies
+    // there (old pages hold anything) reaches the products
+    if constexpr (EDGE) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const int t = 32 * w.unit(place) + tok0 + i;
+        if (t < w.r.lo || t >= w.r.len) {
+          pv[i] = -INFINITY;
+          sb[i][2] = sb[i][3] = 0u;
+        }
+      }
+    }
+    uint32_t scales = 0;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) scales |= sb[i][2];
+    if (lift > 0.0f && __any((scales & 0x40004000u) != 0)) {  // exponents of 2 and more
+      lift -= kTop;
+      base += kTop;
+      rescale(__builtin_amdgcn_exp2f(-kTop));
+#pragma unroll
+      for (int i = 0; i < NT; ++i) pv[i] -= kTop;
+    }
+    float mx = pv[0];
+#pragma unroll
+    for (int i = 1; i < NT; ++i) mx = fmaxf(mx, pv[i]);
+    if (__any(mx > (m == -INFINITY ? m : lift + kSlack))) {
+      if constexpr (!WIDE) mx = fmaxf(mx, column8(mx));
+      const float top = fmaxf(m, base + max_over_groups(mx));
+      const float was = base;
+      base = (top == -INFINITY ? 0.0f : top) - lift;
+      rescale(top == m ? 1.0f : __builtin_amdgcn_exp2f(m - top));
+      m = top;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) pv[i] += was - base;
+    }
+    float p0[NT], p1[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const float p = __builtin_amdgcn_exp2f(pv[i]);
+      l += p;
+      ob0 = __builtin_fmaf(lo_f(sb[i][3]), p, ob0);
+      ob1 = __builtin_fmaf(hi_f(sb[i][3]), p, ob1);
+      const float x = KB == 4 && (i & 2) ? p * kUnit16 : p;  // int4's unit-16 elements
+      p0[i] = lo_f(sb[i][2]) * x;
+      p1[i] = hi_f(sb[i][2]) * x;
+    }
+    const u32x4 off = u32x4{0xE400E400u, 0xE400E400u, 0xE400E400u, 0xE400E400u};  // -1024
+    u32x4 h0, l0, h1, l1;
+    weight_operand<WIDE>(p0, odd, h0, l0);
+    weight_operand<WIDE>(p1, odd, h1, l1);
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) {
+      const u32x4 a = v_operand<KB, 1>(vf, dt, 0, code_base);
+      const u32x4& ph = dt < 4 ? h0 : h1;
+      o[dt] = mfma_f16(off, ph, o[dt]);
+      o[dt] = mfma_f16(a, ph, o[dt]);
+      if constexpr (WIDE) {
+        const u32x4& pl = dt < 4 ? l0 : l1;
+        o[dt] = mfma_f16(off, pl, o[dt]);
+        o[dt] = mfma_f16(a, pl, o[dt]);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (MORE) load_v(slab, next);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  {
+    // (a wave without a unit asks for the part's last one, too: behind a branch
+    // the loop would wait for everything under way)
+    const int u = pages.unit;
+    const uint8_t* slab = pages.slab(geo);
+    pages.ask(w, place + 4);
+    load_k(slab, u);
+    load_sb(slab, u);
+    load_v(slab, u);
+  }
+  // (a wave's units are all full ones, but for its last)
+  for (; place + 4 < w.places; place += 4) step(std::false_type(), std::true_type());
+  if (place < w.full) step(std::false_type(), std::false_type());
+  else if (place < w.places) step(std::true_type(), std::false_type());
+  ob0 = sum_over_groups(ob0);
+  ob1 = sum_over_groups(ob1);
+  if constexpr (!WIDE) {
+    ob0 += column8(ob0);
+    ob1 += column8(ob1);
+    l += column8(l);
+  }
+#pragma unroll
+  for (int dt = 0; dt < 8; ++dt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (!WIDE) o[dt][i] += column8(o[dt][i]);
+      o[dt][i] += dt < 4 ? ob0 : ob1;
+    }
+  dense_finish<0, WIDE>(geo, db, w, o, m == -INFINITY ? m : base, l, out, partials);
+}
+
+// The parts of one (entry, query head) joined: rows of 32 lanes with four dims
+// each take the parts in turn, four of them asked for at once, and are summed
+// in order at the end.  grid (Hq, n)
+constexpr int kJoinRows = 8, kJoinRound = 4;
 template <int DT>
-__global__ __launch_bounds__(128) void k_dense_join(Geometry geo, DenseBatch db, const float* __restrict__ partials,
-                                                    uint16_t* __restrict__ out) {
-  const int hq = blockIdx.x, bi = blockIdx.y, d = threadIdx.x;
+__global__ __launch_bounds__(32 * kJoinRows) void k_dense_join(Geometry geo, DenseBatch db,
+                                                               const float* __restrict__ partials,
+                                                               uint16_t* __restrict__ out) {
+  __shared__ __align__(16) float s_o[kJoinRows][kHeadDim];
+  __shared__ float s_ml[kJoinRows][2];
+  const int hq = blockIdx.x, bi = blockIdx.y;
+  const int row = threadIdx.x >> 5, c = threadIdx.x & 31;
+  const int part0 = uniform(db.part0[bi]);
   const DenseRange r = dense_range(geo, db, db.ids[bi]);
   const int parts = (r.units + db.cu - 1) / db.cu;
   if (parts <= 1) return;
-  const float* pp = partials + ((size_t)db.part0[bi] * geo.hq + hq) * (kHeadDim + 2);
+  const float* pp = partials + ((size_t)part0 * geo.hq + hq) * (kHeadDim + 2);
   const size_t step = (size_t)geo.hq * (kHeadDim + 2);
-  const float sk = db.sinks ? db.sinks[hq] * kLog2e : -INFINITY;
-  float M = sk, L = 0.f, a = 0.f;
-  for (int p = 0; p < parts; ++p) M = fmaxf(M, pp[p * step + kHeadDim]);
-  for (int p = 0; p < parts; ++p) {
-    const float mp = pp[p * step + kHeadDim];
-    const float f = mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mp - M);
-    L += f * pp[p * step + kHeadDim + 1];
-    a += f * pp[p * step + d];
+  float M = -INFINITY, L = 0.f;
+  f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int p0 = row; p0 < parts; p0 += kJoinRows * kJoinRound) {
+    f32x4 x[kJoinRound];
+    float m[kJoinRound], l[kJoinRound];
+#pragma unroll
+    for (int j = 0; j < kJoinRound; ++j) {
+      const int p = min(p0 + j * kJoinRows, parts - 1);
+      const float2* at = (const float2*)(pp + p * step);
+      const float2 xa = at[2 * c], xb = at[2 * c + 1], ml = at[kHeadDim / 2];
+      x[j] = f32x4{xa.x, xa.y, xb.x, xb.y};
+      m[j] = p0 + j * kJoinRows < parts ? ml.x : -INFINITY;
+      l[j] = ml.y;
+    }
+    float top = M;
+#pragma unroll
+    for (int j = 0; j < kJoinRound; ++j) top = fmaxf(top, m[j]);
+    const float f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - top);
+    L *= f;
+    a *= f;
+#pragma unroll
+    for (int j = 0; j < kJoinRound; ++j) {
+      const float g = m[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[j] - top);
+      L += g * l[j];
+      if (m[j] != -INFINITY) a += g * x[j];
+    }
+    M = top;
   }
-  if (sk != -INFINITY) L += __builtin_amdgcn_exp2f(sk - M);
-  out[((size_t)bi * geo.hq + hq) * kHeadDim + d] = from_f32<DT>(L == 0.f ? 0.f : a / L);
+  *(f32x4*)&s_o[row][4 * c] = a;
+  if (c == 0) {
+    s_ml[row][0] = M;
+    s_ml[row][1] = L;
+  }
+  __syncthreads();
+  if (threadIdx.x >= kHeadDim) return;
+  const int d = threadIdx.x;
+  const float sk = db.sinks ? db.sinks[hq] * kLog2e : -INFINITY;
+  float top = sk;
+#pragma unroll
+  for (int i = 0; i < kJoinRows; ++i) top = fmaxf(top, s_ml[i][0]);
+  float Ls = sk == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sk - top), as = 0.f;
+#pragma unroll
+  for (int i = 0; i < kJoinRows; ++i) {
+    const float mi = s_ml[i][0];
+    const float f = mi == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi - top);
+    Ls += f * s_ml[i][1];
+    if (mi != -INFINITY) as += f * s_o[i][d];
+  }
+  out[((size_t)bi * geo.hq + hq) * kHeadDim + d] = from_f32<DT>(Ls == 0.f ? 0.f : as / Ls);
 }
 
 // The parts of a launch: units per part (db.cu) and each entry's first part,
@@ -426,7 +664,10 @@ int dense_plan(const Geometry& g, const int32_t* units, DenseBatch& db) {
     all += units[i];
     most = std::max(most, units[i]);
   }
-  const int64_t want = 4 * (int64_t)std::max(g.cus, 1);
+  // one round of workgroups, two per CU (three fit): 8 x 32k bf16 tokens 163 us
+  // (three per CU 167, four 165, six 169), 4 x 131k int4 98.9 (100, 110, 105),
+  // 4 x 262k int8 in 16-head groups 179 (185, 190, 199)
+  const int64_t want = 2 * (int64_t)std::max(g.cus, 1);
   db.cu = (int)std::min<int64_t>(most, std::max<int64_t>(4, (all * g.hkv + want - 1) / want));
   while (true) {
     db.cu = (db.cu + 3) & ~3;
@@ -440,17 +681,21 @@ int dense_plan(const Geometry& g, const int32_t* units, DenseBatch& db) {
   }
 }
 
-template <int KIND>
+template <bool WIDE>
 static void dense_dispatch(const Geometry& g, const DenseBatch& db, dim3 grid, const uint16_t* q, uint16_t* out,
                            float* partials, hipStream_t s, Timing* prof) {
-  if (g.group > 8) launch(k_dense<KIND, true>, grid, dim3(256), 0, s, prof, kProfDense, g, db, q, out, partials);
-  else launch(k_dense<KIND, false>, grid, dim3(256), 0, s, prof, kProfDense, g, db, q, out, partials);
+  const dim3 blk(256);
+  const int kd = kProfDense;
+  if (g.kv_bits == 4) launch(k_dense_q<4, WIDE>, grid, blk, 0, s, prof, kd, g, db, q, out, partials);
+  else if (g.kv_bits == 8) launch(k_dense_q<8, WIDE>, grid, blk, 0, s, prof, kd, g, db, q, out, partials);
+  else if (g.dtype == 0) launch(k_dense<0, WIDE>, grid, blk, 0, s, prof, kd, g, db, q, out, partials);
+  else launch(k_dense<1, WIDE>, grid, blk, 0, s, prof, kd, g, db, q, out, partials);
 }
 
 template <int DT>
 static hipError_t join_dispatch(const Geometry& g, const DenseBatch& db, const float* ws, uint16_t* out,
                                 hipEvent_t done, hipStream_t s, Timing* prof) {
-  const dim3 grid(g.hq, db.n), blk(128);
+  const dim3 grid(g.hq, db.n), blk(32 * kJoinRows);
   if (done && !prof)  // (the event is the dispatch's own: no packet of its own behind it)
     hipExtLaunchKernelGGL(k_dense_join<DT>, grid, blk, 0u, s, nullptr, done, 0u, g, db, ws, out);
   else
@@ -465,10 +710,8 @@ hipError_t launch_dense(const Geometry& g, const DenseBatch& db, int parts, cons
   const dim3 grid(parts, g.hkv);
   const uint16_t* qq = (const uint16_t*)q;
   uint16_t* oo = (uint16_t*)out;
-  if (g.kv_bits == 4) dense_dispatch<4>(g, db, grid, qq, oo, ws, s, prof);
-  else if (g.kv_bits == 8) dense_dispatch<8>(g, db, grid, qq, oo, ws, s, prof);
-  else if (g.dtype == 0) dense_dispatch<0>(g, db, grid, qq, oo, ws, s, prof);
-  else dense_dispatch<1>(g, db, grid, qq, oo, ws, s, prof);
+  if (g.group > 8) dense_dispatch<true>(g, db, grid, qq, oo, ws, s, prof);
+  else dense_dispatch<false>(g, db, grid, qq, oo, ws, s, prof);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || parts == db.n) return e;
   return g.dtype == 0 ? join_dispatch<0>(g, db, ws, oo, done, s, prof) : join_dispatch<1>(g, db, ws, oo, done, s, prof);
