@@ -229,7 +229,9 @@ int bsattn_prefill(bsattn_cache* cache, const void* q, const int32_t* seq_ids,
  * device-side lengths, so it may follow bsattn_append_step without
  * bsattn_sync.  Long sequences are split over the GPU and joined through the
  * workspace that bsattn_prefill describes; when none can be had the call runs
- * unsplit: slower, and rounded differently. */
+ * unsplit: slower, and rounded differently.  Blocks that sequences of the call
+ * share (bsattn_fork) are read once for several of them, with no window and
+ * outside a capture: then, too, a result may be rounded differently. */
 int bsattn_decode_dense(bsattn_cache* cache, const void* q, const int32_t* seq_ids,
                         int32_t n_seqs, int32_t window, const float* sinks,
                         float scale, void* out, void* stream);

@@ -268,19 +268,36 @@ struct RotateBatch {
   int32_t ids[kMaxBatch];
 };
 hipError_t launch_rotate(const Geometry& g, RotateBatch rb, int n, hipStream_t s, Timing* prof);
-// Dense decode: entry i is the query of sequence ids[i]; its parts of `cu`
-// units of 32 tokens are the launch's part0[i] and on.  window: the last tokens
-// seen (0: all); sinks: [hq] logits of the heads, or null.
-struct DenseBatch {
-  int32_t n, cu, window;
-  float sl2;
-  const float* sinks;
-  int32_t ids[kMaxBatch];
-  int32_t part0[kMaxBatch];
+// Dense decode: entry i is the query of sequence ids[i].  The launch's work is
+// cut into jobs: the tokens of one entry (count 1: units of 32 tokens from
+// `from` to its length; `units` is the most they can be), or the full
+// blocks that several entries share (count > 1: exactly `units` from the
+// beginning, all of them seen), whose queries go through together.  A job's
+// parts of `cu` units are the launch's part0 and on, its partials the blocks
+// of hq rows row0 + part * count + member.
+constexpr int kMaxDenseJobs = kMaxBatch + kMaxBatch / 2;
+struct DenseJob {
+  int32_t part0, row0;
+  int32_t units, from;    // from: the entry's units that its shared job covers (count 1)
+  int32_t seq;            // a member's sequence
+  int16_t first, count;   // members: order[first] ..
+  int16_t entry, shares;  // the first member; whether it (count 1) has a shared job, too
 };
-int dense_plan(const Geometry& g, const int32_t* units, DenseBatch& db);
-// ws: parts * hq rows of kHeadDim + 2 floats (not needed with one part an
-// entry); the launch that joins them records `done` (may be null)
+struct DenseBatch {
+  int32_t n, jobs, cu, window;  // window: the last tokens seen (0: all)
+  float sl2;
+  const float* sinks;           // [hq] logits of the heads, or null
+  int32_t ids[kMaxBatch];
+  int16_t shared[kMaxBatch];    // that job, or -1
+  int16_t alone[kMaxBatch];     // the entry's own
+  int16_t order[2 * kMaxBatch];
+  DenseJob job[kMaxDenseJobs];
+};
+// sets cu, part0 and row0 of the jobs; the number of parts, and in *rows the
+// blocks of partials (0: none are needed, every entry has one part)
+int dense_plan(const Geometry& g, DenseBatch& db, int* rows);
+// ws: rows * hq rows of kHeadDim + 2 floats (null without partials); the launch
+// that joins them records `done` (may be null)
 hipError_t launch_dense(const Geometry& g, const DenseBatch& db, int parts, const void* q, void* out, float* ws,
                         hipEvent_t done, hipStream_t s, Timing* prof);
 hipError_t launch_export(const Geometry& g, const SeqBatch& b, int T, void* k_out,

@@ -7,7 +7,11 @@
 
 #include "stubs.h"
 
-static uint16_t kv[1];
+namespace stub {
+extern bsattn::DenseBatch last_dense;
+}
+
+alignas(16) static uint16_t kv[8];
 static const int kSeqs = 6, kBlocks = 8, kTb = 32;
 
 // tokens of each sequence as the caller knows them, written into the pages
@@ -137,7 +141,86 @@ static void runs(unsigned seed, int num_pages) {
   bsattn_cache_destroy(copy);
 }
 
+// the jobs of a dense decode over forks of forks: what is read for several
+// sequences at once is in the same pages for each of them, and worth it
+static void shared_jobs(unsigned seed, int hq, int hkv) {
+  std::mt19937 rng(seed);
+  auto pick = [&](int n) { return (int)(rng() % (unsigned)n); };
+  const int seqs = 80, blocks = 64;
+  bsattn_desc d = small_desc(seqs, blocks);
+  d.num_q_heads = hq;
+  d.num_kv_heads = hkv;
+  d.block_size = seed % 2 ? 32 : 64;
+  bsattn_cache* c = nullptr;
+  CHECK(bsattn_cache_create(&d, &c) == BSATTN_OK);
+  std::vector<int32_t> len(seqs, 0), ids;
+  for (int s = 0; s < seqs; ++s) {
+    const int from = s ? pick(s) : 0;
+    if (s > 3 && len[from] && pick(5)) {
+      len[s] = 1 + pick(len[from]);
+      if (pick(2)) len[s] = len[from];
+      CHECK(bsattn_fork(c, &from, &s, 1, &len[s], nullptr) == BSATTN_OK);
+    }
+    const int more = pick(3) ? pick(300) : pick(2) * 1500;
+    if (more && len[s] + more <= blocks * d.block_size) {
+      CHECK(bsattn_append(c, kv, kv, &s, 1, more, nullptr) == BSATTN_OK);
+      len[s] += more;
+    }
+    ids.push_back(s);
+  }
+  for (int tries = 0; tries < 20; ++tries) {
+    std::shuffle(ids.begin(), ids.end(), rng);
+    const int n = 1 + pick(64), window = pick(4) ? 0 : 100;
+    stub::splits = 3;
+    CHECK(bsattn_decode_dense(c, kv, ids.data(), n, window, nullptr, 1.f, kv, nullptr) == BSATTN_OK);
+    const bsattn::DenseBatch& db = stub::last_dense;
+    const int per_block = d.block_size / 32, cols = hq / hkv;
+    CHECK(db.n == n);
+    for (int j = 0; j < db.jobs; ++j) {
+      const bsattn::DenseJob& job = db.job[j];
+      CHECK(job.count * cols <= 16);
+      if (job.count == 1) continue;
+      CHECK(window == 0 && job.units >= 16 && job.units % per_block == 0);
+      std::vector<int32_t> lead;
+      for (int k = 0; k < job.count; ++k) {
+        const int seq = ids[db.order[job.first + k]];
+        CHECK(len[seq] >= 32 * job.units);
+        std::vector<int32_t> p(blocks);
+        int32_t held = 0;
+        CHECK(bsattn_seq_pages(c, seq, p.data(), blocks, &held) == BSATTN_OK && held * per_block >= job.units);
+        p.resize(job.units / per_block);
+        if (k == 0) lead = p;
+        CHECK(p == lead);
+      }
+    }
+    // (two of the same prompt are found)
+    stub::capture = hipStreamCaptureStatusActive;
+    CHECK(bsattn_decode_dense(c, kv, ids.data(), n, 0, nullptr, 1.f, kv, nullptr) == BSATTN_OK);
+    CHECK(stub::last_dense.jobs == n);
+    stub::capture = hipStreamCaptureStatusNone;
+  }
+  // eight branches of one prompt of 40 blocks
+  std::vector<int32_t> all(seqs), src(8, 0), dst;
+  for (int s = 0; s < seqs; ++s) all[s] = s;
+  CHECK(bsattn_reset(c, all.data(), seqs, nullptr) == BSATTN_OK);
+  CHECK(bsattn_append(c, kv, kv, all.data(), 1, 40 * d.block_size + 3, nullptr) == BSATTN_OK);
+  for (int i = 0; i < 8; ++i) dst.push_back(10 + i);
+  CHECK(bsattn_fork(c, src.data(), dst.data(), 8, nullptr, nullptr) == BSATTN_OK);
+  CHECK(bsattn_decode_dense(c, kv, dst.data(), 8, 0, nullptr, 1.f, kv, nullptr) == BSATTN_OK);
+  const int per_job = std::min(8, 16 / (hq / hkv));
+  CHECK(stub::last_dense.jobs == 8 + (per_job > 1 ? 8 / per_job : 0));
+  if (per_job > 1) CHECK(stub::last_dense.job[0].count == per_job && stub::last_dense.job[0].units == 40 * d.block_size / 32);
+  stub::splits = 1;
+  bsattn_cache_destroy(c);
+}
+
 int main() {
+  for (unsigned seed = 0; seed < 6; ++seed) {
+    shared_jobs(seed, 8, 2);
+    shared_jobs(seed, 4, 4);
+    shared_jobs(seed, 16, 2);
+    shared_jobs(seed, 16, 1);
+  }
   for (unsigned seed = 0; seed < 40; ++seed) runs(seed, 8 + (int)(seed % 4) * 12);
   // captured: a fork, and a trim that would copy a page, are refused
   const bsattn_desc d = small_desc(4, 8);
@@ -205,21 +288,29 @@ int main() {
   CHECK(norm(buf, buf, 0.f, 1.f / 0.f, buf + 32, buf + 40) == BSATTN_ERR_INVALID);
   CHECK(norm(buf, buf, 0.f, 0.f, buf + 32, buf + 32) == BSATTN_ERR_INVALID);
   CHECK(norm(buf, buf, 0.f, 0.f, buf + 8, buf + 32) == BSATTN_ERR_INVALID);
-  // the dense decode's parts go through the split prefills' workspaces: one
-  // for a stream, the cache's own in a capture, none when there is no memory
+  // the dense decode's parts go through the cache's own workspace where they
+  // fit (64 rows of 8 heads and 2 splits), else through the split prefills':
+  // one for a stream, the cache's own in a capture, none when there is no memory
   auto dense = [&](hipStream_t s) { return bsattn_decode_dense(c, buf, ids, 2, 0, nullptr, 1.f, buf, s); };
   stub::prefills.clear();
   CHECK(dense(nullptr) == BSATTN_OK && stub::prefills.back().ws == nullptr);
   stub::splits = 5;
   CHECK(dense(nullptr) == BSATTN_OK);
+  const stub::Prefill own = stub::prefills.back();
+  CHECK(own.ws && !own.done && own.nsplit == 10 &&
+        stub::memory.at(own.ws) == 64u * 8 * 2 * (bsattn::kHeadDim + 2) * sizeof(float));
+  stub::splits = 64;
+  CHECK(dense(nullptr) == BSATTN_OK && stub::prefills.back().ws == own.ws);
+  stub::splits = 65;
+  CHECK(dense(nullptr) == BSATTN_OK);
   const stub::Prefill first = stub::prefills.back();
-  CHECK(first.ws && first.done && first.nsplit == 10);
+  CHECK(first.ws && first.ws != own.ws && first.done && first.nsplit == 130);
   CHECK(dense(nullptr) == BSATTN_OK && stub::prefills.back().ws == first.ws);
   CHECK(dense((hipStream_t)16) == BSATTN_OK && stub::prefills.back().ws != first.ws);
   stub::capture = hipStreamCaptureStatusActive;
   CHECK(dense(nullptr) == BSATTN_OK);
   const stub::Prefill graph = stub::prefills.back();
-  CHECK(graph.ws && !graph.done && stub::memory.at(graph.ws) == 10u * 8 * (bsattn::kHeadDim + 2) * sizeof(float));
+  CHECK(graph.ws && !graph.done && stub::memory.at(graph.ws) == 130u * 8 * (bsattn::kHeadDim + 2) * sizeof(float));
   stub::capture = hipStreamCaptureStatusNone;
   CHECK(dense(nullptr) == BSATTN_OK && stub::prefills.back().ws == first.ws);
   stub::launches_left = 0;

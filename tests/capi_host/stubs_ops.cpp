@@ -4,17 +4,57 @@
 
 using namespace bsattn;
 
+namespace stub {
+bsattn::DenseBatch last_dense;
+}  // namespace stub
+
+// every entry has a job of its own, and at most one with others, which hold
+// the same units
+static void check_jobs(const bsattn::DenseBatch& db) {
+  stub::last_dense = db;
+  CHECK(db.n >= 1 && db.n <= bsattn::kMaxBatch && db.jobs >= db.n && db.jobs <= bsattn::kMaxDenseJobs);
+  std::vector<int> own(db.n, 0), with(db.n, 0);
+  for (int j = 0; j < db.jobs; ++j) {
+    const bsattn::DenseJob& job = db.job[j];
+    CHECK(job.count >= 1 && job.count <= 16 && job.first >= 0 && job.first + job.count <= 2 * bsattn::kMaxBatch);
+    CHECK(job.units >= 0);
+    CHECK(job.entry == db.order[job.first] && job.seq == db.ids[job.entry]);
+    for (int k = 0; k < job.count; ++k) {
+      const int e = db.order[job.first + k];
+      CHECK(e >= 0 && e < db.n);
+      if (job.count == 1) {
+        ++own[e];
+        CHECK(db.alone[e] == j && job.shares == (db.shared[e] >= 0));
+        CHECK(job.from == (job.shares ? db.job[db.shared[e]].units : 0));
+      } else {
+        ++with[e];
+        CHECK(db.shared[e] == j && db.window == 0);
+      }
+    }
+  }
+  for (int e = 0; e < db.n; ++e) CHECK(own[e] == 1 && with[e] == (db.shared[e] >= 0));
+}
+
 namespace bsattn {
 using stub::run;
 hipError_t launch_rotate(const Geometry& g, RotateBatch, int, hipStream_t, Timing*) { return run(g, nullptr); }
-int dense_plan(const Geometry&, const int32_t*, DenseBatch& db) {
+// (a job of n entries: `splits` parts)
+int dense_plan(const Geometry&, DenseBatch& db, int* rows) {
   db.cu = 4;
-  for (int i = 0; i < db.n; ++i) db.part0[i] = i * stub::splits;
-  return db.n * stub::splits;
+  int parts = 0, blocks = 0;
+  for (int j = 0; j < db.jobs; ++j) {
+    db.job[j].part0 = parts;
+    db.job[j].row0 = blocks;
+    parts += stub::splits;
+    blocks += stub::splits * db.job[j].count;
+  }
+  *rows = parts == db.n ? 0 : blocks;
+  return parts;
 }
 hipError_t launch_dense(const Geometry& g, const DenseBatch& db, int parts, const void*, void*, float* ws,
                         hipEvent_t done, hipStream_t s, Timing*) {
   CHECK((parts > db.n) == (ws != nullptr));
+  check_jobs(db);
   {
     std::lock_guard<std::mutex> lock(stub::mu);
     stub::prefills.push_back({ws, (stub::Event*)done, parts});

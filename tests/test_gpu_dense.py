@@ -353,3 +353,28 @@ def test_refusals(gpu):
     odd = torch.zeros(2 * 8 * D + 1, dtype=torch.float16, device=gpu)[1:].view(2, 8, 1, D)
     with pytest.raises(bsattn.BsattnError):
         c.decodeDense(odd, SCALE)
+
+
+@pytest.mark.parametrize("dtype,bits", KINDS)
+@pytest.mark.parametrize("Hq,Hkv", [(4, 4), (4, 2), (32, 8), (16, 2), (32, 2)])
+def test_joins_agree(gpu, dtype, bits, Hq, Hkv):
+    """The same bits call after call, timed or not, for counts of parts from
+    one to more than a round of the join's rows."""
+    import torch
+    log(f"[dense joins] {dtype} bits={bits} {Hq}/{Hkv}")
+    lens = [1, 129, 300, 1100, 0, 4200, 33]
+    c = _cache(lens, Hq, Hkv, 64, dtype, bits, spare=64)
+    _fill(gpu, c, lens, 7)
+    sinks = torch.linspace(-1, 3, Hq, device=gpu)
+    for step in range(3):
+        for ids in ([0], [1, 2], [3], [5], [6, 5], list(range(7)), [4, 5, 3]):
+            q = _randn(gpu, 10 * step + len(ids), (len(ids), Hq, 1, D), dtype)
+            for kw in (dict(), dict(sinks=sinks), dict(window=1000)):
+                got = [c.decodeDense(q, SCALE, seq_ids=ids, **kw) for _ in range(3)]
+                c.profile(True)
+                want = c.decodeDense(q, SCALE, seq_ids=ids, **kw)
+                c.profile(False)
+                assert all(torch.equal(g, want) for g in got), f"{ids} {kw}"
+            _check(got[0], _reference(c, q, ids=ids, window=1000), dtype, f"{ids}")
+        k = _randn(gpu, 90 + step, (7, Hkv, 17, D), "f16" if bits else dtype)
+        c.append(k, k)

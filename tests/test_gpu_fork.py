@@ -170,6 +170,50 @@ def test_many_and_partial(gpu):
     assert d.freePages == d.desc.max_seqs * d.desc.max_blocks_per_seq
 
 
+@pytest.mark.parametrize("dtype,bits", KINDS)
+@pytest.mark.parametrize("Hq,Hkv", [(4, 4), (8, 4), (16, 4), (16, 2), (16, 1)])
+def test_shared_prefixes(gpu, dtype, bits, Hq, Hkv):
+    """Dense decode of sequences that share their beginnings: branches of two
+    prompts and of a branch, in any order beside sequences of their own; more
+    of them than one workgroup takes; ends at a block's end; sinks."""
+    import torch
+    log(f"[shared] {dtype} bits={bits} {Hq}/{Hkv}")
+    rows = 32
+    c = _cache([2100] * rows, Hq, Hkv, 64, dtype, bits)
+    _fill(gpu, c, [1999, 1024, 777] + [0] * (rows - 3), 21, salient=True)
+    c.fork([0] * 11, list(range(3, 14)))
+    c.fork([1] * 5, list(range(14, 19)))
+    k, v = _tokens(gpu, c, 60, 1, 90)
+    for s in (3, 5, 15, 17):
+        c.append(k, v, seq_ids=[s])
+    c.fork([5, 5, 5, 0, 0], [19, 20, 21, 22, 23], [2050, 2089, 1985, 1500, 511])
+    c.trim(700, seq_ids=[20])
+    g = torch.Generator().manual_seed(4)
+    sinks = torch.linspace(-2, 4, Hq, device=gpu)
+    for ids in (list(range(3, 14)), list(range(rows)), torch.randperm(rows, generator=g).tolist(), [5, 19], [14, 0, 15],
+                [20, 21, 22, 23, 2]):
+        q = _randn(gpu, 70 + len(ids), (len(ids), Hq, 1, D), dtype)
+        _check(c.decodeDense(q, SCALE, seq_ids=ids), _reference(c, q, ids=ids), dtype, f"{ids}")
+        _check(c.decodeDense(q, SCALE, sinks=sinks, seq_ids=ids), _reference(c, q, ids=ids, sinks=sinks), dtype,
+               f"sinks {ids}")
+        _check(c.decodeDense(q, SCALE, window=900, seq_ids=ids), _reference(c, q, ids=ids, window=900), dtype,
+               f"window {ids}")
+    # captured, the sequences may be others by the time of a replay
+    ids = list(range(3, 14))
+    q = _randn(gpu, 90, (len(ids), Hq, 1, D), dtype)
+    c.decodeDense(q, SCALE, seq_ids=ids)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = c.decodeDense(q, SCALE, seq_ids=ids)
+    for step in range(3):
+        graph.replay()
+        _check(out, _reference(c, q, ids=ids), dtype, f"replay {step}")
+        c.trim(600, seq_ids=[4 + step])
+        k, v = _tokens(gpu, c, 80 + step, 1, 500)
+        c.append(k, v, seq_ids=[4 + step])
+
+
 def test_steps_after_forks(gpu):
     """Reserved, captured steps of branches: no branch writes a page that
     another holds."""
