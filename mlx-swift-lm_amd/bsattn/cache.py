@@ -23,6 +23,7 @@ import torch
 from . import _lib
 from ._lib import BsattnError, check, i32_array, lib
 
+_Strides = ctypes.c_int64 * 3
 _DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
 
@@ -69,6 +70,7 @@ class BlockSparseKVCache:
         # take it 38 us, 63 before (one launch a step less included).
         self._lib = lib()
         self._hq, self._hkv, self._dim = num_q_heads, num_kv_heads, head_dim
+        self._index = self.device.index
         info = _lib.Info()
         check(lib().bsattn_cache_info(self._h, ctypes.byref(info)))
         self.nselMax = info.nsel_max
@@ -449,27 +451,34 @@ class BlockSparseKVCache:
     # -- rotary positions ------------------------------------------------------
     def _check_strided(self, t: torch.Tensor, name: str, heads: int):
         """Element strides of t [B, heads, L, D] between sequences, heads and
-        tokens; the dims are contiguous and every row 16-byte aligned."""
-        if t.device != self.device or t.dtype != self.dtype:
+        tokens (None: dense); the dims are contiguous and every row 16-byte
+        aligned."""
+        shape = t.shape
+        if t.dtype is not self.dtype or t.get_device() != self._index:
             raise ValueError(f"{name} must be a {self.dtype} tensor on {self.device}")
-        if t.dim() != 4 or heads < 1 or t.shape[1] != heads or t.shape[3] != self._dim or 0 in t.shape:
-            raise ValueError(f"{name} must be [B, {heads or 'H'}, L, {self._dim}], got {tuple(t.shape)}")
-        # (torch gives a dimension of one element any stride)
-        st = [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
-        if st[3] != 1 or st[0] % 8 or st[1] % 8 or st[2] % 8 or t.data_ptr() % 16:
-            raise ValueError(f"{name} must have contiguous, 16-byte aligned heads, got strides {t.stride()} at "
-                             f"offset {t.storage_offset()}")
-        return (ctypes.c_int64 * 3)(*st[:3])
+        if len(shape) != 4 or heads < 1 or shape[1] != heads or shape[3] != self._dim or 0 in shape:
+            raise ValueError(f"{name} must be [B, {heads or 'H'}, L, {self._dim}], got {tuple(shape)}")
+        if t.is_contiguous():
+            if t.data_ptr() % 16 == 0:
+                return None
+        else:
+            # (torch gives a dimension of one element any stride)
+            s0, s1, s2, s3 = t.stride()
+            s0, s1, s2 = s0 if shape[0] > 1 else 0, s1 if heads > 1 else 0, s2 if shape[2] > 1 else 0
+            if s3 == 1 and not (s0 | s1 | s2) & 7 and t.data_ptr() % 16 == 0:
+                return _Strides(s0, s1, s2)
+        raise ValueError(f"{name} must have contiguous, 16-byte aligned heads, got strides {t.stride()} at "
+                         f"offset {t.storage_offset()}")
 
     def _check_rope(self, rope) -> None:
-        if rope.device != self.device:
+        if rope.index != self._index:
             raise ValueError(f"the rope is on {rope.device}, the cache on {self.device}")
 
     def _check_positions(self, positions: Optional[torch.Tensor], B: int, L: int):
         if positions is None:
             return None
-        if positions.dtype != torch.int32 or positions.device != self.device or not positions.is_contiguous() \
-                or tuple(positions.shape) != (B, L):
+        if positions.dtype is not torch.int32 or positions.get_device() != self._index \
+                or not positions.is_contiguous() or positions.shape != (B, L):
             raise ValueError(f"positions must be a contiguous int32 tensor ({B}, {L}) on {self.device}, got "
                              f"{positions.dtype} {tuple(positions.shape)}")
         return positions.data_ptr()
@@ -493,13 +502,13 @@ class BlockSparseKVCache:
         for name, w in (("qWeight", qWeight), ("kWeight", kWeight)):
             if w is None:
                 continue
-            if w.dtype != self.dtype or w.device != self.device or tuple(w.shape) != (self._dim,) \
+            if w.dtype is not self.dtype or w.get_device() != self._index or w.shape != (self._dim,) \
                     or not w.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous {self.dtype} tensor ({self._dim},) on {self.device}")
         self._check_rope(rope)
         pos = self._check_positions(positions, B, L)
-        q = torch.empty(queries.shape, dtype=self.dtype, device=self.device)
-        k = torch.empty(keys.shape, dtype=self.dtype, device=self.device)
+        q = torch.empty_like(queries, memory_format=torch.contiguous_format)
+        k = torch.empty_like(keys, memory_format=torch.contiguous_format)
         check(self._lib.bsattn_norm_rotate(self._h, rope._ref, queries.data_ptr(), qs, keys.data_ptr(), ks,
                                            None if qWeight is None else qWeight.data_ptr(),
                                            None if kWeight is None else kWeight.data_ptr(), eps, weightOffset,

@@ -14,7 +14,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from ._lib import check, i32_array, lib
+from ._lib import check, i32_array
 from .cache import BlockSparseKVCache, _stream
 
 HEAD_DIM = 128
@@ -40,6 +40,7 @@ class RoPE:
         if not all(math.isfinite(t) for t in theta) or not math.isfinite(factor):
             raise ValueError("rope angles and factor must be finite")
         self.device = torch.device("cuda", device if isinstance(device, int) else device.index or 0)
+        self.index = self.device.index
         self.dims, self.traditional, self.factor = dims, bool(traditional), float(factor)
         self.theta = torch.tensor(theta, dtype=torch.float64, device=self.device)
         # (the table is ready before any stream uses it)
@@ -148,9 +149,9 @@ def applyRotaryPosition(rope: RoPE, x: torch.Tensor, cache: BlockSparseKVCache,
     B, _, L, _ = x.shape
     cache._check_rope(rope)
     pos = cache._check_positions(positions, B, L)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    check(lib().bsattn_rotate(cache._h, rope._ref, x.data_ptr(), strides, heads, i32_array(seq_ids), B, L, pos,
-                              out.data_ptr(), _stream(cache.device)))
+    out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    check(cache._lib.bsattn_rotate(cache._h, rope._ref, x.data_ptr(), strides, heads, i32_array(seq_ids), B, L, pos,
+                                   out.data_ptr(), _stream(cache.device)))
     return out
 
 
