@@ -179,5 +179,7 @@ def check(rc: int) -> None:
 def i32_array(values):
     if values is None:
         return None
-    arr = (ctypes.c_int32 * len(values))(*[int(v) for v in values])
-    return arr
+    try:
+        return (ctypes.c_int32 * len(values))(*values)
+    except TypeError:  # numbers that are not Python's own
+        return (ctypes.c_int32 * len(values))(*[int(v) for v in values])

@@ -51,6 +51,21 @@ constexpr float kSlack = 6.0f;
 constexpr float kTop = 14.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 
+// What the 16 columns hold: a group of up to 8 heads of one entry; a group of
+// 16; the queries of a shared job's members, whose blocks other workgroups of
+// the XCD read, too.
+enum Columns { kNarrow, kGroup16, kShared };
+
+// Ahead of the partials in the workspace: where each entry's lie, written by the
+// first part of its own job.  (With the batch among its arguments the join's
+// launch takes the host 4.1 us, with less than 100 bytes 2.8.)
+struct DenseJoin {
+  int32_t shared0, step, shared;  // the shared job's: blocks shared0, shared0 + step, ...
+  int32_t own0, parts;            // then own0 + shared, own0 + shared + 1, ...; `parts` in all
+};
+constexpr int kPartial = kHeadDim + 2;  // floats of a partial: o, its reference, its sum
+constexpr int kJoinRows = (kMaxBatch * (int)sizeof(DenseJoin) / 4 + kPartial - 1) / kPartial;
+
 // x of the lane 8 columns on
 __device__ __forceinline__ float column8(float x) {
   return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x128, 0xF, 0xF, false));
@@ -64,12 +79,12 @@ __device__ __forceinline__ float hi16(uint32_t w) { return to_f32<DT>((uint16_t)
 // B operand of x[0, 8) (tokens 8g .. 8g + 7 of this lane's head): hi rounded
 // to 16 bits, lo what the rounding left.  Narrow groups: the one that this
 // lane's column takes (rest: 1 in columns 8-15, else 0), in hi.
-template <int DT, bool WIDE>
+template <int DT, Columns C>
 __device__ __forceinline__ void split_operand(const float* x, float rest, u32x4& hi, u32x4& lo) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const uint32_t h = cvt_pk<DT>(x[2 * j], x[2 * j + 1]);
-    if constexpr (WIDE) {
+    if constexpr (C != kNarrow) {
       hi[j] = h;
       lo[j] = cvt_pk<DT>(x[2 * j] - lo16<DT>(h), x[2 * j + 1] - hi16<DT>(h));
     } else {
@@ -79,9 +94,9 @@ __device__ __forceinline__ void split_operand(const float* x, float rest, u32x4&
 }
 
 // The same from weights that are shared out (quantized caches): x holds the
-// lane's tokens, all eight (WIDE) or four of them (odd: the last four).  hi, lo
+// lane's tokens, all eight, or (narrow) four of them (odd: the last four).  hi, lo
 // as split_operand's.
-template <bool WIDE, int NT>
+template <Columns C, int NT>
 __device__ __forceinline__ void weight_operand(const float (&x)[NT], bool odd, u32x4& hi, u32x4& lo) {
   uint32_t h[NT / 2], r[NT / 2];
 #pragma unroll
@@ -89,7 +104,7 @@ __device__ __forceinline__ void weight_operand(const float (&x)[NT], bool odd, u
     h[j] = cvt_pk<0>(x[2 * j], x[2 * j + 1]);
     r[j] = cvt_pk<0>(x[2 * j] - lo16<0>(h[j]), x[2 * j + 1] - hi16<0>(h[j]));
   }
-  if constexpr (WIDE) {
+  if constexpr (C != kNarrow) {
     hi = u32x4{h[0], h[1], h[2], h[3]};
     lo = u32x4{r[0], r[1], r[2], r[3]};
   } else {
@@ -125,7 +140,7 @@ struct DensePart {
     return place < full ? fa + place : place == full ? head : r.u0 + r.units - 1;
   }
 };
-__device__ __forceinline__ DensePart dense_part(const Geometry& geo, const DenseBatch& db) {
+__device__ __forceinline__ DensePart dense_part(const Geometry& geo, const DenseBatch& db, float* partials) {
   DensePart w;
   const int lane = threadIdx.x & 63;
   // the job whose parts hold this workgroup's
@@ -142,11 +157,21 @@ __device__ __forceinline__ DensePart dense_part(const Geometry& geo, const Dense
   const bool alone = w.count == 1;
   if (alone) w.r = dense_range(geo, db, job);
   else w.r = DenseRange{32 * job.units, 0, 0, job.units};
-  const int parts = (w.r.units + db.cu - 1) / db.cu;
-  const bool direct = alone && parts <= 1 && !job.shares;
+  // (more tokens than the launch was cut for, as when a graph replays after
+  // further reservations: as many parts, of more units each)
+  int cu = db.cu;
+  if (alone && w.r.units > job.units) {
+    const int most = max(1, (job.units + cu - 1) / cu);
+    cu = max(cu, ((w.r.units + most - 1) / most + 3) & ~3);
+  }
+  const int parts = (w.r.units + cu - 1) / cu;
+  const bool direct = alone && parts <= 1 && job.of < 0;
   w.rows = direct ? -1 : job.row0 + part * w.count;
+  if (alone && part == 0 && blockIdx.y == 0 && partials && threadIdx.x == 0)
+    ((DenseJoin*)partials)[w.entry] =
+        DenseJoin{job.shared0, job.step, job.shared, job.row0 - job.shared, job.shared + parts};
   const int end = w.r.u0 + w.r.units;
-  const int ua = w.r.u0 + part * db.cu, ub = min(ua + db.cu, end);
+  const int ua = w.r.u0 + part * cu, ub = min(ua + cu, end);
   const bool first = ua == w.r.u0 && 32 * ua < w.r.lo;
   const bool last = ub == end && 32 * ub > w.r.len && !(first && ub == ua + 1);
   w.places = max(ub - ua, 0);
@@ -180,8 +205,13 @@ struct DensePages {
   }
 };
 
-// 16 bytes at a uniform address plus a lane's offset, read once
+// 16 bytes at a uniform address plus a lane's offset: read once, unless another
+// shared job reads them, too (8 branches of 8191 bf16 tokens, two jobs: 14.1 us
+// as if read once, 12.6 so; read once, 4 x 262k int8 in groups of 16: 179 and
+// 201)
+template <Columns C>
 __device__ __forceinline__ u32x4 stream16(const uint8_t* base, uint32_t at) {
+  if constexpr (C == kShared) return *(const u32x4*)(base + at);
   return __builtin_nontemporal_load((const u32x4*)(base + at));
 }
 // a lane's offset, kept in 32 bits up to here (the load then adds it to the
@@ -195,12 +225,12 @@ __device__ __forceinline__ uint32_t offset32(uint32_t at) {
 // g), dims 16 dt + 4 g ..), sums l over its own tokens, and their reference
 // (-inf: no token); written as the output (one part) or as partials (o,
 // reference, l).  Column c holds head c % G of member c / G.
-template <int DT, bool WIDE>
+template <int DT, Columns C>
 __device__ __forceinline__ void dense_finish(const Geometry& geo, const DenseBatch& db, const DensePart& w,
                                              const f32x4 (&o)[8], float ref, float l, uint16_t* __restrict__ out,
                                              float* __restrict__ partials) {
   __shared__ float s_m[4][16], s_l[4][16];
-  __shared__ __align__(16) float s_o[4][WIDE ? 16 : 8][kHeadDim + 4];
+  __shared__ __align__(16) float s_o[4][C == kNarrow ? 8 : 16][kHeadDim + 4];
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int n = lane & 15, g = lane >> 4, G = geo.group, h = blockIdx.y;
   const int cols = G * w.count;
@@ -227,7 +257,7 @@ __device__ __forceinline__ void dense_finish(const Geometry& geo, const DenseBat
       L += f * s_l[v][col];
       a += f * s_o[v][col][d];
     }
-    const int member = WIDE ? col / G : 0, hq = h * G + col - member * G;
+    const int member = C == kShared ? col / G : 0, hq = h * G + col - member * G;
     if (w.rows < 0) {
       if (db.sinks && w.r.len > 0) {
         const float sk = db.sinks[hq] * kLog2e, top = fmaxf(M, sk);
@@ -237,7 +267,7 @@ __device__ __forceinline__ void dense_finish(const Geometry& geo, const DenseBat
       }
       out[((size_t)w.entry * geo.hq + hq) * kHeadDim + d] = from_f32<DT>(L == 0.f ? 0.f : a / L);
     } else {
-      float* pp = partials + ((size_t)(w.rows + member) * geo.hq + hq) * (kHeadDim + 2);
+      float* pp = partials + kJoinRows * kPartial + ((size_t)(w.rows + member) * geo.hq + hq) * kPartial;
       pp[d] = a;
       if (d == 0) {
         pp[kHeadDim] = M;
@@ -248,12 +278,12 @@ __device__ __forceinline__ void dense_finish(const Geometry& geo, const DenseBat
 }
 
 // q's row for this lane's column (columns past the members' repeat the first's)
-template <bool WIDE>
+template <Columns C>
 __device__ __forceinline__ const uint16_t* dense_query(const Geometry& geo, const DenseBatch& db, const DensePart& w,
                                                        const uint16_t* __restrict__ q) {
   const int n = threadIdx.x & 15, G = geo.group;
   int bi = w.entry;
-  if constexpr (WIDE) {
+  if constexpr (C == kShared) {
     const int member = n / G;
     if (member > 0 && member < w.count) bi = db.order[w.first + member];
   }
@@ -261,13 +291,13 @@ __device__ __forceinline__ const uint16_t* dense_query(const Geometry& geo, cons
 }
 
 // 16-bit caches.  grid (parts of all entries, Hkv)
-template <int DT, bool WIDE>
+template <int DT, Columns C>
 __global__ __launch_bounds__(256, 2) void k_dense(Geometry geo, DenseBatch db, const uint16_t* __restrict__ q,
                                                uint16_t* __restrict__ out, float* __restrict__ partials) {
   // P's range: fp16 weights are lifted to at most 2^14, so that small ones keep
   // their bits (bf16 has fp32's range)
   constexpr float kLift = DT == 0 ? kTop - kSlack : 0.0f;
-  const DensePart w = dense_part(geo, db);
+  const DensePart w = dense_part(geo, db, partials);
   if (w.full < 0) return;  // nothing here: past the sequence's end
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int n = lane & 15, g = lane >> 4;
@@ -275,7 +305,7 @@ __global__ __launch_bounds__(256, 2) void k_dense(Geometry geo, DenseBatch db, c
   DensePages pages(geo, w, place);
   u32x4 qf[4];
   {
-    const uint16_t* src = dense_query<WIDE>(geo, db, w, q) + 8 * g;
+    const uint16_t* src = dense_query<C>(geo, db, w, q) + 8 * g;
 #pragma unroll
     for (int s = 0; s < 4; ++s) qf[s] = *(const u32x4*)(src + 32 * s);
   }
@@ -286,13 +316,13 @@ __global__ __launch_bounds__(256, 2) void k_dense(Geometry geo, DenseBatch db, c
     const uint8_t* p = slab + geo.k_off + (u & pages.sh) * 8192;
     const uint32_t x = offset32(at);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) kf[i] = stream16(p + i * 1024, x);
+    for (int i = 0; i < 8; ++i) kf[i] = stream16<C>(p + i * 1024, x);
   };
   auto load_v = [&](const uint8_t* slab, int u) __attribute__((always_inline)) {
     const uint8_t* p = slab + geo.v_off + (u & pages.sh) * 1024;
     const uint32_t x = offset32(at);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) vf[i] = stream16(p + (i << pages.sh) * 1024, x);
+    for (int i = 0; i < 8; ++i) vf[i] = stream16<C>(p + (i << pages.sh) * 1024, x);
   };
   f32x4 o[8];
 #pragma unroll
@@ -355,11 +385,11 @@ __global__ __launch_bounds__(256, 2) void k_dense(Geometry geo, DenseBatch db, c
       l += pv[e];
     }
     u32x4 hi, lo;
-    split_operand<DT, WIDE>(pv, rest, hi, lo);
+    split_operand<DT, C>(pv, rest, hi, lo);
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) {
       o[dt] = mfma16x16x32<DT>(vf[dt], hi, o[dt]);
-      if constexpr (WIDE) o[dt] = mfma16x16x32<DT>(vf[dt], lo, o[dt]);
+      if constexpr (C != kNarrow) o[dt] = mfma16x16x32<DT>(vf[dt], lo, o[dt]);
     }
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (MORE) load_v(slab, next);
@@ -378,13 +408,13 @@ __global__ __launch_bounds__(256, 2) void k_dense(Geometry geo, DenseBatch db, c
   for (; place + 4 < w.places; place += 4) step(std::false_type(), std::true_type());
   if (place < w.full) step(std::false_type(), std::false_type());
   else if (place < w.places) step(std::true_type(), std::false_type());
-  if constexpr (!WIDE) {
+  if constexpr (C == kNarrow) {
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt)
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[dt][i] += column8(o[dt][i]);
   }
-  dense_finish<DT, WIDE>(geo, db, w, o, m == -INFINITY ? m : base, l, out, partials);
+  dense_finish<DT, C>(geo, db, w, o, m == -INFINITY ? m : base, l, out, partials);
 }
 
 // Affine caches of KB bits, dequantised inside the products (the codes as fp16
@@ -399,22 +429,22 @@ __global__ __launch_bounds__(256, 2) void k_dense(Geometry geo, DenseBatch db, c
 // rounded weights go to columns 0-7, what the rounding left to 8-15.  sum p vb
 // stays fp32 and per lane until the end.
 // grid (parts of all entries, Hkv)
-template <int KB, bool WIDE>
+template <int KB, Columns C>
 __global__ __launch_bounds__(256, 2) void k_dense_q(Geometry geo, DenseBatch db, const uint16_t* __restrict__ q,
                                                  uint16_t* __restrict__ out, float* __restrict__ partials) {
   constexpr int NK = 2 * QCode<KB>::KF, NV = 8 / QCode<KB>::DPF;  // K and V fragments of a unit
-  constexpr int NT = WIDE ? 8 : 4;                                // tokens of a unit whose scores a lane holds
-  const DensePart w = dense_part(geo, db);
+  constexpr int NT = C == kNarrow ? 4 : 8;                              // tokens of a unit whose scores a lane holds
+  const DensePart w = dense_part(geo, db, partials);
   if (w.full < 0) return;  // nothing here: past the sequence's end
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int n = lane & 15, g = lane >> 4;
-  const bool odd = !WIDE && n >= 8;
+  const bool odd = C == kNarrow && n >= 8;
   const int tok0 = 8 * g + (odd ? 4 : 0);
   int place = wave;  // of the unit that a step takes
   DensePages pages(geo, w, place);
   u32x4 qf[4];
   {
-    const uint16_t* src = dense_query<WIDE>(geo, db, w, q) + 8 * g;
+    const uint16_t* src = dense_query<C>(geo, db, w, q) + 8 * g;
 #pragma unroll
     for (int s = 0; s < 4; ++s) qf[s] = *(const u32x4*)(src + 32 * s);
   }
@@ -429,16 +459,16 @@ __global__ __launch_bounds__(256, 2) void k_dense_q(Geometry geo, DenseBatch db,
     const uint8_t* p = slab + geo.k_off + (u & pages.sh) * (NK * 1024);
     const uint32_t x = offset32(at);
 #pragma unroll
-    for (int i = 0; i < NK; ++i) kf[i] = stream16(p + i * 1024, x);
+    for (int i = 0; i < NK; ++i) kf[i] = stream16<C>(p + i * 1024, x);
   };
   auto load_v = [&](const uint8_t* slab, int u) __attribute__((always_inline)) {
     const uint8_t* p = slab + geo.v_off + (u & pages.sh) * 1024;
     const uint32_t x = offset32(at);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) vf[i] = stream16(p + (i << pages.sh) * 1024, x);
+    for (int i = 0; i < NV; ++i) vf[i] = stream16<C>(p + (i << pages.sh) * 1024, x);
   };
   auto load_sb = [&](const uint8_t* slab, int u) __attribute__((always_inline)) {
-    sbx = stream16(slab + geo.sb_off + (u & pages.sh) * 128, offset32(sb_at));
+    sbx = stream16<C>(slab + geo.sb_off + (u & pages.sh) * 128, offset32(sb_at));
   };
 
   // the queries' sums over each 64 dims: of q, and of the QK operand (int4:
@@ -511,8 +541,8 @@ __global__ __launch_bounds__(256, 2) void k_dense_q(Geometry geo, DenseBatch db,
     float pv[NT];
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      const float a = (WIDE ? r0[i >> 2][i & 3] : odd ? r0[1][i] : r0[0][i]) - q0c;
-      const float b = (WIDE ? r1[i >> 2][i & 3] : odd ? r1[1][i] : r1[0][i]) - q1c;
+      const float a = (C != kNarrow ? r0[i >> 2][i & 3] : odd ? r0[1][i] : r0[0][i]) - q0c;
+      const float b = (C != kNarrow ? r1[i >> 2][i & 3] : odd ? r1[1][i] : r1[0][i]) - q1c;
       float x = lo_f(sb[i][0]) * a;
       x = __builtin_fmaf(hi_f(sb[i][0]), b, x);
       x = __builtin_fmaf(lo_f(sb[i][1]), q0, x);
@@ -545,7 +575,7 @@ __global__ __launch_bounds__(256, 2) void k_dense_q(Geometry geo, DenseBatch db,
 #pragma unroll
     for (int i = 1; i < NT; ++i) mx = fmaxf(mx, pv[i]);
     if (__any(mx > (m == -INFINITY ? m : lift + kSlack))) {
-      if constexpr (!WIDE) mx = fmaxf(mx, column8(mx));
+      if constexpr (C == kNarrow) mx = fmaxf(mx, column8(mx));
       const float top = fmaxf(m, base + max_over_groups(mx));
       const float was = base;
       base = (top == -INFINITY ? 0.0f : top) - lift;
@@ -567,15 +597,15 @@ __global__ __launch_bounds__(256, 2) void k_dense_q(Geometry geo, DenseBatch db,
     }
     const u32x4 off = u32x4{0xE400E400u, 0xE400E400u, 0xE400E400u, 0xE400E400u};  // -1024
     u32x4 h0, l0, h1, l1;
-    weight_operand<WIDE>(p0, odd, h0, l0);
-    weight_operand<WIDE>(p1, odd, h1, l1);
+    weight_operand<C>(p0, odd, h0, l0);
+    weight_operand<C>(p1, odd, h1, l1);
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) {
       const u32x4 a = v_operand<KB, 1>(vf, dt, 0, code_base);
       const u32x4& ph = dt < 4 ? h0 : h1;
       o[dt] = mfma_f16(off, ph, o[dt]);
       o[dt] = mfma_f16(a, ph, o[dt]);
-      if constexpr (WIDE) {
+      if constexpr (C != kNarrow) {
         const u32x4& pl = dt < 4 ? l0 : l1;
         o[dt] = mfma_f16(off, pl, o[dt]);
         o[dt] = mfma_f16(a, pl, o[dt]);
@@ -601,7 +631,7 @@ __global__ __launch_bounds__(256, 2) void k_dense_q(Geometry geo, DenseBatch db,
   else if (place < w.places) step(std::true_type(), std::false_type());
   ob0 = sum_over_groups(ob0);
   ob1 = sum_over_groups(ob1);
-  if constexpr (!WIDE) {
+  if constexpr (C == kNarrow) {
     ob0 += column8(ob0);
     ob1 += column8(ob1);
     l += column8(l);
@@ -610,10 +640,10 @@ __global__ __launch_bounds__(256, 2) void k_dense_q(Geometry geo, DenseBatch db,
   for (int dt = 0; dt < 8; ++dt)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if constexpr (!WIDE) o[dt][i] += column8(o[dt][i]);
+      if constexpr (C == kNarrow) o[dt][i] += column8(o[dt][i]);
       o[dt][i] += dt < 4 ? ob0 : ob1;
     }
-  dense_finish<0, WIDE>(geo, db, w, o, m == -INFINITY ? m : base, l, out, partials);
+  dense_finish<0, C>(geo, db, w, o, m == -INFINITY ? m : base, l, out, partials);
 }
 
 // The parts of one (entry, query head) joined, those of its shared job first:
@@ -621,52 +651,41 @@ __global__ __launch_bounds__(256, 2) void k_dense_q(Geometry geo, DenseBatch db,
 // asked for at once, and are summed in order at the end.  (Joined by the
 // workgroup that arrives last, with device-scope partials, one sequence of 4k
 // tokens takes 11.5 us, against 5.1 and 4.2 for the two launches.)  grid (Hq, n)
-constexpr int kJoinRows = 8, kJoinRound = 4;
+constexpr int kRows = 8, kRound = 4;
 template <int DT>
-__global__ __launch_bounds__(32 * kJoinRows) void k_dense_join(Geometry geo, DenseBatch db,
-                                                               const float* __restrict__ partials,
-                                                               uint16_t* __restrict__ out) {
-  __shared__ __align__(16) float s_o[kJoinRows][kHeadDim];
-  __shared__ float s_ml[kJoinRows][2];
-  const int hq = blockIdx.x, bi = blockIdx.y;
+__global__ __launch_bounds__(32 * kRows) void k_dense_join(const float* __restrict__ ws,
+                                                           const float* __restrict__ sinks,
+                                                           uint16_t* __restrict__ out) {
+  __shared__ __align__(16) float s_o[kRows][kHeadDim];
+  __shared__ float s_ml[kRows][2];
+  const int hq = blockIdx.x, hqs = gridDim.x, bi = blockIdx.y;
   const int row = threadIdx.x >> 5, c = threadIdx.x & 31;
-  const int js = db.shared[bi];
-  const DenseJob own = db.job[db.alone[bi]];
-  const DenseRange r = dense_range(geo, db, own);
-  int shared = 0, step = 0, block0 = 0;  // the shared job's parts, its blocks per part, this entry's first block
-  if (js >= 0) {
-    const DenseJob job = db.job[js];
-    shared = (job.units + db.cu - 1) / db.cu;
-    step = job.count;
-    while (db.order[job.first + block0] != bi) ++block0;
-    block0 += job.row0;
-  }
-  const int parts = shared + (r.units + db.cu - 1) / db.cu;
-  if (parts <= 1 && js < 0) return;  // (the launch before wrote the output)
-  const int own0 = own.row0 - shared;
+  const DenseJoin at = ((const DenseJoin*)ws)[bi];
+  const float* partials = ws + kJoinRows * kPartial;
+  if (at.parts <= 1 && at.shared == 0) return;  // (the launch before wrote the output)
   float M = -INFINITY, L = 0.f;
   f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int p0 = row; p0 < parts; p0 += kJoinRows * kJoinRound) {
-    f32x4 x[kJoinRound];
-    float m[kJoinRound], l[kJoinRound];
+  for (int p0 = row; p0 < at.parts; p0 += kRows * kRound) {
+    f32x4 x[kRound];
+    float m[kRound], l[kRound];
 #pragma unroll
-    for (int j = 0; j < kJoinRound; ++j) {
-      const int p = min(p0 + j * kJoinRows, parts - 1);
-      const int block = p < shared ? block0 + p * step : own0 + p;
-      const float2* at = (const float2*)(partials + ((size_t)block * geo.hq + hq) * (kHeadDim + 2));
-      const float2 xa = at[2 * c], xb = at[2 * c + 1], ml = at[kHeadDim / 2];
+    for (int j = 0; j < kRound; ++j) {
+      const int p = min(p0 + j * kRows, at.parts - 1);
+      const int block = p < at.shared ? at.shared0 + p * at.step : at.own0 + p;
+      const float2* part = (const float2*)(partials + ((size_t)block * hqs + hq) * kPartial);
+      const float2 xa = part[2 * c], xb = part[2 * c + 1], ml = part[kHeadDim / 2];
       x[j] = f32x4{xa.x, xa.y, xb.x, xb.y};
-      m[j] = p0 + j * kJoinRows < parts ? ml.x : -INFINITY;
+      m[j] = p0 + j * kRows < at.parts ? ml.x : -INFINITY;
       l[j] = ml.y;
     }
     float top = M;
 #pragma unroll
-    for (int j = 0; j < kJoinRound; ++j) top = fmaxf(top, m[j]);
+    for (int j = 0; j < kRound; ++j) top = fmaxf(top, m[j]);
     const float f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - top);
     L *= f;
     a *= f;
 #pragma unroll
-    for (int j = 0; j < kJoinRound; ++j) {
+    for (int j = 0; j < kRound; ++j) {
       const float g = m[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[j] - top);
       L += g * l[j];
       if (m[j] != -INFINITY) a += g * x[j];
@@ -681,23 +700,23 @@ __global__ __launch_bounds__(32 * kJoinRows) void k_dense_join(Geometry geo, Den
   __syncthreads();
   if (threadIdx.x >= kHeadDim) return;
   const int d = threadIdx.x;
-  const float sk = db.sinks ? db.sinks[hq] * kLog2e : -INFINITY;
+  const float sk = sinks ? sinks[hq] * kLog2e : -INFINITY;
   float top = sk;
 #pragma unroll
-  for (int i = 0; i < kJoinRows; ++i) top = fmaxf(top, s_ml[i][0]);
+  for (int i = 0; i < kRows; ++i) top = fmaxf(top, s_ml[i][0]);
   float Ls = sk == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sk - top), as = 0.f;
 #pragma unroll
-  for (int i = 0; i < kJoinRows; ++i) {
+  for (int i = 0; i < kRows; ++i) {
     const float mi = s_ml[i][0];
     const float f = mi == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi - top);
     Ls += f * s_ml[i][1];
     if (mi != -INFINITY) as += f * s_o[i][d];
   }
-  out[((size_t)bi * geo.hq + hq) * kHeadDim + d] = from_f32<DT>(Ls == 0.f ? 0.f : as / Ls);
+  out[((size_t)bi * hqs + hq) * kHeadDim + d] = from_f32<DT>(Ls == 0.f ? 0.f : as / Ls);
 }
 
 // Cuts the jobs into parts.
-int dense_plan(const Geometry& g, DenseBatch& db, int* rows) {
+int dense_plan(const Geometry& g, DenseBatch& db, int64_t* rows) {
   int64_t all = 0;
   int most = 1;
   for (int j = 0; j < db.jobs; ++j) {
@@ -715,44 +734,51 @@ int dense_plan(const Geometry& g, DenseBatch& db, int* rows) {
     bool joined = false;
     for (int j = 0; j < db.jobs; ++j) {
       DenseJob& job = db.job[j];
-      const bool direct = job.count == 1 && !job.shares;
+      const bool direct = job.count == 1 && job.of < 0;
       int n = (job.units + db.cu - 1) / db.cu;
-      if (direct) n = std::max(n, 1);  // (zeros for no tokens)
+      if (job.count == 1) n = std::max(n, 1);  // (zeros for no tokens; the join's table)
       // (jobs of the same blocks: their n-th parts lie a multiple of 8
       // workgroups apart, on the same XCD, whose L2 then holds them; two jobs of
       // 4 x 8191 bf16 tokens 17.1 -> 14.6 us)
       if (job.count > 1) n = (n + 7) & ~7;
       job.part0 = (int32_t)parts;
       job.row0 = (int32_t)blocks;
+      if (job.of >= 0) {  // (shared jobs come first)
+        const DenseJob& with = db.job[job.of];
+        job.shared = (int16_t)((with.units + db.cu - 1) / db.cu);
+        job.step = with.count;
+        job.shared0 = with.row0;
+        while (db.order[with.first + job.shared0 - with.row0] != job.entry) ++job.shared0;
+      }
       parts += n;
       blocks += (int64_t)n * job.count;
       joined = joined || n > 1 || !direct;
     }
-    *rows = joined ? (int)blocks : 0;
-    if (!joined || blocks * g.hq <= kPrefillRows) return (int)parts;
+    *rows = joined ? kJoinRows + blocks * g.hq : 0;
+    if (*rows <= kPrefillRows) return (int)parts;
     db.cu *= 2;
   }
 }
 
-template <bool WIDE>
+template <Columns C>
 static void dense_dispatch(const Geometry& g, const DenseBatch& db, dim3 grid, const uint16_t* q, uint16_t* out,
-                           float* partials, hipStream_t s, Timing* prof) {
+                           float* ws, hipStream_t s, Timing* prof) {
   const dim3 blk(256);
   const int kd = kProfDense;
-  if (g.kv_bits == 4) launch(k_dense_q<4, WIDE>, grid, blk, 0, s, prof, kd, g, db, q, out, partials);
-  else if (g.kv_bits == 8) launch(k_dense_q<8, WIDE>, grid, blk, 0, s, prof, kd, g, db, q, out, partials);
-  else if (g.dtype == 0) launch(k_dense<0, WIDE>, grid, blk, 0, s, prof, kd, g, db, q, out, partials);
-  else launch(k_dense<1, WIDE>, grid, blk, 0, s, prof, kd, g, db, q, out, partials);
+  if (g.kv_bits == 4) launch(k_dense_q<4, C>, grid, blk, 0, s, prof, kd, g, db, q, out, ws);
+  else if (g.kv_bits == 8) launch(k_dense_q<8, C>, grid, blk, 0, s, prof, kd, g, db, q, out, ws);
+  else if (g.dtype == 0) launch(k_dense<0, C>, grid, blk, 0, s, prof, kd, g, db, q, out, ws);
+  else launch(k_dense<1, C>, grid, blk, 0, s, prof, kd, g, db, q, out, ws);
 }
 
 template <int DT>
 static hipError_t join_dispatch(const Geometry& g, const DenseBatch& db, const float* ws, uint16_t* out,
                                 hipEvent_t done, hipStream_t s, Timing* prof) {
-  const dim3 grid(g.hq, db.n), blk(32 * kJoinRows);
+  const dim3 grid(g.hq, db.n), blk(32 * kRows);
   if (done && !prof)  // (the event is the dispatch's own: no packet of its own behind it)
-    hipExtLaunchKernelGGL(k_dense_join<DT>, grid, blk, 0u, s, nullptr, done, 0u, g, db, ws, out);
+    hipExtLaunchKernelGGL(k_dense_join<DT>, grid, blk, 0u, s, nullptr, done, 0u, ws, db.sinks, out);
   else
-    launch(k_dense_join<DT>, grid, blk, 0, s, prof, kProfCombine, g, db, ws, out);
+    launch(k_dense_join<DT>, grid, blk, 0, s, prof, kProfCombine, ws, db.sinks, out);
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && done && prof) e = hipEventRecord(done, s);
   return e;
@@ -764,10 +790,11 @@ hipError_t launch_dense(const Geometry& g, const DenseBatch& db, int parts, cons
   const dim3 grid(parts, g.hkv);
   const uint16_t* qq = (const uint16_t*)q;
   uint16_t* oo = (uint16_t*)out;
-  bool wide = g.group > 8;  // (shared jobs fill more than 8 columns, or may as well)
-  for (int j = 0; j < db.jobs; ++j) wide = wide || db.job[j].count > 1;
-  if (wide) dense_dispatch<true>(g, db, grid, qq, oo, ws, s, prof);
-  else dense_dispatch<false>(g, db, grid, qq, oo, ws, s, prof);
+  bool shared = false;
+  for (int j = 0; j < db.jobs; ++j) shared = shared || db.job[j].count > 1;
+  if (shared) dense_dispatch<kShared>(g, db, grid, qq, oo, ws, s, prof);
+  else if (g.group > 8) dense_dispatch<kGroup16>(g, db, grid, qq, oo, ws, s, prof);
+  else dense_dispatch<kNarrow>(g, db, grid, qq, oo, ws, s, prof);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || !ws) return e;
   return g.dtype == 0 ? join_dispatch<0>(g, db, ws, oo, done, s, prof) : join_dispatch<1>(g, db, ws, oo, done, s, prof);

@@ -322,12 +322,13 @@ inline void cap_patch(const bsattn_cache* c, int seq, Patches& patches) {
 inline int release_pages(bsattn_cache* c, int seq, int keep_blocks,
                   Patches& patches) {
   auto& pg = c->pages[seq];
-  while ((int)pg.size() > keep_blocks) {
-    int32_t& others = c->sharers[pg.back()];
-    if (others > 0) --others;
-    else c->free_pages.push_back(pg.back());
-    pg.pop_back();
+  int32_t* sharers = c->sharers.data();
+  for (size_t i = pg.size(); i > (size_t)keep_blocks; --i) {
+    const int32_t p = pg[i - 1];
+    if (sharers[p] > 0) --sharers[p];
+    else c->free_pages.push_back(p);
   }
+  if (pg.size() > (size_t)keep_blocks) pg.resize(keep_blocks);
   cap_patch(c, seq, patches);
   return BSATTN_OK;
 }

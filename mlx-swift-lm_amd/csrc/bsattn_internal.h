@@ -278,26 +278,27 @@ hipError_t launch_rotate(const Geometry& g, RotateBatch rb, int n, hipStream_t s
 constexpr int kMaxDenseJobs = kMaxBatch + kMaxBatch / 2;
 struct DenseJob {
   int32_t part0, row0;
-  int32_t units, from;    // from: the entry's units that its shared job covers (count 1)
-  int32_t seq;            // a member's sequence
-  int16_t first, count;   // members: order[first] ..
-  int16_t entry, shares;  // the first member; whether it (count 1) has a shared job, too
+  int32_t units, from;   // from: the entry's units that its shared job covers (count 1)
+  int32_t seq;           // a member's sequence
+  // (count 1) the entry's partials from its shared job `of` (-1: none): the
+  // blocks of rows shared0, shared0 + step, ..., `shared` of them
+  int32_t shared0;
+  int16_t shared, step, of;
+  int16_t first, count;  // members: order[first] ..
+  int16_t entry;         // the first member
 };
 struct DenseBatch {
   int32_t n, jobs, cu, window;  // window: the last tokens seen (0: all)
   float sl2;
   const float* sinks;           // [hq] logits of the heads, or null
-  int32_t ids[kMaxBatch];
-  int16_t shared[kMaxBatch];    // that job, or -1
-  int16_t alone[kMaxBatch];     // the entry's own
   int16_t order[2 * kMaxBatch];
   DenseJob job[kMaxDenseJobs];
 };
-// sets cu, part0 and row0 of the jobs; the number of parts, and in *rows the
-// blocks of partials (0: none are needed, every entry has one part)
-int dense_plan(const Geometry& g, DenseBatch& db, int* rows);
-// ws: rows * hq rows of kHeadDim + 2 floats (null without partials); the launch
-// that joins them records `done` (may be null)
+// sets cu and what follows from it in the jobs; the number of parts, and in
+// *rows the rows of the workspace (0: none is needed, every entry has one part)
+int dense_plan(const Geometry& g, DenseBatch& db, int64_t* rows);
+// ws: rows of kHeadDim + 2 floats (null without partials); the launch that
+// joins them records `done` (may be null)
 hipError_t launch_dense(const Geometry& g, const DenseBatch& db, int parts, const void* q, void* out, float* ws,
                         hipEvent_t done, hipStream_t s, Timing* prof);
 hipError_t launch_export(const Geometry& g, const SeqBatch& b, int T, void* k_out,

@@ -77,13 +77,14 @@ int rotate_impl(bsattn_cache* c, const bsattn_rope& rope, RotateBatch& rb, const
 }
 
 // a job of the `count` entries order[first] ..
-DenseJob& add_job(DenseBatch& db, int first, int count) {
+DenseJob& add_job(DenseBatch& db, const int32_t* ids, int first, int count) {
   DenseJob& job = db.job[db.jobs++];
   job = DenseJob{};
   job.first = (int16_t)first;
   job.count = (int16_t)count;
   job.entry = db.order[first];
-  job.seq = db.ids[job.entry];
+  job.seq = ids[job.entry];
+  job.of = -1;
   return job;
 }
 
@@ -93,32 +94,33 @@ DenseJob& add_job(DenseBatch& db, int first, int count) {
 // of 8191 35.5 and 78.9, but 32 of 600 17.9 and 15.7.
 constexpr int kSharedUnits = 32;
 
-// Jobs of a launch (ids are set): the full blocks that entries share, read once
-// for as many as fill the columns, and each entry's rest.  A block is shared
-// only with all those before it (forks share from the beginning, trims take
+// Jobs of a launch of the sequences ids[0, n): the full blocks that entries
+// share, read once for as many as fill the columns, and each entry's rest.  A
+// block is shared only with all those before it (forks share from the beginning, trims take
 // from the end), so the longest common prefix is found by bisection.  Not with
 // a window, and not in a capture: its replays may find other sequences.
-void dense_jobs(const bsattn_cache* c, DenseBatch& db, hipStream_t s) {
+void dense_jobs(const bsattn_cache* c, const int32_t* ids, DenseBatch& db, hipStream_t s) {
   const Geometry& g = c->geo;
   const int per_block = g.tb / 32, most = 16 / g.group;
-  std::fill(db.shared, db.shared + kMaxBatch, (int16_t)-1);
+  int16_t of[kMaxBatch];  // an entry's shared job, or -1
+  std::fill(of, of + kMaxBatch, (int16_t)-1);
   db.jobs = 0;
   int placed = 0;
   auto sharing = [&](int i) {
-    const auto& pg = c->pages[db.ids[i]];
+    const auto& pg = c->pages[ids[i]];
     return !pg.empty() && c->sharers[pg[0]] > 0;
   };
   bool any = false;
   for (int i = 0; i < db.n && !any; ++i) any = sharing(i);
   if (any && db.window == 0 && most > 1 && !capturing(s)) {
     for (int i = 0; i < db.n; ++i) {
-      if (db.shared[i] >= 0 || !sharing(i)) continue;
-      const auto& pi = c->pages[db.ids[i]];
+      if (of[i] >= 0 || !sharing(i)) continue;
+      const auto& pi = c->pages[ids[i]];
       std::pair<int32_t, int32_t> found[kMaxBatch];  // blocks in common, entry
       int n = 0;
       for (int j = i + 1; j < db.n; ++j) {
-        const auto& pj = c->pages[db.ids[j]];
-        if (db.shared[j] >= 0 || pj.empty() || pj[0] != pi[0]) continue;
+        const auto& pj = c->pages[ids[j]];
+        if (of[j] >= 0 || pj.empty() || pj[0] != pi[0]) continue;
         int lo = 1, hi = (int)std::min(pi.size(), pj.size());  // the first lo are common, none from hi on
         while (lo < hi) {
           const int mid = (lo + hi) / 2;
@@ -138,20 +140,19 @@ void dense_jobs(const bsattn_cache* c, DenseBatch& db, hipStream_t s) {
       const int units = found[best - 1].first * per_block;
       db.order[placed] = (int16_t)i;
       for (int k = 0; k < best; ++k) db.order[placed + 1 + k] = (int16_t)found[k].second;
-      for (int k = 0; k <= best; ++k) db.shared[db.order[placed + k]] = (int16_t)db.jobs;
-      add_job(db, placed, best + 1).units = units;
+      for (int k = 0; k <= best; ++k) of[db.order[placed + k]] = (int16_t)db.jobs;
+      add_job(db, ids, placed, best + 1).units = units;
       placed += best + 1;
     }
   }
   for (int i = 0; i < db.n; ++i) {
     db.order[placed] = (int16_t)i;
-    db.alone[i] = (int16_t)db.jobs;
-    DenseJob& job = add_job(db, placed++, 1);
-    job.shares = db.shared[i] >= 0;
-    job.from = job.shares ? db.job[db.shared[i]].units : 0;
+    DenseJob& job = add_job(db, ids, placed++, 1);
+    job.of = of[i];
+    job.from = of[i] >= 0 ? db.job[of[i]].units : 0;
     // (the pages may hold fewer tokens than fit them; a window can begin and
     // end inside a unit)
-    int64_t units = (int64_t)c->pages[db.ids[i]].size() * per_block - job.from;
+    int64_t units = (int64_t)c->pages[ids[i]].size() * per_block - job.from;
     if (db.window > 0) units = std::min<int64_t>(units, ((int64_t)db.window + 62) / 32);
     job.units = (int)units;
   }
@@ -194,9 +195,9 @@ int bsattn_decode_dense(bsattn_cache* c, const void* q, const int32_t* seq_ids, 
     db.window = window;
     db.sl2 = scale * 1.4426950408889634f;
     db.sinks = sinks;
-    for (int i = 0; i < db.n; ++i) db.ids[i] = seqs[i0 + i];
-    dense_jobs(c, db, s);
-    int rows = 0;
+    const int32_t* ids = seqs.data() + i0;
+    dense_jobs(c, ids, db, s);
+    int64_t rows = 0;
     const int parts = dense_plan(g, db, &rows);
     const uint16_t* qq = (const uint16_t*)q + (size_t)i0 * g.hq * kHeadDim;
     uint16_t* oo = (uint16_t*)out + (size_t)i0 * g.hq * kHeadDim;
@@ -209,14 +210,12 @@ int bsattn_decode_dense(bsattn_cache* c, const void* q, const int32_t* seq_ids, 
       whole.jobs = 0;
       for (int i = 0; i < db.n; ++i) {
         whole.order[i] = (int16_t)i;
-        whole.alone[i] = (int16_t)i;
-        whole.shared[i] = -1;
-        add_job(whole, i, 1).part0 = i;
+        add_job(whole, ids, i, 1).part0 = i;
       }
       return launch_dense(g, whole, db.n, qq, oo, nullptr, nullptr, s, prof);
     };
     const hipError_t e = rows == 0 ? launch_dense(g, db, parts, qq, oo, nullptr, nullptr, s, prof)
-                                   : with_partials(c, (int64_t)rows * g.hq, s, run);
+                                   : with_partials(c, rows, s, run);
     prof_collect(c, prof);
     if (e != hipSuccess) return hip_fail(e, "dense decode launch");
   }
@@ -293,7 +292,8 @@ int bsattn_fork(bsattn_cache* c, const int32_t* src_ids, const int32_t* dst_ids,
   }
   c->free_pages.resize(c->free_pages.size() - tails.size());
   for (int i = 0; i < n; ++i) {
-    for (int b = 0; b < tokens[i] / tb; ++b) ++c->sharers[rows[i][b]];
+    int32_t* sharers = c->sharers.data();
+    for (const int32_t *p = rows[i].data(), *end = p + tokens[i] / tb; p != end; ++p) ++sharers[*p];
     c->pages[dst[i]].swap(rows[i]);
     c->len[dst[i]] = tokens[i];
   }

@@ -13,33 +13,33 @@ bsattn::DenseBatch last_dense;
 static void check_jobs(const bsattn::DenseBatch& db) {
   stub::last_dense = db;
   CHECK(db.n >= 1 && db.n <= bsattn::kMaxBatch && db.jobs >= db.n && db.jobs <= bsattn::kMaxDenseJobs);
-  std::vector<int> own(db.n, 0), with(db.n, 0);
+  std::vector<int> own(db.n, 0), with(db.n, 0), of(db.n, -1);
   for (int j = 0; j < db.jobs; ++j) {
     const bsattn::DenseJob& job = db.job[j];
     CHECK(job.count >= 1 && job.count <= 16 && job.first >= 0 && job.first + job.count <= 2 * bsattn::kMaxBatch);
     CHECK(job.units >= 0);
-    CHECK(job.entry == db.order[job.first] && job.seq == db.ids[job.entry]);
+    CHECK(job.entry == db.order[job.first]);
     for (int k = 0; k < job.count; ++k) {
       const int e = db.order[job.first + k];
       CHECK(e >= 0 && e < db.n);
       if (job.count == 1) {
         ++own[e];
-        CHECK(db.alone[e] == j && job.shares == (db.shared[e] >= 0));
-        CHECK(job.from == (job.shares ? db.job[db.shared[e]].units : 0));
+        CHECK(job.of == of[e] && job.from == (of[e] >= 0 ? db.job[of[e]].units : 0));
       } else {
         ++with[e];
-        CHECK(db.shared[e] == j && db.window == 0);
+        of[e] = j;
+        CHECK(db.window == 0 && job.of < 0);
       }
     }
   }
-  for (int e = 0; e < db.n; ++e) CHECK(own[e] == 1 && with[e] == (db.shared[e] >= 0));
+  for (int e = 0; e < db.n; ++e) CHECK(own[e] == 1 && with[e] <= 1);
 }
 
 namespace bsattn {
 using stub::run;
 hipError_t launch_rotate(const Geometry& g, RotateBatch, int, hipStream_t, Timing*) { return run(g, nullptr); }
 // (a job of n entries: `splits` parts)
-int dense_plan(const Geometry&, DenseBatch& db, int* rows) {
+int dense_plan(const Geometry& g, DenseBatch& db, int64_t* rows) {
   db.cu = 4;
   int parts = 0, blocks = 0;
   for (int j = 0; j < db.jobs; ++j) {
@@ -48,7 +48,7 @@ int dense_plan(const Geometry&, DenseBatch& db, int* rows) {
     parts += stub::splits;
     blocks += stub::splits * db.job[j].count;
   }
-  *rows = parts == db.n ? 0 : blocks;
+  *rows = parts == db.n ? 0 : (int64_t)blocks * g.hq;
   return parts;
 }
 hipError_t launch_dense(const Geometry& g, const DenseBatch& db, int parts, const void*, void*, float* ws,

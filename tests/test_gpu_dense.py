@@ -285,6 +285,36 @@ def test_steps_and_capture(gpu):
     _check(other, _reference(c, q), "bf16")
 
 
+@pytest.mark.parametrize("dtype,bits", KINDS)
+@pytest.mark.parametrize("Hq,Hkv", [(8, 4), (16, 1)])
+def test_replayed_at_other_lengths(gpu, dtype, bits, Hq, Hkv):
+    """A graph that was captured over short sequences replays over ones that
+    have grown many times over since, in pages taken later, and shrunk."""
+    import torch
+    log(f"[replay] {dtype} bits={bits} {Hq}/{Hkv}")
+    c = _cache([9000] * 4, Hq, Hkv, 64, dtype, bits)
+    _fill(gpu, c, [200, 0, 1, 640], 3, salient=True)
+    q = _randn(gpu, 4, (4, Hq, 1, D), dtype)
+    c.decodeDense(q, SCALE)
+    torch.cuda.synchronize()
+    graphs = []
+    for window in (None, 500):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = c.decodeDense(q, SCALE, window=window)
+        graphs.append((graph, out, window))
+    for step, more in enumerate((0, 70, 2000, 6000, -7500, 300)):
+        if more > 0:
+            n = 4 - step % 2
+            k, v = (_randn(gpu, 50 + 2 * step + i, (n, Hkv, more, D), dtype) for i in range(2))
+            c.append(k, v, seq_ids=list(range(n)))
+        elif more < 0:
+            c.trim(-more, seq_ids=[0, 1, 2, 3])
+        for graph, out, window in graphs:
+            graph.replay()
+            _check(out, _reference(c, q, window=window), dtype, f"step {step} window {window}")
+
+
 def test_streams_rows_and_repeats(gpu):
     """Many rows; other streams at once on their own caches; the same bits
     every time."""
