@@ -52,9 +52,9 @@ constexpr float kTop = 14.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // What the 16 columns hold: a group of up to 8 heads of one entry; a group of
-// 16; the queries of a shared job's members, whose blocks other workgroups of
-// the XCD read, too.
-enum Columns { kNarrow, kGroup16, kShared };
+// 16, or the queries of a shared job's members; the latter where another job of
+// the launch reads the same blocks.
+enum Columns { kNarrow, kWide, kAgain };
 
 // Ahead of the partials in the workspace: where each entry's lie, written by the
 // first part of its own job.  (With the batch among its arguments the join's
@@ -207,11 +207,12 @@ struct DensePages {
 
 // 16 bytes at a uniform address plus a lane's offset: read once, unless another
 // shared job reads them, too (8 branches of 8191 bf16 tokens, two jobs: 14.1 us
-// as if read once, 12.6 so; read once, 4 x 262k int8 in groups of 16: 179 and
-// 201)
+// as if read once, 12.2 so; four prompts of 16001 int8 tokens, one job each,
+// with fork and append 53 us read once and 61 so, out of different caches in
+// turn)
 template <Columns C>
 __device__ __forceinline__ u32x4 stream16(const uint8_t* base, uint32_t at) {
-  if constexpr (C == kShared) return *(const u32x4*)(base + at);
+  if constexpr (C == kAgain) return *(const u32x4*)(base + at);
   return __builtin_nontemporal_load((const u32x4*)(base + at));
 }
 // a lane's offset, kept in 32 bits up to here (the load then adds it to the
@@ -257,7 +258,7 @@ __device__ __forceinline__ void dense_finish(const Geometry& geo, const DenseBat
       L += f * s_l[v][col];
       a += f * s_o[v][col][d];
     }
-    const int member = C == kShared ? col / G : 0, hq = h * G + col - member * G;
+    const int member = C != kNarrow ? col / G : 0, hq = h * G + col - member * G;
     if (w.rows < 0) {
       if (db.sinks && w.r.len > 0) {
         const float sk = db.sinks[hq] * kLog2e, top = fmaxf(M, sk);
@@ -283,7 +284,7 @@ __device__ __forceinline__ const uint16_t* dense_query(const Geometry& geo, cons
                                                        const uint16_t* __restrict__ q) {
   const int n = threadIdx.x & 15, G = geo.group;
   int bi = w.entry;
-  if constexpr (C == kShared) {
+  if constexpr (C != kNarrow) {
     const int member = n / G;
     if (member > 0 && member < w.count) bi = db.order[w.first + member];
   }
@@ -790,10 +791,9 @@ hipError_t launch_dense(const Geometry& g, const DenseBatch& db, int parts, cons
   const dim3 grid(parts, g.hkv);
   const uint16_t* qq = (const uint16_t*)q;
   uint16_t* oo = (uint16_t*)out;
-  bool shared = false;
-  for (int j = 0; j < db.jobs; ++j) shared = shared || db.job[j].count > 1;
-  if (shared) dense_dispatch<kShared>(g, db, grid, qq, oo, ws, s, prof);
-  else if (g.group > 8) dense_dispatch<kGroup16>(g, db, grid, qq, oo, ws, s, prof);
+  const bool wide = g.group > 8 || db.job[0].count > 1;  // (shared jobs come first)
+  if (db.again) dense_dispatch<kAgain>(g, db, grid, qq, oo, ws, s, prof);
+  else if (wide) dense_dispatch<kWide>(g, db, grid, qq, oo, ws, s, prof);
   else dense_dispatch<kNarrow>(g, db, grid, qq, oo, ws, s, prof);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || !ws) return e;

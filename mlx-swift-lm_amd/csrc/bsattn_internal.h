@@ -261,9 +261,9 @@ struct RotateBatch {
   const int32_t* pos;
   int32_t heads[2];
   int32_t L, b0, dims, interleaved;
-  // set by launch_rotate: heads per workgroup, log2 of the tokens per
-  // workgroup and of the pairs (rounded up)
-  int32_t share, tsh, hsh;
+  // set by launch_rotate: heads per workgroup, workgroups of x[0]'s heads, log2
+  // of the tokens per workgroup and of the pairs (rounded up)
+  int32_t share, shares0, tsh, hsh;
   float m, eps, woff;
   int32_t ids[kMaxBatch];
 };
@@ -290,6 +290,7 @@ struct DenseJob {
 struct DenseBatch {
   int32_t n, jobs, cu, window;  // window: the last tokens seen (0: all)
   float sl2;
+  int32_t again;                // whether two shared jobs read the same blocks
   const float* sinks;           // [hq] logits of the heads, or null
   int16_t order[2 * kMaxBatch];
   DenseJob job[kMaxDenseJobs];

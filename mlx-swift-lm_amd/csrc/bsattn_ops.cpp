@@ -141,6 +141,7 @@ void dense_jobs(const bsattn_cache* c, const int32_t* ids, DenseBatch& db, hipSt
       db.order[placed] = (int16_t)i;
       for (int k = 0; k < best; ++k) db.order[placed + 1 + k] = (int16_t)found[k].second;
       for (int k = 0; k <= best; ++k) of[db.order[placed + k]] = (int16_t)db.jobs;
+      for (int j = 0; j < db.jobs; ++j) db.again |= c->pages[db.job[j].seq][0] == pi[0];
       add_job(db, ids, placed, best + 1).units = units;
       placed += best + 1;
     }
