@@ -231,7 +231,9 @@ int bsattn_prefill(bsattn_cache* cache, const void* q, const int32_t* seq_ids,
  * workspace that bsattn_prefill describes; when none can be had the call runs
  * unsplit: slower, and rounded differently.  Blocks that sequences of the call
  * share (bsattn_fork) are read once for several of them, with no window and
- * outside a capture: then, too, a result may be rounded differently. */
+ * outside a capture: then, too, a result may be rounded differently.  A
+ * captured call holds for any later lengths (its launches keep their size).
+ * Where an attended value is infinite, that dim is infinite or NaN. */
 int bsattn_decode_dense(bsattn_cache* cache, const void* q, const int32_t* seq_ids,
                         int32_t n_seqs, int32_t window, const float* sinks,
                         float scale, void* out, void* stream);
@@ -269,8 +271,8 @@ int bsattn_rotate(bsattn_cache* cache, const bsattn_rope* rope, const void* x,
  * one pass: y = x * rsqrt(mean(x^2) + eps) * (weight_offset + weight), rotated
  * as bsattn_rotate does, in fp32 and rounded once.  q / q_out
  * [n_seqs, Hq, n_tokens, D], k / k_out [n_seqs, Hkv, n_tokens, D], weights
- * [D] in the cache's dtype (both null: no norm, the positions alone).  Strides, positions and aliasing as in
- * bsattn_rotate: q and k may be views into one fused projection, the outputs
+ * [D] in the cache's dtype (both null: no norm, the positions alone).  Strides,
+ * positions and aliasing as in bsattn_rotate: q and k may be views into one fused projection, the outputs
  * are what bsattn_append and the decodes take.  Replaces the qNorm / kNorm and
  * rope calls ahead of attentionWithCacheUpdate. */
 int bsattn_norm_rotate(bsattn_cache* cache, const bsattn_rope* rope, const void* q,

@@ -24,7 +24,8 @@ class RoPE:
     """Rotary positions of the first `dims` dims of each head: pair i turns by
     `scale * base^(-2i / dims)` radians per position, or by theta[i];
     traditional: pairs are neighbours (2i, 2i + 1), otherwise (i, i + dims / 2);
-    factor multiplies the rotated dims."""
+    factor multiplies the rotated dims.  Keep the object while calls or graphs
+    that use it are pending."""
 
     def __init__(self, dims: int, traditional: bool = False, base: float = 10000.0, scale: float = 1.0, *,
                  theta: Optional[Sequence[float]] = None, factor: float = 1.0, device: int | torch.device = 0):

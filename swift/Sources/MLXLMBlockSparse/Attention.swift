@@ -16,7 +16,8 @@ extension BlockSparseKVCache: AttendingKVCache {
     /// queries [B, Hq, L, D], keys / values [B, Hkv, L, D].  L = 1 is one
     /// decode step (mask .none, as BaseKVCache.makeMask gives for n = 1);
     /// a longer pass takes the causal mask and runs as a speculative-verify
-    /// pass up to blockSparseMaxQueries tokens, else as a prefill chunk.
+    /// pass up to blockSparseMaxQueries tokens, else as a prefill chunk; a
+    /// cache that attends densely takes the dense form of both.
     public func updateAndAttend(
         queries: MLXArray, keys: MLXArray, values: MLXArray, scale: Float,
         mask: MLXFast.ScaledDotProductAttentionMaskMode
@@ -26,13 +27,17 @@ extension BlockSparseKVCache: AttendingKVCache {
             guard case .none = mask else {
                 fatalError("decode (L == 1) takes no mask (BaseKVCache.makeMask returns .none)")
             }
+            if attendsDensely {
+                append(keys: keys, values: values)
+                return decodeDense(queries: queries, scale: scale)
+            }
             return appendDecode(keys: keys, values: values, queries: queries, scale: scale)
         }
         guard case .causal = mask else {
             fatalError("a multi-token pass over a BlockSparseKVCache takes the causal mask")
         }
         append(keys: keys, values: values)
-        if L <= blockSparseMaxQueries {
+        if L <= blockSparseMaxQueries && !attendsDensely {
             return decodeMulti(queries: queries, scale: scale)
         }
         return prefill(queries: queries, scale: scale)

@@ -22,6 +22,10 @@ public class BlockSparseKVCache: KVCache {
     public let desc: bsattn_desc
     public let device: BlockSparseDevice
 
+    /// Whether attentionWithCacheUpdate attends to every token instead of the
+    /// selected blocks, for layers that take no selection.
+    public var attendsDensely = false
+
     /// The cache a library handle belongs to; `copy()` makes its subclass's
     /// instances through this initializer.
     public required init(adopting handle: OpaquePointer, desc: bsattn_desc, device: BlockSparseDevice) {
@@ -213,7 +217,9 @@ public class BlockSparseKVCache: KVCache {
     public func copy() -> any KVCache {
         var h: OpaquePointer? = nil
         bsCheck(bsattn_copy(handle, &h, stream), "bsattn_copy")
-        return type(of: self).init(adopting: h!, desc: desc, device: device)
+        let c = type(of: self).init(adopting: h!, desc: desc, device: device)
+        c.attendsDensely = attendsDensely
+        return c
     }
 
     // MARK: block-sparse attention

@@ -95,7 +95,8 @@ def test_rotate(gpu, dtype, R, interleaved, B, H, L):
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("Hq,Hkv", [(32, 8), (64, 4), (2, 1), (16, 16)])
 @pytest.mark.parametrize("R,interleaved,offset,L", [(128, False, 0.0, 1), (128, False, 1.0, 19), (128, True, 0.0, 5),
-                                                    (64, False, 0.0, 16), (96, True, 1.0, 3)])
+                                                    (64, False, 0.0, 16), (96, True, 1.0, 3), (96, False, 0.0, 18),
+                                                    (20, False, 1.0, 7), (126, False, 0.0, 3), (2, True, 1.0, 4)])
 def test_norm_rotate(gpu, dtype, Hq, Hkv, R, interleaved, offset, L):
     import torch
     import bsattn
@@ -226,6 +227,52 @@ def test_many_rows_and_streams(gpu):
     for i in (0, 63, 64, 149):
         one = bsattn.applyRotaryPosition(rope, q[i:i + 1].contiguous(), c, positions=pos[i:i + 1].contiguous())
         assert torch.equal(whole[i:i + 1], one)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("R,interleaved", [(64, False), (64, True), (20, False), (20, True), (96, False)])
+def test_dims_that_stay(gpu, dtype, R, interleaved):
+    """Dims past the rotated ones come through bit for bit, infinities, the
+    smallest and largest numbers and -0 among them, and touch no other dim."""
+    import torch
+    import bsattn
+    c = _cache(gpu, dtype)
+    rope = bsattn.RoPE(R, interleaved, factor=1.25)
+    x = _randn(gpu, R, (2, 8, 19, 128), dtype)
+    plain = bsattn.applyRotaryPosition(rope, x, c)
+    f = torch.finfo(_dt(dtype))
+    odd = torch.tensor([math.inf, -math.inf, f.max, f.min, f.tiny, -0.0, 2.0 ** (-24 if dtype == "f16" else -133)],
+                       device=gpu).to(_dt(dtype))
+    x[..., R:R + 7] = odd
+    x[..., 121:] = odd
+    got = bsattn.applyRotaryPosition(rope, x, c)
+    assert torch.equal(got[..., :R], plain[..., :R])
+    assert torch.equal(got[..., R:].view(torch.int16), x[..., R:].view(torch.int16))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("R,interleaved", [(128, False), (64, False), (128, True), (20, False)])
+def test_large_inputs(gpu, dtype, R, interleaved):
+    """More than the caches hold at once: what the rows give on their own."""
+    import torch
+    import bsattn
+    log(f"[large] {dtype} R={R} interleaved={interleaved}")
+    B, L, Hq, Hkv = 9, 1301, 32, 4
+    c = _cache(gpu, dtype, Hq, Hkv, rows=B)
+    rope = bsattn.RoPE(R, interleaved)
+    g = torch.Generator(device=gpu).manual_seed(R)
+    p = torch.randn((B, L, Hq + Hkv, 128), generator=g, device=gpu).to(_dt(dtype))
+    q, k = p.transpose(1, 2)[:, :Hq], p.transpose(1, 2)[:, Hq:]
+    assert p.numel() * 2 > 96 << 20
+    w = [_randn(gpu, 5 + i, (128,), dtype) for i in range(2)]
+    pos = torch.arange(B * L, dtype=torch.int32, device=gpu).reshape(B, L)
+    alone = bsattn.applyRotaryPosition(rope, p.transpose(1, 2), c, positions=pos)
+    whole = c.normRotate(q, k, w[0], w[1], 1e-6, rope, positions=pos)
+    for b in (0, 4, 8):
+        one = pos[b:b + 1].contiguous()
+        assert torch.equal(alone[b:b + 1], bsattn.applyRotaryPosition(rope, p[b:b + 1].transpose(1, 2), c, positions=one))
+        part = c.normRotate(q[b:b + 1], k[b:b + 1], w[0], w[1], 1e-6, rope, positions=one)
+        assert torch.equal(whole[0][b:b + 1], part[0]) and torch.equal(whole[1][b:b + 1], part[1])
 
 
 def test_in_place(gpu):
