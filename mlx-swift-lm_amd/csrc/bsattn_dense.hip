@@ -651,7 +651,7 @@ __global__ __launch_bounds__(256, 2) void k_dense_q(Geometry geo, DenseBatch db,
 // rows of 32 lanes with four dims each take the parts in turn, four of them
 // asked for at once, and are summed in order at the end.  (Joined by the
 // workgroup that arrives last, with device-scope partials, one sequence of 4k
-// tokens takes 11.5 us, against 5.1 and 4.2 for the two launches.)  grid (Hq, n)
+// tokens takes 11.5 us, against 5.1 and 3.3 for the two launches.)  grid (Hq, n)
 constexpr int kRows = 8, kRound = 4;
 template <int DT>
 __global__ __launch_bounds__(32 * kRows) void k_dense_join(const float* __restrict__ ws,

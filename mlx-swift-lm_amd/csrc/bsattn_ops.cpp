@@ -89,9 +89,9 @@ DenseJob& add_job(DenseBatch& db, const int32_t* ids, int first, int count) {
 }
 
 // Units of 32 tokens that a shared prefix must have to be read apart from its
-// sequences' rest (again and again over the same cache, bf16, 8 kv heads, call
-// to call): 8 branches of 1100 tokens take 12.9 us with it and 15.1 without, 32
-// of 8191 35.5 and 78.9, but 32 of 600 17.9 and 15.7.
+// sequences' rest.  Over one cache again and again (bf16, 8 kv heads), 8
+// branches of 1100 tokens take 11.7 us with it and 14.2 without, 32 of 8191 26
+// and 79, but 32 of 600 16.9 and 14.1.
 constexpr int kSharedUnits = 32;
 
 // Jobs of a launch of the sequences ids[0, n): the full blocks that entries

@@ -171,6 +171,70 @@ def test_many_and_partial(gpu):
 
 
 @pytest.mark.parametrize("dtype,bits", KINDS)
+def test_pages_far_apart(gpu, dtype, bits):
+    """Pages all over a pool of more than 4 GiB: what a small pool gives."""
+    import torch
+    log(f"[far pages] {dtype} bits={bits}")
+    near = _cache([3000] * 10, 32, 8, 64, dtype, bits)
+    page = 64 * 8 * {0: 512, 4: 144, 8: 272}[bits]
+    far = _cache([3000] * 10, 32, 8, 64, dtype, bits, num_pages=(5 << 30) // page)
+    far.shuffleFreePages(3)
+    outs = []
+    for c in (near, far):
+        k, v = (_randn(gpu, i, (1, 8, 2500, D), dtype) for i in (1, 2))
+        c.append(k, v, seq_ids=[0])
+        c.fork([0] * 8, list(range(1, 9)))
+        k, v = (_randn(gpu, i, (9, 8, 1, D), dtype) for i in (3, 4))
+        c.append(k, v)
+        c.trim(40, seq_ids=[3])
+        q = _randn(gpu, 5, (9, 32, 1, D), dtype)
+        outs.append((c.decodeDense(q, SCALE), c.decodeDense(q, SCALE, window=1000), c.decode(q, SCALE)))
+    assert max(p for s in range(9) for p in far.seqPages(s)) * page > 1 << 32
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+def test_calls_at_once(gpu):
+    """Two threads, each with its caches and stream: what one after the other
+    gives."""
+    import threading
+    import torch
+    jobs = []
+    for i in range(4):
+        c = _cache([9000] * 4, 32, 8, 64, "bf16")
+        _fill(gpu, c, [8191, 0, 0, 0], 60 + i)
+        q = _randn(gpu, 80 + i, (4, 32, 1, D), "bf16")
+        jobs.append((c, q))
+    torch.cuda.synchronize()
+
+    def work(c, q, out):
+        for _ in range(5):
+            c.fork([0, 0, 0], [1, 2, 3], [8191, 5000, 63])
+            out.append(c.decodeDense(q, SCALE))
+            c.reset([1, 2, 3])
+
+    want = []
+    for c, q in jobs:
+        work(c, q, got := [])
+        want.append(got[0])
+        assert all(torch.equal(g, got[0]) for g in got)
+    torch.cuda.synchronize()
+    results = [[] for _ in jobs]
+
+    def thread(i):
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            work(*jobs[i], results[i])
+        st.synchronize()
+
+    threads = [threading.Thread(target=thread, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(len(r) == 5 and all(torch.equal(g, w) for g in r) for r, w in zip(results, want))
+
+
+@pytest.mark.parametrize("dtype,bits", KINDS)
 @pytest.mark.parametrize("Hq,Hkv", [(4, 4), (8, 4), (16, 4), (16, 2), (16, 1)])
 def test_shared_prefixes(gpu, dtype, bits, Hq, Hkv):
     """Dense decode of sequences that share their beginnings: branches of two

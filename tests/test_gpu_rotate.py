@@ -275,6 +275,27 @@ def test_large_inputs(gpu, dtype, R, interleaved):
         assert torch.equal(whole[0][b:b + 1], part[0]) and torch.equal(whole[1][b:b + 1], part[1])
 
 
+def test_offsets_past_32_bits(gpu):
+    """A tensor of more than 2^31 elements, whole and through its strides."""
+    import torch
+    import bsattn
+    log("[rotate] 2^31 elements")
+    H, L = 64, 270001
+    c = _cache(gpu, "bf16")
+    rope = bsattn.RoPE(128)
+    x = torch.zeros((1, H, L, 128), dtype=torch.bfloat16, device=gpu)
+    assert x.numel() > 2 ** 31
+    tail = _randn(gpu, 1, (1, H, 21, 128), "bf16")
+    x[:, :, -21:] = tail
+    pos = torch.arange(L, dtype=torch.int32, device=gpu)[None]
+    want = bsattn.applyRotaryPosition(rope, tail, c, positions=pos[:, -21:].contiguous())
+    got = bsattn.applyRotaryPosition(rope, x, c, positions=pos)
+    assert torch.equal(got[:, :, -21:], want) and not got[:, :, :-21].any()
+    view = x.view(1, L, H, 128).transpose(1, 2)  # the same memory, tokens first
+    assert torch.equal(bsattn.applyRotaryPosition(rope, view[:, :, -3:], c, positions=pos[:, -3:].contiguous()),
+                       bsattn.applyRotaryPosition(rope, view[:, :, -3:].contiguous(), c, positions=pos[:, -3:].contiguous()))
+
+
 def test_in_place(gpu):
     import torch
     import bsattn
