@@ -99,20 +99,27 @@ constexpr int kSharedUnits = 32;
 // block is shared only with all those before it (forks share from the beginning, trims take
 // from the end), so the longest common prefix is found by bisection.  Not with
 // a window, and not in a capture: its replays may find other sequences.
-void dense_jobs(const bsattn_cache* c, const int32_t* ids, DenseBatch& db, hipStream_t s) {
+//
+// Shared jobs fill all 16 columns, and then every job of the launch does: for
+// affine caches a unit takes about 5 / 4 of the time of one with half of them
+// (2 branches of 2000 tokens beside 4 sequences of 60k int4 tokens 74 us with
+// the branches together and 60 apart; int8, 40k, 69 and 58; bf16, 16k, 47 both).
+void dense_jobs(const bsattn_cache* c, const int32_t* ids, DenseBatch& db, hipStream_t s, bool share = true) {
   const Geometry& g = c->geo;
   const int per_block = g.tb / 32, most = 16 / g.group;
   int16_t of[kMaxBatch];  // an entry's shared job, or -1
   std::fill(of, of + kMaxBatch, (int16_t)-1);
   db.jobs = 0;
+  db.again = 0;
   int placed = 0;
+  int64_t saved = 0, left = 0;  // units read fewer times, and read
   auto sharing = [&](int i) {
     const auto& pg = c->pages[ids[i]];
     return !pg.empty() && c->sharers[pg[0]] > 0;
   };
   bool any = false;
   for (int i = 0; i < db.n && !any; ++i) any = sharing(i);
-  if (any && db.window == 0 && most > 1 && !capturing(s)) {
+  if (share && any && db.window == 0 && most > 1 && !capturing(s)) {
     for (int i = 0; i < db.n; ++i) {
       if (of[i] >= 0 || !sharing(i)) continue;
       const auto& pi = c->pages[ids[i]];
@@ -143,6 +150,8 @@ void dense_jobs(const bsattn_cache* c, const int32_t* ids, DenseBatch& db, hipSt
       for (int k = 0; k <= best; ++k) of[db.order[placed + k]] = (int16_t)db.jobs;
       for (int j = 0; j < db.jobs; ++j) db.again |= c->pages[db.job[j].seq][0] == pi[0];
       add_job(db, ids, placed, best + 1).units = units;
+      left += units;
+      saved += (int64_t)best * units;
       placed += best + 1;
     }
   }
@@ -156,7 +165,9 @@ void dense_jobs(const bsattn_cache* c, const int32_t* ids, DenseBatch& db, hipSt
     int64_t units = (int64_t)c->pages[ids[i]].size() * per_block - job.from;
     if (db.window > 0) units = std::min<int64_t>(units, ((int64_t)db.window + 62) / 32);
     job.units = (int)units;
+    left += units;
   }
+  if (saved > 0 && g.kv_bits != 0 && 4 * saved < left) dense_jobs(c, ids, db, s, false);
 }
 
 // workspace and event for the parts of a call: the cache's own where they fit

@@ -210,6 +210,28 @@ static void shared_jobs(unsigned seed, int hq, int hkv) {
   const int per_job = std::min(8, 16 / (hq / hkv));
   CHECK(stub::last_dense.jobs == 8 + (per_job > 1 ? 8 / per_job : 0));
   if (per_job > 1) CHECK(stub::last_dense.job[0].count == per_job && stub::last_dense.job[0].units == 40 * d.block_size / 32);
+  // beside a sequence that is many times as long: not worth the other columns
+  // of affine caches
+  for (int bits : {0, 4}) {
+    bsattn_desc b = small_desc(8, 512);
+    b.num_q_heads = hq;
+    b.num_kv_heads = hkv;
+    b.kv_bits = bits;
+    b.group_size = 64;
+    b.num_pages = 500;
+    b.block_size = 64;
+    bsattn_cache* q = nullptr;
+    CHECK(bsattn_cache_create(&b, &q) == BSATTN_OK);
+    const int32_t two[2] = {0, 1}, from[3] = {1, 1, 1}, to[3] = {2, 3, 4}, with[4] = {0, 2, 3, 4};
+    CHECK(bsattn_append(q, kv, kv, &two[0], 1, 400 * 64, nullptr) == BSATTN_OK);
+    CHECK(bsattn_append(q, kv, kv, &two[1], 1, 20 * 64 + 1, nullptr) == BSATTN_OK);
+    CHECK(bsattn_fork(q, from, to, 3, nullptr, nullptr) == BSATTN_OK);
+    CHECK(bsattn_decode_dense(q, kv, to, 3, 0, nullptr, 1.f, kv, nullptr) == BSATTN_OK);
+    CHECK(stub::last_dense.jobs == (per_job > 1 ? 4 : 3));
+    CHECK(bsattn_decode_dense(q, kv, with, 4, 0, nullptr, 1.f, kv, nullptr) == BSATTN_OK);
+    CHECK(stub::last_dense.jobs == (per_job > 1 && bits == 0 ? 5 : 4) && stub::last_dense.again == 0);
+    bsattn_cache_destroy(q);
+  }
   stub::splits = 1;
   bsattn_cache_destroy(c);
 }
