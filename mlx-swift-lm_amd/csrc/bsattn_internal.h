@@ -291,6 +291,7 @@ struct DenseBatch {
   int32_t n, jobs, cu, window;  // window: the last tokens seen (0: all)
   float sl2;
   int32_t again;                // whether two shared jobs read the same blocks
+  int32_t heads_first;          // the grid's order: (kv heads, parts), or (parts, kv heads)
   const float* sinks;           // [hq] logits of the heads, or null
   int16_t order[2 * kMaxBatch];
   DenseJob job[kMaxDenseJobs];

@@ -220,6 +220,7 @@ int bsattn_decode_dense(bsattn_cache* c, const void* q, const int32_t* seq_ids, 
       DenseBatch whole = db;  // (without a workspace: one part an entry)
       whole.cu = INT32_MAX / 32;
       whole.jobs = 0;
+      whole.again = whole.heads_first = 0;
       for (int i = 0; i < db.n; ++i) {
         whole.order[i] = (int16_t)i;
         add_job(whole, ids, i, 1).part0 = i;
