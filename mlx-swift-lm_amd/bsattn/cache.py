@@ -443,30 +443,30 @@ class BlockSparseKVCache:
         sinks: [Hq] float32 logits that join each head's softmax without a
         value.  A sequence without tokens gives zeros."""
         B = self._check_q(queries)
+        window, logits = self._check_window(window), self._check_sinks(sinks)
         out = torch.empty_like(queries)
-        check(self._lib.bsattn_decode_dense(self._h, queries.data_ptr(), i32_array(seq_ids), B,
-                                            self._check_window(window), self._check_sinks(sinks), scale, out.data_ptr(), _stream(self.device)))
+        check(self._lib.bsattn_decode_dense(self._h, queries.data_ptr(), i32_array(seq_ids), B, window, logits, scale,
+                                            out.data_ptr(), _stream(self.device)))
         return out
 
     # -- rotary positions ------------------------------------------------------
-    def _check_strided(self, t: torch.Tensor, name: str, heads: int):
-        """Element strides of t [B, heads, L, D] between sequences, heads and
-        tokens (None: dense); the dims are contiguous and every row 16-byte
-        aligned."""
+    def _check_strided(self, t: torch.Tensor, name: str, heads: Optional[int] = None):
+        """(element strides between sequences, heads and tokens, shape) of
+        t [B, heads, L, D]; no strides where t is dense.  The dims are
+        contiguous and every row 16-byte aligned."""
         shape = t.shape
         if t.dtype is not self.dtype or t.get_device() != self._index:
             raise ValueError(f"{name} must be a {self.dtype} tensor on {self.device}")
-        if len(shape) != 4 or heads < 1 or shape[1] != heads or shape[3] != self._dim or 0 in shape:
+        if len(shape) != 4 or (heads is not None and shape[1] != heads) or shape[3] != self._dim or 0 in shape:
             raise ValueError(f"{name} must be [B, {heads or 'H'}, L, {self._dim}], got {tuple(shape)}")
-        if t.is_contiguous():
-            if t.data_ptr() % 16 == 0:
-                return None
-        else:
+        if t.data_ptr() & 15 == 0:
+            if t.is_contiguous():
+                return None, shape
             # (torch gives a dimension of one element any stride)
             s0, s1, s2, s3 = t.stride()
-            s0, s1, s2 = s0 if shape[0] > 1 else 0, s1 if heads > 1 else 0, s2 if shape[2] > 1 else 0
-            if s3 == 1 and not (s0 | s1 | s2) & 7 and t.data_ptr() % 16 == 0:
-                return _Strides(s0, s1, s2)
+            s0, s1, s2 = s0 if shape[0] > 1 else 0, s1 if shape[1] > 1 else 0, s2 if shape[2] > 1 else 0
+            if s3 == 1 and not (s0 | s1 | s2) & 7:
+                return _Strides(s0, s1, s2), shape
         raise ValueError(f"{name} must have contiguous, 16-byte aligned heads, got strides {t.stride()} at "
                          f"offset {t.storage_offset()}")
 
@@ -483,6 +483,12 @@ class BlockSparseKVCache:
                              f"{positions.dtype} {tuple(positions.shape)}")
         return positions.data_ptr()
 
+    def _check_weight(self, w: torch.Tensor, name: str) -> int:
+        if w.dtype is not self.dtype or w.get_device() != self._index or w.shape != (self._dim,) \
+                or not w.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {self.dtype} tensor ({self._dim},) on {self.device}")
+        return w.data_ptr()
+
     def normRotate(self, queries: torch.Tensor, keys: torch.Tensor, qWeight: Optional[torch.Tensor],
                    kWeight: Optional[torch.Tensor], eps: float, rope, positions: Optional[torch.Tensor] = None,
                    seq_ids: Optional[Sequence[int]] = None, weightOffset: float = 0.0):
@@ -492,28 +498,22 @@ class BlockSparseKVCache:
         the results are dense.  Both weights None: the positions alone.
         positions [B, L] int32; by default each sequence's tokens follow those
         that the cache holds."""
-        qs = self._check_strided(queries, "queries", self._hq)
-        ks = self._check_strided(keys, "keys", self._hkv)
-        B, _, L, _ = queries.shape
-        if keys.shape[0] != B or keys.shape[2] != L:
+        qs, (B, _, L, _) = self._check_strided(queries, "queries", self._hq)
+        ks, (Bk, _, Lk, _) = self._check_strided(keys, "keys", self._hkv)
+        if Bk != B or Lk != L:
             raise ValueError("queries and keys disagree on B or L")
         if (qWeight is None) != (kWeight is None):
             raise ValueError("give both norm weights or neither")
-        for name, w in (("qWeight", qWeight), ("kWeight", kWeight)):
-            if w is None:
-                continue
-            if w.dtype is not self.dtype or w.get_device() != self._index or w.shape != (self._dim,) \
-                    or not w.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous {self.dtype} tensor ({self._dim},) on {self.device}")
+        qw = kw = None
+        if qWeight is not None:
+            qw, kw = self._check_weight(qWeight, "qWeight"), self._check_weight(kWeight, "kWeight")
         self._check_rope(rope)
         pos = self._check_positions(positions, B, L)
         q = torch.empty_like(queries, memory_format=torch.contiguous_format)
         k = torch.empty_like(keys, memory_format=torch.contiguous_format)
         check(self._lib.bsattn_norm_rotate(self._h, rope._ref, queries.data_ptr(), qs, keys.data_ptr(), ks,
-                                           None if qWeight is None else qWeight.data_ptr(),
-                                           None if kWeight is None else kWeight.data_ptr(), eps, weightOffset,
-                                           i32_array(seq_ids), B, L, pos, q.data_ptr(), k.data_ptr(),
-                                           _stream(self.device)))
+                                           qw, kw, eps, weightOffset, i32_array(seq_ids), B, L, pos, q.data_ptr(),
+                                           k.data_ptr(), _stream(self.device)))
         return q, k
 
     # -- kernel timing -------------------------------------------------------

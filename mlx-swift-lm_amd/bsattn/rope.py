@@ -145,9 +145,7 @@ def applyRotaryPosition(rope: RoPE, x: torch.Tensor, cache: BlockSparseKVCache,
     positions rotated in, as a dense tensor.  positions [B, L] int32; by
     default each sequence's tokens follow those that the cache holds (rotate,
     then append)."""
-    heads = x.shape[1] if x.dim() == 4 else 0
-    strides = cache._check_strided(x, "x", heads)
-    B, _, L, _ = x.shape
+    strides, (B, heads, L, _) = cache._check_strided(x, "x")
     cache._check_rope(rope)
     pos = cache._check_positions(positions, B, L)
     out = torch.empty_like(x, memory_format=torch.contiguous_format)
