@@ -738,6 +738,9 @@ int dense_plan(const Geometry& g, DenseBatch& db, int64_t* rows) {
   // 4 x 262k int8 in 16-head groups 179 (185, 190, 199)
   const int64_t want = 2 * (int64_t)std::max(g.cus, 1);
   db.cu = (int)std::min<int64_t>(most, std::max<int64_t>(4, (all * g.hkv + want - 1) / want));
+  // (it ends: jobs of one part each, shared ones padded to 8, fit)
+  static_assert((8 + 1) * kMaxBatch * 128 + kJoinRows <= kPrefillRows && kMaxBatch * 256 + kJoinRows <= kPrefillRows,
+                "up to 128 query heads with shared jobs, 256 without");
   while (true) {
     db.cu = (db.cu + 3) & ~3;
     int64_t parts = 0, blocks = 0;
