@@ -286,6 +286,21 @@ def test_steps_and_capture(gpu):
 
 
 @pytest.mark.parametrize("dtype,bits", KINDS)
+@pytest.mark.parametrize("lens,Hq,Hkv", [([4700] * 9, 32, 16), ([100 + 131 * i for i in range(40)], 16, 8),
+                                         ([700] * 33, 32, 16), ([20000, 3, 900], 8, 8)])
+def test_uneven_batches(gpu, dtype, bits, lens, Hq, Hkv):
+    """Batches whose parts fit a round of workgroups only with rest, fill
+    several, or come one a sequence."""
+    log(f"[uneven] {dtype} bits={bits} {len(lens)} of {min(lens)}..{max(lens)} {Hq}/{Hkv}")
+    c = _cache(lens, Hq, Hkv, 64, dtype, bits)
+    _fill(gpu, c, lens, 17, salient=True)
+    q = _randn(gpu, 6, (len(lens), Hq, 1, D), dtype)
+    _check(c.decodeDense(q, SCALE), _reference(c, q), dtype)
+    some = list(range(len(lens)))[::-1][:7]
+    _check(c.decodeDense(q[some].contiguous(), SCALE, seq_ids=some), _reference(c, q[some], ids=some), dtype)
+
+
+@pytest.mark.parametrize("dtype,bits", KINDS)
 @pytest.mark.parametrize("Hq,Hkv", [(8, 4), (16, 1)])
 def test_replayed_at_other_lengths(gpu, dtype, bits, Hq, Hkv):
     """A graph that was captured over short sequences replays over ones that
