@@ -54,13 +54,15 @@ def attentionWithCacheUpdate(queries: torch.Tensor, keys: torch.Tensor, values: 
         queries, keys = cache.normRotate(queries, keys, qw, kw, eps, rope, weightOffset=offset)
     if L == 1 and not dense:
         return cache.appendDecode(keys, values, queries, scale)
-    if dense:
-        # nothing is appended that could not be attended to
-        cache._check_q(queries, multi=L > 1)
+    # nothing is appended that could not be attended to
+    cache._check_q(queries, multi=L > 1)
+    if queries.shape[0] != keys.shape[0] or L != keys.shape[2]:
+        raise ValueError("keys / values and queries disagree on B or L")
+    if dense and L == 1:
         cache._check_sinks(sinks)
         cache._check_window(window)
-        if queries.shape[0] != keys.shape[0] or L != keys.shape[2]:
-            raise ValueError("keys / values and queries disagree on B or L")
+        if queries.data_ptr() % 16:
+            raise ValueError("queries must be 16-byte aligned")
     cache.append(keys, values)
     if L == 1:
         return cache.decodeDense(queries, scale, window=window, sinks=sinks)
