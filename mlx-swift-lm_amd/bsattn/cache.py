@@ -37,6 +37,16 @@ def _ptr(t: torch.Tensor):
     return t.data_ptr()
 
 
+def _row_ids(seq_ids: Optional[Sequence[int]], rows: int):
+    """The sequences of a call's rows as the library takes them (None: rows
+    0, 1, ...); it reads one for each row."""
+    if seq_ids is None:
+        return None
+    if len(seq_ids) != rows:
+        raise ValueError(f"{len(seq_ids)} sequence ids for {rows} rows")
+    return i32_array(seq_ids)
+
+
 class BlockSparseKVCache:
     """One layer's paged KV cache for up to `max_seqs` sequences."""
 
@@ -172,7 +182,7 @@ class BlockSparseKVCache:
         if keys.shape != values.shape:
             raise ValueError("keys and values shapes differ")
         B, _, L, _ = keys.shape
-        ids = i32_array(seq_ids)
+        ids = _row_ids(seq_ids, B)
         check(lib().bsattn_append(self._h, _ptr(keys), _ptr(values), ids, B, L,
                                   _stream(self.device)))
 
@@ -193,7 +203,8 @@ class BlockSparseKVCache:
         self._check_kv(values, "values")
         if keys.shape != values.shape or keys.shape[2] != 1:
             raise ValueError("keys / values must both be [B, Hkv, 1, D]")
-        check(lib().bsattn_append_step(self._h, _ptr(keys), _ptr(values), i32_array(seq_ids), keys.shape[0],
+        B = keys.shape[0]
+        check(lib().bsattn_append_step(self._h, _ptr(keys), _ptr(values), _row_ids(seq_ids, B), B,
                                        _stream(self.device)))
 
     def sync(self) -> None:
@@ -237,7 +248,7 @@ class BlockSparseKVCache:
                 raise ValueError(f"{name} must be a contiguous {dt} tensor {shape} on {self.device}, "
                                  f"got {t.dtype} {tuple(t.shape)}")
         check(lib().bsattn_append_quantized(self._h, _ptr(kw), _ptr(ks), _ptr(kb), _ptr(vw), _ptr(vs),
-                                            _ptr(vb), i32_array(seq_ids), B, L, _stream(self.device)))
+                                            _ptr(vb), _row_ids(seq_ids, B), B, L, _stream(self.device)))
 
     def exportQuantized(self, seq_ids: Sequence[int]):
         """((kw, ks, kb), (vw, vs, vb)) of the listed sequences, MLX layout."""
@@ -302,7 +313,7 @@ class BlockSparseKVCache:
         B = self._check_q(queries)
         idx = torch.empty((B, self.desc.num_kv_heads, self.nselMax), dtype=torch.int32,
                           device=self.device)
-        check(lib().bsattn_select(self._h, _ptr(queries), i32_array(seq_ids), B, _ptr(idx),
+        check(lib().bsattn_select(self._h, _ptr(queries), _row_ids(seq_ids, B), B, _ptr(idx),
                                   _stream(self.device)))
         return idx
 
@@ -313,7 +324,7 @@ class BlockSparseKVCache:
                 or tuple(idx.shape) != (B, self.desc.num_kv_heads, self.nselMax):
             raise ValueError("idx must be a contiguous int32 [B, Hkv, nselMax] tensor on the cache device")
         out = torch.empty_like(queries)
-        check(lib().bsattn_attend(self._h, _ptr(queries), i32_array(seq_ids), B, _ptr(idx),
+        check(lib().bsattn_attend(self._h, _ptr(queries), _row_ids(seq_ids, B), B, _ptr(idx),
                                   scale, _ptr(out), _stream(self.device)))
         return out
 
@@ -327,7 +338,7 @@ class BlockSparseKVCache:
             if idx_out.dtype != torch.int32 or tuple(idx_out.shape) != (B, self.desc.num_kv_heads, self.nselMax):
                 raise ValueError("idx_out must be int32 [B, Hkv, nselMax]")
             idx_p = _ptr(idx_out)
-        check(lib().bsattn_decode(self._h, _ptr(queries), i32_array(seq_ids), B,
+        check(lib().bsattn_decode(self._h, _ptr(queries), _row_ids(seq_ids, B), B,
                                   scale, _ptr(out), idx_p, _stream(self.device)))
         return out
 
@@ -346,7 +357,7 @@ class BlockSparseKVCache:
             if idx_out.dtype != torch.int32 or tuple(idx_out.shape) != (B, self.desc.num_kv_heads, self.nselMax):
                 raise ValueError("idx_out must be int32 [B, Hkv, nselMax]")
             idx_p = _ptr(idx_out)
-        check(lib().bsattn_decode_noalloc(self._h, _ptr(queries), i32_array(seq_ids), B,
+        check(lib().bsattn_decode_noalloc(self._h, _ptr(queries), _row_ids(seq_ids, B), B,
                                           scale, _ptr(out), idx_p, _stream(self.device)))
         return out
 
@@ -377,7 +388,7 @@ class BlockSparseKVCache:
                 raise ValueError("idx_out must be int32 [B, Hkv, nselMax]")
             idx_p = _ptr(idx_out)
         rc = self._lib.bsattn_append_decode(self._h, keys.data_ptr(), values.data_ptr(), queries.data_ptr(),
-                                            None if seq_ids is None else i32_array(seq_ids), B, scale,
+                                            _row_ids(seq_ids, B), B, scale,
                                             out.data_ptr(), idx_p, _stream(self.device))
         if rc:
             check(rc)
@@ -401,7 +412,7 @@ class BlockSparseKVCache:
                     or tuple(idx_out.shape) != (B, L, self.desc.num_kv_heads, self.nselMax):
                 raise ValueError("idx_out must be a contiguous int32 [B, L, Hkv, nselMax] tensor")
             idx_p = _ptr(idx_out)
-        check(lib().bsattn_decode_multi(self._h, _ptr(queries), i32_array(seq_ids), B, L,
+        check(lib().bsattn_decode_multi(self._h, _ptr(queries), _row_ids(seq_ids, B), B, L,
                                         scale, _ptr(out), idx_p, _stream(self.device)))
         return out
 
@@ -414,7 +425,7 @@ class BlockSparseKVCache:
         mask.  queries / result [B, Hq, L, D] (fp16 on a quantized cache)."""
         B = self._check_q(queries, multi=True)
         out = torch.empty_like(queries)
-        check(lib().bsattn_prefill(self._h, _ptr(queries), i32_array(seq_ids), B, queries.shape[2],
+        check(lib().bsattn_prefill(self._h, _ptr(queries), _row_ids(seq_ids, B), B, queries.shape[2],
                                    scale, _ptr(out), _stream(self.device)))
         return out
 
@@ -445,7 +456,7 @@ class BlockSparseKVCache:
         B = self._check_q(queries)
         window, logits = self._check_window(window), self._check_sinks(sinks)
         out = torch.empty_like(queries)
-        check(self._lib.bsattn_decode_dense(self._h, queries.data_ptr(), i32_array(seq_ids), B, window, logits, scale,
+        check(self._lib.bsattn_decode_dense(self._h, queries.data_ptr(), _row_ids(seq_ids, B), B, window, logits, scale,
                                             out.data_ptr(), _stream(self.device)))
         return out
 
@@ -512,7 +523,7 @@ class BlockSparseKVCache:
         q = torch.empty_like(queries, memory_format=torch.contiguous_format)
         k = torch.empty_like(keys, memory_format=torch.contiguous_format)
         check(self._lib.bsattn_norm_rotate(self._h, rope._ref, queries.data_ptr(), qs, keys.data_ptr(), ks,
-                                           qw, kw, eps, weightOffset, i32_array(seq_ids), B, L, pos, q.data_ptr(),
+                                           qw, kw, eps, weightOffset, _row_ids(seq_ids, B), B, L, pos, q.data_ptr(),
                                            k.data_ptr(), _stream(self.device)))
         return q, k
 

@@ -14,8 +14,8 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from ._lib import check, i32_array
-from .cache import BlockSparseKVCache, _stream
+from ._lib import check
+from .cache import BlockSparseKVCache, _row_ids, _stream
 
 HEAD_DIM = 128
 
@@ -149,7 +149,7 @@ def applyRotaryPosition(rope: RoPE, x: torch.Tensor, cache: BlockSparseKVCache,
     cache._check_rope(rope)
     pos = cache._check_positions(positions, B, L)
     out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    check(cache._lib.bsattn_rotate(cache._h, rope._ref, x.data_ptr(), strides, heads, i32_array(seq_ids), B, L, pos,
+    check(cache._lib.bsattn_rotate(cache._h, rope._ref, x.data_ptr(), strides, heads, _row_ids(seq_ids, B), B, L, pos,
                                    out.data_ptr(), _stream(cache.device)))
     return out
 

@@ -123,7 +123,7 @@ public class BlockSparseKVCache: KVCache {
     public func append(keys: MLXArray, values: MLXArray, seqIds: [Int]? = nil) {
         precondition(keys.shape == values.shape && keys.ndim == 4, "keys / values must both be [B, Hkv, L, D]")
         let (kp, vp) = (device.pointer(keys), device.pointer(values))
-        withSeqIds(seqIds) { ids in
+        withSeqIds(seqIds, rows: keys.dim(0)) { ids in
             bsCheck(bsattn_append(handle, kp, vp, ids, Int32(keys.dim(0)), Int32(keys.dim(2)), stream),
                     "bsattn_append")
         }
@@ -194,7 +194,7 @@ public class BlockSparseKVCache: KVCache {
 
     /// Empties sequences `seqIds` and returns their pages to the pool.
     public func reset(_ seqIds: [Int]) {
-        withSeqIds(seqIds) { ids in
+        withSeqIds(seqIds, rows: seqIds.count) { ids in
             bsCheck(bsattn_reset(handle, ids, Int32(seqIds.count), stream), "bsattn_reset")
         }
     }
@@ -236,7 +236,7 @@ public class BlockSparseKVCache: KVCache {
         checkQueries(queries)
         let idx = device.empty([queries.dim(0), kvHeads, nselMax], dtype: .int32)
         let (qp, ip) = (device.pointer(queries), device.pointer(idx))
-        withSeqIds(seqIds) { ids in
+        withSeqIds(seqIds, rows: queries.dim(0)) { ids in
             bsCheck(bsattn_select(handle, qp, ids, Int32(queries.dim(0)), ip.assumingMemoryBound(to: Int32.self),
                                   stream), "bsattn_select")
         }
@@ -250,7 +250,7 @@ public class BlockSparseKVCache: KVCache {
                      "indices must be int32 [B, Hkv, nselMax]")
         let out = device.empty(queries.shape, dtype: dtype)
         let (qp, ip, op) = (device.pointer(queries), device.pointer(indices), device.pointer(out))
-        withSeqIds(seqIds) { ids in
+        withSeqIds(seqIds, rows: queries.dim(0)) { ids in
             bsCheck(bsattn_attend(handle, qp, ids, Int32(queries.dim(0)), ip.assumingMemoryBound(to: Int32.self),
                                   scale, op, stream), "bsattn_attend")
         }
@@ -263,7 +263,7 @@ public class BlockSparseKVCache: KVCache {
         checkQueries(queries)
         let out = device.empty(queries.shape, dtype: dtype)
         let (qp, op) = (device.pointer(queries), device.pointer(out))
-        withSeqIds(seqIds) { ids in
+        withSeqIds(seqIds, rows: queries.dim(0)) { ids in
             bsCheck(bsattn_decode(handle, qp, ids, Int32(queries.dim(0)), scale, op, nil, stream), "bsattn_decode")
         }
         return out
@@ -281,7 +281,7 @@ public class BlockSparseKVCache: KVCache {
         let out = device.empty(queries.shape, dtype: dtype)
         let (kp, vp, qp, op) = (device.pointer(keys), device.pointer(values), device.pointer(queries),
                                 device.pointer(out))
-        withSeqIds(seqIds) { ids in
+        withSeqIds(seqIds, rows: queries.dim(0)) { ids in
             bsCheck(bsattn_append_decode(handle, kp, vp, qp, ids, Int32(queries.dim(0)), scale, op, nil, stream),
                     "bsattn_append_decode")
         }
@@ -295,7 +295,7 @@ public class BlockSparseKVCache: KVCache {
         checkQueries(queries, multi: true)
         let out = device.empty(queries.shape, dtype: dtype)
         let (qp, op) = (device.pointer(queries), device.pointer(out))
-        withSeqIds(seqIds) { ids in
+        withSeqIds(seqIds, rows: queries.dim(0)) { ids in
             bsCheck(bsattn_decode_multi(handle, qp, ids, Int32(queries.dim(0)), Int32(queries.dim(2)), scale, op,
                                         nil, stream), "bsattn_decode_multi")
         }
@@ -308,7 +308,7 @@ public class BlockSparseKVCache: KVCache {
         checkQueries(queries, multi: true)
         let out = device.empty(queries.shape, dtype: dtype)
         let (qp, op) = (device.pointer(queries), device.pointer(out))
-        withSeqIds(seqIds) { ids in
+        withSeqIds(seqIds, rows: queries.dim(0)) { ids in
             bsCheck(bsattn_prefill(handle, qp, ids, Int32(queries.dim(0)), Int32(queries.dim(2)), scale, op,
                                    stream), "bsattn_prefill")
         }
@@ -327,7 +327,7 @@ public class BlockSparseKVCache: KVCache {
             let shape = [1, kvHeads, seqLen(s), headDim]
             var k = device.empty(shape, dtype: dtype)
             var v = device.empty(shape, dtype: dtype)
-            withSeqIds([s]) { ids in
+            withSeqIds([s], rows: 1) { ids in
                 bsCheck(bsattn_export(handle, ids, 1, device.pointer(k), device.pointer(v), stream), "bsattn_export")
             }
             if dtype != .float16 {
@@ -395,7 +395,7 @@ public final class QuantizedBlockSparseKVCache: BlockSparseKVCache, QuantizedKVC
         precondition(keys.0.shape == ws && values.0.shape == ws && keys.1.shape == ss && kb.shape == ss
                      && values.1.shape == ss && vb.shape == ss, "quantized tuples must be MLX-layout \(ws) / \(ss)")
         let p = [keys.0, keys.1, kb, values.0, values.1, vb].map { device.pointer($0) }
-        withSeqIds(seqIds) { ids in
+        withSeqIds(seqIds, rows: ws[0]) { ids in
             bsCheck(bsattn_append_quantized(handle, p[0].assumingMemoryBound(to: UInt32.self), p[1], p[2],
                                             p[3].assumingMemoryBound(to: UInt32.self), p[4], p[5], ids,
                                             Int32(ws[0]), Int32(ws[2]), stream), "bsattn_append_quantized")

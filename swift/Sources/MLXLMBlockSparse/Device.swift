@@ -38,9 +38,11 @@ func bsCheck(_ rc: Int32, _ what: StaticString) {
     }
 }
 
-/// Calls `body` with a pointer to `ids` as int32, or nil for rows 0..<n.
-func withSeqIds<R>(_ ids: [Int]?, _ body: (UnsafePointer<Int32>?) -> R) -> R {
+/// Calls `body` with a pointer to `ids` as int32, or nil for rows 0..<n.  The
+/// library reads one for each of the call's `rows`.
+func withSeqIds<R>(_ ids: [Int]?, rows: Int, _ body: (UnsafePointer<Int32>?) -> R) -> R {
     guard let ids else { return body(nil) }
+    precondition(ids.count == rows, "\(ids.count) sequence ids for \(rows) rows")
     let ids32 = ids.map { Int32($0) }
     return ids32.withUnsafeBufferPointer { body($0.baseAddress) }
 }

@@ -48,7 +48,7 @@ extension BlockSparseKVCache {
         let out = device.empty(queries.shape, dtype: dtype)
         let (qp, op) = (device.pointer(queries), device.pointer(out))
         let sp = sinks.map { UnsafePointer(device.pointer($0).assumingMemoryBound(to: Float.self)) }
-        withSeqIds(seqIds) { ids in
+        withSeqIds(seqIds, rows: queries.dim(0)) { ids in
             bsCheck(bsattn_decode_dense(handle, qp, ids, Int32(queries.dim(0)), Int32(window ?? 0), sp, scale, op,
                                         stream), "bsattn_decode_dense")
         }
@@ -61,9 +61,9 @@ extension BlockSparseKVCache {
     public func fork(_ src: [Int], to dst: [Int], tokens: [Int]? = nil) {
         precondition(src.count == dst.count && (tokens == nil || tokens!.count == src.count),
                      "src, dst and tokens must have one entry per fork")
-        withSeqIds(src) { from in
-            withSeqIds(dst) { to in
-                withSeqIds(tokens) { n in
+        withSeqIds(src, rows: src.count) { from in
+            withSeqIds(dst, rows: src.count) { to in
+                withSeqIds(tokens, rows: src.count) { n in
                     bsCheck(bsattn_fork(handle, from, to, Int32(src.count), n, stream), "bsattn_fork")
                 }
             }
@@ -80,7 +80,7 @@ extension BlockSparseKVCache {
         let out = device.empty(x.shape, dtype: dtype)
         let (xp, op) = (device.pointer(x), device.pointer(out))
         var angles = rope.angles
-        withSeqIds(seqIds) { ids in
+        withSeqIds(seqIds, rows: x.dim(0)) { ids in
             bsCheck(bsattn_rotate(handle, &angles, xp, nil, Int32(x.dim(1)), ids, Int32(x.dim(0)), Int32(x.dim(2)),
                                   pos, op, stream), "bsattn_rotate")
         }
@@ -105,7 +105,7 @@ extension BlockSparseKVCache {
         let (qp, kp, qo, ko) = (device.pointer(queries), device.pointer(keys), device.pointer(q), device.pointer(k))
         let (qw, kw) = (qWeight.map { device.pointer($0) }, kWeight.map { device.pointer($0) })
         var angles = rope.angles
-        withSeqIds(seqIds) { ids in
+        withSeqIds(seqIds, rows: queries.dim(0)) { ids in
             bsCheck(bsattn_norm_rotate(handle, &angles, qp, nil, kp, nil, qw, kw, eps, weightOffset, ids,
                                        Int32(queries.dim(0)), Int32(queries.dim(2)), pos, qo, ko, stream),
                     "bsattn_norm_rotate")
