@@ -49,6 +49,10 @@ __device__ __forceinline__ u32x4 v_operand(const u32x4* vf, int dt, int s2, uint
   else return byte_to_f16(f[2 * (dt & 1)], f[2 * (dt & 1) + 1]);
 }
 
+// products of the fp16 halves
+__device__ __forceinline__ uint32_t f16x2_mul(uint32_t x, uint32_t y) {
+  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, x) * __builtin_bit_cast(f16x2, y));
+}
 // x * 1/16 on both fp16 halves (exact unless the result is below fp16's
 // normal range)
 __device__ __forceinline__ uint32_t f16x2_unit16(uint32_t x) {

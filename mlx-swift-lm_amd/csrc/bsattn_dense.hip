@@ -500,18 +500,21 @@ __global__ __launch_bounds__(256, 2) void k_dense_q(Geometry geo, DenseBatch db,
   f32x4 o[8];
 #pragma unroll
   for (int dt = 0; dt < 8; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  // P's range: lifted to at most 2^14 as for fp16 caches; a weight also meets
-  // its token's scale, and where one of 2 or more turns up the weights are at
-  // most 1 from there on (65504 times that still fits)
-  float lift = kTop - kSlack;
-  float m = -INFINITY, base = 0.0f, l = 0.0f, ob0 = 0.0f, ob1 = 0.0f;
-  auto rescale = [&](float f) __attribute__((always_inline)) {
-    l *= f;
-    ob0 *= f;
-    ob1 *= f;
-#pragma unroll
-    for (int dt = 0; dt < 8; ++dt) o[dt] *= f;
-  };
+  // P's range: lifted to at most 2^14 as for fp16 caches.  A weight also meets
+  // its token's scale; in units where a product would pass 2^15 the scales of
+  // that half of the dims are lowered by as much, and its sums with them, so
+  // that the other tokens' weights keep their bits (all weights at most 1 from
+  // the first scale of 2 on, whatever its own weight, put them among fp16's
+  // subnormals: outputs were off by 8 half steps of fp16 at their root mean
+  // square where one token in 32 had such a scale and e^-12 of the largest
+  // weight).  Done with the raise
+  // of the reference, behind one branch: 4 x 131k int4 tokens 100.1 us, as before;
+  // with a scale of 2 and more in every unit 141 (118 before).
+  constexpr float kLift = kTop - kSlack;
+  float m = -INFINITY, base = 0.0f, limit = -INFINITY, l = 0.0f, ob0 = 0.0f, ob1 = 0.0f;
+  uint32_t lower = 0x3C003C00u;  // what the scales of dims 0-63 and 64-127 are multiplied by (fp16)
+  // 1 / x of a power of two
+  auto inverse = [](float x) { return __uint_as_float(0x7F000000u - __float_as_uint(x)); };
 
   // EDGE: some of the unit's tokens are not seen.  MORE: the wave has another
   // unit, which is asked for (without a branch: behind one the compiler must
@@ -566,28 +569,50 @@ __global__ __launch_bounds__(256, 2) void k_dense_q(Geometry geo, DenseBatch db,
         }
       }
     }
-    uint32_t scales = 0;
-#pragma unroll
-    for (int i = 0; i < NT; ++i) scales |= sb[i][2];
-    if (lift > 0.0f && __any((scales & 0x40004000u) != 0)) {  // exponents of 2 and more
-      lift -= kTop;
-      base += kTop;
-      rescale(__builtin_amdgcn_exp2f(-kTop));
-#pragma unroll
-      for (int i = 0; i < NT; ++i) pv[i] -= kTop;
-    }
     float mx = pv[0];
+    uint32_t scales = sb[0][2];
 #pragma unroll
-    for (int i = 1; i < NT; ++i) mx = fmaxf(mx, pv[i]);
-    if (__any(mx > (m == -INFINITY ? m : lift + kSlack))) {
+    for (int i = 1; i < NT; ++i) {
+      mx = fmaxf(mx, pv[i]);
+      scales |= sb[i][2];
+    }
+    // (weights are at most 2^14: only a scale of 2 or more can pass 2^15)
+    if (__any(mx > limit || ((scales & 0x40004000u) | (lower ^ 0x3C003C00u)) != 0)) {
       if constexpr (C == kNarrow) mx = fmaxf(mx, column8(mx));
-      const float top = fmaxf(m, base + max_over_groups(mx));
-      const float was = base;
-      base = (top == -INFINITY ? 0.0f : top) - lift;
-      rescale(top == m ? 1.0f : __builtin_amdgcn_exp2f(m - top));
+      const float top = fmaxf(m, base + max_over_groups(mx)), was = base;
+      const float f = top == m ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+      base = (top == -INFINITY ? 0.0f : top) - kLift;
+      limit = top == -INFINITY ? top : kTop;
       m = top;
+      l *= f;
+      ob0 *= f;
+      ob1 *= f;
+      float w0 = 0.f, w1 = 0.f;
 #pragma unroll
-      for (int i = 0; i < NT; ++i) pv[i] += was - base;
+      for (int i = 0; i < NT; ++i) {
+        pv[i] += was - base;
+        float p = pv[i];
+        asm volatile("" : "+v"(p));  // (not taken out of here to be shared with the weights below)
+        p = __builtin_amdgcn_exp2f(p);
+        w0 = fmaxf(w0, fabsf(lo_f(sb[i][2])) * p);
+        w1 = fmaxf(w1, fabsf(hi_f(sb[i][2])) * p);
+      }
+      if constexpr (C == kNarrow) {
+        w0 = fmaxf(w0, column8(w0));
+        w1 = fmaxf(w1, column8(w1));
+      }
+      // 2^(14 - e) for products of 2^e and more, e >= 15 (at most 2^14 * 65504)
+      auto factor = [](float x) {
+        return x < 32768.0f ? 1.0f : __uint_as_float((268u - min(__float_as_uint(x) >> 23, 157u)) << 23);
+      };
+      w0 = factor(max_over_groups(w0));
+      w1 = factor(max_over_groups(w1));
+      const float f0 = f * w0 * inverse(lo_f(lower)), f1 = f * w1 * inverse(hi_f(lower));
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt) o[dt] *= dt < 4 ? f0 : f1;
+      lower = cvt_pk<0>(w0, w1);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) sb[i][2] = f16x2_mul(sb[i][2], lower);
     }
     float p0[NT], p1[NT];
 #pragma unroll
@@ -641,12 +666,13 @@ __global__ __launch_bounds__(256, 2) void k_dense_q(Geometry geo, DenseBatch db,
     ob1 += column8(ob1);
     l += column8(l);
   }
+  const float f0 = inverse(lo_f(lower)), f1 = inverse(hi_f(lower));
 #pragma unroll
   for (int dt = 0; dt < 8; ++dt)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if constexpr (C == kNarrow) o[dt][i] += column8(o[dt][i]);
-      o[dt][i] += dt < 4 ? ob0 : ob1;
+      o[dt][i] = __builtin_fmaf(o[dt][i], dt < 4 ? f0 : f1, dt < 4 ? ob0 : ob1);
     }
   dense_finish<0, C>(geo, db, w, o, m == -INFINITY ? m : base, l, out, partials);
 }

@@ -30,3 +30,103 @@ def test_a_refused_step_appends_nothing(gpu):
     got = bsattn.attentionWithCacheUpdate(q, new, new, c, SCALE, dense=True)
     assert [c.seqLen(b) for b in range(2)] == [41, 41]
     assert torch.equal(got, c.decodeDense(q, SCALE))
+
+
+def _spread(gpu, bits, Hq, Hkv, T, seed):
+    """Queries [2, Hq, 1, D] and tokens [2, Hkv, T, D] whose scores differ by
+    several units, with nothing but what the caller adds along dim 0: there the
+    queries hold 4, so a key of x there adds 4 x SCALE to its scores."""
+    import torch
+    g = torch.Generator(device=gpu).manual_seed(seed)
+    q = 2 * torch.randn((2, Hq, 1, D), generator=g, device=gpu)
+    q[..., 0] = 4
+    k, v = (torch.randn((2, Hkv, T, D), generator=g, device=gpu) for _ in range(2))
+    k[..., 0] = 0
+    return q.half(), k, v
+
+
+def _run(gpu, bits, Hq, Hkv, q, k, v):
+    """The dense decode over these tokens and the formula over what the cache
+    holds, both [2, Hq, 1, D] and [2, Hq, D]."""
+    import torch
+    from test_gpu_dense import _cache, _reference
+    T = k.shape[2]
+    c = _cache([T] * 2, Hq, Hkv, 64, "f16", bits)
+    c.append(k.half(), v.half())
+    got, want = c.decodeDense(q, SCALE), _reference(c, q)
+    assert want.abs().max() < 60000 and torch.equal(got, c.decodeDense(q, SCALE))
+    return got, want
+
+
+# Tolerances of the next tests are those of the dense decode's own, row by row:
+# rounding to fp16, and 0.3 of half a step of the row's root mean square for all
+# before it.  For N(0, 1) values those are the offset of 1024 that is taken off
+# the codes twice a unit of 32 tokens, with roundings of 2^-24 / sqrt 3 of 1024
+# sum p s each (s: the scale, 1 / 3.2 of a value's deviation for int4, 1 / 54
+# for int8): 0.75 sqrt(2 / 3) 2^-14 32 / 3.2 / sqrt 32 = 2^-13.9 of the output,
+# 0.13 of half a step, for equal weights and less for others; and the scores,
+# whose offset of 1024 sum q costs each weight up to 2^-14 |sum q| s SCALE
+# (|sum q| < 60: 2^-13.3, 0.2 of half a step, and the weights' errors differ).
+SHAPES = [(8, 2), (32, 8), (32, 2)]  # groups of 4 and of 16
+
+
+@pytest.mark.parametrize("bits,out", [(4, 10.0), (8, 200.0)])
+@pytest.mark.parametrize("Hq,Hkv", SHAPES)
+@pytest.mark.parametrize("T", [300, 2100, 20000])
+@pytest.mark.parametrize("score", [3.0, -5.0])
+def test_large_scales_of_little_weight(gpu, bits, out, Hq, Hkv, T, score):
+    """One token in 32 has values, and so a scale, many times the others', and
+    e^-4 or e^-12 of the weight of the largest: the others keep their bits."""
+    from test_gpu_dense import _check
+    q, k, v = _spread(gpu, bits, Hq, Hkv, T, 100 * bits + T)
+    odd = slice(5, None, 32)
+    k[:, :, odd, 1:] *= 0.1
+    k[:, :, odd, 0] = score / (4 * SCALE)
+    v[:, :, odd] *= out
+    _check(*_run(gpu, bits, Hq, Hkv, q, k, v), "f16", f"{T} tokens")
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("Hq,Hkv", SHAPES)
+@pytest.mark.parametrize("T", [300, 5000])
+@pytest.mark.parametrize("half", [0, 1])
+def test_large_scales_in_one_half(gpu, bits, Hq, Hkv, T, half):
+    """Tokens of large values in dims 0-63 or 64-127 alone, with scores like
+    any other's: the other half of the dims keeps its bits."""
+    from test_gpu_dense import _check
+    q, k, v = _spread(gpu, bits, Hq, Hkv, T, 7 * bits + T + half)
+    v[:, :, 3::16, 64 * half:64 * half + 64] *= 1000
+    got, want = _run(gpu, bits, Hq, Hkv, q, k, v)
+    for i in range(2):
+        dims = slice(64 * i, 64 * i + 64)
+        _check(got[..., dims], want[..., dims], "f16", f"half {i}")
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("Hq,Hkv", SHAPES)
+@pytest.mark.parametrize("times", [30.0, 1000.0, 6000.0])
+def test_large_scales_everywhere(gpu, bits, Hq, Hkv, times):
+    from test_gpu_dense import _check
+    q, k, v = _spread(gpu, bits, Hq, Hkv, 3000, 11 * bits)
+    _check(*_run(gpu, bits, Hq, Hkv, q, k, v * times), "f16", f"times {times}")
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("Hq,Hkv", SHAPES)
+@pytest.mark.parametrize("slope", [30.0, -30.0])
+def test_large_scales_that_lose_their_weight(gpu, bits, Hq, Hkv, slope):
+    """Scores that rise along the sequence, from tokens of large values whose
+    weight is all there is at first to ones of small values, and the other way
+    round."""
+    import torch
+    from test_gpu_dense import _check
+    T = 4000
+    q, k, v = _spread(gpu, bits, Hq, Hkv, T, 13 * bits)
+    ramp = torch.linspace(0, 1, T, device=gpu)
+    # (int4 keys of up to 85 have scales of 6: a small sum of the queries' dims)
+    q[..., 1:] *= 0.125
+    k *= 0.3
+    k[..., 0] = (ramp if slope > 0 else 1 - ramp) * abs(slope) / (4 * SCALE)
+    large = torch.where(ramp < 0.3, 500.0, 1.0)
+    v *= large[:, None]
+    _check(*_run(gpu, bits, Hq, Hkv, q, k, v), "f16", f"slope {slope}")
