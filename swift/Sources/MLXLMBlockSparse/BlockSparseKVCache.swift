@@ -23,7 +23,9 @@ public class BlockSparseKVCache: KVCache {
     public let device: BlockSparseDevice
 
     /// Whether attentionWithCacheUpdate attends to every token instead of the
-    /// selected blocks, for layers that take no selection.
+    /// selected blocks, for layers that take no selection.  `copy()` and
+    /// `toQuantized` keep it; prompt-cache files do not hold it
+    /// (`registerPromptCacheClass`).
     public var attendsDensely = false
 
     /// The cache a library handle belongs to; `copy()` makes its subclass's
@@ -323,6 +325,7 @@ public class BlockSparseKVCache: KVCache {
             blockSize: blockSize, topK: topK, sinkBlocks: sinkBlocks, recentBlocks: recentBlocks,
             maxBlocksPerSeq: Int(desc.max_blocks_per_seq), numPages: Int(desc.num_pages), bits: bits,
             groupSize: groupSize, device: device)
+        q.attendsDensely = attendsDensely
         for s in 0 ..< Int(desc.max_seqs) where seqLen(s) > 0 {
             let shape = [1, kvHeads, seqLen(s), headDim]
             var k = device.empty(shape, dtype: dtype)

@@ -22,8 +22,12 @@ extension BlockSparse {
     /// per sequence and `maxSeqs` (default: the rows in the file) size the
     /// new cache.  loadPromptCache then sets `state` (the tokens) and
     /// `metaState` (which checks the geometry and the token count of row 0).
+    /// `attendsDensely` is the model's as well: what it says here holds for
+    /// every layer of the file, so a model in which only some layers take no
+    /// selection sets their caches' `attendsDensely` after loading.
     public static func registerPromptCacheClass(
-        qHeads: Int, maxTokens: Int, maxSeqs: Int? = nil, device: BlockSparseDevice? = nil
+        qHeads: Int, maxTokens: Int, maxSeqs: Int? = nil, attendsDensely: Bool = false,
+        device: BlockSparseDevice? = nil
     ) {
         PromptCacheClasses.register(promptCacheClassName) { metaState, state in
             let v = metaState.compactMap { Int($0) }
@@ -42,16 +46,20 @@ extension BlockSparse {
             let kvHeads = state[0].dim(1)
             let headDim = kvBits == 0 ? state[0].dim(3) : state[0].dim(3) * 32 / kvBits
             let blocks = (max(maxTokens, state[0].dim(2)) + blockSize - 1) / blockSize
+            let cache: BlockSparseKVCache
             if kvBits == 0 {
-                return BlockSparseKVCache(
+                cache = BlockSparseKVCache(
                     maxSeqs: rows, qHeads: qHeads, kvHeads: kvHeads, headDim: headDim,
                     blockSize: blockSize, dtype: state[0].dtype, topK: topK, sinkBlocks: sinkBlocks,
                     recentBlocks: recentBlocks, maxBlocksPerSeq: blocks, device: device)
+            } else {
+                cache = QuantizedBlockSparseKVCache(
+                    maxSeqs: rows, qHeads: qHeads, kvHeads: kvHeads, headDim: headDim,
+                    blockSize: blockSize, topK: topK, sinkBlocks: sinkBlocks, recentBlocks: recentBlocks,
+                    maxBlocksPerSeq: blocks, bits: kvBits, groupSize: groupSize, device: device)
             }
-            return QuantizedBlockSparseKVCache(
-                maxSeqs: rows, qHeads: qHeads, kvHeads: kvHeads, headDim: headDim,
-                blockSize: blockSize, topK: topK, sinkBlocks: sinkBlocks, recentBlocks: recentBlocks,
-                maxBlocksPerSeq: blocks, bits: kvBits, groupSize: groupSize, device: device)
+            cache.attendsDensely = attendsDensely
+            return cache
         }
     }
 }
