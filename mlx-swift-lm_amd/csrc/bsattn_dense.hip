@@ -56,16 +56,6 @@ constexpr float kLog2e = 1.4426950408889634f;
 // the launch reads the same blocks.
 enum Columns { kNarrow, kWide, kAgain };
 
-// Ahead of the partials in the workspace: where each entry's lie, written by the
-// first part of its own job.  (With the batch among its arguments the join's
-// launch takes the host 4.1 us, with less than 100 bytes 2.8.)
-struct DenseJoin {
-  int32_t shared0, step, shared;  // the shared job's: blocks shared0, shared0 + step, ...
-  int32_t own0, parts;            // then own0 + shared, own0 + shared + 1, ...; `parts` in all
-};
-constexpr int kPartial = kHeadDim + 2;  // floats of a partial: o, its reference, its sum
-constexpr int kJoinRows = (kMaxBatch * (int)sizeof(DenseJoin) / 4 + kPartial - 1) / kPartial;
-
 // x of the lane 8 columns on
 __device__ __forceinline__ float column8(float x) {
   return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x128, 0xF, 0xF, false));
@@ -744,84 +734,6 @@ __global__ __launch_bounds__(32 * kRows) void k_dense_join(const float* __restri
     if (mi != -INFINITY) as += f * s_o[i][d];
   }
   out[((size_t)bi * hqs + hq) * kHeadDim + d] = from_f32<DT>(Ls == 0.f ? 0.f : as / Ls);
-}
-
-// Cuts the jobs into parts.
-int dense_plan(const Geometry& g, DenseBatch& db, int64_t* rows) {
-  int64_t all = 0;
-  int most = 1;
-  for (int j = 0; j < db.jobs; ++j) {
-    all += db.job[j].units;
-    most = std::max(most, db.job[j].units);
-  }
-  // Shared jobs first, for every head, then what the entries have of their own:
-  // four prompts of 16001 int8 tokens, four branches each, 33.2 -> 29.8 us.
-  // Where the entries are alike their parts stay together (8 x 32k bf16 161.6
-  // us, head by head 163.4; 32 ragged windows 83.4 and 86.6)
-  db.heads_first = db.job[0].count > 1;
-  // One round of workgroups, two per CU: 8 x 32k bf16 tokens 162 us (three per
-  // CU 167, four 165, six 169), 4 x 131k int4 99 (100, 110, 105), 4 x 262k int8
-  // in 16-head groups 179 (185, 190, 199).  The parts are cut so that they all
-  // fit into it: 9 x 13563 fp16 tokens, 16 kv heads, 153 us (576 workgroups 174),
-  // 5 x 40k bf16 131 (152).
-  const int64_t want = 2 * (int64_t)std::max(g.cus, 1);
-  auto fits = [&](int cu) {
-    int64_t n = 0;
-    for (int j = 0; j < db.jobs; ++j) n += std::max(1, (db.job[j].units + cu - 1) / cu);
-    return n * g.hkv <= want;
-  };
-  auto cut = [&](int64_t workgroups) {
-    const int64_t cu = std::max<int64_t>(4, (all * g.hkv + workgroups - 1) / workgroups);
-    return ((int)std::min<int64_t>(cu, most) + 3) & ~3;
-  };
-  db.cu = cut(want);
-  int lo = db.cu / 4, hi = (most + 3) / 4;  // in fours: the smallest that fits
-  while (lo < hi) {
-    const int mid = lo + (hi - lo) / 2;
-    if (fits(4 * mid)) hi = mid;
-    else lo = mid + 1;
-  }
-  // Many sequences of different lengths, where the largest part of a round would
-  // be far from the average: smaller parts, one after another (48 sequences of
-  // 100 to 6000 bf16 tokens 104 us, in one round 111; affine caches, whose parts
-  // cost more to begin, less small: 64 of 400 to 4000 int4 42 and 44).  More
-  // sequences than a round takes: whole ones (33 x 300 tokens, 16 kv heads, 19
-  // us, 24 in parts).
-  const bool even = 4 * lo <= 32 || 2 * (int64_t)4 * lo * want <= 3 * all * g.hkv;
-  if (!fits(4 * lo)) db.cu = cut(want);
-  else db.cu = even ? 4 * lo : cut(g.kv_bits ? want : 3 * want);
-  // (it ends: jobs of one part each, shared ones padded to 8, fit)
-  static_assert((8 + 1) * kMaxBatch * 128 + kJoinRows <= kPrefillRows && kMaxBatch * 256 + kJoinRows <= kPrefillRows,
-                "up to 128 query heads with shared jobs, 256 without");
-  while (true) {
-    int64_t parts = 0, blocks = 0;
-    bool joined = false;
-    for (int j = 0; j < db.jobs; ++j) {
-      DenseJob& job = db.job[j];
-      const bool direct = job.count == 1 && job.of < 0;
-      int n = (job.units + db.cu - 1) / db.cu;
-      if (job.count == 1) n = std::max(n, 1);  // (zeros for no tokens; the join's table)
-      // (jobs of the same blocks: their n-th parts lie a multiple of 8
-      // workgroups apart, whatever the grid's order, on the same XCD, whose L2
-      // then holds them; two jobs of 4 x 8191 bf16 tokens 17.1 -> 14.6 us)
-      if (job.count > 1) n = (n + 7) & ~7;
-      job.part0 = (int32_t)parts;
-      job.row0 = (int32_t)blocks;
-      if (job.of >= 0) {  // (shared jobs come first)
-        const DenseJob& with = db.job[job.of];
-        job.shared = (int16_t)((with.units + db.cu - 1) / db.cu);
-        job.step = with.count;
-        job.shared0 = with.row0;
-        while (db.order[with.first + job.shared0 - with.row0] != job.entry) ++job.shared0;
-      }
-      parts += n;
-      blocks += (int64_t)n * job.count;
-      joined = joined || n > 1 || !direct;
-    }
-    *rows = joined ? kJoinRows + blocks * g.hq : 0;
-    if (*rows <= kPrefillRows) return (int)parts;
-    db.cu *= 2;
-  }
 }
 
 template <Columns C>
