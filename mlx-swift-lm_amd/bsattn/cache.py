@@ -47,6 +47,12 @@ def _row_ids(seq_ids: Optional[Sequence[int]], rows: int):
     return i32_array(seq_ids)
 
 
+def _common(a: Sequence[int], b: Sequence[int]) -> int:
+    """How many leading entries two lists have in common."""
+    n = min(len(a), len(b))
+    return next((i for i in range(n) if a[i] != b[i]), n)
+
+
 class BlockSparseKVCache:
     """One layer's paged KV cache for up to `max_seqs` sequences."""
 
@@ -629,7 +635,7 @@ class BlockSparseKVCache:
         `bits`-bit codes with fp16 scales / biases (exported and quantized on
         append, on the device), with the summaries of the dequantized keys.
         Quantized caches hold fp16, so a bf16 cache's tokens are rounded to
-        fp16 first."""
+        fp16 first.  Blocks that sequences share (fork) stay shared."""
         if self.bits:
             raise ValueError("toQuantized: the cache is already quantized")
         d = self.desc
@@ -639,12 +645,20 @@ class BlockSparseKVCache:
             group_size=groupSize, top_k=d.top_k, sink_blocks=d.sink_blocks,
             recent_blocks=d.recent_blocks, max_blocks_per_seq=d.max_blocks_per_seq,
             num_pages=d.num_pages, device=self.device.index)
+        Tb, pages = d.block_size, {}  # of the sequences converted so far
         for s in range(d.max_seqs):
-            if self.seqLen(s) == 0:
+            n = self.seqLen(s)
+            if n == 0:
                 continue
-            k, v = self.export([s])
-            if self.dtype != torch.float16:
-                k, v = k.half(), v.half()
+            # (pages that two sequences hold are full blocks of the same tokens)
+            pages[s] = self.seqPages(s)
+            like, shared = max(((r, _common(p, pages[s])) for r, p in pages.items() if r != s),
+                               key=lambda x: x[1], default=(s, 0))
+            if shared:
+                qc.fork([like], [s], [shared * Tb])
+            if shared * Tb == n:
+                continue
+            k, v = (x[:, :, shared * Tb:].to(torch.float16).contiguous() for x in self.export([s]))
             qc.append(k, v, seq_ids=[s])
             del k, v
         return qc

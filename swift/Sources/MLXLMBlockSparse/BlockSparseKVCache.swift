@@ -318,7 +318,9 @@ public class BlockSparseKVCache: KVCache {
     }
 
     /// KVCacheSimple.toQuantized (KVCache.swift:407-427): a cache of the same
-    /// geometry holding every sequence as `bits`-bit MLX-affine codes.
+    /// geometry holding every sequence as `bits`-bit MLX-affine codes.  Each
+    /// sequence gets pages of its own, forks included: `numPages` has to do
+    /// for that.
     public func toQuantized(groupSize: Int = 64, bits: Int = 4) -> QuantizedBlockSparseKVCache {
         let q = QuantizedBlockSparseKVCache(
             maxSeqs: Int(desc.max_seqs), qHeads: qHeads, kvHeads: kvHeads, headDim: headDim,

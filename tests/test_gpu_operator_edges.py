@@ -130,3 +130,42 @@ def test_large_scales_that_lose_their_weight(gpu, bits, Hq, Hkv, slope):
     large = torch.where(ramp < 0.3, 500.0, 1.0)
     v *= large[:, None]
     _check(*_run(gpu, bits, Hq, Hkv, q, k, v), "f16", f"slope {slope}")
+
+
+@pytest.mark.parametrize("dtype,bits", [("bf16", 8), ("f16", 4)])
+def test_quantizing_keeps_forks_shared(gpu, dtype, bits):
+    """toQuantized of a cache whose sequences share blocks, in a pool that
+    holds no more: the same codes as sequence by sequence, as many free pages
+    as before, and sequences that are independent from then on."""
+    import torch
+    from test_gpu_dense import _check, _dt, _randn, _reference
+    import bsattn
+    geometry = dict(max_seqs=9, num_q_heads=8, num_kv_heads=2, block_size=32, top_k=2, max_blocks_per_seq=40, device=0)
+    c = bsattn.BlockSparseKVCache(dtype=_dt(dtype), num_pages=60, **geometry)
+    plain = bsattn.BlockSparseKVCache(dtype=torch.float16, kv_bits=bits, **geometry)
+    k, v = (_randn(gpu, i, (1, 2, 1010, D), dtype) for i in (1, 2))
+    c.append(k, v, seq_ids=[8])
+    c.fork([8] * 4, [0, 1, 2, 3], [1010, 992, 500, 31])
+    more = _randn(gpu, 3, (1, 2, 70, D), dtype)
+    c.append(more, more, seq_ids=[1])
+    c.fork([1, 1], [4, 5], [1062, 1000])
+    c.append(more, more, seq_ids=[6])
+    c.trim(400, seq_ids=[4])
+    lens = [c.seqLen(s) for s in range(9)]
+    q = c.toQuantized(bits=bits)
+    assert [q.seqLen(s) for s in range(9)] == lens and q.freePages == c.freePages
+    for s in range(9):
+        if lens[s]:
+            k, v = c.export([s])
+            plain.append(k.half(), v.half(), seq_ids=[s])
+            for a, b in zip(sum(q.exportQuantized([s]), ()), sum(plain.exportQuantized([s]), ())):
+                assert torch.equal(a, b), f"sequence {s}"
+            assert torch.equal(q.exportSummaries(s), plain.exportSummaries(s)), f"sequence {s}"
+    new = _randn(gpu, 5, (9, 2, 1, D), "f16")
+    for x in (q, plain):
+        x.append(new, new)
+    x = _randn(gpu, 6, (9, 8, 1, D), "f16")
+    assert torch.equal(q.decode(x, SCALE), plain.decode(x, SCALE))
+    _check(q.decodeDense(x, SCALE), _reference(plain, x), "f16")
+    q.reset(list(range(9)))
+    assert q.freePages == 60
