@@ -223,8 +223,8 @@ int bsattn_prefill(bsattn_cache* cache, const void* q, const int32_t* seq_ids,
  * computes for L = 1 (AttentionUtils.swift:46-52, :68-75; KVCache.swift:
  * 1533-1621), for the layers and models that take no block selection.  The
  * token's own key and value have been appended.  q / out [n_seqs, Hq, 1, D];
- * sinks: [Hq] float logits (device) that join each head's softmax without a
- * value, or null.  A sequence that holds no token gives zeros.  Like
+ * (both 16-byte aligned); sinks: [Hq] float logits (device) that join each
+ * head's softmax without a value, or null.  A sequence that holds no token gives zeros.  Like
  * bsattn_decode it sizes its launches from the held pages and reads the
  * device-side lengths, so it may follow bsattn_append_step without
  * bsattn_sync.  Long sequences are split over the GPU and joined through the
@@ -233,7 +233,8 @@ int bsattn_prefill(bsattn_cache* cache, const void* q, const int32_t* seq_ids,
  * share (bsattn_fork) are read once for several of them, with no window and
  * outside a capture: then, too, a result may be rounded differently.  A
  * captured call holds for any later lengths (its launches keep their size).
- * Where an attended value is infinite, that dim is infinite or NaN. */
+ * Where an attended value is infinite, that dim is infinite or NaN (a weight
+ * enters as two 16-bit parts, of which the second may be zero or negative). */
 int bsattn_decode_dense(bsattn_cache* cache, const void* q, const int32_t* seq_ids,
                         int32_t n_seqs, int32_t window, const float* sinks,
                         float scale, void* out, void* stream);

@@ -32,7 +32,8 @@ def attentionWithCacheUpdate(queries: torch.Tensor, keys: torch.Tensor, values: 
     keys come without positions and get those behind the cached tokens first;
     norms: (qWeight, kWeight, eps) or (qWeight, kWeight, eps, weightOffset) of
     the per-head RMS norms ahead of the rope, in the same pass.  Queries and
-    keys may then be views into a fused projection."""
+    keys may then be views into a fused projection; values are contiguous in any
+    case (of a view, the caller makes a copy)."""
     if not isinstance(cache, BlockSparseKVCache):
         raise TypeError("attentionWithCacheUpdate here handles BlockSparseKVCache only; "
                         "other caches use the reference's dense path")

@@ -458,7 +458,8 @@ class BlockSparseKVCache:
         sequences hold (the new one appended), or over the last `window`: the
         reference's dense decode, for layers that take no block selection.
         sinks: [Hq] float32 logits that join each head's softmax without a
-        value.  A sequence without tokens gives zeros."""
+        value.  A sequence without tokens gives zeros.  queries are 16-byte
+        aligned."""
         B = self._check_q(queries)
         window, logits = self._check_window(window), self._check_sinks(sinks)
         out = torch.empty_like(queries)
@@ -512,9 +513,10 @@ class BlockSparseKVCache:
         """RMS norms of the heads of queries [B, Hq, L, D] and keys
         [B, Hkv, L, D], scaled by weightOffset + weight ([D]), then their
         rotary positions, in one pass.  Views into a fused projection will do;
-        the results are dense.  Both weights None: the positions alone.
-        positions [B, L] int32; by default each sequence's tokens follow those
-        that the cache holds."""
+        the results are dense.  (append takes the values as a contiguous
+        tensor: a projection's view of them has to be copied first.)  Both
+        weights None: the positions alone.  positions [B, L] int32; by default
+        each sequence's tokens follow those that the cache holds."""
         qs, (B, _, L, _) = self._check_strided(queries, "queries", self._hq)
         ks, (Bk, _, Lk, _) = self._check_strided(keys, "keys", self._hkv)
         if Bk != B or Lk != L:

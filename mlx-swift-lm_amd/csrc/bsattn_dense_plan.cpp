@@ -25,6 +25,9 @@ int dense_plan(const Geometry& g, DenseBatch& db, int64_t* rows) {
   // fit into it: 9 x 13563 fp16 tokens, 16 kv heads, 153 us (576 workgroups 174),
   // 5 x 40k bf16 131 (152).
   const int64_t want = 2 * (int64_t)std::max(g.cus, 1);
+  // (A branch's rest of a unit or two counts as a workgroup like any other: four
+  // prompts of 16001 int8 tokens, four branches each, have 384 workgroups for
+  // what is shared, of 44 units each, and 128 for the rests: 28.9 us.)
   auto fits = [&](int cu) {
     int64_t n = 0;
     for (int j = 0; j < db.jobs; ++j) n += std::max(1, (db.job[j].units + cu - 1) / cu);
@@ -63,7 +66,9 @@ int dense_plan(const Geometry& g, DenseBatch& db, int64_t* rows) {
       if (job.count == 1) n = std::max(n, 1);  // (zeros for no tokens; the join's table)
       // (jobs of the same blocks: their n-th parts lie a multiple of 8
       // workgroups apart, whatever the grid's order, on the same XCD, whose L2
-      // then holds them; two jobs of 4 x 8191 bf16 tokens 17.1 -> 14.6 us)
+      // then holds them; two jobs of 4 x 8191 bf16 tokens 17.1 -> 14.6 us.
+      // Where no two jobs read the same blocks the padding is empty workgroups
+      // and nothing else.)
       if (job.count > 1) n = (n + 7) & ~7;
       job.part0 = (int32_t)parts;
       job.row0 = (int32_t)blocks;

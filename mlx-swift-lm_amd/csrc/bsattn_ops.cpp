@@ -89,9 +89,16 @@ DenseJob& add_job(DenseBatch& db, const int32_t* ids, int first, int count) {
 }
 
 // Units of 32 tokens that a shared prefix must have to be read apart from its
-// sequences' rest.  Over one cache again and again (bf16, 8 kv heads), 8
-// branches of 1100 tokens take 11.7 us with it and 14.2 without, 32 of 8191 26
-// and 79, but 32 of 600 16.9 and 14.1.
+// sequences' rest.  32 heads in groups of 4, one cache again and again (and
+// caches in turn, past what the Infinity Cache holds), together against apart:
+//   bf16  2 branches of 2048 tokens  9.8 and 10.1 us (9.9 and 11.2), of 4096
+//         10.1, 13.2 (11.6, 16.1), of 8191 11.6, 12.5 (15.7, 14.6), of 16384
+//         18.2, 26.0 (19.8, 28.6); 8 of 1100 10.1, 14.0 (10.1, 17.4)
+//   int8  2 of 8191 11.7, 11.3 (12.4, 11.7), of 16384 15.1, 17.2 (16.2, 19.0)
+//   int4  2 of 8191 11.5, 11.0 (11.6, 11.2), of 65536 25.4, 31.2 (25.5, 30.8)
+// Two branches in groups of 8 lose most: 8191 bf16 tokens 11.1 and 9.6 us
+// (11.5, 10.5).  Below this 32 branches of 600 tokens take 16.9 together, 14.1
+// apart.
 constexpr int kSharedUnits = 32;
 
 // Jobs of a launch of the sequences ids[0, n): the full blocks that entries

@@ -25,7 +25,9 @@ public class BlockSparseKVCache: KVCache {
     /// Whether attentionWithCacheUpdate attends to every token instead of the
     /// selected blocks, for layers that take no selection.  `copy()` and
     /// `toQuantized` keep it; prompt-cache files do not hold it
-    /// (`registerPromptCacheClass`).
+    /// (`registerPromptCacheClass`).  Windows, sinks, rotary positions and norms
+    /// are not part of it: a model that has them calls `normRotate`, `append`
+    /// and `decodeDense` itself.
     public var attendsDensely = false
 
     /// The cache a library handle belongs to; `copy()` makes its subclass's
