@@ -57,7 +57,7 @@ def attentionWithCacheUpdate(queries: torch.Tensor, keys: torch.Tensor, values: 
         return cache.appendDecode(keys, values, queries, scale)
     # nothing is appended that could not be attended to
     cache._check_q(queries, multi=L > 1)
-    if queries.shape[0] != keys.shape[0] or L != keys.shape[2]:
+    if keys.dim() != 4 or queries.shape[0] != keys.shape[0] or L != keys.shape[2]:
         raise ValueError("keys / values and queries disagree on B or L")
     if dense and L == 1:
         cache._check_sinks(sinks)

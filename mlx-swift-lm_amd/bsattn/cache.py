@@ -647,15 +647,17 @@ class BlockSparseKVCache:
             group_size=groupSize, top_k=d.top_k, sink_blocks=d.sink_blocks,
             recent_blocks=d.recent_blocks, max_blocks_per_seq=d.max_blocks_per_seq,
             num_pages=d.num_pages, device=self.device.index)
-        Tb, pages = d.block_size, {}  # of the sequences converted so far
+        Tb, converted = d.block_size, {}  # first page -> [(sequence, pages)]
         for s in range(d.max_seqs):
             n = self.seqLen(s)
             if n == 0:
                 continue
-            # (pages that two sequences hold are full blocks of the same tokens)
-            pages[s] = self.seqPages(s)
-            like, shared = max(((r, _common(p, pages[s])) for r, p in pages.items() if r != s),
-                               key=lambda x: x[1], default=(s, 0))
+            # (pages that two sequences hold are full blocks of the same tokens,
+            # from the beginning on)
+            pages = self.seqPages(s)
+            alike = converted.setdefault(pages[0], [])
+            like, shared = max(((r, _common(p, pages)) for r, p in alike), key=lambda x: x[1], default=(s, 0))
+            alike.append((s, pages))
             if shared:
                 qc.fork([like], [s], [shared * Tb])
             if shared * Tb == n:
