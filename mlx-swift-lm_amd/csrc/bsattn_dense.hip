@@ -498,8 +498,8 @@ __global__ __launch_bounds__(256, 2) void k_dense_q(Geometry geo, DenseBatch db,
   // subnormals: outputs were off by 8 half steps of fp16 at their root mean
   // square where one token in 32 had such a scale and e^-12 of the largest
   // weight).  Done with the raise
-  // of the reference, behind one branch: 4 x 131k int4 tokens 100.1 us, as before;
-  // with a scale of 2 and more in every unit 141 (118 before).
+  // of the reference, behind one branch: 4 x 131k int4 tokens 99.6 us (99.0
+  // before); with scales of 10 everywhere 117 (115), on one token in 32 108 (103).
   constexpr float kLift = kTop - kSlack;
   float m = -INFINITY, base = 0.0f, limit = -INFINITY, l = 0.0f, ob0 = 0.0f, ob1 = 0.0f;
   uint32_t lower = 0x3C003C00u;  // what the scales of dims 0-63 and 64-127 are multiplied by (fp16)
@@ -566,8 +566,16 @@ __global__ __launch_bounds__(256, 2) void k_dense_q(Geometry geo, DenseBatch db,
       mx = fmaxf(mx, pv[i]);
       scales |= sb[i][2];
     }
-    // (weights are at most 2^14: only a scale of 2 or more can pass 2^15)
-    if (__any(mx > limit || ((scales & 0x40004000u) | (lower ^ 0x3C003C00u)) != 0)) {
+    // (weights are at most 2^14: only a scale of 2 or more can pass 2^15; then
+    // the largest weight and scale say whether one does)
+    bool move = mx > limit || lower != 0x3C003C00u;
+    if (__any((scales & 0x40004000u) != 0)) {
+      float most = 0.f;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) most = fmaxf(most, fmaxf(fabsf(lo_f(sb[i][2])), fabsf(hi_f(sb[i][2]))));
+      move = move || most * __builtin_amdgcn_exp2f(mx) >= 32768.0f;
+    }
+    if (__any(move)) {
       if constexpr (C == kNarrow) mx = fmaxf(mx, column8(mx));
       const float top = fmaxf(m, base + max_over_groups(mx)), was = base;
       const float f = top == m ? 1.0f : __builtin_amdgcn_exp2f(m - top);
