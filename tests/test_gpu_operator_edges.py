@@ -169,3 +169,27 @@ def test_quantizing_keeps_forks_shared(gpu, dtype, bits):
     _check(q.decodeDense(x, SCALE), _reference(plain, x), "f16")
     q.reset(list(range(9)))
     assert q.freePages == 60
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("Hq,Hkv", SHAPES)
+def test_large_scales_of_branches(gpu, bits, Hq, Hkv):
+    """Large scales in blocks that branches share and in what they have of
+    their own; a window and sinks beside them."""
+    import torch
+    from test_gpu_dense import _cache, _check, _reference
+    q, k, v = _spread(gpu, bits, Hq, Hkv, 2500, 17 * bits)
+    v[:, :, 5::32] *= 100
+    v[:, :, 9::32, :64] *= 1000
+    c = _cache([2600] * 14, Hq, Hkv, 64, "f16", bits)
+    c.append(k.half(), v.half(), seq_ids=[0, 1])
+    c.fork([0] * 9 + [1] * 3, list(range(2, 14)))
+    c.append((k[:1, :, :70] * 1.5).half().expand(12, -1, -1, -1).contiguous(),
+             v[:1, :, :70].half().expand(12, -1, -1, -1).contiguous(), seq_ids=list(range(2, 14)))
+    q = torch.cat([q[:1] * (1 - 0.05 * i) for i in range(14)]).contiguous()
+    sinks = torch.linspace(-2, 6, Hq, device=gpu)
+    for kw in (dict(), dict(sinks=sinks), dict(window=900, sinks=sinks)):
+        got, want = c.decodeDense(q, SCALE, **kw), _reference(c, q, **kw)
+        for i in range(2):
+            dims = slice(64 * i, 64 * i + 64)
+            _check(got[..., dims], want[..., dims], "f16", f"half {i} {list(kw)}")
