@@ -303,6 +303,88 @@ int bsattn_append_step(bsattn_cache* cache, const void* k, const void* v,
                        const int32_t* seq_ids, int32_t n_seqs, void* stream);
 int bsattn_sync(bsattn_cache* cache, void* stream);
 
+/* Verification steps: requests that each bring their own number of new
+ * tokens, as a tree of drafts or as a chain, at the device-side lengths.  The
+ * new tokens are packed along rows: tensors are [rows, heads, D], request i's
+ * tokens the rows starts[i] .. starts[i] + taken[i] - 1.  A round is
+ * bsattn_step_map once for all layers, then for each layer
+ * bsattn_append_packed, bsattn_attend_tree and, once the accepted path is
+ * known, bsattn_keep; nothing in it needs the host, and all of it can be
+ * captured.  Its generalisation of SpeculativeTokenIterator.speculateRound
+ * (Evaluate.swift:841-931), which verifies one chain of drafts and trims.
+ *
+ * The caller owns the arrays (device memory) and keeps them and the struct
+ * while calls or graphs that use them are pending; a step is used with one
+ * stream at a time, and with the caches that it was last mapped for. */
+#define BSATTN_STEP_SEQS 64    /* most requests of a step */
+#define BSATTN_STEP_CACHES 128 /* most caches of a step */
+#define BSATTN_TREE_NODES 64   /* most tokens of a request whose tree can be attended or kept */
+typedef struct bsattn_step {
+  int32_t n_caches;    /* 1..BSATTN_STEP_CACHES */
+  int32_t rows;        /* rows of the packed tensors: >= 1 */
+  int32_t max_tokens;  /* most tokens that a request brings: >= 1 */
+  int32_t n_seqs;      /* requests of the last map (written by it) */
+  /* written by bsattn_step_map */
+  int32_t* starts;     /* [n_seqs + 1]: the counts' sums; rows behind the last are nobody's */
+  int32_t* taken;      /* [n_seqs]: tokens of the request, 0 where it does not fit */
+  int32_t* requests;   /* [rows]: the row's request, -1: none */
+  int32_t* positions;  /* [rows]: its position (cached tokens + depth in the tree), 0: none */
+  uint64_t* ancestors; /* [rows]: its ancestors among its request's tokens and itself, a bit
+                          each (0: absent, or none).  May be null where max_tokens >
+                          BSATTN_TREE_NODES */
+  int32_t* slots;      /* [n_caches, rows]: page * block_size + place in it, -1: none */
+  int32_t* ends;       /* [n_caches, n_seqs]: the request's length with its new tokens */
+  int32_t ids[BSATTN_STEP_SEQS]; /* the requests' sequences */
+  uint64_t stamp;      /* names the map to the caches */
+} bsattn_step;
+
+/* Where the new tokens of a step lie: builds the step's arrays on the device.
+ * counts (device, [n_seqs] int32): tokens of each request; parents (device,
+ * [rows] int32, packed; null: chains): a node's parent among its request's
+ * tokens, or -1 for a node that follows the cached ones.  A node whose parent
+ * is neither -1 nor an earlier node is absent, with all that descends from it:
+ * it has a row and a slot, but sees nothing and is not seen.  A request is
+ * taken whole or not at all: not if it brings more than max_tokens, its rows
+ * end past `rows`, or the pages it holds (bsattn_reserve) in some cache do not
+ * fit them.  All caches are of one GPU and hold the requests' sequences at the
+ * same lengths (checked where the host knows them).  seq_ids (host) as in
+ * bsattn_append.  The caches do not change. */
+int bsattn_step_map(bsattn_cache* const* caches, bsattn_step* step, const int32_t* counts,
+                    const int32_t* parents, const int32_t* seq_ids, int32_t n_seqs, void* stream);
+
+/* Appends the step's rows of k and v [rows, Hkv, D] to one of its caches, at
+ * the slots that the map gave them (quantized where the cache is), with the
+ * summaries of the blocks they fill, and sets the device-side lengths to
+ * `ends`.  strides: elements between rows and between heads, multiples of 8
+ * (null: dense); the dims are contiguous, 16-byte aligned.  A step can be
+ * appended again (the rows are overwritten) until the host changes the
+ * cache's sequences.  As after bsattn_append_step the host's view is behind
+ * until bsattn_sync. */
+int bsattn_append_packed(bsattn_cache* cache, const bsattn_step* step, const void* k,
+                         const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                         void* stream);
+
+/* Dense attention of the step's rows, q [rows, Hq, D] (strides as above) ->
+ * out [rows, Hq, D] (dense, 16-byte aligned): a node sees the tokens its
+ * request held before the step and its own ancestors, or with a window those
+ * of them at the last `window` positions (0: all).  sinks: as in
+ * bsattn_decode_dense.  Absent nodes give zeros; rows of no request are left
+ * as they were.  max_tokens is at most BSATTN_TREE_NODES.  Workspaces, split
+ * sequences and infinite attended values as in bsattn_decode_dense. */
+int bsattn_attend_tree(bsattn_cache* cache, const bsattn_step* step, const void* q,
+                       const int64_t* q_strides, int32_t window, const float* sinks, float scale,
+                       void* out, void* stream);
+
+/* Keeps accepted paths: of the tokens that the step appended, request i's
+ * become its nodes kept[i, 0], .., kept[i, n_kept[i] - 1] (device, kept
+ * [n_seqs, width] int32, strictly ascending; the list ends at the first entry
+ * that is not, or that is no node), moved together behind what it held before;
+ * its device-side length is that and the kept ones.  Blocks that are full then
+ * get their summary.  With no node kept the step is taken back (also after
+ * another bsattn_keep of it).  max_tokens is at most BSATTN_TREE_NODES. */
+int bsattn_keep(bsattn_cache* cache, const bsattn_step* step, const int32_t* kept, int32_t width,
+                const int32_t* n_kept, void* stream);
+
 /* Forks: sequence dst_ids[i] becomes the first n_tokens[i] tokens of sequence
  * src_ids[i] (n_tokens null: all that it holds), for samples or beams that
  * continue one prompt, or a prompt that many requests begin with.  A source
@@ -370,6 +452,9 @@ int bsattn_export_summaries(const bsattn_cache* cache, int32_t seq, void* out,
 #define BSATTN_KERNEL_ROTATE 7  /* rotary positions, with the norms or alone */
 #define BSATTN_KERNEL_DENSE 8   /* dense decode attention (its join counts as BSATTN_KERNEL_COMBINE) */
 #define BSATTN_KERNEL_FORK 9    /* forks */
+#define BSATTN_KERNEL_MAP 10    /* step maps (recorded by the step's first cache) */
+#define BSATTN_KERNEL_TREE 11   /* tree attention (its join counts as BSATTN_KERNEL_COMBINE) */
+#define BSATTN_KERNEL_KEEP 12   /* kept paths */
 int bsattn_profile_enable(bsattn_cache* cache, int32_t enable);
 int bsattn_profile_read(bsattn_cache* cache, int32_t kernel, double* total_ms,
                         int64_t* launches);

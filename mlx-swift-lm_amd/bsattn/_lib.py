@@ -48,6 +48,10 @@ EXPORTS = (
     "bsattn_reserve",
     "bsattn_append_step",
     "bsattn_sync",
+    "bsattn_step_map",
+    "bsattn_append_packed",
+    "bsattn_attend_tree",
+    "bsattn_keep",
     "bsattn_fork",
     "bsattn_trim",
     "bsattn_reset",
@@ -109,6 +113,29 @@ class Rope(ctypes.Structure):
     ]
 
 
+STEP_SEQS = 64    # most requests of a step
+STEP_CACHES = 128  # most caches of a step
+TREE_NODES = 64   # most tokens of a request's tree
+
+
+class Step(ctypes.Structure):
+    _fields_ = [
+        ("n_caches", ctypes.c_int32),
+        ("rows", ctypes.c_int32),
+        ("max_tokens", ctypes.c_int32),
+        ("n_seqs", ctypes.c_int32),
+        ("starts", ctypes.c_void_p),
+        ("taken", ctypes.c_void_p),
+        ("requests", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("ancestors", ctypes.c_void_p),
+        ("slots", ctypes.c_void_p),
+        ("ends", ctypes.c_void_p),
+        ("ids", ctypes.c_int32 * STEP_SEQS),
+        ("stamp", ctypes.c_uint64),
+    ]
+
+
 _lib = None
 
 
@@ -151,6 +178,10 @@ def lib() -> ctypes.CDLL:
         "bsattn_reserve": (ctypes.c_int, [P, PI32, i32, i32, P]),
         "bsattn_append_step": (ctypes.c_int, [P, P, P, PI32, i32, P]),
         "bsattn_sync": (ctypes.c_int, [P, P]),
+        "bsattn_step_map": (ctypes.c_int, [PP, ctypes.POINTER(Step), P, P, PI32, i32, P]),
+        "bsattn_append_packed": (ctypes.c_int, [P, ctypes.POINTER(Step), P, PI64, P, PI64, P]),
+        "bsattn_attend_tree": (ctypes.c_int, [P, ctypes.POINTER(Step), P, PI64, i32, P, ctypes.c_float, P, P]),
+        "bsattn_keep": (ctypes.c_int, [P, ctypes.POINTER(Step), P, i32, P, P]),
         "bsattn_fork": (ctypes.c_int, [P, PI32, PI32, i32, PI32, P]),
         "bsattn_trim": (ctypes.c_int, [P, PI32, i32, i32, PI32, P]),
         "bsattn_reset": (ctypes.c_int, [P, PI32, i32, P]),

@@ -23,7 +23,7 @@ MAX_QUERIES = 16
 
 def attentionWithCacheUpdate(queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
                              cache, scale: float, mask="none", *, dense: bool = False, window=None, sinks=None,
-                             rope=None, norms=None) -> torch.Tensor:
+                             rope=None, norms=None, step=None) -> torch.Tensor:
     """queries [B, Hq, L, D], keys / values [B, Hkv, L, D] -> [B, Hq, L, D].
 
     dense: attention over every token instead of the selected blocks, for
@@ -33,10 +33,27 @@ def attentionWithCacheUpdate(queries: torch.Tensor, keys: torch.Tensor, values: 
     norms: (qWeight, kWeight, eps) or (qWeight, kWeight, eps, weightOffset) of
     the per-head RMS norms ahead of the rope, in the same pass.  Queries and
     keys may then be views into a fused projection; values are contiguous in any
-    case (of a view, the caller makes a copy)."""
+    case (of a view, the caller makes a copy).
+
+    step: a Step that was mapped for the new tokens.  queries [rows, Hq, D] and
+    keys / values [rows, Hkv, D] are its packed rows, with their positions
+    (step.positions), all of them views if need be; they are appended and
+    attend densely, each to what its request held and to its ancestors (mask
+    "none": the step says who sees whom)."""
     if not isinstance(cache, BlockSparseKVCache):
         raise TypeError("attentionWithCacheUpdate here handles BlockSparseKVCache only; "
                         "other caches use the reference's dense path")
+    if step is not None:
+        if rope is not None or norms is not None or mask not in ("none", None):
+            raise ValueError("a step's rows come with their positions, and take no mask")
+        # nothing is appended that could not be attended to
+        cache._check_packed(queries, "queries", cache._hq, step.rows)
+        cache._check_window(window)
+        cache._check_sinks(sinks)
+        if step.ancestors is None:
+            raise ValueError("a step of more than 64 tokens a request can be appended, not attended to")
+        cache.appendPacked(keys, values, step)
+        return cache.attendTree(queries, step, scale, window=window, sinks=sinks)
     if (window is not None or sinks is not None) and not dense:
         raise ValueError("window and sinks belong to dense attention (dense=True)")
     if norms is not None and rope is None:

@@ -24,6 +24,7 @@ from . import _lib
 from ._lib import BsattnError, check, i32_array, lib
 
 _Strides = ctypes.c_int64 * 3
+_RowStrides = ctypes.c_int64 * 2
 _DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
 
@@ -534,6 +535,69 @@ class BlockSparseKVCache:
                                            qw, kw, eps, weightOffset, _row_ids(seq_ids, B), B, L, pos, q.data_ptr(),
                                            k.data_ptr(), _stream(self.device)))
         return q, k
+
+    # -- verification steps ------------------------------------------------------
+    def _check_packed(self, t: torch.Tensor, name: str, heads: int, rows: int):
+        """(element strides between rows and heads of t [rows, heads, D]; none
+        where it is dense)."""
+        shape = t.shape
+        if t.dtype is not self.dtype or t.get_device() != self._index:
+            raise ValueError(f"{name} must be a {self.dtype} tensor on {self.device}")
+        if len(shape) != 3 or shape[0] != rows or shape[1] != heads or shape[2] != self._dim:
+            raise ValueError(f"{name} must be [{rows}, {heads}, {self._dim}], got {tuple(shape)}")
+        if t.data_ptr() & 15 == 0:
+            if t.is_contiguous():
+                return None
+            # (torch gives a dimension of one element any stride)
+            s0, s1, s2 = t.stride()
+            s0, s1 = s0 if rows > 1 else 0, s1 if heads > 1 else 0
+            if s2 == 1 and not (s0 | s1) & 7:
+                return _RowStrides(s0, s1)
+        raise ValueError(f"{name} must have contiguous, 16-byte aligned heads, got strides {t.stride()} at "
+                         f"offset {t.storage_offset()}")
+
+    def appendPacked(self, keys: torch.Tensor, values: torch.Tensor, step) -> None:
+        """Appends a step's rows, keys / values [rows, Hkv, D] (views into a
+        fused projection will do), where step.map put them, at the device-side
+        lengths; the host's view follows with sync()."""
+        ks = self._check_packed(keys, "keys", self._hkv, step.rows)
+        vs = self._check_packed(values, "values", self._hkv, step.rows)
+        rc = self._lib.bsattn_append_packed(self._h, step._ref, keys.data_ptr(), ks, values.data_ptr(), vs,
+                                            _stream(self.device))
+        if rc:
+            check(rc)
+
+    def attendTree(self, queries: torch.Tensor, step, scale: float, window: Optional[int] = None,
+                   sinks: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Dense attention of a step's rows, queries [rows, Hq, D] (a view will
+        do): each sees what its request held before and its ancestors in the
+        tree, or those of them at the last `window` positions.  sinks as in
+        decodeDense.  Rows of no request are left as they are in out [rows, Hq,
+        D]."""
+        qs = self._check_packed(queries, "queries", self._hq, step.rows)
+        window, logits = self._check_window(window), self._check_sinks(sinks)
+        if out is None:
+            out = torch.empty_like(queries, memory_format=torch.contiguous_format)
+        elif out.shape != queries.shape or out.dtype is not self.dtype or out.get_device() != self._index \
+                or not out.is_contiguous() or out.data_ptr() & 15:
+            raise ValueError("out must be a contiguous, 16-byte aligned tensor shaped and typed like queries")
+        rc = self._lib.bsattn_attend_tree(self._h, step._ref, queries.data_ptr(), qs, window, logits, scale,
+                                          out.data_ptr(), _stream(self.device))
+        if rc:
+            check(rc)
+        return out
+
+    def keep(self, step, kept: torch.Tensor, nKept: torch.Tensor) -> None:
+        """Of the tokens that the step appended, request i keeps its nodes
+        kept[i, :nKept[i]] (int32 [n, width] and [n], ascending), moved together
+        behind what it held before; the others are dropped."""
+        n = step._n
+        if kept.dim() != 2 or kept.shape[1] < 1:
+            raise ValueError(f"kept must be [{n}, width], got {tuple(kept.shape)}")
+        rc = self._lib.bsattn_keep(self._h, step._ref, step._check_ints(kept, "kept", (n, kept.shape[1])), kept.shape[1],
+                                   step._check_ints(nKept, "nKept", (n,)), _stream(self.device))
+        if rc:
+            check(rc)
 
     # -- kernel timing -------------------------------------------------------
     def profile(self, enable: bool = True) -> None:

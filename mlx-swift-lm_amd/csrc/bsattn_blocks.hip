@@ -59,27 +59,21 @@ __device__ __forceinline__ int append_page(const Geometry& geo, const AppendPage
 // (0, 0, 0) applies the metadata patches for the launches that follow (nothing
 // here reads the metadata then).  grid (blocks touched, Hkv, n)
 // ---------------------------------------------------------------------------
+// block blk (on `page`) of a sequence that grows from old to end tokens: the
+// row of position p is row0 + p of k and v, whose rows are kld / vld elements
+// apart
 template <int DT, int TB>
-__global__ __launch_bounds__(4 * TB) void k_append_blocks(Geometry geo, AppendBatch ab, AppendPages pg,
-                                                          PatchBatch pb, const uint16_t* __restrict__ k,
-                                                          const uint16_t* __restrict__ v) {
+__device__ __forceinline__ void append_block(const Geometry& geo, int seq, int h, int old, int end, int blk, int page,
+                                             const uint16_t* __restrict__ k, int64_t kld, const uint16_t* __restrict__ v,
+                                             int64_t vld, int64_t row0) {
   constexpr int SEG = TB / 32;  // 32-token segments of a block
   __shared__ u32x4 s_v[SEG][512];
   __shared__ u32x4 s_k[TB][17];  // a padded row per token
-  const int x = blockIdx.x, h = blockIdx.y, bi = blockIdx.z;
-  if (x == 0 && h == 0 && bi == 0)
-    for (int i = threadIdx.x; i < pb.n; i += 4 * TB) geo.meta[pb.idx[i]] = pb.val[i];
-  const int old = ab.old_len[bi], end = old + ab.L;
-  const int blk = old / TB + x;
-  if (blk * TB >= end) return;
-  const int seq = ab.seq[bi];
-  const int page = append_page(geo, pg, seq, bi, x, blk);
   const bool fills = (blk + 1) * TB <= end;
   uint8_t* slab = geo.pool + ((size_t)page * geo.hkv + h) * geo.slab_bytes;
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int seg = wave % SEG;
   const int seg0 = blk * TB + 32 * seg;  // the segment's first position
-  const int64_t row0 = ((int64_t)bi * geo.hkv + h) * ab.L - old;  // row of position p: row0 + p
   if (wave < SEG) {
     if (seg0 < end && seg0 + 32 > old) {
       const int g = lane >> 4, c = lane & 15;
@@ -87,7 +81,7 @@ __global__ __launch_bounds__(4 * TB) void k_append_blocks(Geometry geo, AppendBa
       u32x4 row[8], out[8];
   #pragma unroll
       for (int i = 0; i < 8; ++i)  // positions that are not appended read a neighbour's row
-        row[i] = *(const u32x4*)(v + (row0 + min(max(p0 + i, old), end - 1)) * kHeadDim + 8 * c);
+        row[i] = *(const u32x4*)(v + (row0 + min(max(p0 + i, old), end - 1)) * vld + 8 * c);
       transpose8x8(row, out);
   #pragma unroll
       for (int e = 0; e < 8; ++e) s_v[seg][v_place(c >> 1, 16 * g + 8 * (c & 1) + e)] = out[e];
@@ -117,7 +111,7 @@ __global__ __launch_bounds__(4 * TB) void k_append_blocks(Geometry geo, AppendBa
 #pragma unroll
     for (int f = 0; f < 8; ++f) {
       const int p = seg0 + k_seg_tok(f >> 2, m);
-      const u32x4* src = p >= old && p < end ? (const u32x4*)(k + (row0 + p) * kHeadDim + 32 * (f & 3) + 8 * g)
+      const u32x4* src = p >= old && p < end ? (const u32x4*)(k + (row0 + p) * kld + 32 * (f & 3) + 8 * g)
                                              : Kf + f * 64;
       kr[f] = *src;
     }
@@ -145,6 +139,68 @@ __global__ __launch_bounds__(4 * TB) void k_append_blocks(Geometry geo, AppendBa
     constexpr float inv = 1.0f / (float)TB;
     ((uint32_t*)summary_row(geo, seq, h, blk))[threadIdx.x] = pack2<DT>(__fmul_rn(a, inv), __fmul_rn(b, inv));
   }
+}
+
+template <int DT, int TB>
+__global__ __launch_bounds__(4 * TB) void k_append_blocks(Geometry geo, AppendBatch ab, AppendPages pg,
+                                                          PatchBatch pb, const uint16_t* __restrict__ k,
+                                                          const uint16_t* __restrict__ v) {
+  const int x = blockIdx.x, h = blockIdx.y, bi = blockIdx.z;
+  if (x == 0 && h == 0 && bi == 0)
+    for (int i = threadIdx.x; i < pb.n; i += 4 * TB) geo.meta[pb.idx[i]] = pb.val[i];
+  const int old = ab.old_len[bi], end = old + ab.L;
+  const int blk = old / TB + x;
+  if (blk * TB >= end) return;
+  const int seq = ab.seq[bi];
+  const int page = append_page(geo, pg, seq, bi, x, blk);
+  append_block<DT, TB>(geo, seq, h, old, end, blk, page, k, kHeadDim, v, kHeadDim,
+                       ((int64_t)bi * geo.hkv + h) * ab.L - old);
+}
+
+// ---------------------------------------------------------------------------
+// append of a step's packed rows, by the blocks that its requests touch.  Each
+// workgroup finds its block from the requests' lengths (a lane each) and takes
+// its page from the slot of the block's first new token: the metadata is not
+// read, so the first workgroup can set the lengths.  grid (most blocks touched,
+// Hkv)
+// ---------------------------------------------------------------------------
+struct PackedBlock {
+  int seq, old, end, blk, page;  // page: -1 past the last block
+  int64_t row0;                  // the row of position p: row0 + p
+};
+template <int TB>
+__device__ __forceinline__ PackedBlock packed_block(const Geometry& geo, const StepRows& sr) {
+  const int lane = threadIdx.x & 63, x = blockIdx.x;
+  const int at = min(lane, sr.n - 1);
+  const int taken = lane < sr.n ? sr.taken[at] : 0, end = sr.ends[at];
+  if (x == 0 && blockIdx.y == 0 && (int)threadIdx.x < sr.n && taken > 0) geo.meta[sr.ids[at]] = end;
+  const int blocks = taken > 0 ? (end - 1) / TB - (end - taken) / TB + 1 : 0;
+  const int upto = wave_scan_incl(blocks);
+  const uint64_t holds = __ballot(x >= upto - blocks && x < upto);
+  PackedBlock b;
+  b.page = -1;
+  if (holds == 0) return b;
+  const int i = __ffsll((unsigned long long)holds) - 1;
+  b.seq = sr.ids[i];
+  b.end = __builtin_amdgcn_readlane(end, i);
+  b.old = b.end - __builtin_amdgcn_readlane(taken, i);
+  b.blk = b.old / TB + x - __builtin_amdgcn_readlane(upto - blocks, i);
+  b.row0 = (int64_t)uniform(sr.starts[i]) - b.old;
+  const int64_t row = b.row0 + max(b.blk * TB, b.old);
+  const int slot = row >= 0 && row < sr.rows ? uniform(sr.slots[row]) : -1;
+  const int page = slot / TB;
+  if (slot >= 0 && page < sr.pages) b.page = page;
+  return b;
+}
+
+template <int DT, int TB>
+__global__ __launch_bounds__(4 * TB) void k_append_packed(Geometry geo, StepRows sr, const uint16_t* __restrict__ k,
+                                                          int64_t kr, int64_t kh, const uint16_t* __restrict__ v,
+                                                          int64_t vr, int64_t vh) {
+  const int h = blockIdx.y;
+  const PackedBlock b = packed_block<TB>(geo, sr);
+  if (b.page < 0) return;
+  append_block<DT, TB>(geo, b.seq, h, b.old, b.end, b.blk, b.page, k + h * kh, kr, v + h * vh, vr, b.row0);
 }
 
 // ---------------------------------------------------------------------------
@@ -302,23 +358,16 @@ struct QuantDst {
 // codes are brought into the tile's order in LDS, which is also what the
 // summary's fold reads.  grid (blocks touched, Hkv, n)
 // ---------------------------------------------------------------------------
+// (arguments as append_block's; kld, vld: of k16 / v16)
 template <int KB, int TB, bool QUANTIZE>
-__global__ __launch_bounds__(4 * TB) void k_append_blocks_q(Geometry geo, AppendBatch ab, AppendPages pg,
-                                                            PatchBatch pb, QuantSrc src) {
+__device__ __forceinline__ void append_block_q(const Geometry& geo, int seq, int h, int old, int end, int blk, int page,
+                                               const QuantSrc& src, int64_t kld, int64_t vld, int64_t row0) {
   constexpr int SEG = TB / 32, W = KB / 4, WPR = QCode<KB>::WPR;
   constexpr int NVF = KB / 2;      // V fragments of a segment
   constexpr int KF = KB / 4;       // K fragments of a 16-token tile
   __shared__ u32x4 s_v[SEG][NVF * 64];
   __shared__ u32x4 s_k[TB * KB];   // the K code tile
   __shared__ u32x4 s_sb[TB];       // scales / biases, by sb_entry
-  const int x = blockIdx.x, h = blockIdx.y, bi = blockIdx.z;
-  if (x == 0 && h == 0 && bi == 0)
-    for (int i = threadIdx.x; i < pb.n; i += 4 * TB) geo.meta[pb.idx[i]] = pb.val[i];
-  const int old = ab.old_len[bi], end = old + ab.L;
-  const int blk = old / TB + x;
-  if (blk * TB >= end) return;
-  const int seq = ab.seq[bi];
-  const int page = append_page(geo, pg, seq, bi, x, blk);
   const bool fills = (blk + 1) * TB <= end;
   uint8_t* slab = geo.pool + ((size_t)page * geo.hkv + h) * geo.slab_bytes;
   u32x4* Sb = (u32x4*)(slab + geo.sb_off);
@@ -326,7 +375,6 @@ __global__ __launch_bounds__(4 * TB) void k_append_blocks_q(Geometry geo, Append
   const int seg = wave % SEG;
   const bool is_v = wave < SEG;
   const int seg0 = blk * TB + 32 * seg;
-  const int64_t row0 = ((int64_t)bi * geo.hkv + h) * ab.L - old;  // row of position p: row0 + p
   auto appended = [&](int p) { return p >= old && p < end; };
   if (seg0 < end && seg0 + 32 > old) {
     const int g = lane >> 4, c = lane & 15;
@@ -336,7 +384,7 @@ __global__ __launch_bounds__(4 * TB) void k_append_blocks_q(Geometry geo, Append
       u32x4 raw[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i)  // positions that are not appended read a neighbour's row
-        raw[i] = *(const u32x4*)((is_v ? src.v16 : src.k16) + (row0 + min(max(p0 + i, old), end - 1)) * kHeadDim + 8 * c);
+        raw[i] = *(const u32x4*)((is_v ? src.v16 : src.k16) + (row0 + min(max(p0 + i, old), end - 1)) * (is_v ? vld : kld) + 8 * c);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         uint32_t codes[8];
@@ -437,6 +485,35 @@ __global__ __launch_bounds__(4 * TB) void k_append_blocks_q(Geometry geo, Append
     summary_row(geo, seq, h, blk)[tid] = fold_block_q<KB>((const uint8_t*)s_k, (const uint16_t*)s_sb, TB, tid);
 }
 
+template <int KB, int TB, bool QUANTIZE>
+__global__ __launch_bounds__(4 * TB) void k_append_blocks_q(Geometry geo, AppendBatch ab, AppendPages pg,
+                                                            PatchBatch pb, QuantSrc src) {
+  const int x = blockIdx.x, h = blockIdx.y, bi = blockIdx.z;
+  if (x == 0 && h == 0 && bi == 0)
+    for (int i = threadIdx.x; i < pb.n; i += 4 * TB) geo.meta[pb.idx[i]] = pb.val[i];
+  const int old = ab.old_len[bi], end = old + ab.L;
+  const int blk = old / TB + x;
+  if (blk * TB >= end) return;
+  const int seq = ab.seq[bi];
+  const int page = append_page(geo, pg, seq, bi, x, blk);
+  append_block_q<KB, TB, QUANTIZE>(geo, seq, h, old, end, blk, page, src, kHeadDim, kHeadDim,
+                                   ((int64_t)bi * geo.hkv + h) * ab.L - old);
+}
+
+// a step's packed rows (as k_append_packed)
+template <int KB, int TB>
+__global__ __launch_bounds__(4 * TB) void k_append_packed_q(Geometry geo, StepRows sr, const uint16_t* __restrict__ k,
+                                                            int64_t kr, int64_t kh, const uint16_t* __restrict__ v,
+                                                            int64_t vr, int64_t vh) {
+  const int h = blockIdx.y;
+  const PackedBlock b = packed_block<TB>(geo, sr);
+  if (b.page < 0) return;
+  QuantSrc src{};
+  src.k16 = k + h * kh;
+  src.v16 = v + h * vh;
+  append_block_q<KB, TB, true>(geo, b.seq, h, b.old, b.end, b.blk, b.page, src, kr, vr, b.row0);
+}
+
 // ---------------------------------------------------------------------------
 // export in the MLX layout: kw / vw [n, Hkv, T, D*b/32] uint32 (LSB first),
 // scales / biases [n, Hkv, T, D/64] fp16.  grid (ceil(T / TB), Hkv, n)
@@ -529,6 +606,21 @@ hipError_t launch_append(const Geometry& g, const AppendBatch& ab, const AppendP
     if (g.dtype == 0) launch(k_append_blocks<0, 32>, grid, dim3(128), 0, s, prof, kind, g, ab, pg, pb, kk, vv);
     else launch(k_append_blocks<1, 32>, grid, dim3(128), 0, s, prof, kind, g, ab, pg, pb, kk, vv);
   }
+  return hipGetLastError();
+}
+
+hipError_t launch_append_packed(const Geometry& g, const StepRows& sr, const void* k, int64_t kr, int64_t kh,
+                                const void* v, int64_t vr, int64_t vh, hipStream_t s, Timing* prof) {
+  // a request of c tokens touches at most (c + tb - 2) / tb + 1 blocks
+  const int64_t each = ((int64_t)sr.max_tokens + g.tb - 2) / g.tb + 1;
+  const int64_t blocks = std::min<int64_t>(sr.n * each, sr.rows / g.tb + 2 * (int64_t)sr.n);
+  const dim3 grid((unsigned)blocks, g.hkv), blk(4 * g.tb);
+  const uint16_t *kk = (const uint16_t*)k, *vv = (const uint16_t*)v;
+  auto go = [&](auto kernel) { launch(kernel, grid, blk, 0, s, prof, kProfAppend, g, sr, kk, kr, kh, vv, vr, vh); };
+  if (g.kv_bits == 4) g.tb == 64 ? go(k_append_packed_q<4, 64>) : go(k_append_packed_q<4, 32>);
+  else if (g.kv_bits == 8) g.tb == 64 ? go(k_append_packed_q<8, 64>) : go(k_append_packed_q<8, 32>);
+  else if (g.dtype == 0) g.tb == 64 ? go(k_append_packed<0, 64>) : go(k_append_packed<0, 32>);
+  else g.tb == 64 ? go(k_append_packed<1, 64>) : go(k_append_packed<1, 32>);
   return hipGetLastError();
 }
 

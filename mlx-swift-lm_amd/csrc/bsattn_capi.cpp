@@ -372,6 +372,7 @@ int bsattn_append_step(bsattn_cache* c, const void* k, const void* v, const int3
     if (e != hipSuccess) return hip_fail(e, "append step launch");
   }
   c->stale = true;
+  c->step = 0;
   return BSATTN_OK;
 } catch (...) {
   return on_exception();
@@ -455,6 +456,7 @@ int append_impl(bsattn_cache* c, const int32_t* seq_ids, int32_t n_seqs, int32_t
     if (e != hipSuccess) return hip_fail(e, "append launch");
   }
   ap.sent();
+  c->step = 0;
   for (int s_ : seqs) c->len[s_] += n_tokens;
   return BSATTN_OK;
 }
@@ -776,6 +778,7 @@ int bsattn_append_decode(bsattn_cache* c, const void* k, const void* v, const vo
   prof_collect(c, prof);
   if (e != hipSuccess) return hip_fail(e, "append-decode launch");
   patches.sent();
+  c->step = 0;
   for (int sq : seqs) c->len[sq] += 1;
   return BSATTN_OK;
 } catch (...) {
@@ -924,6 +927,7 @@ int bsattn_trim(bsattn_cache* c, const int32_t* seq_ids, int32_t n_seqs, int32_t
   UnsharedTails tails;
   rc = unshare_tails(c, seqs, n_tokens, (hipStream_t)stream, tails);
   if (rc) return rc;
+  c->step = 0;
   c->free_pages.resize(c->free_pages.size() - tails.from_free);
   for (int i = 0; i < n_seqs; ++i) {
     const int sq = seqs[i];
@@ -958,6 +962,7 @@ int bsattn_reset(bsattn_cache* c, const int32_t* seq_ids, int32_t n_seqs, void* 
   if (rc) return rc;
   Patches patches;
   patches.reserve(2 * seqs.size());  // the loop below then cannot throw
+  c->step = 0;
   for (int sq : seqs) {
     c->len[sq] = 0;
     release_pages(c, sq, 0, patches);

@@ -103,6 +103,10 @@ struct bsattn_cache {
   // metadata words that a failed launch may have left unset (or set ahead of
   // the host): sent before the next call's own (send_unsent)
   bsattn::Patches unsent;
+  // the step that the cache was last mapped for (0: none, or the host has
+  // changed its sequences since), and its place among the step's caches
+  uint64_t step = 0;
+  int32_t step_layer = 0;
   // opt-in per-kernel timing (bsattn_profile_*)
   bool profiling = false;
   std::vector<hipEvent_t> event_pool;
@@ -371,8 +375,20 @@ inline void prof_collect(bsattn_cache* c, Timing* tm) {
   }
 }
 
+// workspace and event for the parts of a call: the cache's own where they fit
+// (no event: a cache's calls follow each other), otherwise as for a split
+// prefill
+template <typename F>
+hipError_t with_partials(bsattn_cache* c, int64_t rows, hipStream_t s, F launch) {
+  if (rows <= (int64_t)std::min(kMaxBatch, c->d.max_seqs * kMaxQueries) * c->geo.hq * c->geo.nsplit)
+    return launch(c->partials, nullptr);
+  if (capturing(s)) return launch(graph_workspace(c, rows), nullptr);
+  PrefillSpaces* spaces = PrefillSpaces::of(c->d.device);
+  return spaces ? spaces->with(s, launch) : launch(nullptr, nullptr);
+}
+
 // Calls that need the exact token counts refuse while device-side appends
-// (bsattn_append_step) may have advanced them past the host's view.
+// (bsattn_append_step, bsattn_append_packed) may have moved them past the host's view.
 inline int check_synced(const bsattn_cache* c) {
   if (c->stale)
     return fail(BSATTN_ERR_INVALID, "device-side lengths may be ahead of the host's view "

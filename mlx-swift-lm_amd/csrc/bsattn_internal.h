@@ -116,7 +116,8 @@ struct StepAppend {
 enum ProfKind {
   kProfScore = 0, kProfTopk = 1, kProfAttend = 2, kProfCombine = 3, kProfAppend = 4,
   kProfSummary = 5, kProfPrefill = 6, kProfRotate = 7, kProfDense = 8, kProfFork = 9,
-  kProfKinds = 10
+  kProfMap = 10, kProfTree = 11, kProfKeep = 12,
+  kProfKinds = 13
 };
 struct Timing {
   hipEvent_t start = nullptr, stop = nullptr;
@@ -312,6 +313,66 @@ int dense_plan(const Geometry& g, DenseBatch& db, int64_t* rows);
 // joins them records `done` (may be null)
 hipError_t launch_dense(const Geometry& g, const DenseBatch& db, int parts, const void* q, void* out, float* ws,
                         hipEvent_t done, hipStream_t s, Timing* prof);
+// ---------------------------------------------------------------------------
+// Verification steps (bsattn_step.hip, bsattn_tree.hip; packed appends in
+// bsattn_blocks.hip): requests of a step, and what its map wrote
+// ---------------------------------------------------------------------------
+constexpr int kMaxStepCaches = 128;  // caches a map serves (24 bytes each of its arguments)
+constexpr int kMaxNodes = 64;        // tokens of a request's tree: a bit each
+struct StepCache {
+  int32_t* meta;
+  int32_t bt_off, cap_off, mbps, tb;
+};
+struct StepMap {
+  int32_t n, rows, max_tokens, caches;
+  const int32_t* counts;
+  const int32_t* parents;  // or null: chains
+  int32_t* starts;
+  int32_t* taken;
+  int32_t* requests;
+  int32_t* positions;
+  uint64_t* ancestors;  // or null
+  int32_t* slots;       // [caches][rows]
+  int32_t* ends;        // [caches][n]
+  int32_t ids[kMaxBatch];
+  StepCache cache[kMaxStepCaches];
+};
+hipError_t launch_step_map(const StepMap& sm, hipStream_t s, Timing* prof);
+// a step as the launches on one of its caches take it (slots and ends are the
+// cache's own)
+struct StepRows {
+  int32_t n, rows, max_tokens;
+  int64_t pages;  // of the cache's pool
+  const int32_t* starts;
+  const int32_t* taken;
+  const int32_t* slots;
+  const int32_t* ends;
+  int32_t ids[kMaxBatch];
+};
+// rows of k / v: kr / vr elements apart, their heads kh / vh
+hipError_t launch_append_packed(const Geometry& g, const StepRows& sr, const void* k, int64_t kr, int64_t kh,
+                                const void* v, int64_t vr, int64_t vh, hipStream_t s, Timing* prof);
+hipError_t launch_keep(const Geometry& g, const StepRows& sr, const int32_t* kept, int width, const int32_t* n_kept,
+                       hipStream_t s, Timing* prof);
+// Tree attention.  Request i's tokens are cut into parts of `cu` units of 32;
+// they are the launch's parts part0[i] .. part0[i + 1] - 1, their partials the
+// blocks of hq rows (row0[i] + part * max_tokens + node).
+struct TreeBatch {
+  int32_t n, max_tokens, cu, window;
+  int32_t tiles, groups;  // column tiles of 16 in a workgroup, workgroups for a request's columns
+  float sl2;
+  const float* sinks;  // [hq], or null
+  const int32_t* starts;
+  const int32_t* taken;
+  const uint64_t* ancestors;
+  int64_t qr, qh;      // elements between rows and heads of q
+  int32_t ids[kMaxBatch], units[kMaxBatch], row0[kMaxBatch], part0[kMaxBatch + 1];
+};
+// sets cu, tiles, groups, row0 and part0 from units (the most of each request);
+// the rows of the workspace (0: none is needed)
+int64_t tree_plan(const Geometry& g, TreeBatch& tb);
+hipError_t launch_tree(const Geometry& g, const TreeBatch& tb, const void* q, void* out, float* ws, hipEvent_t done,
+                       hipStream_t s, Timing* prof);
 hipError_t launch_export(const Geometry& g, const SeqBatch& b, int T, void* k_out,
                          void* v_out, hipStream_t s);
 hipError_t launch_export_quantized(const Geometry& g, const SeqBatch& b, int T,

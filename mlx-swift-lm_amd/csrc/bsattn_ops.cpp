@@ -177,18 +177,6 @@ void dense_jobs(const bsattn_cache* c, const int32_t* ids, DenseBatch& db, hipSt
   if (saved > 0 && g.kv_bits != 0 && 4 * saved < left) dense_jobs(c, ids, db, s, false);
 }
 
-// workspace and event for the parts of a call: the cache's own where they fit
-// (no event: a cache's calls follow each other), otherwise as for a split
-// prefill
-template <typename F>
-hipError_t with_partials(bsattn_cache* c, int64_t rows, hipStream_t s, F launch) {
-  if (rows <= (int64_t)std::min(kMaxBatch, c->d.max_seqs * kMaxQueries) * c->geo.hq * c->geo.nsplit)
-    return launch(c->partials, nullptr);
-  if (capturing(s)) return launch(graph_workspace(c, rows), nullptr);
-  PrefillSpaces* spaces = PrefillSpaces::of(c->d.device);
-  return spaces ? spaces->with(s, launch) : launch(nullptr, nullptr);
-}
-
 }  // namespace
 
 extern "C" {
@@ -317,6 +305,7 @@ int bsattn_fork(bsattn_cache* c, const int32_t* src_ids, const int32_t* dst_ids,
     c->pages[dst[i]].swap(rows[i]);
     c->len[dst[i]] = tokens[i];
   }
+  c->step = 0;
   return BSATTN_OK;
 } catch (...) {
   return on_exception();

@@ -1,0 +1,244 @@
+// bsattn_steps.cpp -- the C ABI's verification steps: maps, packed appends,
+// tree attention, kept paths.  Argument checking and kernel sequencing.
+#include <hip/hip_runtime_api.h>
+
+#include <algorithm>
+#include <atomic>
+#include <climits>
+#include <vector>
+
+#include "bsattn_host.h"
+
+using namespace bsattn;
+
+static_assert(BSATTN_STEP_SEQS == kMaxBatch && BSATTN_STEP_CACHES == kMaxStepCaches && BSATTN_TREE_NODES == kMaxNodes,
+              "the header's limits are the kernels'");
+
+namespace {
+
+std::atomic<uint64_t> g_steps{0};  // names of the steps' maps
+
+int check_sizes(const bsattn_step& st) {
+  if (st.n_caches < 1 || st.n_caches > kMaxStepCaches)
+    return fail(BSATTN_ERR_INVALID, "n_caches %d out of range [1, %d]", st.n_caches, kMaxStepCaches);
+  if (st.rows < 1) return fail(BSATTN_ERR_INVALID, "rows must be >= 1 (got %d)", st.rows);
+  if (st.max_tokens < 1) return fail(BSATTN_ERR_INVALID, "max_tokens must be >= 1 (got %d)", st.max_tokens);
+  if (!st.starts || !st.taken || !st.requests || !st.positions || !st.slots || !st.ends ||
+      (!st.ancestors && st.max_tokens <= kMaxNodes))
+    return fail(BSATTN_ERR_INVALID, "null array in the step");
+  return BSATTN_OK;
+}
+
+// the step's last map is the last that the cache was mapped for, and the
+// cache's sequences are as they were then
+int check_step(const bsattn_cache* c, const bsattn_step* st) {
+  if (!c || !st) return fail(BSATTN_ERR_INVALID, "null argument");
+  if (int rc = check_sizes(*st)) return rc;
+  if (st->stamp == 0 || c->step != st->stamp)
+    return fail(BSATTN_ERR_INVALID, "the cache was not mapped for this step, or has changed since: call bsattn_step_map");
+  if (st->n_seqs < 1 || st->n_seqs > std::min(kMaxBatch, c->d.max_seqs) || c->step_layer >= st->n_caches)
+    return fail(BSATTN_ERR_INVALID, "the step has changed since its map");
+  for (int i = 0; i < st->n_seqs; ++i)
+    if (st->ids[i] < 0 || st->ids[i] >= c->d.max_seqs) return fail(BSATTN_ERR_INVALID, "the step has changed since its map");
+  return BSATTN_OK;
+}
+
+int check_tree(const bsattn_step* st) {
+  if (st->max_tokens > kMaxNodes)
+    return fail(BSATTN_ERR_INVALID, "a step of up to %d tokens a request: trees have at most %d", st->max_tokens,
+                kMaxNodes);
+  return BSATTN_OK;
+}
+
+StepRows step_rows(const bsattn_cache* c, const bsattn_step& st) {
+  StepRows sr{};
+  sr.n = st.n_seqs;
+  sr.rows = st.rows;
+  sr.max_tokens = st.max_tokens;
+  sr.pages = c->num_pages;
+  sr.starts = st.starts;
+  sr.taken = st.taken;
+  sr.slots = st.slots + (size_t)c->step_layer * st.rows;
+  sr.ends = st.ends + (size_t)c->step_layer * st.n_seqs;
+  std::copy(st.ids, st.ids + st.n_seqs, sr.ids);
+  return sr;
+}
+
+// rows [rows, heads, D] and the elements between their rows and heads
+int packed_strides(const char* name, const void* x, const int64_t* strides, int heads, int64_t (&out)[2]) {
+  if (!x) return fail(BSATTN_ERR_INVALID, "null argument");
+  if ((uintptr_t)x % 16) return fail(BSATTN_ERR_INVALID, "%s must be 16-byte aligned", name);
+  out[0] = strides ? strides[0] : (int64_t)heads * kHeadDim;
+  out[1] = strides ? strides[1] : kHeadDim;
+  for (int64_t st : out)
+    if (st % 8 || st < 0)
+      return fail(BSATTN_ERR_INVALID, "%s strides must be multiples of 8 elements and >= 0 (got %lld)", name,
+                  (long long)st);
+  return BSATTN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int bsattn_step_map(bsattn_cache* const* caches, bsattn_step* st, const int32_t* counts, const int32_t* parents,
+                    const int32_t* seq_ids, int32_t n_seqs, void* stream) try {
+  if (!caches || !st || !counts) return fail(BSATTN_ERR_INVALID, "null argument");
+  if (int rc = check_sizes(*st)) return rc;
+  if (n_seqs > kMaxBatch) return fail(BSATTN_ERR_RANGE, "n_seqs %d exceeds the %d requests of a step", n_seqs, kMaxBatch);
+  if (parents && st->max_tokens > kMaxNodes)
+    return fail(BSATTN_ERR_INVALID, "a tree has at most %d nodes (max_tokens is %d)", kMaxNodes, st->max_tokens);
+  std::vector<int32_t> seqs;
+  bool synced = true;
+  for (int l = 0; l < st->n_caches; ++l) {
+    const bsattn_cache* c = caches[l];
+    if (!c) return fail(BSATTN_ERR_INVALID, "null cache");
+    if (c->d.device != caches[0]->d.device) return fail(BSATTN_ERR_INVALID, "the step's caches are on different GPUs");
+    for (int k = 0; k < l; ++k)
+      if (caches[k] == c) return fail(BSATTN_ERR_INVALID, "a cache is listed twice");
+    if (int rc = seq_list(c, seq_ids, n_seqs, seqs)) return rc;
+    if (c->num_pages * c->d.block_size > INT32_MAX)
+      return fail(BSATTN_ERR_RANGE, "a pool of %lld tokens: slots are 32-bit", (long long)(c->num_pages * c->d.block_size));
+    synced = synced && !c->stale;
+  }
+  if (synced)
+    for (int l = 1; l < st->n_caches; ++l)
+      for (int s : seqs)
+        if (caches[l]->len[s] != caches[0]->len[s])
+          return fail(BSATTN_ERR_INVALID, "sequence %d holds %d tokens in the step's first cache and %d in another", s,
+                      caches[0]->len[s], caches[l]->len[s]);
+  DeviceGuard dg(caches[0]->d.device);
+  if (!dg.ok) return fail(BSATTN_ERR_HIP, "hipSetDevice(%d) failed", caches[0]->d.device);
+  hipStream_t s = (hipStream_t)stream;
+  StepMap sm{};
+  sm.n = n_seqs;
+  sm.rows = st->rows;
+  sm.max_tokens = st->max_tokens;
+  sm.caches = st->n_caches;
+  sm.counts = counts;
+  sm.parents = parents;
+  sm.starts = st->starts;
+  sm.taken = st->taken;
+  sm.requests = st->requests;
+  sm.positions = st->positions;
+  sm.ancestors = st->ancestors;
+  sm.slots = st->slots;
+  sm.ends = st->ends;
+  std::copy(seqs.begin(), seqs.end(), sm.ids);
+  for (int l = 0; l < st->n_caches; ++l) {
+    if (int rc = send_unsent(caches[l], s)) return rc;
+    const Geometry& g = caches[l]->geo;
+    sm.cache[l] = StepCache{g.meta, g.bt_off, g.cap_off, g.mbps, g.tb};
+  }
+  Timing tm[kProfKinds];
+  Timing* prof = prof_slots(caches[0], s, tm);
+  const hipError_t e = launch_step_map(sm, s, prof);
+  prof_collect(caches[0], prof);
+  if (e != hipSuccess) return hip_fail(e, "step map launch");
+  st->n_seqs = n_seqs;
+  std::copy(seqs.begin(), seqs.end(), st->ids);
+  st->stamp = ++g_steps;
+  for (int l = 0; l < st->n_caches; ++l) {
+    caches[l]->step = st->stamp;
+    caches[l]->step_layer = l;
+  }
+  return BSATTN_OK;
+} catch (...) {
+  return on_exception();
+}
+
+int bsattn_append_packed(bsattn_cache* c, const bsattn_step* st, const void* k, const int64_t* k_strides,
+                         const void* v, const int64_t* v_strides, void* stream) try {
+  if (int rc = check_step(c, st)) return rc;
+  int64_t ks[2], vs[2];
+  if (int rc = packed_strides("k", k, k_strides, c->geo.hkv, ks)) return rc;
+  if (int rc = packed_strides("v", v, v_strides, c->geo.hkv, vs)) return rc;
+  DeviceGuard dg(c->d.device);
+  if (!dg.ok) return fail(BSATTN_ERR_HIP, "hipSetDevice(%d) failed", c->d.device);
+  hipStream_t s = (hipStream_t)stream;
+  if (int rc = send_unsent(c, s)) return rc;
+  Timing tm[kProfKinds];
+  Timing* prof = prof_slots(c, s, tm);
+  const hipError_t e = launch_append_packed(c->geo, step_rows(c, *st), k, ks[0], ks[1], v, vs[0], vs[1], s, prof);
+  prof_collect(c, prof);
+  if (e != hipSuccess) return hip_fail(e, "packed append launch");
+  c->stale = true;
+  return BSATTN_OK;
+} catch (...) {
+  return on_exception();
+}
+
+int bsattn_attend_tree(bsattn_cache* c, const bsattn_step* st, const void* q, const int64_t* q_strides, int32_t window,
+                       const float* sinks, float scale, void* out, void* stream) try {
+  if (int rc = check_step(c, st)) return rc;
+  if (int rc = check_tree(st)) return rc;
+  if (!out) return fail(BSATTN_ERR_INVALID, "null argument");
+  if ((uintptr_t)out % 16) return fail(BSATTN_ERR_INVALID, "out must be 16-byte aligned");
+  if (window < 0) return fail(BSATTN_ERR_INVALID, "window must be >= 0 (got %d)", window);
+  if ((uintptr_t)sinks % 4) return fail(BSATTN_ERR_INVALID, "sinks must be 4-byte aligned");
+  const Geometry& g = c->geo;
+  int64_t qs[2];
+  if (int rc = packed_strides("q", q, q_strides, g.hq, qs)) return rc;
+  DeviceGuard dg(c->d.device);
+  if (!dg.ok) return fail(BSATTN_ERR_HIP, "hipSetDevice(%d) failed", c->d.device);
+  hipStream_t s = (hipStream_t)stream;
+  if (int rc = send_unsent(c, s)) return rc;
+  TreeBatch tb{};
+  tb.n = st->n_seqs;
+  tb.max_tokens = std::min(st->max_tokens, st->rows);
+  tb.window = window;
+  tb.sl2 = scale * 1.4426950408889634f;
+  tb.sinks = sinks;
+  tb.starts = st->starts;
+  tb.taken = st->taken;
+  tb.ancestors = st->ancestors;
+  tb.qr = qs[0];
+  tb.qh = qs[1];
+  for (int i = 0; i < tb.n; ++i) {
+    tb.ids[i] = st->ids[i];
+    // (the device-side length is at most what the pages hold; a window can
+    // begin and end inside a unit, and the tree's positions follow it)
+    int64_t units = (int64_t)c->pages[tb.ids[i]].size() * (g.tb / 32);
+    if (window > 0) units = std::min<int64_t>(units, ((int64_t)window + tb.max_tokens + 62) / 32);
+    tb.units[i] = (int32_t)units;
+  }
+  const int64_t rows = tree_plan(g, tb);
+  Timing tm[kProfKinds];
+  Timing* prof = prof_slots(c, s, tm);
+  auto run = [&](float* ws, hipEvent_t done) {
+    if (ws) return launch_tree(g, tb, q, out, ws, done, s, prof);
+    TreeBatch whole = tb;  // (without a workspace: one part a request)
+    whole.cu = INT32_MAX / 32;
+    for (int i = 0; i <= whole.n; ++i) whole.part0[i] = i;
+    return launch_tree(g, whole, q, out, nullptr, nullptr, s, prof);
+  };
+  const hipError_t e = rows == 0 ? launch_tree(g, tb, q, out, nullptr, nullptr, s, prof) : with_partials(c, rows, s, run);
+  prof_collect(c, prof);
+  if (e != hipSuccess) return hip_fail(e, "tree attention launch");
+  return BSATTN_OK;
+} catch (...) {
+  return on_exception();
+}
+
+int bsattn_keep(bsattn_cache* c, const bsattn_step* st, const int32_t* kept, int32_t width, const int32_t* n_kept,
+                void* stream) try {
+  if (int rc = check_step(c, st)) return rc;
+  if (int rc = check_tree(st)) return rc;
+  if (!kept || !n_kept) return fail(BSATTN_ERR_INVALID, "null argument");
+  if (width < 1) return fail(BSATTN_ERR_INVALID, "width must be >= 1 (got %d)", width);
+  DeviceGuard dg(c->d.device);
+  if (!dg.ok) return fail(BSATTN_ERR_HIP, "hipSetDevice(%d) failed", c->d.device);
+  hipStream_t s = (hipStream_t)stream;
+  if (int rc = send_unsent(c, s)) return rc;
+  Timing tm[kProfKinds];
+  Timing* prof = prof_slots(c, s, tm);
+  const hipError_t e = launch_keep(c->geo, step_rows(c, *st), kept, width, n_kept, s, prof);
+  prof_collect(c, prof);
+  if (e != hipSuccess) return hip_fail(e, "keep launch");
+  c->stale = true;
+  return BSATTN_OK;
+} catch (...) {
+  return on_exception();
+}
+
+}  // extern "C"

@@ -1,0 +1,577 @@
+// bsattn_tree.hip -- attention of a tree of drafted tokens over the paged cache:
+// node j of a request, N nodes behind P tokens, sees the tokens t < P (or those
+// at the last `window` positions up to its own) and its ancestors P + a,
+//   o = sum_t p_t v_t / (sum_t p_t + exp(sink - m)),  p_t = exp(scale q.k_t - m)
+// for 16-bit and affine caches.
+//
+// A workgroup takes a part of one (request, kv head)'s tokens, in units of 32,
+// for up to 16 CT columns, each a (node, query head) pair; its four waves take
+// every fourth unit of the part for all of the columns.  K and V lie in the slabs as
+// the matrix instructions take them, so a wave works in registers alone:
+//   S^T[token][col] = K[token][:] . Q^T      (A = K rows, B = Q^T)
+//   O^T[dim][col]  += V^T[dim][token] . P^T  (A = V^T,    B = P^T)
+// A lane (column n, group g) holds column n's share of tokens 8g .. 8g + 7 in
+// both, and the next unit's K is asked for as soon as this one's is used, its V
+// likewise.  P enters as two 16-bit parts, for 16 (bf16) or 22 (fp16) bits.
+// Only the units that hold drafted tokens, or where a window begins, are masked.
+#include <hip/hip_ext.h>
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "bsattn_append.h"
+#include "bsattn_codes.h"
+#include "bsattn_device.h"
+
+namespace bsattn {
+
+constexpr float kTreeLog2e = 1.4426950408889634f;
+// The softmax's reference is raised when a score passes it by more than 2^kSlack
+constexpr float kTreeSlack = 6.0f;
+constexpr float kTreeTop = 14.0f;
+
+// What a request brings to a launch, and the units of its part
+struct TreeRange {
+  int T, N, P, lo, u0, units, cu;
+};
+__device__ __forceinline__ TreeRange tree_range(const Geometry& geo, const TreeBatch& tb, int i) {
+  TreeRange r;
+  r.T = uniform(geo.meta[tb.ids[i]]);
+  r.N = min(min(uniform(tb.taken[i]), tb.max_tokens), r.T);
+  r.P = r.T - r.N;
+  r.lo = tb.window > 0 ? max(0, r.P - tb.window + 1) : 0;  // the first token that a root sees
+  r.u0 = r.lo >> 5;
+  r.units = r.N > 0 ? ((r.T - 1) >> 5) - r.u0 + 1 : 0;
+  // (more tokens than the launch was cut for, as when a graph replays after
+  // further reservations: as many parts, of more units each)
+  r.cu = tb.cu;
+  if (r.units > tb.units[i]) {
+    const int most = max(1, tb.part0[i + 1] - tb.part0[i]);
+    r.cu = max(r.cu, ((r.units + most - 1) / most + 3) & ~3);
+  }
+  return r;
+}
+
+// slabs of the units that a wave takes, the block table read through the scalar
+// cache one unit ahead
+struct TreePages {
+  const int32_t* bt;
+  int h, sh, last, unit, page;
+  __device__ __forceinline__ TreePages(const Geometry& geo, int seq, int h_, int last_, int u) : h(h_), last(last_) {
+    sh = geo.tb == 64 ? 1 : 0;
+    bt = block_table(geo, seq);
+    ask(u);
+  }
+  // (past the part's units: its last one)
+  __device__ __forceinline__ void ask(int u) {
+    unit = min(u, last);
+    page = *((const __attribute__((address_space(4))) int32_t*)(uintptr_t)(bt + (unit >> sh)));
+  }
+  __device__ __forceinline__ const uint8_t* slab(const Geometry& geo) const {
+    return geo.pool + ((size_t)page * geo.hkv + h) * geo.slab_bytes;
+  }
+};
+
+// weights x[0, 8) as an operand's two parts: hi cut to 16 bits, lo what is left, rounded
+template <int DT>
+__device__ __forceinline__ void tree_split(const float* x, u32x4& hi, u32x4& lo) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (DT == 1) {
+      const uint32_t a = __float_as_uint(x[2 * j]), b = __float_as_uint(x[2 * j + 1]);
+      hi[j] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+      lo[j] = cvt_pk<1>(x[2 * j] - __uint_as_float(a & 0xFFFF0000u), x[2 * j + 1] - __uint_as_float(b & 0xFFFF0000u));
+    } else {
+      const uint32_t w = cvt_pk<0>(x[2 * j], x[2 * j + 1]);
+      hi[j] = w;
+      lo[j] = cvt_pk<0>(x[2 * j] - lo_f(w), x[2 * j + 1] - hi_f(w));
+    }
+  }
+}
+
+// eight codes of a V fragment's dim tile as bf16 (exact)
+template <int KB>
+__device__ __forceinline__ u32x4 codes_bf16(const u32x4* vf, int dt) {
+  constexpr int DPF = QCode<KB>::DPF;
+  const u32x4& f = vf[dt / DPF];
+  u32x4 o;
+  auto pair = [](float a, float b) { return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u); };
+  if constexpr (KB == 4) {
+    // element e sits in nibble q_nib(e): even ones in the low half of the word
+    const uint32_t w = f[dt & 3], a = w & 0x0F0F0F0Fu, b = (w >> 4) & 0x0F0F0F0Fu;
+    auto el = [&](int e) {
+      const int nb = q_nib(e);
+      return (float)(((nb & 1 ? b : a) >> (8 * (nb >> 1))) & 0xFFu);
+    };
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = pair(el(2 * j), el(2 * j + 1));
+  } else {
+    const uint32_t a = f[2 * (dt & 1)], b = f[2 * (dt & 1) + 1];
+    auto el = [&](int e) { return (float)(((e < 4 ? a : b) >> (8 * (e & 3))) & 0xFFu); };
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = pair(el(2 * j), el(2 * j + 1));
+  }
+  return o;
+}
+
+// grid (8-fold interleaved (part, kv head) pairs and column groups): the
+// workgroups of one pair's groups lie a multiple of 8 apart, on one XCD, whose
+// L2 then holds the K and V they share
+template <int DT, int KB, int CT>
+__global__ __launch_bounds__(256, CT > 2 ? 1 : 2) void k_tree(Geometry geo, TreeBatch tb, const uint16_t* __restrict__ q,
+                                                             uint16_t* __restrict__ out, float* __restrict__ partials) {
+  static_assert(KB == 0 || DT == 0, "affine caches: fp16");
+  constexpr int PT = KB ? 1 : DT;  // P's type: weights times scales need bf16's range, and codes are exact in it
+  constexpr float kLift = PT == 0 ? kTreeTop - kTreeSlack : 0.0f;
+  constexpr int NK = KB ? 2 * QCode<KB ? KB : 4>::KF : 8, NV = KB ? 8 / QCode<KB ? KB : 4>::DPF : 8;
+  __shared__ uint64_t s_seen[kMaxNodes];  // each node's ancestors, those in its window
+  __shared__ int s_from[kMaxNodes];       // the first cached token it sees
+  __shared__ u32x4 s_sb[KB ? 4 : 1][KB ? 32 : 1];
+  __shared__ float s_m[4][16], s_l[4][16];
+  __shared__ __align__(16) float s_o[4][16][kHeadDim + 4];
+
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int n = lane & 15, g = lane >> 4, G = geo.group;
+  // which part, head and columns
+  const int total = tb.part0[tb.n], chunk = blockIdx.x / (8 * tb.groups), in = blockIdx.x - chunk * 8 * tb.groups;
+  const int pair = 8 * chunk + (in & 7), group = in >> 3;
+  const int h = uniform(pair / total), at = pair - h * total;
+  if (h >= geo.hkv) return;
+  const int i = uniform(__popcll(__ballot(lane < tb.n && tb.part0[min(lane, tb.n - 1)] <= at)) - 1);
+  const int part = at - tb.part0[i];
+  const TreeRange r = tree_range(geo, tb, i);
+  const int col0 = group * 16 * CT, cols = r.N * G;
+  const int parts = (r.units + r.cu - 1) / r.cu;
+  if (col0 >= cols || part >= parts) return;
+  const bool direct = tb.part0[i + 1] - tb.part0[i] <= 1;
+  const int start = uniform(tb.starts[i]);
+  const int ua = r.u0 + part * r.cu, ub = min(ua + r.cu, r.u0 + r.units);
+  const int seq = tb.ids[i];
+
+  if (threadIdx.x < kMaxNodes) {
+    const int j = threadIdx.x;
+    uint64_t seen = j < r.N ? tb.ancestors[start + j] : 0;
+    const int depth = __popcll(seen) - 1;
+    s_from[j] = tb.window > 0 ? r.P + depth - tb.window + 1 : 0;
+    if (tb.window > 0)
+      for (int k = depth + 1; k > tb.window; --k) seen &= seen - 1;  // (the furthest come first)
+    s_seen[j] = seen;
+  }
+  // units that every column sees whole
+  const int full0 = tb.window > 0 ? max(0, r.P + r.N - tb.window) : 0, full1 = r.P;
+
+  int unit = ua + wave;
+  TreePages pages(geo, seq, h, ub - 1, unit);
+  u32x4 qf[CT][4];
+  [[maybe_unused]] float q0[CT], q1[CT], q0c[CT], q1c[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int col = min(col0 + 16 * ct + n, cols - 1), node = col / G;
+    const uint16_t* src = q + (int64_t)(start + node) * tb.qr + (int64_t)(h * G + col - node * G) * tb.qh + 8 * g;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) qf[ct][s] = *(const u32x4*)(src + 32 * s);
+    if constexpr (KB != 0) {
+      // the queries' sums over each 64 dims: of q, and of the QK operand (int4:
+      // with its unit-16 elements scaled) times 1024
+      const u32x4 ones = u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
+      const f32x4 zero = f32x4{0.f, 0.f, 0.f, 0.f};
+      q0[ct] = mfma_f16(ones, qf[ct][1], mfma_f16(ones, qf[ct][0], zero))[0];
+      q1[ct] = mfma_f16(ones, qf[ct][3], mfma_f16(ones, qf[ct][2], zero))[0];
+      if constexpr (KB == 4)
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          qf[ct][s][1] = f16x2_unit16(qf[ct][s][1]);
+          qf[ct][s][3] = f16x2_unit16(qf[ct][s][3]);
+        }
+      q0c[ct] = mfma_f16(ones, qf[ct][1], mfma_f16(ones, qf[ct][0], zero))[0] * -kDecOff;
+      q1c[ct] = mfma_f16(ones, qf[ct][3], mfma_f16(ones, qf[ct][2], zero))[0] * -kDecOff;
+    }
+  }
+  [[maybe_unused]] const uint32_t code_base = KB ? f16_pair_1024() : 0u;
+  const uint32_t lane16 = (uint32_t)lane * 16;
+  const uint32_t sb_at = 16u * (uint32_t)(((lane >> 3) & 3) * (geo.tb >> 2) + (lane & 7));
+  u32x4 kf[NK], vf[NV];
+  [[maybe_unused]] u32x4 sbx;
+  auto load_k = [&](const uint8_t* slab, int u) __attribute__((always_inline)) {
+    const uint8_t* p = slab + geo.k_off + (u & pages.sh) * (NK * 1024);
+#pragma unroll
+    for (int x = 0; x < NK; ++x) kf[x] = *(const u32x4*)(p + x * 1024 + lane16);
+    if constexpr (KB != 0) sbx = *(const u32x4*)(slab + geo.sb_off + (u & pages.sh) * 128 + sb_at);
+  };
+  auto load_v = [&](const uint8_t* slab, int u) __attribute__((always_inline)) {
+    const uint8_t* p = slab + geo.v_off + (u & pages.sh) * 1024;
+#pragma unroll
+    for (int x = 0; x < NV; ++x) vf[x] = *(const u32x4*)(p + (x << pages.sh) * 1024 + lane16);
+  };
+  f32x4 o[CT][8];
+  float m[CT], base[CT], l[CT];
+  [[maybe_unused]] float ob0[CT], ob1[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) o[ct][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m[ct] = -INFINITY;
+    base[ct] = l[ct] = 0.f;
+    if constexpr (KB != 0) ob0[ct] = ob1[ct] = 0.f;
+  }
+  __syncthreads();
+
+  auto step = [&](auto more) __attribute__((always_inline)) {
+    constexpr bool MORE = decltype(more)::value;
+    const int next = pages.unit;
+    const uint8_t* slab = pages.slab(geo);
+    if constexpr (MORE) pages.ask(unit + 8);
+    __builtin_amdgcn_sched_barrier(0);
+    f32x4 acc[CT][KB ? 4 : 2];
+    if constexpr (KB == 0) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) acc[ct][0] = acc[ct][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) acc[ct][t] = mfma16x16x32<DT>(kf[4 * t + s], qf[ct][s], acc[ct][t]);
+    } else {
+      constexpr int KQ = KB ? KB : 4;
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        acc[ct][0] = acc[ct][1] = f32x4{q0c[ct], q0c[ct], q0c[ct], q0c[ct]};
+        acc[ct][2] = acc[ct][3] = f32x4{q1c[ct], q1c[ct], q1c[ct], q1c[ct]};
+      }
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const u32x4 a = k_operand<KQ>(kf + t * QCode<KQ>::KF, s, code_base);
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) acc[ct][2 * (s >> 1) + t] = mfma_f16(a, qf[ct][s], acc[ct][2 * (s >> 1) + t]);
+        }
+      s_sb[wave][lane & 31] = sbx;
+      wave_lds_order();
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (MORE) load_k(slab, next);
+    __builtin_amdgcn_sched_barrier(0);
+    [[maybe_unused]] u32x4 sb[KB ? 8 : 1], vc[KB ? 8 : 1];
+    if constexpr (KB != 0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sb[e] = s_sb[wave][8 * g + e];
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt) vc[dt] = codes_bf16<KB ? KB : 4>(vf, dt);
+    }
+    const int t0 = 32 * unit + 8 * g;  // this lane's first token
+    const bool edge = 32 * unit < full0 || 32 * unit + 32 > full1;
+    uint64_t odd = 0;  // (16-bit) tokens of the unit with a value that is no number, or infinite
+    if constexpr (KB == 0) {
+      if (edge) {
+        // values of tokens that no node sees (old pages hold anything) are taken as
+        // zeros; so are infinities and NaN, which a weight of zero does not
+        // take out of a product: they are added below to the columns that see them
+        uint32_t any = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const bool a = t0 + 2 * j >= r.lo && t0 + 2 * j < r.T, b = t0 + 2 * j + 1 >= r.lo && t0 + 2 * j + 1 < r.T;
+          const uint32_t keep = (a ? 0x0000FFFFu : 0u) | (b ? 0xFFFF0000u : 0u);
+          constexpr uint32_t INF = DT == 0 ? 0x7C00u : 0x7F80u;
+          uint32_t got = 0;
+#pragma unroll
+          for (int dt = 0; dt < 8; ++dt) {
+            uint32_t w = vf[dt][j] & keep;
+            const uint32_t x = (w & INF) == INF ? 0xFFFFu : 0u, y = (w >> 16 & INF) == INF ? 0xFFFF0000u : 0u;
+            got |= x | y;
+            vf[dt][j] = w & ~(x | y);
+          }
+          any |= (got & 0xFFFFu ? 1u << (2 * j) : 0u) | (got >> 16 ? 2u << (2 * j) : 0u);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint64_t who = __ballot(any >> e & 1);
+#pragma unroll
+          for (int gg = 0; gg < 4; ++gg)
+            if (who >> (16 * gg) & 0xFFFF) odd |= 1ull << (8 * gg + e);
+        }
+      }
+    }
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      // scores of tokens t0 + e in the log2 domain
+      float pv[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if constexpr (KB == 0) {
+          pv[e] = acc[ct][e >> 2][e & 3] * tb.sl2;
+        } else {
+          float x = lo_f(sb[e][0]) * acc[ct][e >> 2][e & 3];
+          x = __builtin_fmaf(hi_f(sb[e][0]), acc[ct][2 + (e >> 2)][e & 3], x);
+          x = __builtin_fmaf(lo_f(sb[e][1]), q0[ct], x);
+          x = __builtin_fmaf(hi_f(sb[e][1]), q1[ct], x);
+          pv[e] = x * tb.sl2;
+        }
+      }
+      uint32_t sees = 0xFFu;  // bit e: whether the column sees token t0 + e
+      if (edge) {
+        const int node = min(col0 + 16 * ct + n, cols - 1) / G;
+        const uint64_t seen = s_seen[node];
+        const int from = max(s_from[node], 0);
+        sees = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int t = t0 + e, a = t - r.P;
+          const bool ok = a < 0 ? t >= from && seen != 0 : a < r.N && (seen >> (a & 63) & 1);
+          sees |= ok ? 1u << e : 0u;
+          pv[e] = ok ? pv[e] : -INFINITY;
+        }
+      }
+      float mx = pv[0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) mx = fmaxf(mx, pv[e]);
+      if (__any(mx > m[ct] + kTreeSlack)) {
+        const float top = fmaxf(m[ct], max_over_groups(mx));
+        const float f = top == m[ct] ? 1.0f : __builtin_amdgcn_exp2f(m[ct] - top);
+        m[ct] = top;
+        base[ct] = (top == -INFINITY ? 0.0f : top) - kLift;
+        l[ct] *= f;
+        if constexpr (KB != 0) {
+          ob0[ct] *= f;
+          ob1[ct] *= f;
+        }
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) o[ct][dt] *= f;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        pv[e] = __builtin_amdgcn_exp2f(pv[e] - base[ct]);
+        l[ct] += pv[e];
+      }
+      if constexpr (KB == 0) {
+        if (odd) {
+          // token by token: the weight from the lane that has it, the values from
+          // the slab as it is stored
+#pragma unroll 1
+          for (uint64_t left = odd; left; left &= left - 1) {
+            const int t = __ffsll((unsigned long long)left) - 1, e = t & 7, src = n + 16 * (t >> 3);
+            float p = pv[0];
+#pragma unroll
+            for (int x = 1; x < 8; ++x) p = x == e ? pv[x] : p;
+            p = __shfl(p, src, 64);
+            const bool ok = __shfl((int)(sees >> e & 1), src, 64) != 0;
+            const int tok = 32 * (unit & pages.sh) + t;
+            const int32_t page = block_table(geo, seq)[unit >> pages.sh];
+            const uint16_t* vs = (const uint16_t*)(geo.pool + ((size_t)page * geo.hkv + h) * geo.slab_bytes + geo.v_off);
+#pragma unroll
+            for (int dt = 0; dt < 8; ++dt)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const float v = to_f32<DT>(vs[v_elem(geo.tb, tok, 16 * dt + 4 * g + x)]);
+                if (ok && !__builtin_isfinite(v)) o[ct][dt][x] = __builtin_fmaf(p, v, o[ct][dt][x]);
+              }
+          }
+        }
+        u32x4 hi, lo;
+        tree_split<PT>(pv, hi, lo);
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) {
+          o[ct][dt] = mfma16x16x32<DT>(vf[dt], hi, o[ct][dt]);
+          o[ct][dt] = mfma16x16x32<DT>(vf[dt], lo, o[ct][dt]);
+        }
+      } else {
+        // o_d = sum_t (p_t vs_j) c_td + sum_t p_t vb_j for group j of 64 dims
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float w[8];
+          float& ob = half ? ob1[ct] : ob0[ct];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float vs = half ? hi_f(sb[e][2]) : lo_f(sb[e][2]), vb = half ? hi_f(sb[e][3]) : lo_f(sb[e][3]);
+            if (edge) {  // (a token that the column does not see may have any scale)
+              vs = sees >> e & 1 ? vs : 0.f;
+              vb = sees >> e & 1 ? vb : 0.f;
+            }
+            w[e] = pv[e] * vs;
+            ob = __builtin_fmaf(pv[e], vb, ob);
+          }
+          u32x4 hi, lo;
+          tree_split<1>(w, hi, lo);
+#pragma unroll
+          for (int dt = 4 * half; dt < 4 * half + 4; ++dt) {
+            o[ct][dt] = mfma16x16x32<1>(vc[dt], hi, o[ct][dt]);
+            o[ct][dt] = mfma16x16x32<1>(vc[dt], lo, o[ct][dt]);
+          }
+        }
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (MORE) load_v(slab, next);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  {
+    // (a wave without a unit asks for the part's last one: behind a branch the
+    // loop would wait for everything under way)
+    const int u = pages.unit;
+    const uint8_t* slab = pages.slab(geo);
+    pages.ask(unit + 4);
+    load_k(slab, u);
+    load_v(slab, u);
+  }
+  for (; unit + 4 < ub; unit += 4) step(std::true_type());
+  if (unit < ub) step(std::false_type());
+
+  // the four waves' shares joined, a column tile at a time
+#pragma unroll 1
+  for (int ct = 0; ct < CT; ++ct) {
+    f32x4 oc[8];
+    float lc = 0.f, mc = 0.f;
+#pragma unroll
+    for (int x = 0; x < CT; ++x)
+      if (x == ct) {
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) {
+          oc[dt] = o[x][dt];
+          if constexpr (KB != 0) {
+            const float b = sum_over_groups(dt < 4 ? ob0[x] : ob1[x]);
+#pragma unroll
+            for (int y = 0; y < 4; ++y) oc[dt][y] += b;
+          }
+        }
+        lc = sum_over_groups(l[x]);
+        mc = m[x] == -INFINITY ? m[x] : base[x];
+      }
+    const int first = col0 + 16 * ct;
+    if (first >= cols) break;
+    __syncthreads();
+    if (g == 0) {
+      s_m[wave][n] = mc;
+      s_l[wave][n] = lc;
+    }
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) *(f32x4*)&s_o[wave][n][16 * dt + 4 * g] = oc[dt];
+    __syncthreads();
+    for (int e = threadIdx.x; e < 16 * kHeadDim; e += 256) {
+      const int c = e >> 7, d = e & 127, col = first + c;
+      if (col >= cols) break;
+      float M = s_m[0][c];
+#pragma unroll
+      for (int v = 1; v < 4; ++v) M = fmaxf(M, s_m[v][c]);
+      float L = 0.f, a = 0.f;
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const float mv = s_m[v][c];
+        const float f = mv == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mv - M);
+        L += f * s_l[v][c];
+        if (mv != -INFINITY) a += f * s_o[v][c][d];
+      }
+      const int node = col / G, hq = h * G + col - node * G;
+      if (s_seen[node] == 0) {  // absent: nothing is seen
+        M = -INFINITY;
+        L = a = 0.f;
+      }
+      if (direct) {
+        if (tb.sinks && M != -INFINITY) {
+          const float sk = tb.sinks[hq] * kTreeLog2e, top = fmaxf(M, sk), f = __builtin_amdgcn_exp2f(M - top);
+          L = L * f + (sk == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sk - top));
+          a *= f;
+        }
+        out[((int64_t)(start + node) * geo.hq + hq) * kHeadDim + d] = from_f32<DT>(L == 0.f ? 0.f : a / L);
+      } else {
+        float* pp = partials + ((int64_t)(tb.row0[i] + part * tb.max_tokens + node) * geo.hq + hq) * kPartial;
+        pp[d] = a;
+        if (d == 0) {
+          pp[kHeadDim] = M;
+          pp[kHeadDim + 1] = L;
+        }
+      }
+    }
+  }
+}
+
+// The parts of one (node, query head) joined, eight rows of 32 lanes with four
+// dims each taking the parts in turn.  grid (Hq, n * max_tokens)
+constexpr int kTreeRows = 8;
+template <int DT>
+__global__ __launch_bounds__(32 * kTreeRows) void k_tree_join(Geometry geo, TreeBatch tb, const float* __restrict__ ws,
+                                                              uint16_t* __restrict__ out) {
+  __shared__ __align__(16) float s_o[kTreeRows][kHeadDim];
+  __shared__ float s_ml[kTreeRows][2];
+  const int hq = blockIdx.x, i = blockIdx.y / tb.max_tokens, node = blockIdx.y - i * tb.max_tokens;
+  if (tb.part0[i + 1] - tb.part0[i] <= 1) return;  // (the launch before wrote the output)
+  const TreeRange r = tree_range(geo, tb, i);
+  if (node >= r.N) return;
+  const int parts = (r.units + r.cu - 1) / r.cu;
+  const int y = threadIdx.x >> 5, c = threadIdx.x & 31;
+  float M = -INFINITY, L = 0.f;
+  f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int p = y; p < parts; p += kTreeRows) {
+    const float2* part = (const float2*)(ws + ((int64_t)(tb.row0[i] + p * tb.max_tokens + node) * geo.hq + hq) * kPartial);
+    const float2 xa = part[2 * c], xb = part[2 * c + 1], ml = part[kHeadDim / 2];
+    // (without a token that is seen: no reference, and a sum of 0, or NaN)
+    const float top = fmaxf(M, ml.x), f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - top);
+    const float w = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - top);
+    L = L * f + w * ml.y;
+    a *= f;
+    if (ml.x != -INFINITY) a += w * f32x4{xa.x, xa.y, xb.x, xb.y};
+    M = top;
+  }
+  *(f32x4*)&s_o[y][4 * c] = a;
+  if (c == 0) {
+    s_ml[y][0] = M;
+    s_ml[y][1] = L;
+  }
+  __syncthreads();
+  if (threadIdx.x >= kHeadDim) return;
+  const int d = threadIdx.x;
+  float top = -INFINITY;
+#pragma unroll
+  for (int x = 0; x < kTreeRows; ++x) top = fmaxf(top, s_ml[x][0]);
+  const bool none = top == -INFINITY;
+  const float sk = tb.sinks && !none ? tb.sinks[hq] * kTreeLog2e : -INFINITY;
+  top = fmaxf(top, sk);
+  float Ls = sk == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sk - top), as = 0.f;
+#pragma unroll
+  for (int x = 0; x < kTreeRows; ++x) {
+    const float mx = s_ml[x][0], f = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - top);
+    Ls += f * s_ml[x][1];
+    if (mx != -INFINITY) as += f * s_o[x][d];
+  }
+  out[((int64_t)(tb.starts[i] + node) * geo.hq + hq) * kHeadDim + d] = from_f32<DT>(Ls == 0.f ? 0.f : as / Ls);
+}
+
+template <int DT, int KB>
+static void tree_dispatch(const Geometry& g, const TreeBatch& tb, const uint16_t* q, uint16_t* out, float* ws,
+                          hipStream_t s, Timing* prof) {
+  const int64_t pairs = ((int64_t)tb.part0[tb.n] * g.hkv + 7) & ~7ll;
+  const dim3 grid((unsigned)(pairs * tb.groups)), blk(256);
+  if (tb.tiles == 1) launch(k_tree<DT, KB, 1>, grid, blk, 0, s, prof, kProfTree, g, tb, q, out, ws);
+  else if (tb.tiles == 2) launch(k_tree<DT, KB, 2>, grid, blk, 0, s, prof, kProfTree, g, tb, q, out, ws);
+  else launch(k_tree<DT, KB, 4>, grid, blk, 0, s, prof, kProfTree, g, tb, q, out, ws);
+}
+
+static_assert(sizeof(Geometry) + sizeof(TreeBatch) <= 4000, "a launch's arguments stay under 4 KiB");
+hipError_t launch_tree(const Geometry& g, const TreeBatch& tb, const void* q, void* out, float* ws, hipEvent_t done,
+                       hipStream_t s, Timing* prof) {
+  const uint16_t* qq = (const uint16_t*)q;
+  uint16_t* oo = (uint16_t*)out;
+  if (g.kv_bits == 4) tree_dispatch<0, 4>(g, tb, qq, oo, ws, s, prof);
+  else if (g.kv_bits == 8) tree_dispatch<0, 8>(g, tb, qq, oo, ws, s, prof);
+  else if (g.dtype == 0) tree_dispatch<0, 0>(g, tb, qq, oo, ws, s, prof);
+  else tree_dispatch<1, 0>(g, tb, qq, oo, ws, s, prof);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !ws) return e;
+  const dim3 grid(g.hq, tb.n * tb.max_tokens), blk(32 * kTreeRows);
+  const float* cws = ws;
+  auto join = [&](auto kernel) {
+    if (done && !prof)  // (the event is the dispatch's own: no packet of its own behind it)
+      hipExtLaunchKernelGGL(kernel, grid, blk, 0u, s, nullptr, done, 0u, g, tb, cws, oo);
+    else
+      launch(kernel, grid, blk, 0, s, prof, kProfCombine, g, tb, cws, oo);
+  };
+  if (g.dtype == 0) join(k_tree_join<0>);
+  else join(k_tree_join<1>);
+  e = hipGetLastError();
+  if (e == hipSuccess && done && prof) e = hipEventRecord(done, s);
+  return e;
+}
+
+}  // namespace bsattn

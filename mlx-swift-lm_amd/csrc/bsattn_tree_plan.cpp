@@ -1,0 +1,56 @@
+// bsattn_tree_plan.cpp -- how a tree attention's tokens are cut into the parts
+// that its workgroups take (bsattn_tree.hip), and where their partials lie.
+#include <algorithm>
+
+#include "bsattn_internal.h"
+
+namespace bsattn {
+
+int64_t tree_plan(const Geometry& g, TreeBatch& tb) {
+  const int cols = tb.max_tokens * g.group;
+  tb.tiles = cols <= 16 ? 1 : cols <= 32 ? 2 : 4;
+  tb.groups = (cols + 16 * tb.tiles - 1) / (16 * tb.tiles);
+  int64_t all = 0;
+  int most = 1;
+  for (int i = 0; i < tb.n; ++i) {
+    all += tb.units[i];
+    most = std::max(most, tb.units[i]);
+  }
+  // one round of workgroups
+  const int64_t want = (tb.tiles > 2 ? 1 : 2) * (int64_t)std::max(g.cus, 1), each = (int64_t)g.hkv * tb.groups;
+  auto parts = [&](int i, int cu) { return std::max(1, (tb.units[i] + cu - 1) / cu); };
+  auto fits = [&](int cu) {
+    int64_t n = 0;
+    for (int i = 0; i < tb.n; ++i) n += parts(i, cu);
+    return n * each <= want;
+  };
+  auto cut = [&](int64_t workgroups) {
+    const int64_t cu = std::max<int64_t>(4, (all * each + workgroups - 1) / workgroups);
+    return ((int)std::min<int64_t>(cu, most) + 3) & ~3;
+  };
+  tb.cu = cut(want);
+  int lo = tb.cu / 4, hi = (most + 3) / 4;  // in fours: the smallest that fits
+  while (lo < hi) {
+    const int mid = lo + (hi - lo) / 2;
+    if (fits(4 * mid)) hi = mid;
+    else lo = mid + 1;
+  }
+  const bool even = 4 * lo <= 32 || 2 * (int64_t)4 * lo * want <= 3 * all * each;
+  tb.cu = !fits(4 * lo) ? cut(want) : even ? 4 * lo : cut(3 * want);
+  // (it ends: a request of one part has no partials)
+  while (true) {
+    int64_t n = 0, blocks = 0;
+    for (int i = 0; i < tb.n; ++i) {
+      const int p = parts(i, tb.cu);
+      tb.part0[i] = (int32_t)n;
+      tb.row0[i] = (int32_t)blocks;
+      n += p;
+      if (p > 1) blocks += (int64_t)p * tb.max_tokens;
+    }
+    tb.part0[tb.n] = (int32_t)n;
+    if (blocks * g.hq <= kPrefillRows) return blocks * g.hq;
+    tb.cu *= 2;
+  }
+}
+
+}  // namespace bsattn
