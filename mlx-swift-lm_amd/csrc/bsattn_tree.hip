@@ -58,15 +58,14 @@ __device__ __forceinline__ TreeRange tree_range(const Geometry& geo, const TreeB
 // cache one unit ahead
 struct TreePages {
   const int32_t* bt;
-  int h, sh, last, unit, page;
-  __device__ __forceinline__ TreePages(const Geometry& geo, int seq, int h_, int last_, int u) : h(h_), last(last_) {
+  int h, sh, unit, page;  // sh: log2 of the units per block; the unit asked for last, and its page
+  __device__ __forceinline__ TreePages(const Geometry& geo, int seq, int h_, int u) : h(h_) {
     sh = geo.tb == 64 ? 1 : 0;
     bt = block_table(geo, seq);
     ask(u);
   }
-  // (past the part's units: its last one)
   __device__ __forceinline__ void ask(int u) {
-    unit = min(u, last);
+    unit = u;
     page = *((const __attribute__((address_space(4))) int32_t*)(uintptr_t)(bt + (unit >> sh)));
   }
   __device__ __forceinline__ const uint8_t* slab(const Geometry& geo) const {
@@ -128,7 +127,10 @@ __global__ __launch_bounds__(256, CT > 2 ? 1 : 2) void k_tree(Geometry geo, Tree
   constexpr int NK = KB ? 2 * QCode<KB ? KB : 4>::KF : 8, NV = KB ? 8 / QCode<KB ? KB : 4>::DPF : 8;
   __shared__ uint64_t s_seen[kMaxNodes];  // each node's ancestors, those in its window
   __shared__ int s_from[kMaxNodes];       // the first cached token it sees
-  __shared__ u32x4 s_sb[KB ? 4 : 1][KB ? 32 : 1];
+  // (affine) a unit's scales and biases, the keys' and the values'; the waves' own
+  __shared__ uint2 s_sb[KB ? 4 : 1][KB ? 32 : 1], s_sv[KB ? 4 : 1][KB ? 32 : 1];
+  // units with values of this kind (a wave has at most two with columns that do not see all of them), and their tokens
+  __shared__ uint2 s_odd[4][2];
   __shared__ float s_m[4][16], s_l[4][16];
   __shared__ __align__(16) float s_o[4][16][kHeadDim + 4];
 
@@ -150,6 +152,7 @@ __global__ __launch_bounds__(256, CT > 2 ? 1 : 2) void k_tree(Geometry geo, Tree
   const int ua = r.u0 + part * r.cu, ub = min(ua + r.cu, r.u0 + r.units);
   const int seq = tb.ids[i];
 
+  if (lane < 2) s_odd[wave][lane] = make_uint2(0u, 0u);
   if (threadIdx.x < kMaxNodes) {
     const int j = threadIdx.x;
     uint64_t seen = j < r.N ? tb.ancestors[start + j] : 0;
@@ -159,11 +162,21 @@ __global__ __launch_bounds__(256, CT > 2 ? 1 : 2) void k_tree(Geometry geo, Tree
       for (int k = depth + 1; k > tb.window; --k) seen &= seen - 1;  // (the furthest come first)
     s_seen[j] = seen;
   }
-  // units that every column sees whole
-  const int full0 = tb.window > 0 ? max(0, r.P + r.N - tb.window) : 0, full1 = r.P;
-
-  int unit = ua + wave;
-  TreePages pages(geo, seq, h, ub - 1, unit);
+  // The part's units: those that every column sees whole (from fa on, `full` of
+  // them), then the others, in front of them and behind
+  const int whole0 = tb.window > 0 ? (max(0, r.P + r.N - tb.window) + 31) >> 5 : 0, whole1 = r.P >> 5;
+  const int fa = min(max(ua, whole0), ub), full = max(min(ub, whole1) - fa, 0), places = ub - ua;
+  // (places past the part's: its last one)
+  auto unit_at = [&](int at) {
+    const int p = min(at, places - 1), k = ua + p - full;
+    return p < full ? fa + p : k < fa ? k : k + full;
+  };
+  int place = wave;  // a wave takes every fourth
+  TreePages pages(geo, seq, h, unit_at(place));
+  // scores are products times |scale|, of queries with its sign: the largest is
+  // found on the products
+  const float sc = fmaxf(fabsf(tb.sl2), 1e-30f);  // (-inf, of what is not seen, times it is -inf)
+  const uint32_t qflip = tb.sl2 < 0.f ? 0x80008000u : 0u;
   u32x4 qf[CT][4];
   [[maybe_unused]] float q0[CT], q1[CT], q0c[CT], q1c[CT];
 #pragma unroll
@@ -171,7 +184,7 @@ __global__ __launch_bounds__(256, CT > 2 ? 1 : 2) void k_tree(Geometry geo, Tree
     const int col = min(col0 + 16 * ct + n, cols - 1), node = col / G;
     const uint16_t* src = q + (int64_t)(start + node) * tb.qr + (int64_t)(h * G + col - node * G) * tb.qh + 8 * g;
 #pragma unroll
-    for (int s = 0; s < 4; ++s) qf[ct][s] = *(const u32x4*)(src + 32 * s);
+    for (int s = 0; s < 4; ++s) qf[ct][s] = *(const u32x4*)(src + 32 * s) ^ qflip;
     if constexpr (KB != 0) {
       // the queries' sums over each 64 dims: of q, and of the QK operand (int4:
       // with its unit-16 elements scaled) times 1024
@@ -206,26 +219,32 @@ __global__ __launch_bounds__(256, CT > 2 ? 1 : 2) void k_tree(Geometry geo, Tree
     for (int x = 0; x < NV; ++x) vf[x] = *(const u32x4*)(p + (x << pages.sh) * 1024 + lane16);
   };
   f32x4 o[CT][8];
-  float m[CT], base[CT], l[CT];
+  float m[CT], base[CT], limit[CT], l[CT];  // limit: the product past which the reference is raised
   [[maybe_unused]] float ob0[CT], ob1[CT];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) o[ct][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    m[ct] = -INFINITY;
+    m[ct] = limit[ct] = -INFINITY;
     base[ct] = l[ct] = 0.f;
     if constexpr (KB != 0) ob0[ct] = ob1[ct] = 0.f;
   }
   __syncthreads();
 
-  auto step = [&](auto more) __attribute__((always_inline)) {
-    constexpr bool MORE = decltype(more)::value;
+  // One unit.  (The next one's K is asked for as soon as this one's is used, its
+  // V likewise; a wave's last step asks for its own unit again: behind a branch
+  // the compiler must wait as if nothing had been asked for, and a second copy of
+  // the step spills.)
+  auto step = [&]() __attribute__((always_inline)) {
     const int next = pages.unit;
     const uint8_t* slab = pages.slab(geo);
-    if constexpr (MORE) pages.ask(unit + 8);
+    pages.ask(unit_at(place + 8));
     __builtin_amdgcn_sched_barrier(0);
-    f32x4 acc[CT][KB ? 4 : 2];
+    // S^T: entry e is token 8 g + e of the unit.  Affine caches: the codes' products
+    // of each 64 dims, then with the token's scales and biases
+    float sv[CT][8];
     if constexpr (KB == 0) {
+      f32x4 acc[CT][2];
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) acc[ct][0] = acc[ct][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -234,8 +253,18 @@ __global__ __launch_bounds__(256, CT > 2 ? 1 : 2) void k_tree(Geometry geo, Tree
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int ct = 0; ct < CT; ++ct) acc[ct][t] = mfma16x16x32<DT>(kf[4 * t + s], qf[ct][s], acc[ct][t]);
+      __builtin_amdgcn_sched_barrier(0);
+      load_k(slab, next);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sv[ct][e] = acc[ct][e >> 2][e & 3];
     } else {
       constexpr int KQ = KB ? KB : 4;
+      f32x4 acc[CT][4];
+      s_sb[wave][lane & 31] = make_uint2(sbx[0], sbx[1]);
+      s_sv[wave][lane & 31] = make_uint2(sbx[2], sbx[3]);
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
         acc[ct][0] = acc[ct][1] = f32x4{q0c[ct], q0c[ct], q0c[ct], q0c[ct]};
@@ -249,27 +278,43 @@ __global__ __launch_bounds__(256, CT > 2 ? 1 : 2) void k_tree(Geometry geo, Tree
 #pragma unroll
           for (int ct = 0; ct < CT; ++ct) acc[ct][2 * (s >> 1) + t] = mfma_f16(a, qf[ct][s], acc[ct][2 * (s >> 1) + t]);
         }
-      s_sb[wave][lane & 31] = sbx;
       wave_lds_order();
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    if constexpr (MORE) load_k(slab, next);
-    __builtin_amdgcn_sched_barrier(0);
-    [[maybe_unused]] u32x4 sb[KB ? 8 : 1], vc[KB ? 8 : 1];
-    if constexpr (KB != 0) {
+      __builtin_amdgcn_sched_barrier(0);
+      load_k(slab, next);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sb[e] = s_sb[wave][8 * g + e];
+      for (int e = 0; e < 8; ++e) {
+        const uint2 sb = s_sb[wave][8 * g + e];
 #pragma unroll
-      for (int dt = 0; dt < 8; ++dt) vc[dt] = codes_bf16<KB ? KB : 4>(vf, dt);
+        for (int ct = 0; ct < CT; ++ct) {
+          float x = lo_f(sb.x) * acc[ct][e >> 2][e & 3];
+          x = __builtin_fmaf(hi_f(sb.x), acc[ct][2 + (e >> 2)][e & 3], x);
+          x = __builtin_fmaf(lo_f(sb.y), q0[ct], x);
+          sv[ct][e] = __builtin_fmaf(hi_f(sb.y), q1[ct], x);
+        }
+      }
     }
-    const int t0 = 32 * unit + 8 * g;  // this lane's first token
-    const bool edge = 32 * unit < full0 || 32 * unit + 32 > full1;
-    uint64_t odd = 0;  // (16-bit) tokens of the unit with a value that is no number, or infinite
-    if constexpr (KB == 0) {
-      if (edge) {
-        // values of tokens that no node sees (old pages hold anything) are taken as
-        // zeros; so are infinities and NaN, which a weight of zero does not
-        // take out of a product: they are added below to the columns that see them
+    if (place >= full) {
+      // Some columns do not see all of the unit.  Values of tokens that none sees
+      // (old pages hold anything) are taken as zeros; so are infinities and NaN,
+      // which a weight of zero does not take out of a product: they are noted, and
+      // reach the columns that see them at the end.  Of affine caches these are
+      // tokens with such scales or biases, for their 64 dims.
+      const int unit = unit_at(place), t0 = 32 * unit + 8 * g;
+      uint32_t odd = 0;  // tokens with such values
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        const int node = min(col0 + 16 * ct + n, cols - 1) / G;
+        const uint64_t seen = s_seen[node];
+        const int from = seen ? s_from[node] : r.T;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int t = t0 + e, a = t - r.P;
+          const bool ok = a < 0 ? t >= from : a < r.N && (seen >> (a & 63) & 1);
+          sv[ct][e] = ok ? sv[ct][e] : -INFINITY;
+        }
+      }
+      if constexpr (KB == 0) {
         uint32_t any = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -279,7 +324,7 @@ __global__ __launch_bounds__(256, CT > 2 ? 1 : 2) void k_tree(Geometry geo, Tree
           uint32_t got = 0;
 #pragma unroll
           for (int dt = 0; dt < 8; ++dt) {
-            uint32_t w = vf[dt][j] & keep;
+            const uint32_t w = vf[dt][j] & keep;
             const uint32_t x = (w & INF) == INF ? 0xFFFFu : 0u, y = (w >> 16 & INF) == INF ? 0xFFFF0000u : 0u;
             got |= x | y;
             vf[dt][j] = w & ~(x | y);
@@ -291,48 +336,38 @@ __global__ __launch_bounds__(256, CT > 2 ? 1 : 2) void k_tree(Geometry geo, Tree
           const uint64_t who = __ballot(any >> e & 1);
 #pragma unroll
           for (int gg = 0; gg < 4; ++gg)
-            if (who >> (16 * gg) & 0xFFFF) odd |= 1ull << (8 * gg + e);
+            if (who >> (16 * gg) & 0xFFFF) odd |= 1u << (8 * gg + e);
         }
+      } else {
+        const uint2 f = s_sv[wave][lane & 31];
+        auto inf = [](uint32_t w) {
+          return ((w & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u) | ((w >> 16 & 0x7C00u) == 0x7C00u ? 0xFFFF0000u : 0u);
+        };
+        const uint32_t bad = inf(f.x) | inf(f.y);
+        odd = (uint32_t)__ballot(bad != 0 && lane < 32);
+        s_sv[wave][lane & 31] = make_uint2(f.x & ~bad, f.y & ~bad);
+        wave_lds_order();
       }
+      if (odd && lane == 0) s_odd[wave][(place - full) >> 2] = make_uint2(unit, odd);
     }
+    // the largest scores, and one branch for all columns' references
+    float mx[CT];
+    bool raise = false;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      // scores of tokens t0 + e in the log2 domain
-      float pv[8];
+      mx[ct] = sv[ct][0];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if constexpr (KB == 0) {
-          pv[e] = acc[ct][e >> 2][e & 3] * tb.sl2;
-        } else {
-          float x = lo_f(sb[e][0]) * acc[ct][e >> 2][e & 3];
-          x = __builtin_fmaf(hi_f(sb[e][0]), acc[ct][2 + (e >> 2)][e & 3], x);
-          x = __builtin_fmaf(lo_f(sb[e][1]), q0[ct], x);
-          x = __builtin_fmaf(hi_f(sb[e][1]), q1[ct], x);
-          pv[e] = x * tb.sl2;
-        }
-      }
-      uint32_t sees = 0xFFu;  // bit e: whether the column sees token t0 + e
-      if (edge) {
-        const int node = min(col0 + 16 * ct + n, cols - 1) / G;
-        const uint64_t seen = s_seen[node];
-        const int from = max(s_from[node], 0);
-        sees = 0;
+      for (int e = 1; e < 8; ++e) mx[ct] = fmaxf(mx[ct], sv[ct][e]);
+      raise = raise || mx[ct] > limit[ct];
+    }
+    if (__any(raise)) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int t = t0 + e, a = t - r.P;
-          const bool ok = a < 0 ? t >= from && seen != 0 : a < r.N && (seen >> (a & 63) & 1);
-          sees |= ok ? 1u << e : 0u;
-          pv[e] = ok ? pv[e] : -INFINITY;
-        }
-      }
-      float mx = pv[0];
-#pragma unroll
-      for (int e = 1; e < 8; ++e) mx = fmaxf(mx, pv[e]);
-      if (__any(mx > m[ct] + kTreeSlack)) {
-        const float top = fmaxf(m[ct], max_over_groups(mx));
+      for (int ct = 0; ct < CT; ++ct) {
+        const float top = fmaxf(m[ct], max_over_groups(mx[ct]) * sc);
         const float f = top == m[ct] ? 1.0f : __builtin_amdgcn_exp2f(m[ct] - top);
         m[ct] = top;
         base[ct] = (top == -INFINITY ? 0.0f : top) - kLift;
+        limit[ct] = (top + kTreeSlack) / sc;
         l[ct] *= f;
         if constexpr (KB != 0) {
           ob0[ct] *= f;
@@ -341,83 +376,99 @@ __global__ __launch_bounds__(256, CT > 2 ? 1 : 2) void k_tree(Geometry geo, Tree
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt) o[ct][dt] *= f;
       }
+    }
+    [[maybe_unused]] u32x4 vc[KB ? 8 : 1];
+    if constexpr (KB != 0) {
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt) vc[dt] = codes_bf16<KB ? KB : 4>(vf, dt);
+      __builtin_amdgcn_sched_barrier(0);
+      load_v(slab, next);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      float (&pv)[8] = sv[ct];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        pv[e] = __builtin_amdgcn_exp2f(pv[e] - base[ct]);
+        pv[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(pv[e], sc, -base[ct]));
         l[ct] += pv[e];
       }
       if constexpr (KB == 0) {
-        if (odd) {
-          // token by token: the weight from the lane that has it, the values from
-          // the slab as it is stored
-#pragma unroll 1
-          for (uint64_t left = odd; left; left &= left - 1) {
-            const int t = __ffsll((unsigned long long)left) - 1, e = t & 7, src = n + 16 * (t >> 3);
-            float p = pv[0];
-#pragma unroll
-            for (int x = 1; x < 8; ++x) p = x == e ? pv[x] : p;
-            p = __shfl(p, src, 64);
-            const bool ok = __shfl((int)(sees >> e & 1), src, 64) != 0;
-            const int tok = 32 * (unit & pages.sh) + t;
-            const int32_t page = block_table(geo, seq)[unit >> pages.sh];
-            const uint16_t* vs = (const uint16_t*)(geo.pool + ((size_t)page * geo.hkv + h) * geo.slab_bytes + geo.v_off);
-#pragma unroll
-            for (int dt = 0; dt < 8; ++dt)
-#pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                const float v = to_f32<DT>(vs[v_elem(geo.tb, tok, 16 * dt + 4 * g + x)]);
-                if (ok && !__builtin_isfinite(v)) o[ct][dt][x] = __builtin_fmaf(p, v, o[ct][dt][x]);
-              }
-          }
-        }
         u32x4 hi, lo;
         tree_split<PT>(pv, hi, lo);
 #pragma unroll
-        for (int dt = 0; dt < 8; ++dt) {
-          o[ct][dt] = mfma16x16x32<DT>(vf[dt], hi, o[ct][dt]);
-          o[ct][dt] = mfma16x16x32<DT>(vf[dt], lo, o[ct][dt]);
-        }
+        for (int dt = 0; dt < 8; ++dt) o[ct][dt] = mfma16x16x32<DT>(vf[dt], hi, o[ct][dt]);
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) o[ct][dt] = mfma16x16x32<DT>(vf[dt], lo, o[ct][dt]);
       } else {
         // o_d = sum_t (p_t vs_j) c_td + sum_t p_t vb_j for group j of 64 dims
+        float w0[8], w1[8];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float w[8];
-          float& ob = half ? ob1[ct] : ob0[ct];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float vs = half ? hi_f(sb[e][2]) : lo_f(sb[e][2]), vb = half ? hi_f(sb[e][3]) : lo_f(sb[e][3]);
-            if (edge) {  // (a token that the column does not see may have any scale)
-              vs = sees >> e & 1 ? vs : 0.f;
-              vb = sees >> e & 1 ? vb : 0.f;
-            }
-            w[e] = pv[e] * vs;
-            ob = __builtin_fmaf(pv[e], vb, ob);
-          }
-          u32x4 hi, lo;
-          tree_split<1>(w, hi, lo);
-#pragma unroll
-          for (int dt = 4 * half; dt < 4 * half + 4; ++dt) {
-            o[ct][dt] = mfma16x16x32<1>(vc[dt], hi, o[ct][dt]);
-            o[ct][dt] = mfma16x16x32<1>(vc[dt], lo, o[ct][dt]);
-          }
+        for (int e = 0; e < 8; ++e) {
+          const uint2 sb = s_sv[wave][8 * g + e];
+          w0[e] = pv[e] * lo_f(sb.x);
+          w1[e] = pv[e] * hi_f(sb.x);
+          ob0[ct] = __builtin_fmaf(pv[e], lo_f(sb.y), ob0[ct]);
+          ob1[ct] = __builtin_fmaf(pv[e], hi_f(sb.y), ob1[ct]);
         }
+        u32x4 h0, l0, h1, l1;
+        tree_split<1>(w0, h0, l0);
+        tree_split<1>(w1, h1, l1);
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) o[ct][dt] = mfma16x16x32<1>(vc[dt], dt < 4 ? h0 : h1, o[ct][dt]);
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) o[ct][dt] = mfma16x16x32<1>(vc[dt], dt < 4 ? l0 : l1, o[ct][dt]);
       }
     }
-    __builtin_amdgcn_sched_barrier(0);
-    if constexpr (MORE) load_v(slab, next);
-    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (KB == 0) {
+      __builtin_amdgcn_sched_barrier(0);
+      load_v(slab, next);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
   {
-    // (a wave without a unit asks for the part's last one: behind a branch the
-    // loop would wait for everything under way)
     const int u = pages.unit;
     const uint8_t* slab = pages.slab(geo);
-    pages.ask(unit + 4);
+    pages.ask(unit_at(place + 4));
     load_k(slab, u);
     load_v(slab, u);
   }
-  for (; unit + 4 < ub; unit += 4) step(std::true_type());
-  if (unit < ub) step(std::false_type());
+#pragma unroll 1
+  for (; place < places; place += 4) step();
+  // what was noted: a value that is infinite or no number is so in the output,
+  // whatever its weight
+#pragma unroll 1
+  for (int x = 0; x < 2; ++x) {
+    const int unit = uniform((int)s_odd[wave][x].x);
+#pragma unroll 1
+    for (uint32_t odd = (uint32_t)uniform((int)s_odd[wave][x].y); odd; odd &= odd - 1) {
+      const int t = __ffs(odd) - 1, tok = 32 * (unit & pages.sh) + t, a = 32 * unit + t - r.P;
+      const int32_t page = block_table(geo, seq)[unit >> pages.sh];
+      const uint8_t* own = geo.pool + ((size_t)page * geo.hkv + h) * geo.slab_bytes;
+      float v[32];
+#pragma unroll
+      for (int y = 0; y < 32; ++y) {
+        const int d = 16 * (y >> 2) + 4 * g + (y & 3);
+        if constexpr (KB == 0) {
+          v[y] = to_f32<DT>(((const uint16_t*)(own + geo.v_off))[v_elem(geo.tb, tok, d)]);
+        } else {
+          int sh;
+          const uint2 f = *(const uint2*)(own + geo.sb_off + 16 * sb_entry(geo.tb, tok) + 8);
+          const float code = (float)(own[geo.v_off + vq_byte(KB, geo.tb, tok, d, &sh)] >> sh & ((1 << KB) - 1));
+          v[y] = y < 16 ? __builtin_fmaf(lo_f(f.x), code, lo_f(f.y)) : __builtin_fmaf(hi_f(f.x), code, hi_f(f.y));
+        }
+        if (__builtin_isfinite(v[y])) v[y] = 0.f;
+      }
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        const int node = min(col0 + 16 * ct + n, cols - 1) / G;
+        const uint64_t seen = s_seen[node];
+        const bool ok = seen && (a < 0 ? a + r.P >= s_from[node] : a < r.N && (seen >> (a & 63) & 1));
+#pragma unroll
+        for (int y = 0; y < 32; ++y) o[ct][y >> 2][y & 3] += ok ? v[y] : 0.f;
+      }
+    }
+  }
 
   // the four waves' shares joined, a column tile at a time
 #pragma unroll 1
@@ -545,6 +596,7 @@ static void tree_dispatch(const Geometry& g, const TreeBatch& tb, const uint16_t
   const dim3 grid((unsigned)(pairs * tb.groups)), blk(256);
   if (tb.tiles == 1) launch(k_tree<DT, KB, 1>, grid, blk, 0, s, prof, kProfTree, g, tb, q, out, ws);
   else if (tb.tiles == 2) launch(k_tree<DT, KB, 2>, grid, blk, 0, s, prof, kProfTree, g, tb, q, out, ws);
+  else if (tb.tiles == 3) launch(k_tree<DT, KB, 3>, grid, blk, 0, s, prof, kProfTree, g, tb, q, out, ws);
   else launch(k_tree<DT, KB, 4>, grid, blk, 0, s, prof, kProfTree, g, tb, q, out, ws);
 }
 

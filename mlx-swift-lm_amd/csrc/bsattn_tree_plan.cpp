@@ -8,8 +8,12 @@ namespace bsattn {
 
 int64_t tree_plan(const Geometry& g, TreeBatch& tb) {
   const int cols = tb.max_tokens * g.group;
-  tb.tiles = cols <= 16 ? 1 : cols <= 32 ? 2 : 4;
-  tb.groups = (cols + 16 * tb.tiles - 1) / (16 * tb.tiles);
+  // Column tiles per workgroup: two leave room for two waves a SIMD (8 x 32k bf16
+  // tokens, trees of 16: 208 us, 216 with four); dequantising affine caches for
+  // more of them at once pays (4 x 262k int8, 96 columns: 556 us with three, 764 with two)
+  const int tiles = (cols + 15) / 16, most_tiles = g.kv_bits ? 4 : 2;
+  tb.groups = (tiles + most_tiles - 1) / most_tiles;
+  tb.tiles = (tiles + tb.groups - 1) / tb.groups;
   int64_t all = 0;
   int most = 1;
   for (int i = 0; i < tb.n; ++i) {
