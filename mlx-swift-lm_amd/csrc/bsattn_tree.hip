@@ -34,13 +34,14 @@ constexpr float kTreeTop = 14.0f;
 
 // What a request brings to a launch, and the units of its part
 struct TreeRange {
-  int T, N, P, lo, u0, units, cu;
+  int T, N, P, lo, u0, units, cu, G;
 };
 __device__ __forceinline__ TreeRange tree_range(const Geometry& geo, const TreeBatch& tb, int i) {
   TreeRange r;
   r.T = uniform(geo.meta[tb.ids[i]]);
   r.N = min(min(uniform(tb.taken[i]), tb.max_tokens), r.T);
   r.P = r.T - r.N;
+  r.G = geo.group;
   r.lo = tb.window > 0 ? max(0, r.P - tb.window + 1) : 0;  // the first token that a root sees
   r.u0 = r.lo >> 5;
   r.units = r.N > 0 ? ((r.T - 1) >> 5) - r.u0 + 1 : 0;
@@ -90,36 +91,179 @@ __device__ __forceinline__ void tree_split(const float* x, u32x4& hi, u32x4& lo)
   }
 }
 
-// eight codes of a V fragment's dim tile as bf16 (exact)
+// eight codes as bf16 (exact): an int4 word (element e in nibble q_nib(e)), or two
+// int8 words
+__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
+  return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+__device__ __forceinline__ u32x4 nib_to_bf16(uint32_t w) {
+  const uint32_t a = w & 0x0F0F0F0Fu, b = (w >> 4) & 0x0F0F0F0Fu;
+  auto el = [&](int e) {
+    const int nb = q_nib(e);
+    return (float)(((nb & 1 ? b : a) >> (8 * (nb >> 1))) & 0xFFu);
+  };
+  return u32x4{bf16_pair(el(0), el(1)), bf16_pair(el(2), el(3)), bf16_pair(el(4), el(5)), bf16_pair(el(6), el(7))};
+}
+__device__ __forceinline__ u32x4 byte_to_bf16(uint32_t lo, uint32_t hi) {
+  auto el = [&](int e) { return (float)(((e < 4 ? lo : hi) >> (8 * (e & 3))) & 0xFFu); };
+  return u32x4{bf16_pair(el(0), el(1)), bf16_pair(el(2), el(3)), bf16_pair(el(4), el(5)), bf16_pair(el(6), el(7))};
+}
+// those of dim tile dt, from a unit's V fragments
 template <int KB>
 __device__ __forceinline__ u32x4 codes_bf16(const u32x4* vf, int dt) {
-  constexpr int DPF = QCode<KB>::DPF;
-  const u32x4& f = vf[dt / DPF];
-  u32x4 o;
-  auto pair = [](float a, float b) { return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u); };
-  if constexpr (KB == 4) {
-    // element e sits in nibble q_nib(e): even ones in the low half of the word
-    const uint32_t w = f[dt & 3], a = w & 0x0F0F0F0Fu, b = (w >> 4) & 0x0F0F0F0Fu;
-    auto el = [&](int e) {
-      const int nb = q_nib(e);
-      return (float)(((nb & 1 ? b : a) >> (8 * (nb >> 1))) & 0xFFu);
-    };
-#pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = pair(el(2 * j), el(2 * j + 1));
-  } else {
-    const uint32_t a = f[2 * (dt & 1)], b = f[2 * (dt & 1) + 1];
-    auto el = [&](int e) { return (float)(((e < 4 ? a : b) >> (8 * (e & 3))) & 0xFFu); };
-#pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = pair(el(2 * j), el(2 * j + 1));
-  }
-  return o;
+  const u32x4& f = vf[dt / QCode<KB>::DPF];
+  if constexpr (KB == 4) return nib_to_bf16(f[dt & 3]);
+  else return byte_to_bf16(f[2 * (dt & 1)], f[2 * (dt & 1) + 1]);
 }
 
-// grid (8-fold interleaved (part, kv head) pairs and column groups): the
-// workgroups of one pair's groups lie a multiple of 8 apart, on one XCD, whose
-// L2 then holds the K and V they share
+// which of the tokens t0 .. t0 + 7 a node sees: bit e of the cached ones (from
+// `from` on) and of the tree's, which begin at token P
+__device__ __forceinline__ uint32_t seen_tokens(const uint64_t* s_seen, const int* s_from, int node, int P, int t0) {
+  const uint64_t seen = s_seen[node];
+  auto below = [](int x) { return (1u << min(max(x, 0), 8)) - 1; };
+  const int a = P - t0;
+  const uint32_t cached = seen ? below(a) & ~below(s_from[node] - t0) : 0u;
+  const uint32_t tree = a > 0 ? (a < 8 ? (uint32_t)(seen << a) : 0u) : a > -64 ? (uint32_t)(seen >> -a) : 0u;
+  return (cached | tree) & 0xFFu;
+}
+
+// What a workgroup takes of the launch: workgroup x is one column group of one
+// (part, kv head) pair; the groups of a pair lie a multiple of 8 apart, on one
+// XCD, whose L2 then holds the K and V they share.
+struct TreePlace {
+  int i, h, group, part;  // h: -1 where there is nothing
+};
+__device__ __forceinline__ TreePlace tree_place(const Geometry& geo, const TreeBatch& tb) {
+  TreePlace p;
+  const int lane = threadIdx.x & 63, total = tb.part0[tb.n];
+  const int chunk = blockIdx.x / (8 * tb.groups), in = blockIdx.x - chunk * 8 * tb.groups;
+  const int pair = 8 * chunk + (in & 7);
+  p.group = in >> 3;
+  p.h = uniform(pair / total);
+  const int at = pair - p.h * total;
+  p.i = uniform(__popcll(__ballot(lane < tb.n && tb.part0[min(lane, tb.n - 1)] <= at)) - 1);
+  p.part = at - tb.part0[p.i];
+  if (p.h >= geo.hkv) p.h = -1;
+  return p;
+}
+
+// Each node's ancestors, those in its window, and the first cached token it
+// sees, by the first 64 threads
+__device__ __forceinline__ void tree_nodes(const TreeBatch& tb, const TreeRange& r, int start, uint64_t* s_seen, int* s_from) {
+  const int j = threadIdx.x;
+  if (j >= kMaxNodes) return;
+  uint64_t seen = j < r.N ? tb.ancestors[start + j] : 0;
+  const int depth = __popcll(seen) - 1;
+  s_from[j] = tb.window > 0 ? r.P + depth - tb.window + 1 : 0;
+  if (tb.window > 0)
+    for (int k = depth + 1; k > tb.window; --k) seen &= seen - 1;  // (the furthest come first)
+  s_seen[j] = seen;
+}
+
+// The units of a part: those that every column sees whole (from fa on, `full` of
+// them), then the others, in front of them and behind (at most 7 in all)
+struct TreePart {
+  int ua, fa, full, places;
+  __device__ __forceinline__ TreePart(const TreeBatch& tb, const TreeRange& r, int part) {
+    ua = r.u0 + part * r.cu;
+    const int ub = min(ua + r.cu, r.u0 + r.units);
+    const int whole0 = tb.window > 0 ? (max(0, r.P + r.N - tb.window) + 31) >> 5 : 0, whole1 = r.P >> 5;
+    fa = min(max(ua, whole0), ub);
+    full = max(min(ub, whole1) - fa, 0);
+    places = ub - ua;
+  }
+  // (places past the part's: its last one)
+  __device__ __forceinline__ int unit(int at) const {
+    const int p = min(at, places - 1), k = ua + p - full;
+    return p < full ? fa + p : k < fa ? k : k + full;
+  }
+};
+
+// What was noted: a value that is infinite or no number is so in the output of
+// every column that sees its token, whatever its weight
 template <int DT, int KB, int CT>
-__global__ __launch_bounds__(256, CT > 2 ? 1 : 2) void k_tree(Geometry geo, TreeBatch tb, const uint16_t* __restrict__ q,
+__device__ __forceinline__ void tree_odd(const Geometry& geo, const TreeRange& r, int seq, int h, const uint2* noted, int n_noted,
+                                         const uint64_t* s_seen, const int* s_from, int col0, int cols, f32x4 (&o)[CT][8]) {
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, sh = geo.tb == 64 ? 1 : 0;
+#pragma unroll 1
+  for (int x = 0; x < n_noted; ++x) {
+    const int unit = uniform((int)noted[x].x);
+#pragma unroll 1
+    for (uint32_t odd = (uint32_t)uniform((int)noted[x].y); odd; odd &= odd - 1) {
+      const int t = __ffs(odd) - 1, tok = 32 * (unit & sh) + t;
+      const int32_t page = block_table(geo, seq)[unit >> sh];
+      const uint8_t* own = geo.pool + ((size_t)page * geo.hkv + h) * geo.slab_bytes;
+      float v[32];
+#pragma unroll
+      for (int y = 0; y < 32; ++y) {
+        const int d = 16 * (y >> 2) + 4 * g + (y & 3);
+        if constexpr (KB == 0) {
+          v[y] = to_f32<DT>(((const uint16_t*)(own + geo.v_off))[v_elem(geo.tb, tok, d)]);
+        } else {
+          int bit;
+          const uint2 f = *(const uint2*)(own + geo.sb_off + 16 * sb_entry(geo.tb, tok) + 8);
+          const float code = (float)(own[geo.v_off + vq_byte(KB, geo.tb, tok, d, &bit)] >> bit & ((1 << KB) - 1));
+          v[y] = y < 16 ? __builtin_fmaf(lo_f(f.x), code, lo_f(f.y)) : __builtin_fmaf(hi_f(f.x), code, hi_f(f.y));
+        }
+        if (__builtin_isfinite(v[y])) v[y] = 0.f;
+      }
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        const int node = min(col0 + 16 * ct + n, cols - 1) / r.G;
+        const bool ok = seen_tokens(s_seen, s_from, node, r.P, 32 * unit + t) & 1;
+#pragma unroll
+        for (int y = 0; y < 32; ++y) o[ct][y >> 2][y & 3] += ok ? v[y] : 0.f;
+      }
+    }
+  }
+}
+
+// Columns first .. first + count - 1 out of W shares (references s_m, sums s_l,
+// o): the outputs, or the part's partials
+template <int DT, int W, int C, int THREADS>
+__device__ __forceinline__ void tree_write(const Geometry& geo, const TreeBatch& tb, const TreeRange& r, int i, int h, int part,
+                                           int start, int first, int count, bool direct, const float (&s_m)[W][C],
+                                           const float (&s_l)[W][C], const float (*s_o)[C][kHeadDim + 4],
+                                           const uint64_t* s_seen, uint16_t* __restrict__ out, float* __restrict__ partials) {
+  for (int e = threadIdx.x; e < count * kHeadDim; e += THREADS) {
+    const int c = e >> 7, d = e & 127, col = first + c;
+    float M = s_m[0][c];
+#pragma unroll
+    for (int v = 1; v < W; ++v) M = fmaxf(M, s_m[v][c]);
+    float L = 0.f, a = 0.f;
+#pragma unroll
+    for (int v = 0; v < W; ++v) {
+      const float mv = s_m[v][c];
+      const float f = mv == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mv - M);
+      L += f * s_l[v][c];
+      if (mv != -INFINITY) a += f * s_o[v][c][d];
+    }
+    const int node = col / r.G, hq = h * r.G + col - node * r.G;
+    if (s_seen[node] == 0) {  // absent: nothing is seen
+      M = -INFINITY;
+      L = a = 0.f;
+    }
+    if (direct) {
+      if (tb.sinks && M != -INFINITY) {
+        const float sk = tb.sinks[hq] * kTreeLog2e, top = fmaxf(M, sk), f = __builtin_amdgcn_exp2f(M - top);
+        L = L * f + (sk == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sk - top));
+        a *= f;
+      }
+      out[((int64_t)(start + node) * geo.hq + hq) * kHeadDim + d] = from_f32<DT>(L == 0.f ? 0.f : a / L);
+    } else {
+      float* pp = partials + ((int64_t)(tb.row0[i] + part * tb.max_tokens + node) * geo.hq + hq) * kPartial;
+      pp[d] = a;
+      if (d == 0) {
+        pp[kHeadDim] = M;
+        pp[kHeadDim + 1] = L;
+      }
+    }
+  }
+}
+
+// grid: see tree_place
+template <int DT, int KB, int CT>
+__global__ __launch_bounds__(256, 2) void k_tree(Geometry geo, TreeBatch tb, const uint16_t* __restrict__ q,
                                                              uint16_t* __restrict__ out, float* __restrict__ partials) {
   static_assert(KB == 0 || DT == 0, "affine caches: fp16");
   constexpr int PT = KB ? 1 : DT;  // P's type: weights times scales need bf16's range, and codes are exact in it
@@ -136,41 +280,22 @@ __global__ __launch_bounds__(256, CT > 2 ? 1 : 2) void k_tree(Geometry geo, Tree
 
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int n = lane & 15, g = lane >> 4, G = geo.group;
-  // which part, head and columns
-  const int total = tb.part0[tb.n], chunk = blockIdx.x / (8 * tb.groups), in = blockIdx.x - chunk * 8 * tb.groups;
-  const int pair = 8 * chunk + (in & 7), group = in >> 3;
-  const int h = uniform(pair / total), at = pair - h * total;
-  if (h >= geo.hkv) return;
-  const int i = uniform(__popcll(__ballot(lane < tb.n && tb.part0[min(lane, tb.n - 1)] <= at)) - 1);
-  const int part = at - tb.part0[i];
+  const TreePlace at = tree_place(geo, tb);
+  if (at.h < 0) return;
+  const int i = at.i, h = at.h, part = at.part;
   const TreeRange r = tree_range(geo, tb, i);
-  const int col0 = group * 16 * CT, cols = r.N * G;
+  const int col0 = at.group * 16 * CT, cols = r.N * G;
   const int parts = (r.units + r.cu - 1) / r.cu;
   if (col0 >= cols || part >= parts) return;
   const bool direct = tb.part0[i + 1] - tb.part0[i] <= 1;
   const int start = uniform(tb.starts[i]);
-  const int ua = r.u0 + part * r.cu, ub = min(ua + r.cu, r.u0 + r.units);
   const int seq = tb.ids[i];
 
   if (lane < 2) s_odd[wave][lane] = make_uint2(0u, 0u);
-  if (threadIdx.x < kMaxNodes) {
-    const int j = threadIdx.x;
-    uint64_t seen = j < r.N ? tb.ancestors[start + j] : 0;
-    const int depth = __popcll(seen) - 1;
-    s_from[j] = tb.window > 0 ? r.P + depth - tb.window + 1 : 0;
-    if (tb.window > 0)
-      for (int k = depth + 1; k > tb.window; --k) seen &= seen - 1;  // (the furthest come first)
-    s_seen[j] = seen;
-  }
-  // The part's units: those that every column sees whole (from fa on, `full` of
-  // them), then the others, in front of them and behind
-  const int whole0 = tb.window > 0 ? (max(0, r.P + r.N - tb.window) + 31) >> 5 : 0, whole1 = r.P >> 5;
-  const int fa = min(max(ua, whole0), ub), full = max(min(ub, whole1) - fa, 0), places = ub - ua;
-  // (places past the part's: its last one)
-  auto unit_at = [&](int at) {
-    const int p = min(at, places - 1), k = ua + p - full;
-    return p < full ? fa + p : k < fa ? k : k + full;
-  };
+  tree_nodes(tb, r, start, s_seen, s_from);
+  const TreePart pt(tb, r, part);
+  const int full = pt.full, places = pt.places;
+  auto unit_at = [&](int at) { return pt.unit(at); };
   int place = wave;  // a wave takes every fourth
   TreePages pages(geo, seq, h, unit_at(place));
   // scores are products times |scale|, of queries with its sign: the largest is
@@ -304,15 +429,9 @@ __global__ __launch_bounds__(256, CT > 2 ? 1 : 2) void k_tree(Geometry geo, Tree
       uint32_t odd = 0;  // tokens with such values
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
-        const int node = min(col0 + 16 * ct + n, cols - 1) / G;
-        const uint64_t seen = s_seen[node];
-        const int from = seen ? s_from[node] : r.T;
+        const uint32_t mask = seen_tokens(s_seen, s_from, min(col0 + 16 * ct + n, cols - 1) / G, r.P, t0);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int t = t0 + e, a = t - r.P;
-          const bool ok = a < 0 ? t >= from : a < r.N && (seen >> (a & 63) & 1);
-          sv[ct][e] = ok ? sv[ct][e] : -INFINITY;
-        }
+        for (int e = 0; e < 8; ++e) sv[ct][e] = mask >> e & 1 ? sv[ct][e] : -INFINITY;
       }
       if constexpr (KB == 0) {
         uint32_t any = 0;
@@ -435,40 +554,7 @@ __global__ __launch_bounds__(256, CT > 2 ? 1 : 2) void k_tree(Geometry geo, Tree
   }
 #pragma unroll 1
   for (; place < places; place += 4) step();
-  // what was noted: a value that is infinite or no number is so in the output,
-  // whatever its weight
-#pragma unroll 1
-  for (int x = 0; x < 2; ++x) {
-    const int unit = uniform((int)s_odd[wave][x].x);
-#pragma unroll 1
-    for (uint32_t odd = (uint32_t)uniform((int)s_odd[wave][x].y); odd; odd &= odd - 1) {
-      const int t = __ffs(odd) - 1, tok = 32 * (unit & pages.sh) + t, a = 32 * unit + t - r.P;
-      const int32_t page = block_table(geo, seq)[unit >> pages.sh];
-      const uint8_t* own = geo.pool + ((size_t)page * geo.hkv + h) * geo.slab_bytes;
-      float v[32];
-#pragma unroll
-      for (int y = 0; y < 32; ++y) {
-        const int d = 16 * (y >> 2) + 4 * g + (y & 3);
-        if constexpr (KB == 0) {
-          v[y] = to_f32<DT>(((const uint16_t*)(own + geo.v_off))[v_elem(geo.tb, tok, d)]);
-        } else {
-          int sh;
-          const uint2 f = *(const uint2*)(own + geo.sb_off + 16 * sb_entry(geo.tb, tok) + 8);
-          const float code = (float)(own[geo.v_off + vq_byte(KB, geo.tb, tok, d, &sh)] >> sh & ((1 << KB) - 1));
-          v[y] = y < 16 ? __builtin_fmaf(lo_f(f.x), code, lo_f(f.y)) : __builtin_fmaf(hi_f(f.x), code, hi_f(f.y));
-        }
-        if (__builtin_isfinite(v[y])) v[y] = 0.f;
-      }
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        const int node = min(col0 + 16 * ct + n, cols - 1) / G;
-        const uint64_t seen = s_seen[node];
-        const bool ok = seen && (a < 0 ? a + r.P >= s_from[node] : a < r.N && (seen >> (a & 63) & 1));
-#pragma unroll
-        for (int y = 0; y < 32; ++y) o[ct][y >> 2][y & 3] += ok ? v[y] : 0.f;
-      }
-    }
-  }
+  tree_odd<DT, KB, CT>(geo, r, seq, h, &s_odd[wave][0], 2, s_seen, s_from, col0, cols, o);
 
   // the four waves' shares joined, a column tile at a time
 #pragma unroll 1
@@ -500,42 +586,380 @@ __global__ __launch_bounds__(256, CT > 2 ? 1 : 2) void k_tree(Geometry geo, Tree
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) *(f32x4*)&s_o[wave][n][16 * dt + 4 * g] = oc[dt];
     __syncthreads();
-    for (int e = threadIdx.x; e < 16 * kHeadDim; e += 256) {
-      const int c = e >> 7, d = e & 127, col = first + c;
-      if (col >= cols) break;
-      float M = s_m[0][c];
+    tree_write<DT, 4, 16, 256>(geo, tb, r, i, h, part, start, first, min(cols - first, 16), direct, s_m, s_l, s_o, s_seen, out,
+                               partials);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// More than 32 columns: eight waves share what they read through LDS.  CW waves
+// hold 32 columns each and take the same unit, 8 / CW groups of them different
+// ones: a step is 8 / CW units.  In step s a wave writes its share of unit s + 1
+// of its group (16-bit operands, affine codes as fp16 and bf16) to LDS, which it
+// loaded in step s - 1, asks for that of s + 2, and takes unit s from LDS.
+// grid: see tree_place
+// ---------------------------------------------------------------------------
+template <int KB>
+struct Raw {  // a lane's part of a 16-bit operand fragment, as stored
+  typedef uint2 T;
+};
+template <>
+struct Raw<0> {
+  typedef u32x4 T;
+};
+template <>
+struct Raw<4> {
+  typedef uint32_t T;
+};
+
+// a workgroup barrier that orders LDS only: the global loads of later units stay
+// in flight across it
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+template <int DT, int KB, int CW>
+__global__ __launch_bounds__(512, 2) void k_tree_wide(Geometry geo, TreeBatch tb, const uint16_t* __restrict__ q,
+                                                      uint16_t* __restrict__ out, float* __restrict__ partials) {
+  static_assert(KB == 0 || DT == 0, "affine caches: fp16");
+  constexpr int TW = 8 / CW, CT = 2, F = 8 / CW;  // F: K, and V, operand fragments of a unit that a wave brings
+  constexpr int PT = KB ? 1 : DT;
+  constexpr float kLift = PT == 0 ? kTreeTop - kTreeSlack : 0.0f;
+  constexpr int COLS = 32 * CW;
+  using R = typename Raw<KB>::T;
+  // two units of each group ([slot][group][8 K, 8 V fragments][lane]), and in the
+  // end the groups' sums
+  constexpr int RING = 2 * TW * 16 * 64, SUMS = TW * COLS * (kHeadDim + 4) / 4;
+  __shared__ u32x4 s_mem[RING > SUMS ? RING : SUMS];
+  __shared__ u32x4 s_ent[KB ? 2 * TW : 1][KB ? 32 : 1];  // (affine) scales and biases
+  __shared__ uint64_t s_seen[kMaxNodes];
+  __shared__ int s_from[kMaxNodes];
+  __shared__ uint2 s_odd[8][8];  // units with values that are infinite or no numbers, and their tokens
+  __shared__ float s_m[TW][COLS], s_l[TW][COLS];
+
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int n = lane & 15, g = lane >> 4, G = geo.group;
+  const int cw = wave % CW, tw = wave / CW;
+  const TreePlace at = tree_place(geo, tb);
+  if (at.h < 0) return;
+  const int i = at.i, h = at.h, part = at.part;
+  const TreeRange r = tree_range(geo, tb, i);
+  const int col0 = at.group * COLS + 32 * cw, cols = r.N * G;
+  const int parts = (r.units + r.cu - 1) / r.cu;
+  if (at.group * COLS >= cols || part >= parts) return;
+  const bool direct = tb.part0[i + 1] - tb.part0[i] <= 1;
+  const int start = uniform(tb.starts[i]);
+  const int seq = tb.ids[i];
+  if (lane < 8) s_odd[wave][lane] = make_uint2(0u, 0u);
+  tree_nodes(tb, r, start, s_seen, s_from);
+  const TreePart pt(tb, r, part);
+  const int steps = (pt.places + TW - 1) / TW, whole = pt.full / TW;  // (steps of whole units come first)
+
+  const float sc = fmaxf(fabsf(tb.sl2), 1e-30f);
+  const uint32_t qflip = tb.sl2 < 0.f ? 0x80008000u : 0u;
+  u32x4 qf[CT][4];
+  [[maybe_unused]] float q0[CT], q1[CT], q0c[CT], q1c[CT];
 #pragma unroll
-      for (int v = 1; v < 4; ++v) M = fmaxf(M, s_m[v][c]);
-      float L = 0.f, a = 0.f;
+  for (int ct = 0; ct < CT; ++ct) {
+    const int col = min(col0 + 16 * ct + n, cols - 1), node = col / G;
+    const uint16_t* src = q + (int64_t)(start + node) * tb.qr + (int64_t)(h * G + col - node * G) * tb.qh + 8 * g;
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const float mv = s_m[v][c];
-        const float f = mv == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mv - M);
-        L += f * s_l[v][c];
-        if (mv != -INFINITY) a += f * s_o[v][c][d];
-      }
-      const int node = col / G, hq = h * G + col - node * G;
-      if (s_seen[node] == 0) {  // absent: nothing is seen
-        M = -INFINITY;
-        L = a = 0.f;
-      }
-      if (direct) {
-        if (tb.sinks && M != -INFINITY) {
-          const float sk = tb.sinks[hq] * kTreeLog2e, top = fmaxf(M, sk), f = __builtin_amdgcn_exp2f(M - top);
-          L = L * f + (sk == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sk - top));
-          a *= f;
+    for (int s = 0; s < 4; ++s) qf[ct][s] = *(const u32x4*)(src + 32 * s) ^ qflip;
+    if constexpr (KB != 0) {
+      const u32x4 ones = u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
+      const f32x4 zero = f32x4{0.f, 0.f, 0.f, 0.f};
+      q0[ct] = mfma_f16(ones, qf[ct][1], mfma_f16(ones, qf[ct][0], zero))[0];
+      q1[ct] = mfma_f16(ones, qf[ct][3], mfma_f16(ones, qf[ct][2], zero))[0];
+      if constexpr (KB == 4)
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          qf[ct][s][1] = f16x2_unit16(qf[ct][s][1]);
+          qf[ct][s][3] = f16x2_unit16(qf[ct][s][3]);
         }
-        out[((int64_t)(start + node) * geo.hq + hq) * kHeadDim + d] = from_f32<DT>(L == 0.f ? 0.f : a / L);
+      q0c[ct] = mfma_f16(ones, qf[ct][1], mfma_f16(ones, qf[ct][0], zero))[0] * -kDecOff;
+      q1c[ct] = mfma_f16(ones, qf[ct][3], mfma_f16(ones, qf[ct][2], zero))[0] * -kDecOff;
+    }
+  }
+  [[maybe_unused]] const uint32_t code_base = KB ? f16_pair_1024() : 0u;
+
+  // --- units from memory: operand fragments f = cw + CW x of K (key tile f / 4,
+  // k-step f % 4) and of V (dim tile f)
+  TreePages pages(geo, seq, h, pt.unit(tw));
+  R rk[F], rv[F];
+  [[maybe_unused]] u32x4 re;
+  auto load = [&](int step) __attribute__((always_inline)) {  // (pages.unit is the step's unit)
+    const int sub = pages.unit & pages.sh;
+    const uint8_t *slab = pages.slab(geo), *ks = slab + geo.k_off, *vs = slab + geo.v_off;
+    pages.ask(pt.unit((step + 1) * TW + tw));
+#pragma unroll
+    for (int x = 0; x < F; ++x) {
+      const int f = cw + CW * x;
+      if constexpr (KB == 0) {
+        rk[x] = *(const R*)(ks + (8 * sub + f) * 1024 + lane * 16);
+        rv[x] = *(const R*)(vs + ((f << pages.sh) + sub) * 1024 + lane * 16);
+      } else if constexpr (KB == 4) {
+        rk[x] = *(const R*)(ks + (2 * sub + (f >> 2)) * 1024 + 4 * (f & 3) + lane * 16);
+        rv[x] = *(const R*)(vs + (((f >> 2) << pages.sh) + sub) * 1024 + 4 * (f & 3) + lane * 16);
       } else {
-        float* pp = partials + ((int64_t)(tb.row0[i] + part * tb.max_tokens + node) * geo.hq + hq) * kPartial;
-        pp[d] = a;
-        if (d == 0) {
-          pp[kHeadDim] = M;
-          pp[kHeadDim + 1] = L;
+        rk[x] = *(const R*)(ks + (4 * sub + (f >> 1)) * 1024 + 8 * (f & 1) + lane * 16);
+        rv[x] = *(const R*)(vs + (((f >> 1) << pages.sh) + sub) * 1024 + 8 * (f & 1) + lane * 16);
+      }
+    }
+    if constexpr (KB != 0)
+      re = *(const u32x4*)(slab + geo.sb_off + sub * 128 + 16 * (((lane >> 3) & 3) * (geo.tb >> 2) + (lane & 7)));
+  };
+  auto stage = [&](int slot) __attribute__((always_inline)) {
+    u32x4* to = s_mem + (slot * TW + tw) * 16 * 64 + lane;
+#pragma unroll
+    for (int x = 0; x < F; ++x) {
+      const int f = cw + CW * x;
+      if constexpr (KB == 0) {
+        to[f * 64] = rk[x];
+        to[(8 + f) * 64] = rv[x];
+      } else if constexpr (KB == 4) {
+        to[f * 64] = nib_to_f16_dec(rk[x], code_base);
+        to[(8 + f) * 64] = nib_to_bf16(rv[x]);
+      } else {
+        to[f * 64] = byte_to_f16(rk[x].x, rk[x].y);
+        to[(8 + f) * 64] = byte_to_bf16(rv[x].x, rv[x].y);
+      }
+    }
+    if constexpr (KB != 0)
+      if (cw == 0) s_ent[slot * TW + tw][lane & 31] = re;
+  };
+
+  f32x4 o[CT][8];
+  float m[CT], base[CT], limit[CT], l[CT];
+  [[maybe_unused]] float ob0[CT], ob1[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) o[ct][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m[ct] = limit[ct] = -INFINITY;
+    base[ct] = l[ct] = 0.f;
+    if constexpr (KB != 0) ob0[ct] = ob1[ct] = 0.f;
+  }
+
+  auto compute = [&](int step, int slot, auto edge) __attribute__((always_inline)) {
+    constexpr bool EDGE = decltype(edge)::value;
+    const u32x4* in = s_mem + (slot * TW + tw) * 16 * 64 + lane;
+    float sv[CT][8];
+    if constexpr (KB == 0) {
+      f32x4 acc[CT][2];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) acc[ct][0] = acc[ct][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const u32x4 a = in[(4 * t + s) * 64];
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) acc[ct][t] = mfma16x16x32<DT>(a, qf[ct][s], acc[ct][t]);
+        }
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sv[ct][e] = acc[ct][e >> 2][e & 3];
+    } else {
+      f32x4 acc[CT][4];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        acc[ct][0] = acc[ct][1] = f32x4{q0c[ct], q0c[ct], q0c[ct], q0c[ct]};
+        acc[ct][2] = acc[ct][3] = f32x4{q1c[ct], q1c[ct], q1c[ct], q1c[ct]};
+      }
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const u32x4 a = in[(4 * t + s) * 64];
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) acc[ct][2 * (s >> 1) + t] = mfma_f16(a, qf[ct][s], acc[ct][2 * (s >> 1) + t]);
+        }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint2 sb = *(const uint2*)&s_ent[slot * TW + tw][8 * g + e];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          float x = lo_f(sb.x) * acc[ct][e >> 2][e & 3];
+          x = __builtin_fmaf(hi_f(sb.x), acc[ct][2 + (e >> 2)][e & 3], x);
+          x = __builtin_fmaf(lo_f(sb.y), q0[ct], x);
+          sv[ct][e] = __builtin_fmaf(hi_f(sb.y), q1[ct], x);
         }
       }
     }
+    [[maybe_unused]] const int unit = pt.unit(step * TW + tw), t0 = 32 * unit + 8 * g;
+    if constexpr (EDGE) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        const uint32_t mask = seen_tokens(s_seen, s_from, min(col0 + 16 * ct + n, cols - 1) / G, r.P, t0);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sv[ct][e] = mask >> e & 1 ? sv[ct][e] : -INFINITY;
+      }
+    }
+    float mx[CT];
+    bool raise = false;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      mx[ct] = sv[ct][0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) mx[ct] = fmaxf(mx[ct], sv[ct][e]);
+      raise = raise || mx[ct] > limit[ct];
+    }
+    if (__any(raise)) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        const float top = fmaxf(m[ct], max_over_groups(mx[ct]) * sc);
+        const float f = top == m[ct] ? 1.0f : __builtin_amdgcn_exp2f(m[ct] - top);
+        m[ct] = top;
+        base[ct] = (top == -INFINITY ? 0.0f : top) - kLift;
+        limit[ct] = (top + kTreeSlack) / sc;
+        l[ct] *= f;
+        if constexpr (KB != 0) {
+          ob0[ct] *= f;
+          ob1[ct] *= f;
+        }
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) o[ct][dt] *= f;
+      }
+    }
+    // weights, as operands' two parts
+    [[maybe_unused]] uint32_t odd = 0;
+    if constexpr (KB == 0) {
+      u32x4 hi[CT], lo[CT];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          sv[ct][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[ct][e], sc, -base[ct]));
+          l[ct] += sv[ct][e];
+        }
+        tree_split<PT>(sv[ct], hi[ct], lo[ct]);
+      }
+      uint32_t any = 0;
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt) {
+        u32x4 v = in[(8 + dt) * 64];
+        if constexpr (EDGE) {
+          // values of tokens that no node sees (old pages hold anything) are taken
+          // as zeros; so are infinities and NaN, which are noted
+          constexpr uint32_t INF = DT == 0 ? 0x7C00u : 0x7F80u;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int a = t0 + 2 * j;
+            const uint32_t keep = (a >= r.lo && a < r.T ? 0x0000FFFFu : 0u) | (a + 1 >= r.lo && a + 1 < r.T ? 0xFFFF0000u : 0u);
+            const uint32_t w = v[j] & keep;
+            const uint32_t x = (w & INF) == INF ? 0xFFFFu : 0u, y = (w >> 16 & INF) == INF ? 0xFFFF0000u : 0u;
+            any |= (x ? 1u << (2 * j) : 0u) | (y ? 2u << (2 * j) : 0u);
+            v[j] = w & ~(x | y);
+          }
+        }
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) o[ct][dt] = mfma16x16x32<DT>(v, hi[ct], o[ct][dt]);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) o[ct][dt] = mfma16x16x32<DT>(v, lo[ct], o[ct][dt]);
+      }
+      if constexpr (EDGE) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint64_t who = __ballot(any >> e & 1);
+#pragma unroll
+          for (int gg = 0; gg < 4; ++gg)
+            if (who >> (16 * gg) & 0xFFFF) odd |= 1u << (8 * gg + e);
+        }
+      }
+    } else {
+      // o_d = sum_t (p_t vs_j) c_td + sum_t p_t vb_j for group j of 64 dims
+      u32x4 hi[CT][2], lo[CT][2];
+      float w0[CT][8], w1[CT][8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        uint2 sb = *((const uint2*)&s_ent[slot * TW + tw][8 * g + e] + 1);
+        if constexpr (EDGE) {  // (as above; of a token with such a scale or bias, its 64 dims)
+          auto inf = [](uint32_t w) {
+            return ((w & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u) | ((w >> 16 & 0x7C00u) == 0x7C00u ? 0xFFFF0000u : 0u);
+          };
+          const uint32_t bad = inf(sb.x) | inf(sb.y);
+          const uint64_t who = __ballot(bad != 0);
+#pragma unroll
+          for (int gg = 0; gg < 4; ++gg)
+            if (who >> (16 * gg) & 0xFFFF) odd |= 1u << (8 * gg + e);
+          sb = make_uint2(sb.x & ~bad, sb.y & ~bad);
+        }
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[ct][e], sc, -base[ct]));
+          l[ct] += p;
+          w0[ct][e] = p * lo_f(sb.x);
+          w1[ct][e] = p * hi_f(sb.x);
+          ob0[ct] = __builtin_fmaf(p, lo_f(sb.y), ob0[ct]);
+          ob1[ct] = __builtin_fmaf(p, hi_f(sb.y), ob1[ct]);
+        }
+      }
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        tree_split<1>(w0[ct], hi[ct][0], lo[ct][0]);
+        tree_split<1>(w1[ct], hi[ct][1], lo[ct][1]);
+      }
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt) {
+        const u32x4 v = in[(8 + dt) * 64];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) o[ct][dt] = mfma16x16x32<1>(v, hi[ct][dt >> 2], o[ct][dt]);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) o[ct][dt] = mfma16x16x32<1>(v, lo[ct][dt >> 2], o[ct][dt]);
+      }
+    }
+    if constexpr (EDGE)
+      if (odd && lane == 0) s_odd[wave][step - whole] = make_uint2(unit, odd);
+  };
+
+  load(0);
+  stage(0);
+  load(1);
+  lds_barrier();
+#pragma unroll 1
+  for (int s = 0; s < whole; ++s) {
+    stage((s + 1) & 1);
+    load(s + 2);
+    compute(s, s & 1, std::false_type());
+    lds_barrier();
   }
+#pragma unroll 1
+  for (int s = whole; s < steps; ++s) {
+    stage((s + 1) & 1);
+    load(s + 2);
+    if (s * TW + tw < pt.places) compute(s, s & 1, std::true_type());
+    lds_barrier();
+  }
+  tree_odd<DT, KB, CT>(geo, r, seq, h, &s_odd[wave][0], 8, s_seen, s_from, col0, cols, o);
+
+  // the groups' shares joined
+  float (*s_o)[COLS][kHeadDim + 4] = (float (*)[COLS][kHeadDim + 4])s_mem;
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int c = 32 * cw + 16 * ct + n;
+    const float lc = sum_over_groups(l[ct]);
+    if (g == 0) {
+      s_m[tw][c] = m[ct] == -INFINITY ? m[ct] : base[ct];
+      s_l[tw][c] = lc;
+    }
+    float b0 = 0.f, b1 = 0.f;
+    if constexpr (KB != 0) {
+      b0 = sum_over_groups(ob0[ct]);
+      b1 = sum_over_groups(ob1[ct]);
+    }
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) {
+      f32x4 x = o[ct][dt];
+      if constexpr (KB != 0) x += dt < 4 ? b0 : b1;
+      *(f32x4*)&s_o[tw][c][16 * dt + 4 * g] = x;
+    }
+  }
+  __syncthreads();
+  tree_write<DT, TW, COLS, 512>(geo, tb, r, i, h, part, start, at.group * COLS, min(cols - at.group * COLS, COLS), direct,
+                                s_m, s_l, s_o, s_seen, out, partials);
 }
 
 // The parts of one (node, query head) joined, eight rows of 32 lanes with four
@@ -593,11 +1017,13 @@ template <int DT, int KB>
 static void tree_dispatch(const Geometry& g, const TreeBatch& tb, const uint16_t* q, uint16_t* out, float* ws,
                           hipStream_t s, Timing* prof) {
   const int64_t pairs = ((int64_t)tb.part0[tb.n] * g.hkv + 7) & ~7ll;
-  const dim3 grid((unsigned)(pairs * tb.groups)), blk(256);
-  if (tb.tiles == 1) launch(k_tree<DT, KB, 1>, grid, blk, 0, s, prof, kProfTree, g, tb, q, out, ws);
-  else if (tb.tiles == 2) launch(k_tree<DT, KB, 2>, grid, blk, 0, s, prof, kProfTree, g, tb, q, out, ws);
-  else if (tb.tiles == 3) launch(k_tree<DT, KB, 3>, grid, blk, 0, s, prof, kProfTree, g, tb, q, out, ws);
-  else launch(k_tree<DT, KB, 4>, grid, blk, 0, s, prof, kProfTree, g, tb, q, out, ws);
+  const dim3 grid((unsigned)(pairs * tb.groups));
+  auto go = [&](auto kernel, int threads) { launch(kernel, grid, dim3(threads), 0, s, prof, kProfTree, g, tb, q, out, ws); };
+  if (tb.tiles == 1) go(k_tree<DT, KB, 1>, 256);
+  else if (tb.tiles == 2) go(k_tree<DT, KB, 2>, 256);
+  else if (tb.tiles == 4) go(k_tree_wide<DT, KB, 2>, 512);
+  else if (tb.tiles == 8) go(k_tree_wide<DT, KB, 4>, 512);
+  else go(k_tree_wide<DT, KB, 8>, 512);
 }
 
 static_assert(sizeof(Geometry) + sizeof(TreeBatch) <= 4000, "a launch's arguments stay under 4 KiB");

@@ -8,12 +8,8 @@ namespace bsattn {
 
 int64_t tree_plan(const Geometry& g, TreeBatch& tb) {
   const int cols = tb.max_tokens * g.group;
-  // Column tiles per workgroup: two leave room for two waves a SIMD (8 x 32k bf16
-  // tokens, trees of 16: 208 us, 216 with four); dequantising affine caches for
-  // more of them at once pays (4 x 262k int8, 96 columns: 556 us with three, 764 with two)
-  const int tiles = (cols + 15) / 16, most_tiles = g.kv_bits ? 4 : 2;
-  tb.groups = (tiles + most_tiles - 1) / most_tiles;
-  tb.tiles = (tiles + tb.groups - 1) / tb.groups;
+  tb.tiles = cols <= 16 ? 1 : cols <= 32 ? 2 : cols <= 64 ? 4 : cols <= 128 ? 8 : 16;
+  tb.groups = (cols + 16 * tb.tiles - 1) / (16 * tb.tiles);
   int64_t all = 0;
   int most = 1;
   for (int i = 0; i < tb.n; ++i) {
