@@ -5,15 +5,14 @@
 // for 16-bit and affine caches.
 //
 // A workgroup takes a part of one (request, kv head)'s tokens, in units of 32,
-// for up to 16 CT columns, each a (node, query head) pair; its four waves take
-// every fourth unit of the part for all of the columns.  K and V lie in the slabs as
-// the matrix instructions take them, so a wave works in registers alone:
+// for a group of the columns, each a (node, query head) pair:
 //   S^T[token][col] = K[token][:] . Q^T      (A = K rows, B = Q^T)
 //   O^T[dim][col]  += V^T[dim][token] . P^T  (A = V^T,    B = P^T)
-// A lane (column n, group g) holds column n's share of tokens 8g .. 8g + 7 in
-// both, and the next unit's K is asked for as soon as this one's is used, its V
-// likewise.  P enters as two 16-bit parts, for 16 (bf16) or 22 (fp16) bits.
-// Only the units that hold drafted tokens, or where a window begins, are masked.
+// with MFMA 16x16x32.  A lane (column n, group g) holds column n's share of tokens
+// 8g .. 8g + 7 in both, so P goes from one to the other without a shuffle.  P
+// enters as two 16-bit parts, for 16 (bf16) or 22 (fp16) bits.  Affine codes enter
+// as 1024 + c (K, fp16) and c (V, bf16), exactly; scales and biases act on scores
+// and weights.
 #include <hip/hip_ext.h>
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -34,14 +33,15 @@ constexpr float kTreeTop = 14.0f;
 
 // What a request brings to a launch, and the units of its part
 struct TreeRange {
-  int T, N, P, lo, u0, units, cu, G;
+  int T, N, P, lo, u0, units, cu;
+  int lg;  // log2 of the heads of a group
 };
 __device__ __forceinline__ TreeRange tree_range(const Geometry& geo, const TreeBatch& tb, int i) {
   TreeRange r;
   r.T = uniform(geo.meta[tb.ids[i]]);
   r.N = min(min(uniform(tb.taken[i]), tb.max_tokens), r.T);
   r.P = r.T - r.N;
-  r.G = geo.group;
+  r.lg = __builtin_ctz((unsigned)geo.group);
   r.lo = tb.window > 0 ? max(0, r.P - tb.window + 1) : 0;  // the first token that a root sees
   r.u0 = r.lo >> 5;
   r.units = r.N > 0 ? ((r.T - 1) >> 5) - r.u0 + 1 : 0;
@@ -108,12 +108,12 @@ __device__ __forceinline__ u32x4 byte_to_bf16(uint32_t lo, uint32_t hi) {
   auto el = [&](int e) { return (float)(((e < 4 ? lo : hi) >> (8 * (e & 3))) & 0xFFu); };
   return u32x4{bf16_pair(el(0), el(1)), bf16_pair(el(2), el(3)), bf16_pair(el(4), el(5)), bf16_pair(el(6), el(7))};
 }
-// those of dim tile dt, from a unit's V fragments
-template <int KB>
-__device__ __forceinline__ u32x4 codes_bf16(const u32x4* vf, int dt) {
-  const u32x4& f = vf[dt / QCode<KB>::DPF];
-  if constexpr (KB == 4) return nib_to_bf16(f[dt & 3]);
-  else return byte_to_bf16(f[2 * (dt & 1)], f[2 * (dt & 1) + 1]);
+// a workgroup barrier that orders LDS only: the global loads of later units stay
+// in flight across it
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
 // which of the tokens t0 .. t0 + 7 a node sees: bit e of the cached ones (from
@@ -182,11 +182,12 @@ struct TreePart {
 // What was noted: a value that is infinite or no number is so in the output of
 // every column that sees its token, whatever its weight
 template <int DT, int KB, int CT>
-__device__ __forceinline__ void tree_odd(const Geometry& geo, const TreeRange& r, int seq, int h, const uint2* noted, int n_noted,
+__device__ __forceinline__ void tree_odd(const Geometry& geo, const TreeRange& r, int seq, int h, const uint2* noted,
                                          const uint64_t* s_seen, const int* s_from, int col0, int cols, f32x4 (&o)[CT][8]) {
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, sh = geo.tb == 64 ? 1 : 0;
+  if (!__any(noted[lane & 7].y != 0)) return;
 #pragma unroll 1
-  for (int x = 0; x < n_noted; ++x) {
+  for (int x = 0; x < 8; ++x) {
     const int unit = uniform((int)noted[x].x);
 #pragma unroll 1
     for (uint32_t odd = (uint32_t)uniform((int)noted[x].y); odd; odd &= odd - 1) {
@@ -209,7 +210,7 @@ __device__ __forceinline__ void tree_odd(const Geometry& geo, const TreeRange& r
       }
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
-        const int node = min(col0 + 16 * ct + n, cols - 1) / r.G;
+        const int node = min(col0 + 16 * ct + n, cols - 1) >> r.lg;
         const bool ok = seen_tokens(s_seen, s_from, node, r.P, 32 * unit + t) & 1;
 #pragma unroll
         for (int y = 0; y < 32; ++y) o[ct][y >> 2][y & 3] += ok ? v[y] : 0.f;
@@ -238,7 +239,7 @@ __device__ __forceinline__ void tree_write(const Geometry& geo, const TreeBatch&
       L += f * s_l[v][c];
       if (mv != -INFINITY) a += f * s_o[v][c][d];
     }
-    const int node = col / r.G, hq = h * r.G + col - node * r.G;
+    const int node = col >> r.lg, hq = (h << r.lg) + col - (node << r.lg);
     if (s_seen[node] == 0) {  // absent: nothing is seen
       M = -INFINITY;
       L = a = 0.f;
@@ -261,53 +262,104 @@ __device__ __forceinline__ void tree_write(const Geometry& geo, const TreeBatch&
   }
 }
 
+template <int KB>
+struct Raw {  // a lane's part of a 16-bit operand fragment, as stored
+  typedef uint2 T;
+};
+template <>
+struct Raw<0> {
+  typedef u32x4 T;
+};
+template <>
+struct Raw<4> {
+  typedef uint32_t T;
+};
+
+// ---------------------------------------------------------------------------
+// CW waves hold 16 CT columns each and take the same units; TW such teams take
+// different ones, a unit each per step.  A unit passes through LDS, as 16-bit
+// operands: each wave of the team brings its share of the fragments, loaded a
+// step before.  So K and V are read, and affine codes converted, once for all of
+// the columns (each wave on its own with its own loads: 64 columns 208, 256 485 us
+// over 8 x 32k bf16 tokens; 100 columns over 4 x 131k int4 800).  A team of one
+// wave (CW 1) needs no barrier, and one place for its unit.
 // grid: see tree_place
-template <int DT, int KB, int CT>
-__global__ __launch_bounds__(256, 2) void k_tree(Geometry geo, TreeBatch tb, const uint16_t* __restrict__ q,
-                                                             uint16_t* __restrict__ out, float* __restrict__ partials) {
+// ---------------------------------------------------------------------------
+template <int DT, int KB, int CT, int CW>
+__global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, TreeBatch tb, const uint16_t* __restrict__ q,
+                                                                uint16_t* __restrict__ out, float* __restrict__ partials) {
   static_assert(KB == 0 || DT == 0, "affine caches: fp16");
-  constexpr int PT = KB ? 1 : DT;  // P's type: weights times scales need bf16's range, and codes are exact in it
+  constexpr int W = CW == 1 ? 4 : 8, TW = W / CW, SLOTS = CW == 1 ? 1 : 2;
+  constexpr int F = 8 / CW;       // K, and V, operand fragments of a unit that a wave brings: cw + CW x
+  constexpr int PT = KB ? 1 : DT; // P's type: weights times scales need bf16's range, and codes are exact in it
+  // fp16 weights are lifted to at most 2^14, so that small ones keep their bits
   constexpr float kLift = PT == 0 ? kTreeTop - kTreeSlack : 0.0f;
-  constexpr int NK = KB ? 2 * QCode<KB ? KB : 4>::KF : 8, NV = KB ? 8 / QCode<KB ? KB : 4>::DPF : 8;
-  __shared__ uint64_t s_seen[kMaxNodes];  // each node's ancestors, those in its window
-  __shared__ int s_from[kMaxNodes];       // the first cached token it sees
-  // (affine) a unit's scales and biases, the keys' and the values'; the waves' own
-  __shared__ uint2 s_sb[KB ? 4 : 1][KB ? 32 : 1], s_sv[KB ? 4 : 1][KB ? 32 : 1];
-  // units with values of this kind (a wave has at most two with columns that do not see all of them), and their tokens
-  __shared__ uint2 s_odd[4][2];
-  __shared__ float s_m[4][16], s_l[4][16];
-  __shared__ __align__(16) float s_o[4][16][kHeadDim + 4];
+  constexpr int COLS = 16 * CT * CW;
+  using R = typename Raw<KB>::T;
+  // units of each team ([slot][team][8 K, 8 V fragments][lane]), and in the end the
+  // teams' sums
+  constexpr int RING = SLOTS * TW * 16 * 64, SUMS = TW * COLS * (kHeadDim + 4) / 4;
+  __shared__ u32x4 s_mem[RING > SUMS ? RING : SUMS];
+  __shared__ u32x4 s_ent[KB ? SLOTS * TW : 1][KB ? 32 : 1];  // (affine) scales and biases
+  __shared__ uint64_t s_seen[kMaxNodes];
+  __shared__ int s_from[kMaxNodes];
+  __shared__ uint2 s_odd[TW][8];  // units with values that are infinite or no numbers, and their tokens
+  __shared__ float s_m[TW][COLS], s_l[TW][COLS];
 
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int n = lane & 15, g = lane >> 4, G = geo.group;
+  const int n = lane & 15, g = lane >> 4, cw = wave % CW, tw = wave / CW;
   const TreePlace at = tree_place(geo, tb);
   if (at.h < 0) return;
   const int i = at.i, h = at.h, part = at.part;
   const TreeRange r = tree_range(geo, tb, i);
-  const int col0 = at.group * 16 * CT, cols = r.N * G;
+  const int first = at.group * COLS, col0 = first + 16 * CT * cw, cols = r.N << r.lg;
   const int parts = (r.units + r.cu - 1) / r.cu;
-  if (col0 >= cols || part >= parts) return;
+  if (first >= cols || part >= parts) return;
   const bool direct = tb.part0[i + 1] - tb.part0[i] <= 1;
-  const int start = uniform(tb.starts[i]);
-  const int seq = tb.ids[i];
-
-  if (lane < 2) s_odd[wave][lane] = make_uint2(0u, 0u);
-  tree_nodes(tb, r, start, s_seen, s_from);
+  const int start = uniform(tb.starts[i]), seq = tb.ids[i];
   const TreePart pt(tb, r, part);
-  const int full = pt.full, places = pt.places;
-  auto unit_at = [&](int at) { return pt.unit(at); };
-  int place = wave;  // a wave takes every fourth
-  TreePages pages(geo, seq, h, unit_at(place));
+  const int steps = (pt.places + TW - 1) / TW;
+
+  // --- units from memory (pages.unit is the one that a load takes)
+  TreePages pages(geo, seq, h, pt.unit(tw));
+  R rk[F], rv[F];
+  [[maybe_unused]] u32x4 re;
+  const uint32_t lane16 = (uint32_t)lane * 16;
+  const uint32_t ent_at = 16u * (uint32_t)(((lane >> 3) & 3) * (geo.tb >> 2) + (lane & 7));
+  auto load = [&](int next) __attribute__((always_inline)) {  // next: the place that the load after this one takes
+    const int sub = pages.unit & pages.sh;
+    const uint8_t *slab = pages.slab(geo), *ks = slab + geo.k_off, *vs = slab + geo.v_off;
+    pages.ask(pt.unit(next));
+#pragma unroll
+    for (int x = 0; x < F; ++x) {
+      const int f = cw + CW * x;
+      if constexpr (KB == 0) {
+        rk[x] = *(const R*)(ks + (8 * sub + f) * 1024 + lane16);
+        rv[x] = *(const R*)(vs + ((f << pages.sh) + sub) * 1024 + lane16);
+      } else if constexpr (KB == 4) {
+        rk[x] = *(const R*)(ks + (2 * sub + (f >> 2)) * 1024 + 4 * (f & 3) + lane16);
+        rv[x] = *(const R*)(vs + (((f >> 2) << pages.sh) + sub) * 1024 + 4 * (f & 3) + lane16);
+      } else {
+        rk[x] = *(const R*)(ks + (4 * sub + (f >> 1)) * 1024 + 8 * (f & 1) + lane16);
+        rv[x] = *(const R*)(vs + (((f >> 1) << pages.sh) + sub) * 1024 + 8 * (f & 1) + lane16);
+      }
+    }
+    if constexpr (KB != 0) re = *(const u32x4*)(slab + geo.sb_off + sub * 128 + ent_at);
+  };
+  load(TW + tw);
+
+  if (threadIdx.x < 8 * TW) s_odd[threadIdx.x >> 3][threadIdx.x & 7] = make_uint2(0u, 0u);
+  tree_nodes(tb, r, start, s_seen, s_from);
   // scores are products times |scale|, of queries with its sign: the largest is
-  // found on the products
-  const float sc = fmaxf(fabsf(tb.sl2), 1e-30f);  // (-inf, of what is not seen, times it is -inf)
+  // found on the products.  (-inf, of what is not seen, times it is -inf)
+  const float sc = fmaxf(fabsf(tb.sl2), 1e-30f);
   const uint32_t qflip = tb.sl2 < 0.f ? 0x80008000u : 0u;
   u32x4 qf[CT][4];
   [[maybe_unused]] float q0[CT], q1[CT], q0c[CT], q1c[CT];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
-    const int col = min(col0 + 16 * ct + n, cols - 1), node = col / G;
-    const uint16_t* src = q + (int64_t)(start + node) * tb.qr + (int64_t)(h * G + col - node * G) * tb.qh + 8 * g;
+    const int col = min(col0 + 16 * ct + n, cols - 1), node = col >> r.lg;
+    const uint16_t* src = q + (int64_t)(start + node) * tb.qr + (int64_t)((h << r.lg) + col - (node << r.lg)) * tb.qh + 8 * g;
 #pragma unroll
     for (int s = 0; s < 4; ++s) qf[ct][s] = *(const u32x4*)(src + 32 * s) ^ qflip;
     if constexpr (KB != 0) {
@@ -328,21 +380,80 @@ __global__ __launch_bounds__(256, 2) void k_tree(Geometry geo, TreeBatch tb, con
     }
   }
   [[maybe_unused]] const uint32_t code_base = KB ? f16_pair_1024() : 0u;
-  const uint32_t lane16 = (uint32_t)lane * 16;
-  const uint32_t sb_at = 16u * (uint32_t)(((lane >> 3) & 3) * (geo.tb >> 2) + (lane & 7));
-  u32x4 kf[NK], vf[NV];
-  [[maybe_unused]] u32x4 sbx;
-  auto load_k = [&](const uint8_t* slab, int u) __attribute__((always_inline)) {
-    const uint8_t* p = slab + geo.k_off + (u & pages.sh) * (NK * 1024);
+
+  // --- and into LDS, as 16-bit operands
+  auto stage = [&](int place, int slot) __attribute__((always_inline)) {
+    u32x4* to = s_mem + (slot * TW + tw) * 16 * 64 + lane;
 #pragma unroll
-    for (int x = 0; x < NK; ++x) kf[x] = *(const u32x4*)(p + x * 1024 + lane16);
-    if constexpr (KB != 0) sbx = *(const u32x4*)(slab + geo.sb_off + (u & pages.sh) * 128 + sb_at);
-  };
-  auto load_v = [&](const uint8_t* slab, int u) __attribute__((always_inline)) {
-    const uint8_t* p = slab + geo.v_off + (u & pages.sh) * 1024;
+    for (int x = 0; x < F; ++x) {
+      const int f = cw + CW * x;
+      if constexpr (KB == 0) {
+        to[f * 64] = rk[x];
+        to[(8 + f) * 64] = rv[x];
+      } else if constexpr (KB == 4) {
+        to[f * 64] = nib_to_f16_dec(rk[x], code_base);
+        to[(8 + f) * 64] = nib_to_bf16(rv[x]);
+      } else {
+        to[f * 64] = byte_to_f16(rk[x].x, rk[x].y);
+        to[(8 + f) * 64] = byte_to_bf16(rv[x].x, rv[x].y);
+      }
+    }
+    if (place >= pt.full) {
+      // Some columns do not see all of the unit.  Values of tokens that none sees
+      // (old pages hold anything) are taken as zeros; so are infinities and NaN,
+      // which a weight of zero does not take out of a product: they are noted, and
+      // reach the columns that see them at the end.  Of affine caches these are
+      // tokens with such scales or biases, for their 64 dims.
+      const int unit = pt.unit(place);
+      uint32_t odd = 0;
+      if constexpr (KB == 0) {
+        const int t0 = 32 * unit + 8 * g;
+        constexpr uint32_t INF = DT == 0 ? 0x7C00u : 0x7F80u;
+        u32x4 any = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll 1
+        for (int f = 8 + cw; f < 16; f += CW) {
+          u32x4 v = to[f * 64];
 #pragma unroll
-    for (int x = 0; x < NV; ++x) vf[x] = *(const u32x4*)(p + (x << pages.sh) * 1024 + lane16);
+          for (int j = 0; j < 4; ++j) {
+            const int a = t0 + 2 * j;
+            const uint32_t w = v[j] & ((a >= r.lo && a < r.T ? 0x0000FFFFu : 0u) | (a + 1 >= r.lo && a + 1 < r.T ? 0xFFFF0000u : 0u));
+            const uint32_t bad = ((w & INF) == INF ? 0xFFFFu : 0u) | ((w >> 16 & INF) == INF ? 0xFFFF0000u : 0u);
+            any[j] |= bad;
+            v[j] = w & ~bad;
+          }
+          to[f * 64] = v;
+        }
+        if (__any((any[0] | any[1] | any[2] | any[3]) != 0))
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint64_t who = __ballot((any[e >> 1] >> (16 * (e & 1)) & 1) != 0);
+#pragma unroll
+            for (int gg = 0; gg < 4; ++gg)
+              if (who >> (16 * gg) & 0xFFFF) odd |= 1u << (8 * gg + e);
+          }
+      } else {
+        auto inf = [](uint32_t w) {
+          return ((w & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u) | ((w >> 16 & 0x7C00u) == 0x7C00u ? 0xFFFF0000u : 0u);
+        };
+        const uint32_t bad = inf(re[2]) | inf(re[3]);
+        odd = (uint32_t)__ballot(bad != 0 && lane < 32);
+        re[2] &= ~bad;
+        re[3] &= ~bad;
+      }
+      if (odd && lane == 0) {
+        uint2* at = &s_odd[tw][(place - pt.full) / TW];
+        at->x = unit;
+        atomicOr(&at->y, odd);
+      }
+    }
+    if constexpr (KB != 0)
+      if (cw == 0) s_ent[slot * TW + tw][lane & 31] = re;
   };
+  auto sync = [&]() __attribute__((always_inline)) {
+    if constexpr (CW == 1) wave_lds_order();
+    else lds_barrier();
+  };
+
   f32x4 o[CT][8];
   float m[CT], base[CT], limit[CT], l[CT];  // limit: the product past which the reference is raised
   [[maybe_unused]] float ob0[CT], ob1[CT];
@@ -354,120 +465,54 @@ __global__ __launch_bounds__(256, 2) void k_tree(Geometry geo, TreeBatch tb, con
     base[ct] = l[ct] = 0.f;
     if constexpr (KB != 0) ob0[ct] = ob1[ct] = 0.f;
   }
-  __syncthreads();
 
-  // One unit.  (The next one's K is asked for as soon as this one's is used, its
-  // V likewise; a wave's last step asks for its own unit again: behind a branch
-  // the compiler must wait as if nothing had been asked for, and a second copy of
-  // the step spills.)
-  auto step = [&]() __attribute__((always_inline)) {
-    const int next = pages.unit;
-    const uint8_t* slab = pages.slab(geo);
-    pages.ask(unit_at(place + 8));
-    __builtin_amdgcn_sched_barrier(0);
+  auto compute = [&](int place, int slot) __attribute__((always_inline)) {
+    const u32x4* in = s_mem + (slot * TW + tw) * 16 * 64 + lane;
+    [[maybe_unused]] const uint2* ent = (const uint2*)s_ent[KB ? slot * TW + tw : 0];
     // S^T: entry e is token 8 g + e of the unit.  Affine caches: the codes' products
     // of each 64 dims, then with the token's scales and biases
     float sv[CT][8];
-    if constexpr (KB == 0) {
-      f32x4 acc[CT][2];
+    f32x4 acc[CT][KB ? 4 : 2];
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) acc[ct][0] = acc[ct][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct) acc[ct][t] = mfma16x16x32<DT>(kf[4 * t + s], qf[ct][s], acc[ct][t]);
-      __builtin_amdgcn_sched_barrier(0);
-      load_k(slab, next);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sv[ct][e] = acc[ct][e >> 2][e & 3];
-    } else {
-      constexpr int KQ = KB ? KB : 4;
-      f32x4 acc[CT][4];
-      s_sb[wave][lane & 31] = make_uint2(sbx[0], sbx[1]);
-      s_sv[wave][lane & 31] = make_uint2(sbx[2], sbx[3]);
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        acc[ct][0] = acc[ct][1] = f32x4{q0c[ct], q0c[ct], q0c[ct], q0c[ct]};
-        acc[ct][2] = acc[ct][3] = f32x4{q1c[ct], q1c[ct], q1c[ct], q1c[ct]};
+      for (int x = 0; x < (KB ? 4 : 2); ++x) {
+        float c = 0.f;
+        if constexpr (KB != 0) c = x < 2 ? q0c[ct] : q1c[ct];
+        acc[ct][x] = f32x4{c, c, c, c};
       }
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
+    for (int s = 0; s < 4; ++s)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const u32x4 a = k_operand<KQ>(kf + t * QCode<KQ>::KF, s, code_base);
+      for (int t = 0; t < 2; ++t) {
+        const u32x4 a = in[(4 * t + s) * 64];
+        const int x = (KB ? 2 * (s >> 1) : 0) + t;
 #pragma unroll
-          for (int ct = 0; ct < CT; ++ct) acc[ct][2 * (s >> 1) + t] = mfma_f16(a, qf[ct][s], acc[ct][2 * (s >> 1) + t]);
-        }
-      wave_lds_order();
-      __builtin_amdgcn_sched_barrier(0);
-      load_k(slab, next);
-      __builtin_amdgcn_sched_barrier(0);
+        for (int ct = 0; ct < CT; ++ct) acc[ct][x] = mfma16x16x32<DT>(a, qf[ct][s], acc[ct][x]);
+      }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint2 sb = s_sb[wave][8 * g + e];
+    for (int e = 0; e < 8; ++e) {
+      uint2 sb = make_uint2(0u, 0u);
+      if constexpr (KB != 0) sb = ent[2 * (8 * g + e)];
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          float x = lo_f(sb.x) * acc[ct][e >> 2][e & 3];
+      for (int ct = 0; ct < CT; ++ct) {
+        sv[ct][e] = acc[ct][e >> 2][e & 3];
+        if constexpr (KB != 0) {
+          float x = lo_f(sb.x) * sv[ct][e];
           x = __builtin_fmaf(hi_f(sb.x), acc[ct][2 + (e >> 2)][e & 3], x);
           x = __builtin_fmaf(lo_f(sb.y), q0[ct], x);
           sv[ct][e] = __builtin_fmaf(hi_f(sb.y), q1[ct], x);
         }
       }
     }
-    if (place >= full) {
-      // Some columns do not see all of the unit.  Values of tokens that none sees
-      // (old pages hold anything) are taken as zeros; so are infinities and NaN,
-      // which a weight of zero does not take out of a product: they are noted, and
-      // reach the columns that see them at the end.  Of affine caches these are
-      // tokens with such scales or biases, for their 64 dims.
-      const int unit = unit_at(place), t0 = 32 * unit + 8 * g;
-      uint32_t odd = 0;  // tokens with such values
+    if (place >= pt.full) {
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
-        const uint32_t mask = seen_tokens(s_seen, s_from, min(col0 + 16 * ct + n, cols - 1) / G, r.P, t0);
+        const uint32_t mask =
+            seen_tokens(s_seen, s_from, min(col0 + 16 * ct + n, cols - 1) >> r.lg, r.P, 32 * pt.unit(place) + 8 * g);
 #pragma unroll
         for (int e = 0; e < 8; ++e) sv[ct][e] = mask >> e & 1 ? sv[ct][e] : -INFINITY;
       }
-      if constexpr (KB == 0) {
-        uint32_t any = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const bool a = t0 + 2 * j >= r.lo && t0 + 2 * j < r.T, b = t0 + 2 * j + 1 >= r.lo && t0 + 2 * j + 1 < r.T;
-          const uint32_t keep = (a ? 0x0000FFFFu : 0u) | (b ? 0xFFFF0000u : 0u);
-          constexpr uint32_t INF = DT == 0 ? 0x7C00u : 0x7F80u;
-          uint32_t got = 0;
-#pragma unroll
-          for (int dt = 0; dt < 8; ++dt) {
-            const uint32_t w = vf[dt][j] & keep;
-            const uint32_t x = (w & INF) == INF ? 0xFFFFu : 0u, y = (w >> 16 & INF) == INF ? 0xFFFF0000u : 0u;
-            got |= x | y;
-            vf[dt][j] = w & ~(x | y);
-          }
-          any |= (got & 0xFFFFu ? 1u << (2 * j) : 0u) | (got >> 16 ? 2u << (2 * j) : 0u);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint64_t who = __ballot(any >> e & 1);
-#pragma unroll
-          for (int gg = 0; gg < 4; ++gg)
-            if (who >> (16 * gg) & 0xFFFF) odd |= 1u << (8 * gg + e);
-        }
-      } else {
-        const uint2 f = s_sv[wave][lane & 31];
-        auto inf = [](uint32_t w) {
-          return ((w & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u) | ((w >> 16 & 0x7C00u) == 0x7C00u ? 0xFFFF0000u : 0u);
-        };
-        const uint32_t bad = inf(f.x) | inf(f.y);
-        odd = (uint32_t)__ballot(bad != 0 && lane < 32);
-        s_sv[wave][lane & 31] = make_uint2(f.x & ~bad, f.y & ~bad);
-        wave_lds_order();
-      }
-      if (odd && lane == 0) s_odd[wave][(place - full) >> 2] = make_uint2(unit, odd);
     }
     // the largest scores, and one branch for all columns' references
     float mx[CT];
@@ -496,450 +541,70 @@ __global__ __launch_bounds__(256, 2) void k_tree(Geometry geo, TreeBatch tb, con
         for (int dt = 0; dt < 8; ++dt) o[ct][dt] *= f;
       }
     }
-    [[maybe_unused]] u32x4 vc[KB ? 8 : 1];
-    if constexpr (KB != 0) {
+    // the weights, as operands' two parts; affine caches: times the value scales,
+    // o_d = sum_t (p_t vs_j) c_td + sum_t p_t vb_j for group j of 64 dims
+    u32x4 hi[CT][KB ? 2 : 1], lo[CT][KB ? 2 : 1];
+    [[maybe_unused]] float w0[CT][KB ? 8 : 1], w1[CT][KB ? 8 : 1];
 #pragma unroll
-      for (int dt = 0; dt < 8; ++dt) vc[dt] = codes_bf16<KB ? KB : 4>(vf, dt);
-      __builtin_amdgcn_sched_barrier(0);
-      load_v(slab, next);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      float (&pv)[8] = sv[ct];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        pv[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(pv[e], sc, -base[ct]));
-        l[ct] += pv[e];
-      }
-      if constexpr (KB == 0) {
-        u32x4 hi, lo;
-        tree_split<PT>(pv, hi, lo);
-#pragma unroll
-        for (int dt = 0; dt < 8; ++dt) o[ct][dt] = mfma16x16x32<DT>(vf[dt], hi, o[ct][dt]);
-#pragma unroll
-        for (int dt = 0; dt < 8; ++dt) o[ct][dt] = mfma16x16x32<DT>(vf[dt], lo, o[ct][dt]);
-      } else {
-        // o_d = sum_t (p_t vs_j) c_td + sum_t p_t vb_j for group j of 64 dims
-        float w0[8], w1[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint2 sb = s_sv[wave][8 * g + e];
-          w0[e] = pv[e] * lo_f(sb.x);
-          w1[e] = pv[e] * hi_f(sb.x);
-          ob0[ct] = __builtin_fmaf(pv[e], lo_f(sb.y), ob0[ct]);
-          ob1[ct] = __builtin_fmaf(pv[e], hi_f(sb.y), ob1[ct]);
-        }
-        u32x4 h0, l0, h1, l1;
-        tree_split<1>(w0, h0, l0);
-        tree_split<1>(w1, h1, l1);
-#pragma unroll
-        for (int dt = 0; dt < 8; ++dt) o[ct][dt] = mfma16x16x32<1>(vc[dt], dt < 4 ? h0 : h1, o[ct][dt]);
-#pragma unroll
-        for (int dt = 0; dt < 8; ++dt) o[ct][dt] = mfma16x16x32<1>(vc[dt], dt < 4 ? l0 : l1, o[ct][dt]);
-      }
-    }
-    if constexpr (KB == 0) {
-      __builtin_amdgcn_sched_barrier(0);
-      load_v(slab, next);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  };
-  {
-    const int u = pages.unit;
-    const uint8_t* slab = pages.slab(geo);
-    pages.ask(unit_at(place + 4));
-    load_k(slab, u);
-    load_v(slab, u);
-  }
-#pragma unroll 1
-  for (; place < places; place += 4) step();
-  tree_odd<DT, KB, CT>(geo, r, seq, h, &s_odd[wave][0], 2, s_seen, s_from, col0, cols, o);
-
-  // the four waves' shares joined, a column tile at a time
-#pragma unroll 1
-  for (int ct = 0; ct < CT; ++ct) {
-    f32x4 oc[8];
-    float lc = 0.f, mc = 0.f;
-#pragma unroll
-    for (int x = 0; x < CT; ++x)
-      if (x == ct) {
-#pragma unroll
-        for (int dt = 0; dt < 8; ++dt) {
-          oc[dt] = o[x][dt];
-          if constexpr (KB != 0) {
-            const float b = sum_over_groups(dt < 4 ? ob0[x] : ob1[x]);
-#pragma unroll
-            for (int y = 0; y < 4; ++y) oc[dt][y] += b;
-          }
-        }
-        lc = sum_over_groups(l[x]);
-        mc = m[x] == -INFINITY ? m[x] : base[x];
-      }
-    const int first = col0 + 16 * ct;
-    if (first >= cols) break;
-    __syncthreads();
-    if (g == 0) {
-      s_m[wave][n] = mc;
-      s_l[wave][n] = lc;
-    }
-#pragma unroll
-    for (int dt = 0; dt < 8; ++dt) *(f32x4*)&s_o[wave][n][16 * dt + 4 * g] = oc[dt];
-    __syncthreads();
-    tree_write<DT, 4, 16, 256>(geo, tb, r, i, h, part, start, first, min(cols - first, 16), direct, s_m, s_l, s_o, s_seen, out,
-                               partials);
-  }
-}
-
-// ---------------------------------------------------------------------------
-// More than 32 columns: eight waves share what they read through LDS.  CW waves
-// hold 32 columns each and take the same unit, 8 / CW groups of them different
-// ones: a step is 8 / CW units.  In step s a wave writes its share of unit s + 1
-// of its group (16-bit operands, affine codes as fp16 and bf16) to LDS, which it
-// loaded in step s - 1, asks for that of s + 2, and takes unit s from LDS.
-// grid: see tree_place
-// ---------------------------------------------------------------------------
-template <int KB>
-struct Raw {  // a lane's part of a 16-bit operand fragment, as stored
-  typedef uint2 T;
-};
-template <>
-struct Raw<0> {
-  typedef u32x4 T;
-};
-template <>
-struct Raw<4> {
-  typedef uint32_t T;
-};
-
-// a workgroup barrier that orders LDS only: the global loads of later units stay
-// in flight across it
-__device__ __forceinline__ void lds_barrier() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
-
-template <int DT, int KB, int CW>
-__global__ __launch_bounds__(512, 2) void k_tree_wide(Geometry geo, TreeBatch tb, const uint16_t* __restrict__ q,
-                                                      uint16_t* __restrict__ out, float* __restrict__ partials) {
-  static_assert(KB == 0 || DT == 0, "affine caches: fp16");
-  constexpr int TW = 8 / CW, CT = 2, F = 8 / CW;  // F: K, and V, operand fragments of a unit that a wave brings
-  constexpr int PT = KB ? 1 : DT;
-  constexpr float kLift = PT == 0 ? kTreeTop - kTreeSlack : 0.0f;
-  constexpr int COLS = 32 * CW;
-  using R = typename Raw<KB>::T;
-  // two units of each group ([slot][group][8 K, 8 V fragments][lane]), and in the
-  // end the groups' sums
-  constexpr int RING = 2 * TW * 16 * 64, SUMS = TW * COLS * (kHeadDim + 4) / 4;
-  __shared__ u32x4 s_mem[RING > SUMS ? RING : SUMS];
-  __shared__ u32x4 s_ent[KB ? 2 * TW : 1][KB ? 32 : 1];  // (affine) scales and biases
-  __shared__ uint64_t s_seen[kMaxNodes];
-  __shared__ int s_from[kMaxNodes];
-  __shared__ uint2 s_odd[8][8];  // units with values that are infinite or no numbers, and their tokens
-  __shared__ float s_m[TW][COLS], s_l[TW][COLS];
-
-  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int n = lane & 15, g = lane >> 4, G = geo.group;
-  const int cw = wave % CW, tw = wave / CW;
-  const TreePlace at = tree_place(geo, tb);
-  if (at.h < 0) return;
-  const int i = at.i, h = at.h, part = at.part;
-  const TreeRange r = tree_range(geo, tb, i);
-  const int col0 = at.group * COLS + 32 * cw, cols = r.N * G;
-  const int parts = (r.units + r.cu - 1) / r.cu;
-  if (at.group * COLS >= cols || part >= parts) return;
-  const bool direct = tb.part0[i + 1] - tb.part0[i] <= 1;
-  const int start = uniform(tb.starts[i]);
-  const int seq = tb.ids[i];
-  if (lane < 8) s_odd[wave][lane] = make_uint2(0u, 0u);
-  tree_nodes(tb, r, start, s_seen, s_from);
-  const TreePart pt(tb, r, part);
-  const int steps = (pt.places + TW - 1) / TW, whole = pt.full / TW;  // (steps of whole units come first)
-
-  const float sc = fmaxf(fabsf(tb.sl2), 1e-30f);
-  const uint32_t qflip = tb.sl2 < 0.f ? 0x80008000u : 0u;
-  u32x4 qf[CT][4];
-  [[maybe_unused]] float q0[CT], q1[CT], q0c[CT], q1c[CT];
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    const int col = min(col0 + 16 * ct + n, cols - 1), node = col / G;
-    const uint16_t* src = q + (int64_t)(start + node) * tb.qr + (int64_t)(h * G + col - node * G) * tb.qh + 8 * g;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) qf[ct][s] = *(const u32x4*)(src + 32 * s) ^ qflip;
-    if constexpr (KB != 0) {
-      const u32x4 ones = u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
-      const f32x4 zero = f32x4{0.f, 0.f, 0.f, 0.f};
-      q0[ct] = mfma_f16(ones, qf[ct][1], mfma_f16(ones, qf[ct][0], zero))[0];
-      q1[ct] = mfma_f16(ones, qf[ct][3], mfma_f16(ones, qf[ct][2], zero))[0];
-      if constexpr (KB == 4)
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          qf[ct][s][1] = f16x2_unit16(qf[ct][s][1]);
-          qf[ct][s][3] = f16x2_unit16(qf[ct][s][3]);
-        }
-      q0c[ct] = mfma_f16(ones, qf[ct][1], mfma_f16(ones, qf[ct][0], zero))[0] * -kDecOff;
-      q1c[ct] = mfma_f16(ones, qf[ct][3], mfma_f16(ones, qf[ct][2], zero))[0] * -kDecOff;
-    }
-  }
-  [[maybe_unused]] const uint32_t code_base = KB ? f16_pair_1024() : 0u;
-
-  // --- units from memory: operand fragments f = cw + CW x of K (key tile f / 4,
-  // k-step f % 4) and of V (dim tile f)
-  TreePages pages(geo, seq, h, pt.unit(tw));
-  R rk[F], rv[F];
-  [[maybe_unused]] u32x4 re;
-  auto load = [&](int step) __attribute__((always_inline)) {  // (pages.unit is the step's unit)
-    const int sub = pages.unit & pages.sh;
-    const uint8_t *slab = pages.slab(geo), *ks = slab + geo.k_off, *vs = slab + geo.v_off;
-    pages.ask(pt.unit((step + 1) * TW + tw));
-#pragma unroll
-    for (int x = 0; x < F; ++x) {
-      const int f = cw + CW * x;
-      if constexpr (KB == 0) {
-        rk[x] = *(const R*)(ks + (8 * sub + f) * 1024 + lane * 16);
-        rv[x] = *(const R*)(vs + ((f << pages.sh) + sub) * 1024 + lane * 16);
-      } else if constexpr (KB == 4) {
-        rk[x] = *(const R*)(ks + (2 * sub + (f >> 2)) * 1024 + 4 * (f & 3) + lane * 16);
-        rv[x] = *(const R*)(vs + (((f >> 2) << pages.sh) + sub) * 1024 + 4 * (f & 3) + lane * 16);
-      } else {
-        rk[x] = *(const R*)(ks + (4 * sub + (f >> 1)) * 1024 + 8 * (f & 1) + lane * 16);
-        rv[x] = *(const R*)(vs + (((f >> 1) << pages.sh) + sub) * 1024 + 8 * (f & 1) + lane * 16);
-      }
-    }
-    if constexpr (KB != 0)
-      re = *(const u32x4*)(slab + geo.sb_off + sub * 128 + 16 * (((lane >> 3) & 3) * (geo.tb >> 2) + (lane & 7)));
-  };
-  auto stage = [&](int slot) __attribute__((always_inline)) {
-    u32x4* to = s_mem + (slot * TW + tw) * 16 * 64 + lane;
-#pragma unroll
-    for (int x = 0; x < F; ++x) {
-      const int f = cw + CW * x;
-      if constexpr (KB == 0) {
-        to[f * 64] = rk[x];
-        to[(8 + f) * 64] = rv[x];
-      } else if constexpr (KB == 4) {
-        to[f * 64] = nib_to_f16_dec(rk[x], code_base);
-        to[(8 + f) * 64] = nib_to_bf16(rv[x]);
-      } else {
-        to[f * 64] = byte_to_f16(rk[x].x, rk[x].y);
-        to[(8 + f) * 64] = byte_to_bf16(rv[x].x, rv[x].y);
-      }
-    }
-    if constexpr (KB != 0)
-      if (cw == 0) s_ent[slot * TW + tw][lane & 31] = re;
-  };
-
-  f32x4 o[CT][8];
-  float m[CT], base[CT], limit[CT], l[CT];
-  [[maybe_unused]] float ob0[CT], ob1[CT];
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-#pragma unroll
-    for (int dt = 0; dt < 8; ++dt) o[ct][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    m[ct] = limit[ct] = -INFINITY;
-    base[ct] = l[ct] = 0.f;
-    if constexpr (KB != 0) ob0[ct] = ob1[ct] = 0.f;
-  }
-
-  auto compute = [&](int step, int slot, auto edge) __attribute__((always_inline)) {
-    constexpr bool EDGE = decltype(edge)::value;
-    const u32x4* in = s_mem + (slot * TW + tw) * 16 * 64 + lane;
-    float sv[CT][8];
-    if constexpr (KB == 0) {
-      f32x4 acc[CT][2];
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) acc[ct][0] = acc[ct][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const u32x4 a = in[(4 * t + s) * 64];
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct) acc[ct][t] = mfma16x16x32<DT>(a, qf[ct][s], acc[ct][t]);
-        }
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sv[ct][e] = acc[ct][e >> 2][e & 3];
-    } else {
-      f32x4 acc[CT][4];
+    for (int e = 0; e < 8; ++e) {
+      uint2 sb = make_uint2(0u, 0u);
+      if constexpr (KB != 0) sb = ent[2 * (8 * g + e) + 1];
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
-        acc[ct][0] = acc[ct][1] = f32x4{q0c[ct], q0c[ct], q0c[ct], q0c[ct]};
-        acc[ct][2] = acc[ct][3] = f32x4{q1c[ct], q1c[ct], q1c[ct], q1c[ct]};
-      }
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const u32x4 a = in[(4 * t + s) * 64];
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct) acc[ct][2 * (s >> 1) + t] = mfma_f16(a, qf[ct][s], acc[ct][2 * (s >> 1) + t]);
-        }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint2 sb = *(const uint2*)&s_ent[slot * TW + tw][8 * g + e];
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          float x = lo_f(sb.x) * acc[ct][e >> 2][e & 3];
-          x = __builtin_fmaf(hi_f(sb.x), acc[ct][2 + (e >> 2)][e & 3], x);
-          x = __builtin_fmaf(lo_f(sb.y), q0[ct], x);
-          sv[ct][e] = __builtin_fmaf(hi_f(sb.y), q1[ct], x);
-        }
-      }
-    }
-    [[maybe_unused]] const int unit = pt.unit(step * TW + tw), t0 = 32 * unit + 8 * g;
-    if constexpr (EDGE) {
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        const uint32_t mask = seen_tokens(s_seen, s_from, min(col0 + 16 * ct + n, cols - 1) / G, r.P, t0);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sv[ct][e] = mask >> e & 1 ? sv[ct][e] : -INFINITY;
-      }
-    }
-    float mx[CT];
-    bool raise = false;
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      mx[ct] = sv[ct][0];
-#pragma unroll
-      for (int e = 1; e < 8; ++e) mx[ct] = fmaxf(mx[ct], sv[ct][e]);
-      raise = raise || mx[ct] > limit[ct];
-    }
-    if (__any(raise)) {
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        const float top = fmaxf(m[ct], max_over_groups(mx[ct]) * sc);
-        const float f = top == m[ct] ? 1.0f : __builtin_amdgcn_exp2f(m[ct] - top);
-        m[ct] = top;
-        base[ct] = (top == -INFINITY ? 0.0f : top) - kLift;
-        limit[ct] = (top + kTreeSlack) / sc;
-        l[ct] *= f;
-        if constexpr (KB != 0) {
-          ob0[ct] *= f;
-          ob1[ct] *= f;
-        }
-#pragma unroll
-        for (int dt = 0; dt < 8; ++dt) o[ct][dt] *= f;
-      }
-    }
-    // weights, as operands' two parts
-    [[maybe_unused]] uint32_t odd = 0;
-    if constexpr (KB == 0) {
-      u32x4 hi[CT], lo[CT];
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          sv[ct][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[ct][e], sc, -base[ct]));
-          l[ct] += sv[ct][e];
-        }
-        tree_split<PT>(sv[ct], hi[ct], lo[ct]);
-      }
-      uint32_t any = 0;
-#pragma unroll
-      for (int dt = 0; dt < 8; ++dt) {
-        u32x4 v = in[(8 + dt) * 64];
-        if constexpr (EDGE) {
-          // values of tokens that no node sees (old pages hold anything) are taken
-          // as zeros; so are infinities and NaN, which are noted
-          constexpr uint32_t INF = DT == 0 ? 0x7C00u : 0x7F80u;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int a = t0 + 2 * j;
-            const uint32_t keep = (a >= r.lo && a < r.T ? 0x0000FFFFu : 0u) | (a + 1 >= r.lo && a + 1 < r.T ? 0xFFFF0000u : 0u);
-            const uint32_t w = v[j] & keep;
-            const uint32_t x = (w & INF) == INF ? 0xFFFFu : 0u, y = (w >> 16 & INF) == INF ? 0xFFFF0000u : 0u;
-            any |= (x ? 1u << (2 * j) : 0u) | (y ? 2u << (2 * j) : 0u);
-            v[j] = w & ~(x | y);
-          }
-        }
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) o[ct][dt] = mfma16x16x32<DT>(v, hi[ct], o[ct][dt]);
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) o[ct][dt] = mfma16x16x32<DT>(v, lo[ct], o[ct][dt]);
-      }
-      if constexpr (EDGE) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint64_t who = __ballot(any >> e & 1);
-#pragma unroll
-          for (int gg = 0; gg < 4; ++gg)
-            if (who >> (16 * gg) & 0xFFFF) odd |= 1u << (8 * gg + e);
-        }
-      }
-    } else {
-      // o_d = sum_t (p_t vs_j) c_td + sum_t p_t vb_j for group j of 64 dims
-      u32x4 hi[CT][2], lo[CT][2];
-      float w0[CT][8], w1[CT][8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        uint2 sb = *((const uint2*)&s_ent[slot * TW + tw][8 * g + e] + 1);
-        if constexpr (EDGE) {  // (as above; of a token with such a scale or bias, its 64 dims)
-          auto inf = [](uint32_t w) {
-            return ((w & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u) | ((w >> 16 & 0x7C00u) == 0x7C00u ? 0xFFFF0000u : 0u);
-          };
-          const uint32_t bad = inf(sb.x) | inf(sb.y);
-          const uint64_t who = __ballot(bad != 0);
-#pragma unroll
-          for (int gg = 0; gg < 4; ++gg)
-            if (who >> (16 * gg) & 0xFFFF) odd |= 1u << (8 * gg + e);
-          sb = make_uint2(sb.x & ~bad, sb.y & ~bad);
-        }
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[ct][e], sc, -base[ct]));
-          l[ct] += p;
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[ct][e], sc, -base[ct]));
+        l[ct] += p;
+        if constexpr (KB == 0) {
+          sv[ct][e] = p;
+        } else {
           w0[ct][e] = p * lo_f(sb.x);
           w1[ct][e] = p * hi_f(sb.x);
           ob0[ct] = __builtin_fmaf(p, lo_f(sb.y), ob0[ct]);
           ob1[ct] = __builtin_fmaf(p, hi_f(sb.y), ob1[ct]);
         }
       }
+    }
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
+    for (int ct = 0; ct < CT; ++ct) {
+      if constexpr (KB == 0) {
+        tree_split<PT>(sv[ct], hi[ct][0], lo[ct][0]);
+      } else {
         tree_split<1>(w0[ct], hi[ct][0], lo[ct][0]);
         tree_split<1>(w1[ct], hi[ct][1], lo[ct][1]);
       }
-#pragma unroll
-      for (int dt = 0; dt < 8; ++dt) {
-        const u32x4 v = in[(8 + dt) * 64];
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) o[ct][dt] = mfma16x16x32<1>(v, hi[ct][dt >> 2], o[ct][dt]);
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) o[ct][dt] = mfma16x16x32<1>(v, lo[ct][dt >> 2], o[ct][dt]);
-      }
     }
-    if constexpr (EDGE)
-      if (odd && lane == 0) s_odd[wave][step - whole] = make_uint2(unit, odd);
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) {
+      const u32x4 v = in[(8 + dt) * 64];
+      constexpr int HALF = KB ? 4 : 8;
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) o[ct][dt] = mfma16x16x32<PT>(v, hi[ct][dt / HALF], o[ct][dt]);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) o[ct][dt] = mfma16x16x32<PT>(v, lo[ct][dt / HALF], o[ct][dt]);
+    }
   };
 
-  load(0);
-  stage(0);
-  load(1);
-  lds_barrier();
+  __syncthreads();
+  stage(tw, 0);
+  load(2 * TW + tw);
+  sync();
 #pragma unroll 1
-  for (int s = 0; s < whole; ++s) {
-    stage((s + 1) & 1);
-    load(s + 2);
-    compute(s, s & 1, std::false_type());
-    lds_barrier();
+  for (int s = 0; s < steps; ++s) {
+    const int place = s * TW + tw, slot = SLOTS == 1 ? 0 : s & 1;
+    if (place < pt.places) compute(place, slot);
+    if (s + 1 == steps) break;
+    if constexpr (SLOTS == 1) sync();
+    stage(place + TW, SLOTS == 1 ? 0 : slot ^ 1);
+    load(place + 3 * TW);
+    sync();
   }
-#pragma unroll 1
-  for (int s = whole; s < steps; ++s) {
-    stage((s + 1) & 1);
-    load(s + 2);
-    if (s * TW + tw < pt.places) compute(s, s & 1, std::true_type());
-    lds_barrier();
-  }
-  tree_odd<DT, KB, CT>(geo, r, seq, h, &s_odd[wave][0], 8, s_seen, s_from, col0, cols, o);
+  __syncthreads();
+  tree_odd<DT, KB, CT>(geo, r, seq, h, s_odd[tw], s_seen, s_from, col0, cols, o);
 
-  // the groups' shares joined
+  // the teams' shares joined
   float (*s_o)[COLS][kHeadDim + 4] = (float (*)[COLS][kHeadDim + 4])s_mem;
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
-    const int c = 32 * cw + 16 * ct + n;
+    const int c = 16 * (CT * cw + ct) + n;
     const float lc = sum_over_groups(l[ct]);
     if (g == 0) {
       s_m[tw][c] = m[ct] == -INFINITY ? m[ct] : base[ct];
@@ -958,8 +623,8 @@ __global__ __launch_bounds__(512, 2) void k_tree_wide(Geometry geo, TreeBatch tb
     }
   }
   __syncthreads();
-  tree_write<DT, TW, COLS, 512>(geo, tb, r, i, h, part, start, at.group * COLS, min(cols - at.group * COLS, COLS), direct,
-                                s_m, s_l, s_o, s_seen, out, partials);
+  tree_write<DT, TW, COLS, 64 * W>(geo, tb, r, i, h, part, start, first, min(cols - first, COLS), direct, s_m, s_l, s_o, s_seen,
+                                   out, partials);
 }
 
 // The parts of one (node, query head) joined, eight rows of 32 lanes with four
@@ -1019,11 +684,11 @@ static void tree_dispatch(const Geometry& g, const TreeBatch& tb, const uint16_t
   const int64_t pairs = ((int64_t)tb.part0[tb.n] * g.hkv + 7) & ~7ll;
   const dim3 grid((unsigned)(pairs * tb.groups));
   auto go = [&](auto kernel, int threads) { launch(kernel, grid, dim3(threads), 0, s, prof, kProfTree, g, tb, q, out, ws); };
-  if (tb.tiles == 1) go(k_tree<DT, KB, 1>, 256);
-  else if (tb.tiles == 2) go(k_tree<DT, KB, 2>, 256);
-  else if (tb.tiles == 4) go(k_tree_wide<DT, KB, 2>, 512);
-  else if (tb.tiles == 8) go(k_tree_wide<DT, KB, 4>, 512);
-  else go(k_tree_wide<DT, KB, 8>, 512);
+  if (tb.tiles == 1) go(k_tree<DT, KB, 1, 1>, 256);
+  else if (tb.tiles == 2) go(k_tree<DT, KB, 2, 1>, 256);
+  else if (tb.tiles == 4) go(k_tree<DT, KB, 2, 2>, 512);
+  else if (tb.tiles == 8) go(k_tree<DT, KB, 2, 4>, 512);
+  else go(k_tree<DT, KB, 2, 8>, 512);
 }
 
 static_assert(sizeof(Geometry) + sizeof(TreeBatch) <= 4000, "a launch's arguments stay under 4 KiB");
