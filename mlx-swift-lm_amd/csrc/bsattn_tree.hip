@@ -32,14 +32,16 @@ constexpr float kTreeSlack = 6.0f;
 constexpr float kTreeTop = 14.0f;
 
 // What a request brings to a launch, and the units of its part
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
 struct TreeRange {
   int T, N, P, lo, u0, units, cu;
   int lg;  // log2 of the heads of a group
 };
 __device__ __forceinline__ TreeRange tree_range(const Geometry& geo, const TreeBatch& tb, int i) {
   TreeRange r;
-  r.T = uniform(geo.meta[tb.ids[i]]);
-  r.N = min(min(uniform(tb.taken[i]), tb.max_tokens), r.T);
+  r.T = geo.meta[tb.ids[i]];
+  r.N = min(min(tb.taken[i], tb.max_tokens), r.T);
   r.P = r.T - r.N;
   r.lg = __builtin_ctz((unsigned)geo.group);
   r.lo = tb.window > 0 ? max(0, r.P - tb.window + 1) : 0;  // the first token that a root sees
@@ -74,18 +76,29 @@ struct TreePages {
   }
 };
 
-// weights x[0, 8) as an operand's two parts: hi cut to 16 bits, lo what is left, rounded
+// weights x[0, 8) as an operand's two parts: hi rounded to 16 bits, lo what the
+// rounding left.  one: bf16 -1 in the low half, and in the high half (from
+// minus_one: as constants of the product they come out wrong with this compiler)
+struct MinusOne {
+  uint32_t lo, hi;
+};
+__device__ __forceinline__ MinusOne minus_one() {
+  return MinusOne{(uint32_t)__builtin_amdgcn_mov_dpp(0x0000BF80, 0xE4, 0xF, 0xF, false),
+                  (uint32_t)__builtin_amdgcn_mov_dpp((int)0xBF800000u, 0xE4, 0xF, 0xF, false)};
+}
 template <int DT>
-__device__ __forceinline__ void tree_split(const float* x, u32x4& hi, u32x4& lo) {
+__device__ __forceinline__ void tree_split(const float* x, const MinusOne& one, u32x4& hi, u32x4& lo) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
+    const uint32_t w = cvt_pk<DT>(x[2 * j], x[2 * j + 1]);
+    hi[j] = w;
     if constexpr (DT == 1) {
-      const uint32_t a = __float_as_uint(x[2 * j]), b = __float_as_uint(x[2 * j + 1]);
-      hi[j] = __builtin_amdgcn_perm(b, a, 0x07060302u);
-      lo[j] = cvt_pk<1>(x[2 * j] - __uint_as_float(a & 0xFFFF0000u), x[2 * j + 1] - __uint_as_float(b & 0xFFFF0000u));
+      // (a product with -1 and 0 gives the difference in one instruction, exactly)
+      auto less = [&](uint32_t c, float v) {
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, c), v, false);
+      };
+      lo[j] = cvt_pk<1>(less(one.lo, x[2 * j]), less(one.hi, x[2 * j + 1]));
     } else {
-      const uint32_t w = cvt_pk<0>(x[2 * j], x[2 * j + 1]);
-      hi[j] = w;
       lo[j] = cvt_pk<0>(x[2 * j] - lo_f(w), x[2 * j + 1] - hi_f(w));
     }
   }
@@ -127,23 +140,20 @@ __device__ __forceinline__ uint32_t seen_tokens(const uint64_t* s_seen, const in
   return (cached | tree) & 0xFFu;
 }
 
-// What a workgroup takes of the launch: workgroup x is one column group of one
-// (part, kv head) pair; the groups of a pair lie a multiple of 8 apart, on one
-// XCD, whose L2 then holds the K and V they share.
+// What a workgroup takes of the launch: grid (parts, kv heads, column groups),
+// the parts padded so that the groups of a (part, head) lie a multiple of 8
+// workgroups apart, on one XCD, whose L2 then holds the K and V they share
 struct TreePlace {
-  int i, h, group, part;  // h: -1 where there is nothing
+  int i, h, group, part;  // i: -1 where there is nothing
 };
-__device__ __forceinline__ TreePlace tree_place(const Geometry& geo, const TreeBatch& tb) {
+__device__ __forceinline__ TreePlace tree_place(const TreeBatch& tb) {
   TreePlace p;
-  const int lane = threadIdx.x & 63, total = tb.part0[tb.n];
-  const int chunk = blockIdx.x / (8 * tb.groups), in = blockIdx.x - chunk * 8 * tb.groups;
-  const int pair = 8 * chunk + (in & 7);
-  p.group = in >> 3;
-  p.h = uniform(pair / total);
-  const int at = pair - p.h * total;
-  p.i = uniform(__popcll(__ballot(lane < tb.n && tb.part0[min(lane, tb.n - 1)] <= at)) - 1);
-  p.part = at - tb.part0[p.i];
-  if (p.h >= geo.hkv) p.h = -1;
+  const int lane = threadIdx.x & 63, at = blockIdx.x;
+  p.h = blockIdx.y;
+  p.group = blockIdx.z;
+  const uint64_t held = __ballot(lane < tb.n && tb.part0[min(lane, tb.n - 1)] <= at);
+  p.i = at < tb.part0[tb.n] ? uniform(__popcll(held) - 1) : -1;
+  p.part = at - tb.part0[max(p.i, 0)];
   return p;
 }
 
@@ -220,29 +230,36 @@ __device__ __forceinline__ void tree_odd(const Geometry& geo, const TreeRange& r
 }
 
 // Columns first .. first + count - 1 out of W shares (references s_m, sums s_l,
-// o): the outputs, or the part's partials
+// o), four dims a thread: the outputs, or the part's partials
 template <int DT, int W, int C, int THREADS>
 __device__ __forceinline__ void tree_write(const Geometry& geo, const TreeBatch& tb, const TreeRange& r, int i, int h, int part,
                                            int start, int first, int count, bool direct, const float (&s_m)[W][C],
                                            const float (&s_l)[W][C], const float (*s_o)[C][kHeadDim + 4],
                                            const uint64_t* s_seen, uint16_t* __restrict__ out, float* __restrict__ partials) {
-  for (int e = threadIdx.x; e < count * kHeadDim; e += THREADS) {
-    const int c = e >> 7, d = e & 127, col = first + c;
+  const int d = 4 * (threadIdx.x & 31);
+#pragma unroll 4
+  for (int c0 = 0; c0 < C; c0 += THREADS / 32) {
+    const int c = c0 + (threadIdx.x >> 5);
+    if (C % (THREADS / 32) != 0 && c >= C) break;
+    const int col = min(first + c, first + count - 1), node = col >> r.lg, hq = (h << r.lg) + col - (node << r.lg);
     float M = s_m[0][c];
 #pragma unroll
     for (int v = 1; v < W; ++v) M = fmaxf(M, s_m[v][c]);
-    float L = 0.f, a = 0.f;
+    float L = 0.f;
+    f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int v = 0; v < W; ++v) {
       const float mv = s_m[v][c];
       const float f = mv == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mv - M);
       L += f * s_l[v][c];
-      if (mv != -INFINITY) a += f * s_o[v][c][d];
+      const f32x4 x = *(const f32x4*)&s_o[v][c][d];
+      if (mv != -INFINITY) a += f * x;
     }
-    const int node = col >> r.lg, hq = (h << r.lg) + col - (node << r.lg);
+    if (c >= count) continue;
     if (s_seen[node] == 0) {  // absent: nothing is seen
       M = -INFINITY;
-      L = a = 0.f;
+      L = 0.f;
+      a = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     if (direct) {
       if (tb.sinks && M != -INFINITY) {
@@ -250,14 +267,15 @@ __device__ __forceinline__ void tree_write(const Geometry& geo, const TreeBatch&
         L = L * f + (sk == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sk - top));
         a *= f;
       }
-      out[((int64_t)(start + node) * geo.hq + hq) * kHeadDim + d] = from_f32<DT>(L == 0.f ? 0.f : a / L);
+      a = L == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : a / L;
+      *(uint2*)(out + ((int64_t)(start + node) * geo.hq + hq) * kHeadDim + d) =
+          make_uint2(pack2<DT>(a[0], a[1]), pack2<DT>(a[2], a[3]));
     } else {
       float* pp = partials + ((int64_t)(tb.row0[i] + part * tb.max_tokens + node) * geo.hq + hq) * kPartial;
-      pp[d] = a;
-      if (d == 0) {
-        pp[kHeadDim] = M;
-        pp[kHeadDim + 1] = L;
-      }
+      // (partials are 130 floats apart)
+      *(float2*)(pp + d) = make_float2(a[0], a[1]);
+      *(float2*)(pp + d + 2) = make_float2(a[2], a[3]);
+      if (d == 0) *(float2*)(pp + kHeadDim) = make_float2(M, L);
     }
   }
 }
@@ -291,7 +309,12 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
   static_assert(KB == 0 || DT == 0, "affine caches: fp16");
   constexpr int W = CW == 1 ? 4 : 8, TW = W / CW, SLOTS = CW == 1 ? 1 : 2;
   constexpr int F = 8 / CW;       // K, and V, operand fragments of a unit that a wave brings: cw + CW x
-  constexpr int PT = KB ? 1 : DT; // P's type: weights times scales need bf16's range, and codes are exact in it
+  // P's type.  Weights times scales need bf16's range, and codes are exact in it.
+  // bf16 caches: V is brought as fp16 where that takes it as it is, fragment by
+  // fragment, and P then enters once, rounded to fp16's 11 bits (a sixteenth of the
+  // output's half step): half of PV's products and most of the work on P
+  constexpr bool CONV = KB == 0 && DT == 1 && CW >= 2;
+  constexpr int PT = KB ? 1 : CONV ? 0 : DT;
   // fp16 weights are lifted to at most 2^14, so that small ones keep their bits
   constexpr float kLift = PT == 0 ? kTreeTop - kTreeSlack : 0.0f;
   constexpr int COLS = 16 * CT * CW;
@@ -301,6 +324,7 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
   constexpr int RING = SLOTS * TW * 16 * 64, SUMS = TW * COLS * (kHeadDim + 4) / 4;
   __shared__ u32x4 s_mem[RING > SUMS ? RING : SUMS];
   __shared__ u32x4 s_ent[KB ? SLOTS * TW : 1][KB ? 32 : 1];  // (affine) scales and biases
+  __shared__ uint8_t s_raw[SLOTS * TW][8];  // (CONV) per wave of a team: which dim tiles of V are bf16
   __shared__ uint64_t s_seen[kMaxNodes];
   __shared__ int s_from[kMaxNodes];
   __shared__ uint2 s_odd[TW][8];  // units with values that are infinite or no numbers, and their tokens
@@ -308,13 +332,12 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
 
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int n = lane & 15, g = lane >> 4, cw = wave % CW, tw = wave / CW;
-  const TreePlace at = tree_place(geo, tb);
-  if (at.h < 0) return;
+  const TreePlace at = tree_place(tb);
+  if (at.i < 0) return;
   const int i = at.i, h = at.h, part = at.part;
   const TreeRange r = tree_range(geo, tb, i);
   const int first = at.group * COLS, col0 = first + 16 * CT * cw, cols = r.N << r.lg;
-  const int parts = (r.units + r.cu - 1) / r.cu;
-  if (first >= cols || part >= parts) return;
+  if (first >= cols || part * r.cu >= r.units) return;
   const bool direct = tb.part0[i + 1] - tb.part0[i] <= 1;
   const int start = uniform(tb.starts[i]), seq = tb.ids[i];
   const TreePart pt(tb, r, part);
@@ -389,7 +412,7 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
       const int f = cw + CW * x;
       if constexpr (KB == 0) {
         to[f * 64] = rk[x];
-        to[(8 + f) * 64] = rv[x];
+        if constexpr (!CONV) to[(8 + f) * 64] = rv[x];
       } else if constexpr (KB == 4) {
         to[f * 64] = nib_to_f16_dec(rk[x], code_base);
         to[(8 + f) * 64] = nib_to_bf16(rv[x]);
@@ -397,6 +420,32 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
         to[f * 64] = byte_to_f16(rk[x].x, rk[x].y);
         to[(8 + f) * 64] = byte_to_bf16(rv[x].x, rv[x].y);
       }
+    }
+    if constexpr (CONV) {
+      // fp16 takes a tile whose values are below 65536 with the largest at 2^-8 or
+      // more (values below 2^-14 are off by up to 2^-25 then); units with tokens
+      // that are not seen stay as they are
+      uint32_t raw = 0;
+#pragma unroll
+      for (int x = 0; x < F; ++x) {
+        const int f = cw + CW * x;
+        u16x2 big = {0, 0};
+        u32x4 v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t w = rv[x][j], mag = w & 0x7FFF7FFFu;
+          big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2, mag));
+          v[j] = cvt_pk<0>(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+        }
+        const uint32_t top = max((uint32_t)big[0], (uint32_t)big[1]);
+        const bool ok = place < pt.full && !__any(top >= 0x4780u) && (__any(top >= 0x3B80u) || !__any(top != 0));
+        if (!ok) {
+          raw |= 1u << f;
+          v = rv[x];
+        }
+        to[(8 + f) * 64] = v;
+      }
+      if (lane == 0) s_raw[slot * TW + tw][cw] = (uint8_t)raw;
     }
     if (place >= pt.full) {
       // Some columns do not see all of the unit.  Values of tokens that none sees
@@ -455,16 +504,23 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
   };
 
   f32x4 o[CT][8];
-  float m[CT], base[CT], limit[CT], l[CT];  // limit: the product past which the reference is raised
+  float m[CT], base[CT], limit[CT];  // limit: the product past which the reference is raised
+  // the weights' sums, as they enter the products: of 16-bit caches by a product
+  // with ones (rows alike)
+  f32x4 l[CT];
   [[maybe_unused]] float ob0[CT], ob1[CT];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) o[ct][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     m[ct] = limit[ct] = -INFINITY;
-    base[ct] = l[ct] = 0.f;
+    base[ct] = 0.f;
+    l[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
     if constexpr (KB != 0) ob0[ct] = ob1[ct] = 0.f;
   }
+  const MinusOne one = minus_one();
+  [[maybe_unused]] const uint32_t unit_pair = PT == 0 ? 0x3C003C00u : 0x3F803F80u;
+  [[maybe_unused]] const u32x4 ones = u32x4{unit_pair, unit_pair, unit_pair, unit_pair};
 
   auto compute = [&](int place, int slot) __attribute__((always_inline)) {
     const u32x4* in = s_mem + (slot * TW + tw) * 16 * 64 + lane;
@@ -552,10 +608,10 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
         const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[ct][e], sc, -base[ct]));
-        l[ct] += p;
         if constexpr (KB == 0) {
           sv[ct][e] = p;
         } else {
+          l[ct][0] += p;
           w0[ct][e] = p * lo_f(sb.x);
           w1[ct][e] = p * hi_f(sb.x);
           ob0[ct] = __builtin_fmaf(p, lo_f(sb.y), ob0[ct]);
@@ -565,12 +621,52 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
     }
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      if constexpr (KB == 0) {
-        tree_split<PT>(sv[ct], hi[ct][0], lo[ct][0]);
+      if constexpr (CONV) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) hi[ct][0][j] = cvt_pk<0>(sv[ct][2 * j], sv[ct][2 * j + 1]);
+        l[ct] = mfma16x16x32<0>(ones, hi[ct][0], l[ct]);
+      } else if constexpr (KB == 0) {
+        tree_split<PT>(sv[ct], one, hi[ct][0], lo[ct][0]);
+        l[ct] = mfma16x16x32<PT>(ones, hi[ct][0], l[ct]);
+        l[ct] = mfma16x16x32<PT>(ones, lo[ct][0], l[ct]);
       } else {
-        tree_split<1>(w0[ct], hi[ct][0], lo[ct][0]);
-        tree_split<1>(w1[ct], hi[ct][1], lo[ct][1]);
+        tree_split<1>(w0[ct], one, hi[ct][0], lo[ct][0]);
+        tree_split<1>(w1[ct], one, hi[ct][1], lo[ct][1]);
       }
+    }
+    if constexpr (CONV) {
+      uint32_t raw = 0;
+      const uint2 each = *(const uint2*)s_raw[slot * TW + tw];
+#pragma unroll
+      for (int x = 0; x < CW; ++x) raw |= (x < 4 ? each.x : each.y) >> (8 * (x & 3)) & 0xFFu;
+      raw = (uint32_t)uniform((int)raw);
+      if (raw == 0) {
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) {
+          const u32x4 v = in[(8 + dt) * 64];
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) o[ct][dt] = mfma16x16x32<0>(v, hi[ct][0], o[ct][dt]);
+        }
+      } else {
+        u32x4 bh[CT], bl[CT];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) tree_split<1>(sv[ct], one, bh[ct], bl[ct]);
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) {
+          const u32x4 v = in[(8 + dt) * 64];
+          const bool as_is = raw >> dt & 1;
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) {
+            if (as_is) {
+              o[ct][dt] = mfma16x16x32<1>(v, bh[ct], o[ct][dt]);
+              o[ct][dt] = mfma16x16x32<1>(v, bl[ct], o[ct][dt]);
+            } else {
+              o[ct][dt] = mfma16x16x32<0>(v, hi[ct][0], o[ct][dt]);
+            }
+          }
+        }
+      }
+      return;
     }
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) {
@@ -590,7 +686,7 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
 #pragma unroll 1
   for (int s = 0; s < steps; ++s) {
     const int place = s * TW + tw, slot = SLOTS == 1 ? 0 : s & 1;
-    if (place < pt.places) compute(place, slot);
+    if (place < pt.places && col0 < cols) compute(place, slot);
     if (s + 1 == steps) break;
     if constexpr (SLOTS == 1) sync();
     stage(place + TW, SLOTS == 1 ? 0 : slot ^ 1);
@@ -605,7 +701,7 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     const int c = 16 * (CT * cw + ct) + n;
-    const float lc = sum_over_groups(l[ct]);
+    const float lc = KB ? sum_over_groups(l[ct][0]) : l[ct][0];
     if (g == 0) {
       s_m[tw][c] = m[ct] == -INFINITY ? m[ct] : base[ct];
       s_l[tw][c] = lc;
@@ -627,62 +723,88 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
                                    out, partials);
 }
 
-// The parts of one (node, query head) joined, eight rows of 32 lanes with four
-// dims each taking the parts in turn.  grid (Hq, n * max_tokens)
-constexpr int kTreeRows = 8;
-template <int DT>
-__global__ __launch_bounds__(32 * kTreeRows) void k_tree_join(Geometry geo, TreeBatch tb, const float* __restrict__ ws,
-                                                              uint16_t* __restrict__ out) {
-  __shared__ __align__(16) float s_o[kTreeRows][kHeadDim];
-  __shared__ float s_ml[kTreeRows][2];
-  const int hq = blockIdx.x, i = blockIdx.y / tb.max_tokens, node = blockIdx.y - i * tb.max_tokens;
-  if (tb.part0[i + 1] - tb.part0[i] <= 1) return;  // (the launch before wrote the output)
-  const TreeRange r = tree_range(geo, tb, i);
-  if (node >= r.N) return;
-  const int parts = (r.units + r.cu - 1) / r.cu;
-  const int y = threadIdx.x >> 5, c = threadIdx.x & 31;
+// The parts of each (node, query head) joined: 32 lanes with four dims each take
+// the parts four at a time; ROWS of them share a (node, head) where there are many
+// parts.  grid (Hq, nodes of all requests, 8 / ROWS a workgroup)
+template <int DT, int ROWS>
+__global__ __launch_bounds__(256) void k_tree_join(Geometry geo, TreeBatch tb, const float* __restrict__ ws,
+                                                   uint16_t* __restrict__ out) {
+  __shared__ __align__(16) float s_o[8][kHeadDim];
+  __shared__ float s_ml[8][2];
+  const int slot = threadIdx.x >> 5, c = threadIdx.x & 31, y = slot % ROWS;
+  const int hq = blockIdx.x, which = blockIdx.y * (8 / ROWS) + slot / ROWS;
+  const int i = min(which / tb.max_tokens, tb.n - 1), node = which - i * tb.max_tokens;
+  const TreeRange r = tree_range(geo, tb, ROWS == 8 ? uniform(i) : i);
+  // (requests of one part: the launch before wrote the output)
+  const bool there = which < tb.n * tb.max_tokens && node < r.N && tb.part0[i + 1] - tb.part0[i] > 1;
   float M = -INFINITY, L = 0.f;
   f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int p = y; p < parts; p += kTreeRows) {
-    const float2* part = (const float2*)(ws + ((int64_t)(tb.row0[i] + p * tb.max_tokens + node) * geo.hq + hq) * kPartial);
-    const float2 xa = part[2 * c], xb = part[2 * c + 1], ml = part[kHeadDim / 2];
-    // (without a token that is seen: no reference, and a sum of 0, or NaN)
-    const float top = fmaxf(M, ml.x), f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - top);
-    const float w = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - top);
-    L = L * f + w * ml.y;
+  const int parts = there ? (r.units + r.cu - 1) / r.cu : 0;
+  for (int p0 = y; p0 < parts; p0 += 4 * ROWS) {
+    f32x4 x[4];
+    float m[4], l[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int p = min(p0 + j * ROWS, parts - 1);
+      const float2* part = (const float2*)(ws + ((int64_t)(tb.row0[i] + p * tb.max_tokens + node) * geo.hq + hq) * kPartial);
+      const float2 xa = part[2 * c], xb = part[2 * c + 1], ml = part[kHeadDim / 2];
+      x[j] = f32x4{xa.x, xa.y, xb.x, xb.y};
+      // (without a token that is seen: no reference, and a sum of 0, or NaN)
+      m[j] = p0 + j * ROWS < parts ? ml.x : -INFINITY;
+      l[j] = p0 + j * ROWS < parts ? ml.y : 0.f;
+    }
+    float top = M;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top = fmaxf(top, m[j]);
+    const float f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - top);
+    L *= f;
     a *= f;
-    if (ml.x != -INFINITY) a += w * f32x4{xa.x, xa.y, xb.x, xb.y};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float w = m[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[j] - top);
+      L += w * l[j];
+      if (m[j] != -INFINITY) a += w * x[j];
+    }
     M = top;
   }
-  *(f32x4*)&s_o[y][4 * c] = a;
-  if (c == 0) {
-    s_ml[y][0] = M;
-    s_ml[y][1] = L;
-  }
-  __syncthreads();
-  if (threadIdx.x >= kHeadDim) return;
-  const int d = threadIdx.x;
-  float top = -INFINITY;
+  if constexpr (ROWS > 1) {
+    *(f32x4*)&s_o[slot][4 * c] = a;
+    if (c == 0) {
+      s_ml[slot][0] = M;
+      s_ml[slot][1] = L;
+    }
+    __syncthreads();
+    if (y != 0) return;
+    float top = M;
 #pragma unroll
-  for (int x = 0; x < kTreeRows; ++x) top = fmaxf(top, s_ml[x][0]);
-  const bool none = top == -INFINITY;
-  const float sk = tb.sinks && !none ? tb.sinks[hq] * kTreeLog2e : -INFINITY;
-  top = fmaxf(top, sk);
-  float Ls = sk == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sk - top), as = 0.f;
+    for (int x = 1; x < ROWS; ++x) top = fmaxf(top, s_ml[slot + x][0]);
+    const float f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - top);
+    L *= f;
+    a *= f;
 #pragma unroll
-  for (int x = 0; x < kTreeRows; ++x) {
-    const float mx = s_ml[x][0], f = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - top);
-    Ls += f * s_ml[x][1];
-    if (mx != -INFINITY) as += f * s_o[x][d];
+    for (int x = 1; x < ROWS; ++x) {
+      const float mx = s_ml[slot + x][0], w = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - top);
+      L += w * s_ml[slot + x][1];
+      if (mx != -INFINITY) a += w * *(const f32x4*)&s_o[slot + x][4 * c];
+    }
+    M = top;
   }
-  out[((int64_t)(tb.starts[i] + node) * geo.hq + hq) * kHeadDim + d] = from_f32<DT>(Ls == 0.f ? 0.f : as / Ls);
+  if (!there) return;
+  if (tb.sinks && M != -INFINITY) {
+    const float sk = tb.sinks[hq] * kTreeLog2e, top = fmaxf(M, sk), f = __builtin_amdgcn_exp2f(M - top);
+    L = L * f + (sk == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sk - top));
+    a *= f;
+  }
+  a = L == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : a / L;
+  *(uint2*)(out + ((int64_t)(tb.starts[i] + node) * geo.hq + hq) * kHeadDim + 4 * c) =
+      make_uint2(pack2<DT>(a[0], a[1]), pack2<DT>(a[2], a[3]));
 }
 
 template <int DT, int KB>
 static void tree_dispatch(const Geometry& g, const TreeBatch& tb, const uint16_t* q, uint16_t* out, float* ws,
                           hipStream_t s, Timing* prof) {
-  const int64_t pairs = ((int64_t)tb.part0[tb.n] * g.hkv + 7) & ~7ll;
-  const dim3 grid((unsigned)(pairs * tb.groups));
+  const int parts = tb.groups > 1 ? (tb.part0[tb.n] + 7) & ~7 : tb.part0[tb.n];
+  const dim3 grid(parts, g.hkv, tb.groups);
   auto go = [&](auto kernel, int threads) { launch(kernel, grid, dim3(threads), 0, s, prof, kProfTree, g, tb, q, out, ws); };
   if (tb.tiles == 1) go(k_tree<DT, KB, 1, 1>, 256);
   else if (tb.tiles == 2) go(k_tree<DT, KB, 2, 1>, 256);
@@ -702,7 +824,11 @@ hipError_t launch_tree(const Geometry& g, const TreeBatch& tb, const void* q, vo
   else tree_dispatch<1, 0>(g, tb, qq, oo, ws, s, prof);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !ws) return e;
-  const dim3 grid(g.hq, tb.n * tb.max_tokens), blk(32 * kTreeRows);
+  int most = 1;
+  for (int i = 0; i < tb.n; ++i) most = std::max(most, tb.part0[i + 1] - tb.part0[i]);
+  const bool many = most > 8;
+  const int nodes = tb.n * tb.max_tokens;
+  const dim3 grid(g.hq, many ? nodes : (nodes + 7) / 8), blk(256);
   const float* cws = ws;
   auto join = [&](auto kernel) {
     if (done && !prof)  // (the event is the dispatch's own: no packet of its own behind it)
@@ -710,8 +836,8 @@ hipError_t launch_tree(const Geometry& g, const TreeBatch& tb, const void* q, vo
     else
       launch(kernel, grid, blk, 0, s, prof, kProfCombine, g, tb, cws, oo);
   };
-  if (g.dtype == 0) join(k_tree_join<0>);
-  else join(k_tree_join<1>);
+  if (g.dtype == 0) many ? join(k_tree_join<0, 8>) : join(k_tree_join<0, 1>);
+  else many ? join(k_tree_join<1, 8>) : join(k_tree_join<1, 1>);
   e = hipGetLastError();
   if (e == hipSuccess && done && prof) e = hipEventRecord(done, s);
   return e;
