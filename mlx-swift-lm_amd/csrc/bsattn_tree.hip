@@ -57,21 +57,18 @@ __device__ __forceinline__ TreeRange tree_range(const Geometry& geo, const TreeB
   return r;
 }
 
-// slabs of the units that a wave takes, the block table read through the scalar
-// cache one unit ahead
+// slabs of the units that a wave takes, the block table read through the scalar cache
 struct TreePages {
   const int32_t* bt;
-  int h, sh, unit, page;  // sh: log2 of the units per block; the unit asked for last, and its page
-  __device__ __forceinline__ TreePages(const Geometry& geo, int seq, int h_, int u) : h(h_) {
+  int h, sh;  // sh: log2 of the units per block
+  __device__ __forceinline__ TreePages(const Geometry& geo, int seq, int h_) : h(h_) {
     sh = geo.tb == 64 ? 1 : 0;
     bt = block_table(geo, seq);
-    ask(u);
   }
-  __device__ __forceinline__ void ask(int u) {
-    unit = u;
-    page = *((const __attribute__((address_space(4))) int32_t*)(uintptr_t)(bt + (unit >> sh)));
+  __device__ __forceinline__ int page(int unit) const {
+    return *((const __attribute__((address_space(4))) int32_t*)(uintptr_t)(bt + (unit >> sh)));
   }
-  __device__ __forceinline__ const uint8_t* slab(const Geometry& geo) const {
+  __device__ __forceinline__ const uint8_t* slab(const Geometry& geo, int page) const {
     return geo.pool + ((size_t)page * geo.hkv + h) * geo.slab_bytes;
   }
 };
@@ -308,7 +305,14 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
                                                                 uint16_t* __restrict__ out, float* __restrict__ partials) {
   static_assert(KB == 0 || DT == 0, "affine caches: fp16");
   constexpr int W = CW == 1 ? 4 : 8, TW = W / CW, SLOTS = CW == 1 ? 1 : 2;
-  constexpr int F = 8 / CW;       // K, and V, operand fragments of a unit that a wave brings: cw + CW x
+  // units of a team, and of the workgroup, in a step.  16-bit caches: four, however
+  // many teams there are (256 columns over 8 x 32k bf16 tokens, 1 and 4: 394 and 377
+  // us); affine ones one per team, since their units' pieces and entries then stay in
+  // fewer registers (132 columns over 8 x 16k int8 tokens, 1 and 4: 336 and 365 us for
+  // the round, 100 over 4 x 131k int4 ones, 1 and 2: 552 and 566)
+  constexpr int UB = KB == 0 && CW > 2 ? CW / 2 : 1, STEP = TW * UB;
+  constexpr int F = 8 / CW;  // K, and V, operand fragments of a unit that a wave brings: cw + CW x
+  static_assert(4 % STEP == 0, "parts are cut in fours");
   // P's type.  Weights times scales need bf16's range, and codes are exact in it.
   // bf16 caches: V is brought as fp16 where that takes it as it is, fragment by
   // fragment, and P then enters once, rounded to fp16's 11 bits (a sixteenth of the
@@ -319,12 +323,12 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
   constexpr float kLift = PT == 0 ? kTreeTop - kTreeSlack : 0.0f;
   constexpr int COLS = 16 * CT * CW;
   using R = typename Raw<KB>::T;
-  // units of each team ([slot][team][8 K, 8 V fragments][lane]), and in the end the
+  // units ([slot][unit of a step][8 K, 8 V fragments][lane]), and in the end the
   // teams' sums
-  constexpr int RING = SLOTS * TW * 16 * 64, SUMS = TW * COLS * (kHeadDim + 4) / 4;
+  constexpr int RING = SLOTS * STEP * 16 * 64, SUMS = TW * COLS * (kHeadDim + 4) / 4;
   __shared__ u32x4 s_mem[RING > SUMS ? RING : SUMS];
-  __shared__ u32x4 s_ent[KB ? SLOTS * TW : 1][KB ? 32 : 1];  // (affine) scales and biases
-  __shared__ uint8_t s_raw[SLOTS * TW][8];  // (CONV) per wave of a team: which dim tiles of V are bf16
+  __shared__ u32x4 s_ent[KB ? SLOTS * STEP : 1][KB ? 32 : 1];  // (affine) scales and biases
+  __shared__ uint8_t s_raw[SLOTS * STEP][8];  // (CONV) per wave of a team: which dim tiles of V are bf16
   __shared__ uint64_t s_seen[kMaxNodes];
   __shared__ int s_from[kMaxNodes];
   __shared__ uint2 s_odd[TW][8];  // units with values that are infinite or no numbers, and their tokens
@@ -341,35 +345,56 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
   const bool direct = tb.part0[i + 1] - tb.part0[i] <= 1;
   const int start = uniform(tb.starts[i]), seq = tb.ids[i];
   const TreePart pt(tb, r, part);
-  const int steps = (pt.places + TW - 1) / TW;
+  const int steps = (pt.places + STEP - 1) / STEP;  // the team's units of step s: places STEP s + TW u + tw
 
-  // --- units from memory (pages.unit is the one that a load takes)
-  TreePages pages(geo, seq, h, pt.unit(tw));
-  R rk[F], rv[F];
-  [[maybe_unused]] u32x4 re;
+  // --- units from memory, and their pages a step ahead
+  TreePages pages(geo, seq, h);
+  int unit_next[UB], page_next[UB];
+  auto ask = [&](int step) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < UB; ++u) {
+      unit_next[u] = pt.unit(STEP * step + TW * u + tw);
+      page_next[u] = pages.page(unit_next[u]);
+    }
+  };
+  R rk[UB][F], rv[UB][F];
+  [[maybe_unused]] u32x4 re[UB];
   const uint32_t lane16 = (uint32_t)lane * 16;
   const uint32_t ent_at = 16u * (uint32_t)(((lane >> 3) & 3) * (geo.tb >> 2) + (lane & 7));
-  auto load = [&](int next) __attribute__((always_inline)) {  // next: the place that the load after this one takes
-    const int sub = pages.unit & pages.sh;
-    const uint8_t *slab = pages.slab(geo), *ks = slab + geo.k_off, *vs = slab + geo.v_off;
-    pages.ask(pt.unit(next));
+  auto load = [&](int next) __attribute__((always_inline)) {  // the units asked for; then asks for step `next`
+    const uint8_t* slab[UB];
+    int sub[UB];
 #pragma unroll
-    for (int x = 0; x < F; ++x) {
-      const int f = cw + CW * x;
-      if constexpr (KB == 0) {
-        rk[x] = *(const R*)(ks + (8 * sub + f) * 1024 + lane16);
-        rv[x] = *(const R*)(vs + ((f << pages.sh) + sub) * 1024 + lane16);
-      } else if constexpr (KB == 4) {
-        rk[x] = *(const R*)(ks + (2 * sub + (f >> 2)) * 1024 + 4 * (f & 3) + lane16);
-        rv[x] = *(const R*)(vs + (((f >> 2) << pages.sh) + sub) * 1024 + 4 * (f & 3) + lane16);
-      } else {
-        rk[x] = *(const R*)(ks + (4 * sub + (f >> 1)) * 1024 + 8 * (f & 1) + lane16);
-        rv[x] = *(const R*)(vs + (((f >> 1) << pages.sh) + sub) * 1024 + 8 * (f & 1) + lane16);
-      }
+    for (int u = 0; u < UB; ++u) {
+      slab[u] = pages.slab(geo, page_next[u]);
+      sub[u] = unit_next[u] & pages.sh;
     }
-    if constexpr (KB != 0) re = *(const u32x4*)(slab + geo.sb_off + sub * 128 + ent_at);
+    ask(next);
+    // (a lane's offset, kept in 32 bits up to here: the loads add it to a uniform address)
+    uint32_t at = lane16;
+    asm volatile("" : "+v"(at));
+#pragma unroll
+    for (int u = 0; u < UB; ++u) {
+      const uint8_t *ks = slab[u] + geo.k_off, *vs = slab[u] + geo.v_off;
+#pragma unroll
+      for (int x = 0; x < F; ++x) {
+        const int f = cw + CW * x;
+        if constexpr (KB == 0) {
+          rk[u][x] = *(const R*)(ks + (8 * sub[u] + f) * 1024 + at);
+          rv[u][x] = *(const R*)(vs + ((f << pages.sh) + sub[u]) * 1024 + at);
+        } else if constexpr (KB == 4) {
+          rk[u][x] = *(const R*)(ks + (2 * sub[u] + (f >> 2)) * 1024 + 4 * (f & 3) + at);
+          rv[u][x] = *(const R*)(vs + (((f >> 2) << pages.sh) + sub[u]) * 1024 + 4 * (f & 3) + at);
+        } else {
+          rk[u][x] = *(const R*)(ks + (4 * sub[u] + (f >> 1)) * 1024 + 8 * (f & 1) + at);
+          rv[u][x] = *(const R*)(vs + (((f >> 1) << pages.sh) + sub[u]) * 1024 + 8 * (f & 1) + at);
+        }
+      }
+      if constexpr (KB != 0) re[u] = *(const u32x4*)(slab[u] + geo.sb_off + sub[u] * 128 + ent_at);
+    }
   };
-  load(TW + tw);
+  ask(0);
+  load(1);
 
   if (threadIdx.x < 8 * TW) s_odd[threadIdx.x >> 3][threadIdx.x & 7] = make_uint2(0u, 0u);
   tree_nodes(tb, r, start, s_seen, s_from);
@@ -405,98 +430,102 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
   [[maybe_unused]] const uint32_t code_base = KB ? f16_pair_1024() : 0u;
 
   // --- and into LDS, as 16-bit operands
-  auto stage = [&](int place, int slot) __attribute__((always_inline)) {
-    u32x4* to = s_mem + (slot * TW + tw) * 16 * 64 + lane;
+  auto stage = [&](int step, int slot) __attribute__((always_inline)) {
 #pragma unroll
-    for (int x = 0; x < F; ++x) {
-      const int f = cw + CW * x;
-      if constexpr (KB == 0) {
-        to[f * 64] = rk[x];
-        if constexpr (!CONV) to[(8 + f) * 64] = rv[x];
-      } else if constexpr (KB == 4) {
-        to[f * 64] = nib_to_f16_dec(rk[x], code_base);
-        to[(8 + f) * 64] = nib_to_bf16(rv[x]);
-      } else {
-        to[f * 64] = byte_to_f16(rk[x].x, rk[x].y);
-        to[(8 + f) * 64] = byte_to_bf16(rv[x].x, rv[x].y);
-      }
-    }
-    if constexpr (CONV) {
-      // fp16 takes a tile whose values are below 65536 with the largest at 2^-8 or
-      // more (values below 2^-14 are off by up to 2^-25 then); units with tokens
-      // that are not seen stay as they are
-      uint32_t raw = 0;
+    for (int u = 0; u < UB; ++u) {
+      const int place = STEP * step + TW * u + tw, at = slot * STEP + TW * u + tw;
+      u32x4* to = s_mem + at * 16 * 64 + lane;
 #pragma unroll
       for (int x = 0; x < F; ++x) {
         const int f = cw + CW * x;
-        u16x2 big = {0, 0};
-        u32x4 v;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t w = rv[x][j], mag = w & 0x7FFF7FFFu;
-          big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2, mag));
-          v[j] = cvt_pk<0>(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+        if constexpr (KB == 0) {
+          to[f * 64] = rk[u][x];
+          if constexpr (!CONV) to[(8 + f) * 64] = rv[u][x];
+        } else if constexpr (KB == 4) {
+          to[f * 64] = nib_to_f16_dec(rk[u][x], code_base);
+          to[(8 + f) * 64] = nib_to_bf16(rv[u][x]);
+        } else {
+          to[f * 64] = byte_to_f16(rk[u][x].x, rk[u][x].y);
+          to[(8 + f) * 64] = byte_to_bf16(rv[u][x].x, rv[u][x].y);
         }
-        const uint32_t top = max((uint32_t)big[0], (uint32_t)big[1]);
-        const bool ok = place < pt.full && !__any(top >= 0x4780u) && (__any(top >= 0x3B80u) || !__any(top != 0));
-        if (!ok) {
-          raw |= 1u << f;
-          v = rv[x];
-        }
-        to[(8 + f) * 64] = v;
       }
-      if (lane == 0) s_raw[slot * TW + tw][cw] = (uint8_t)raw;
-    }
-    if (place >= pt.full) {
-      // Some columns do not see all of the unit.  Values of tokens that none sees
-      // (old pages hold anything) are taken as zeros; so are infinities and NaN,
-      // which a weight of zero does not take out of a product: they are noted, and
-      // reach the columns that see them at the end.  Of affine caches these are
-      // tokens with such scales or biases, for their 64 dims.
-      const int unit = pt.unit(place);
-      uint32_t odd = 0;
-      if constexpr (KB == 0) {
-        const int t0 = 32 * unit + 8 * g;
-        constexpr uint32_t INF = DT == 0 ? 0x7C00u : 0x7F80u;
-        u32x4 any = u32x4{0u, 0u, 0u, 0u};
-#pragma unroll 1
-        for (int f = 8 + cw; f < 16; f += CW) {
-          u32x4 v = to[f * 64];
+      if constexpr (CONV) {
+        // fp16 takes a tile whose values are below 65536, with one at 2^-10 or more in
+        // each dim's eight tokens (values below 2^-14 are off by up to 2^-25 then, a
+        // 2^-15th of it at most); units with tokens that are not seen stay as they are
+        uint32_t raw = 0;
+#pragma unroll
+        for (int x = 0; x < F; ++x) {
+          const int f = cw + CW * x;
+          u16x2 big = {0, 0};
+          u32x4 v;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const int a = t0 + 2 * j;
-            const uint32_t w = v[j] & ((a >= r.lo && a < r.T ? 0x0000FFFFu : 0u) | (a + 1 >= r.lo && a + 1 < r.T ? 0xFFFF0000u : 0u));
-            const uint32_t bad = ((w & INF) == INF ? 0xFFFFu : 0u) | ((w >> 16 & INF) == INF ? 0xFFFF0000u : 0u);
-            any[j] |= bad;
-            v[j] = w & ~bad;
+            const uint32_t w = rv[u][x][j], mag = w & 0x7FFF7FFFu;
+            big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2, mag));
+            v[j] = cvt_pk<0>(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
           }
-          to[f * 64] = v;
+          const uint32_t top = max((uint32_t)big[0], (uint32_t)big[1]);
+          const bool ok = place < pt.full && __all(top - 0x3A80u < 0x4780u - 0x3A80u);
+          if (!ok) {
+            raw |= 1u << f;
+            v = rv[u][x];
+          }
+          to[(8 + f) * 64] = v;
         }
-        if (__any((any[0] | any[1] | any[2] | any[3]) != 0))
+        if (lane == 0) s_raw[at][cw] = (uint8_t)raw;
+      }
+      if (place >= pt.full) {
+        // Some columns do not see all of the unit.  Values of tokens that none sees
+        // (old pages hold anything) are taken as zeros; so are infinities and NaN,
+        // which a weight of zero does not take out of a product: they are noted, and
+        // reach the columns that see them at the end.  Of affine caches these are
+        // tokens with such scales or biases, for their 64 dims.
+        const int unit = pt.unit(place);
+        uint32_t odd = 0;
+        if constexpr (KB == 0) {
+          const int t0 = 32 * unit + 8 * g;
+          constexpr uint32_t INF = DT == 0 ? 0x7C00u : 0x7F80u;
+          u32x4 any = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll 1
+          for (int f = 8 + cw; f < 16; f += CW) {
+            u32x4 v = to[f * 64];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const uint64_t who = __ballot((any[e >> 1] >> (16 * (e & 1)) & 1) != 0);
-#pragma unroll
-            for (int gg = 0; gg < 4; ++gg)
-              if (who >> (16 * gg) & 0xFFFF) odd |= 1u << (8 * gg + e);
+            for (int j = 0; j < 4; ++j) {
+              const int a = t0 + 2 * j;
+              const uint32_t w = v[j] & ((a >= r.lo && a < r.T ? 0x0000FFFFu : 0u) | (a + 1 >= r.lo && a + 1 < r.T ? 0xFFFF0000u : 0u));
+              const uint32_t bad = ((w & INF) == INF ? 0xFFFFu : 0u) | ((w >> 16 & INF) == INF ? 0xFFFF0000u : 0u);
+              any[j] |= bad;
+              v[j] = w & ~bad;
+            }
+            to[f * 64] = v;
           }
-      } else {
-        auto inf = [](uint32_t w) {
-          return ((w & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u) | ((w >> 16 & 0x7C00u) == 0x7C00u ? 0xFFFF0000u : 0u);
-        };
-        const uint32_t bad = inf(re[2]) | inf(re[3]);
-        odd = (uint32_t)__ballot(bad != 0 && lane < 32);
-        re[2] &= ~bad;
-        re[3] &= ~bad;
+          if (__any((any[0] | any[1] | any[2] | any[3]) != 0))
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const uint64_t who = __ballot((any[e >> 1] >> (16 * (e & 1)) & 1) != 0);
+#pragma unroll
+              for (int gg = 0; gg < 4; ++gg)
+                if (who >> (16 * gg) & 0xFFFF) odd |= 1u << (8 * gg + e);
+            }
+        } else {
+          auto inf = [](uint32_t w) {
+            return ((w & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u) | ((w >> 16 & 0x7C00u) == 0x7C00u ? 0xFFFF0000u : 0u);
+          };
+          const uint32_t bad = inf(re[u][2]) | inf(re[u][3]);
+          odd = (uint32_t)__ballot(bad != 0 && lane < 32);
+          re[u][2] &= ~bad;
+          re[u][3] &= ~bad;
+        }
+        if (odd && lane == 0 && place < pt.places) {
+          uint2* note = &s_odd[tw][place - pt.full];
+          note->x = unit;
+          atomicOr(&note->y, odd);
+        }
       }
-      if (odd && lane == 0) {
-        uint2* at = &s_odd[tw][(place - pt.full) / TW];
-        at->x = unit;
-        atomicOr(&at->y, odd);
-      }
+      if constexpr (KB != 0)
+        if (cw == 0) s_ent[at][lane & 31] = re[u];
     }
-    if constexpr (KB != 0)
-      if (cw == 0) s_ent[slot * TW + tw][lane & 31] = re;
   };
   auto sync = [&]() __attribute__((always_inline)) {
     if constexpr (CW == 1) wave_lds_order();
@@ -522,9 +551,9 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
   [[maybe_unused]] const uint32_t unit_pair = PT == 0 ? 0x3C003C00u : 0x3F803F80u;
   [[maybe_unused]] const u32x4 ones = u32x4{unit_pair, unit_pair, unit_pair, unit_pair};
 
-  auto compute = [&](int place, int slot) __attribute__((always_inline)) {
-    const u32x4* in = s_mem + (slot * TW + tw) * 16 * 64 + lane;
-    [[maybe_unused]] const uint2* ent = (const uint2*)s_ent[KB ? slot * TW + tw : 0];
+  auto compute = [&](int place, int at) __attribute__((always_inline)) {  // at: the unit in the ring
+    const u32x4* in = s_mem + at * 16 * 64 + lane;
+    [[maybe_unused]] const uint2* ent = (const uint2*)s_ent[KB ? at : 0];
     // S^T: entry e is token 8 g + e of the unit.  Affine caches: the codes' products
     // of each 64 dims, then with the token's scales and biases
     float sv[CT][8];
@@ -636,7 +665,7 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
     }
     if constexpr (CONV) {
       uint32_t raw = 0;
-      const uint2 each = *(const uint2*)s_raw[slot * TW + tw];
+      const uint2 each = *(const uint2*)s_raw[at];
 #pragma unroll
       for (int x = 0; x < CW; ++x) raw |= (x < 4 ? each.x : each.y) >> (8 * (x & 3)) & 0xFFu;
       raw = (uint32_t)uniform((int)raw);
@@ -647,23 +676,22 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
 #pragma unroll
           for (int ct = 0; ct < CT; ++ct) o[ct][dt] = mfma16x16x32<0>(v, hi[ct][0], o[ct][dt]);
         }
-      } else {
-        u32x4 bh[CT], bl[CT];
+      }
+      if (raw != 0) {
+        // (the unit's other tiles back to bf16, exactly where they are not below 2^-14)
+        u32x4 bl[CT];
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) tree_split<1>(sv[ct], one, bh[ct], bl[ct]);
+        for (int ct = 0; ct < CT; ++ct) tree_split<1>(sv[ct], one, hi[ct][0], bl[ct]);
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt) {
-          const u32x4 v = in[(8 + dt) * 64];
-          const bool as_is = raw >> dt & 1;
+          u32x4 v = in[(8 + dt) * 64];
+          if (!(raw >> dt & 1))
 #pragma unroll
-          for (int ct = 0; ct < CT; ++ct) {
-            if (as_is) {
-              o[ct][dt] = mfma16x16x32<1>(v, bh[ct], o[ct][dt]);
-              o[ct][dt] = mfma16x16x32<1>(v, bl[ct], o[ct][dt]);
-            } else {
-              o[ct][dt] = mfma16x16x32<0>(v, hi[ct][0], o[ct][dt]);
-            }
-          }
+            for (int j = 0; j < 4; ++j) v[j] = cvt_pk<1>(lo_f(v[j]), hi_f(v[j]));
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) o[ct][dt] = mfma16x16x32<1>(v, hi[ct][0], o[ct][dt]);
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) o[ct][dt] = mfma16x16x32<1>(v, bl[ct], o[ct][dt]);
         }
       }
       return;
@@ -680,17 +708,22 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
   };
 
   __syncthreads();
-  stage(tw, 0);
-  load(2 * TW + tw);
+  stage(0, 0);
+  load(2);
   sync();
 #pragma unroll 1
   for (int s = 0; s < steps; ++s) {
-    const int place = s * TW + tw, slot = SLOTS == 1 ? 0 : s & 1;
-    if (place < pt.places && col0 < cols) compute(place, slot);
+    const int slot = SLOTS == 1 ? 0 : s & 1;
+    if (col0 < cols)
+#pragma unroll 1
+      for (int u = 0; u < UB; ++u) {
+        const int place = STEP * s + TW * u + tw;
+        if (place < pt.places) compute(place, slot * STEP + TW * u + tw);
+      }
     if (s + 1 == steps) break;
     if constexpr (SLOTS == 1) sync();
-    stage(place + TW, SLOTS == 1 ? 0 : slot ^ 1);
-    load(place + 3 * TW);
+    stage(s + 1, SLOTS == 1 ? 0 : slot ^ 1);
+    load(s + 3);
     sync();
   }
   __syncthreads();
