@@ -321,7 +321,7 @@ int bsattn_sync(bsattn_cache* cache, void* stream);
 #define BSATTN_TREE_NODES 64   /* most tokens of a request whose tree can be attended or kept */
 typedef struct bsattn_step {
   int32_t n_caches;    /* 1..BSATTN_STEP_CACHES */
-  int32_t rows;        /* rows of the packed tensors: >= 1 */
+  int32_t rows;        /* rows of the packed tensors: 1..2^24 */
   int32_t max_tokens;  /* most tokens that a request brings: >= 1 */
   int32_t n_seqs;      /* requests of the last map (written by it) */
   /* written by bsattn_step_map */
@@ -365,7 +365,8 @@ int bsattn_append_packed(bsattn_cache* cache, const bsattn_step* step, const voi
                          void* stream);
 
 /* Dense attention of the step's rows, q [rows, Hq, D] (strides as above) ->
- * out [rows, Hq, D] (dense, 16-byte aligned): a node sees the tokens its
+ * out [rows, Hq, D] (dense, 16-byte aligned), after their append and before a
+ * bsattn_keep of them: a node sees the tokens its
  * request held before the step and its own ancestors, or with a window those
  * of them at the last `window` positions (0: all).  sinks: as in
  * bsattn_decode_dense.  Absent nodes give zeros; rows of no request are left

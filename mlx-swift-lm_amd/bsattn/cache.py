@@ -569,8 +569,8 @@ class BlockSparseKVCache:
 
     def attendTree(self, queries: torch.Tensor, step, scale: float, window: Optional[int] = None,
                    sinks: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """Dense attention of a step's rows, queries [rows, Hq, D] (a view will
-        do): each sees what its request held before and its ancestors in the
+        """Dense attention of a step's rows after appendPacked and before keep,
+        queries [rows, Hq, D] (a view will do): each sees what its request held before and its ancestors in the
         tree, or those of them at the last `window` positions.  sinks as in
         decodeDense.  Rows of no request are left as they are in out [rows, Hq,
         D]."""

@@ -107,6 +107,7 @@ struct bsattn_cache {
   // changed its sequences since), and its place among the step's caches
   uint64_t step = 0;
   int32_t step_layer = 0;
+  enum { kMapped, kAppended, kKept } step_state = kMapped;  // the last call with it
   // opt-in per-kernel timing (bsattn_profile_*)
   bool profiling = false;
   std::vector<hipEvent_t> event_pool;

@@ -17,11 +17,13 @@ static_assert(BSATTN_STEP_SEQS == kMaxBatch && BSATTN_STEP_CACHES == kMaxStepCac
 namespace {
 
 std::atomic<uint64_t> g_steps{0};  // names of the steps' maps
+constexpr int kMostRows = 1 << 24;  // (row numbers and the launches' grids stay in 32 bits)
 
 int check_sizes(const bsattn_step& st) {
   if (st.n_caches < 1 || st.n_caches > kMaxStepCaches)
     return fail(BSATTN_ERR_INVALID, "n_caches %d out of range [1, %d]", st.n_caches, kMaxStepCaches);
-  if (st.rows < 1) return fail(BSATTN_ERR_INVALID, "rows must be >= 1 (got %d)", st.rows);
+  if (st.rows < 1 || st.rows > kMostRows)
+    return fail(BSATTN_ERR_INVALID, "rows %d out of range [1, %d]", st.rows, kMostRows);
   if (st.max_tokens < 1) return fail(BSATTN_ERR_INVALID, "max_tokens must be >= 1 (got %d)", st.max_tokens);
   if (!st.starts || !st.taken || !st.requests || !st.positions || !st.slots || !st.ends ||
       (!st.ancestors && st.max_tokens <= kMaxNodes))
@@ -141,6 +143,7 @@ int bsattn_step_map(bsattn_cache* const* caches, bsattn_step* st, const int32_t*
   for (int l = 0; l < st->n_caches; ++l) {
     caches[l]->step = st->stamp;
     caches[l]->step_layer = l;
+    caches[l]->step_state = bsattn_cache::kMapped;
   }
   return BSATTN_OK;
 } catch (...) {
@@ -163,6 +166,7 @@ int bsattn_append_packed(bsattn_cache* c, const bsattn_step* st, const void* k, 
   prof_collect(c, prof);
   if (e != hipSuccess) return hip_fail(e, "packed append launch");
   c->stale = true;
+  c->step_state = bsattn_cache::kAppended;
   return BSATTN_OK;
 } catch (...) {
   return on_exception();
@@ -172,6 +176,10 @@ int bsattn_attend_tree(bsattn_cache* c, const bsattn_step* st, const void* q, co
                        const float* sinks, float scale, void* out, void* stream) try {
   if (int rc = check_step(c, st)) return rc;
   if (int rc = check_tree(st)) return rc;
+  if (c->step_state != bsattn_cache::kAppended)
+    return fail(BSATTN_ERR_INVALID, c->step_state == bsattn_cache::kKept
+                                        ? "the step's tokens have moved (bsattn_keep)"
+                                        : "the step's tokens are not in the cache: call bsattn_append_packed");
   if (!out) return fail(BSATTN_ERR_INVALID, "null argument");
   if ((uintptr_t)out % 16) return fail(BSATTN_ERR_INVALID, "out must be 16-byte aligned");
   if (window < 0) return fail(BSATTN_ERR_INVALID, "window must be >= 0 (got %d)", window);
@@ -224,6 +232,8 @@ int bsattn_keep(bsattn_cache* c, const bsattn_step* st, const int32_t* kept, int
                 void* stream) try {
   if (int rc = check_step(c, st)) return rc;
   if (int rc = check_tree(st)) return rc;
+  if (c->step_state == bsattn_cache::kMapped)
+    return fail(BSATTN_ERR_INVALID, "the step's tokens are not in the cache: call bsattn_append_packed");
   if (!kept || !n_kept) return fail(BSATTN_ERR_INVALID, "null argument");
   if (width < 1) return fail(BSATTN_ERR_INVALID, "width must be >= 1 (got %d)", width);
   DeviceGuard dg(c->d.device);
@@ -236,6 +246,7 @@ int bsattn_keep(bsattn_cache* c, const bsattn_step* st, const int32_t* kept, int
   prof_collect(c, prof);
   if (e != hipSuccess) return hip_fail(e, "keep launch");
   c->stale = true;
+  c->step_state = bsattn_cache::kKept;
   return BSATTN_OK;
 } catch (...) {
   return on_exception();
