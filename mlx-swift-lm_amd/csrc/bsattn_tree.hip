@@ -327,7 +327,9 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
   // teams' sums
   constexpr int RING = SLOTS * STEP * 16 * 64, SUMS = TW * COLS * (kHeadDim + 4) / 4;
   __shared__ u32x4 s_mem[RING > SUMS ? RING : SUMS];
-  __shared__ u32x4 s_ent[KB ? SLOTS * STEP : 1][KB ? 32 : 1];  // (affine) scales and biases
+  // (affine) the tokens' scales and biases: K's in 32 bits, times the scores' scale
+  __shared__ f32x4 s_kent[KB ? SLOTS * STEP : 1][KB ? 32 : 1];
+  __shared__ uint2 s_vent[KB ? SLOTS * STEP : 1][KB ? 32 : 1];
   __shared__ uint8_t s_raw[SLOTS * STEP][8];  // (CONV) per wave of a team: which dim tiles of V are bf16
   __shared__ uint64_t s_seen[kMaxNodes];
   __shared__ int s_from[kMaxNodes];
@@ -340,11 +342,18 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
   if (at.i < 0) return;
   const int i = at.i, h = at.h, part = at.part;
   const TreeRange r = tree_range(geo, tb, i);
-  const int first = at.group * COLS, col0 = first + 16 * CT * cw, cols = r.N << r.lg;
+  const int first = at.group * COLS, cols = r.N << r.lg;
   if (first >= cols || part * r.cu >= r.units) return;
   const bool direct = tb.part0[i + 1] - tb.part0[i] <= 1;
   const int start = uniform(tb.starts[i]), seq = tb.ids[i];
   const TreePart pt(tb, r, part);
+  // the wave's column tiles, spread evenly over the team; waves w and w + 4 share a
+  // SIMD, so that the teams' fuller waves lie on different ones.  (Two a wave as far
+  // as they go, 96 columns over 4 x 262k int8 tokens 546, spread 486 us; 132 over
+  // 8 x 16k ones 336 and 290 for the step.)
+  const int tiles = min((cols - first + 15) >> 4, CT * CW), turn = wave >= 4 && CW < 8 ? CW - 1 - cw : cw;
+  const int own = CW == 1 ? CT : tiles / CW + (turn < tiles % CW ? 1 : 0);
+  const int tile0 = CW == 1 ? 0 : tiles / CW * turn + min(turn, tiles % CW), col0 = first + 16 * tile0;
   const int steps = (pt.places + STEP - 1) / STEP;  // the team's units of step s: places STEP s + TW u + tw
 
   // --- units from memory, and their pages a step ahead
@@ -524,7 +533,10 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
         }
       }
       if constexpr (KB != 0)
-        if (cw == 0) s_ent[at][lane & 31] = re[u];
+        if (cw == 0) {
+          s_kent[at][lane & 31] = sc * f32x4{lo_f(re[u][0]), hi_f(re[u][0]), lo_f(re[u][1]), hi_f(re[u][1])};
+          s_vent[at][lane & 31] = make_uint2(re[u][2], re[u][3]);
+        }
     }
   };
   auto sync = [&]() __attribute__((always_inline)) {
@@ -533,7 +545,7 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
   };
 
   f32x4 o[CT][8];
-  float m[CT], base[CT], limit[CT];  // limit: the product past which the reference is raised
+  float m[CT], base[CT], limit[CT];  // limit: the product (affine caches: exponent) past which the reference is raised
   // the weights' sums, as they enter the products: of 16-bit caches by a product
   // with ones (rows alike)
   f32x4 l[CT];
@@ -551,15 +563,18 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
   [[maybe_unused]] const uint32_t unit_pair = PT == 0 ? 0x3C003C00u : 0x3F803F80u;
   [[maybe_unused]] const u32x4 ones = u32x4{unit_pair, unit_pair, unit_pair, unit_pair};
 
-  auto compute = [&](int place, int at) __attribute__((always_inline)) {  // at: the unit in the ring
+  auto compute = [&](auto count, int place, int at) __attribute__((always_inline)) {  // at: the unit in the ring
+    constexpr int C = decltype(count)::value;  // the wave's column tiles
     const u32x4* in = s_mem + at * 16 * 64 + lane;
-    [[maybe_unused]] const uint2* ent = (const uint2*)s_ent[KB ? at : 0];
+    [[maybe_unused]] const f32x4* kent = s_kent[KB ? at : 0] + 8 * g;
+    [[maybe_unused]] const uint2* vent = s_vent[KB ? at : 0] + 8 * g;
     // S^T: entry e is token 8 g + e of the unit.  Affine caches: the codes' products
-    // of each 64 dims, then with the token's scales and biases
-    float sv[CT][8];
-    f32x4 acc[CT][KB ? 4 : 2];
+    // of each 64 dims, then with the token's scales and biases, which makes the
+    // exponents: times the scale, and less the reference
+    float sv[C][8];
+    f32x4 acc[C][KB ? 4 : 2];
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct)
+    for (int ct = 0; ct < C; ++ct)
 #pragma unroll
       for (int x = 0; x < (KB ? 4 : 2); ++x) {
         float c = 0.f;
@@ -573,26 +588,27 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
         const u32x4 a = in[(4 * t + s) * 64];
         const int x = (KB ? 2 * (s >> 1) : 0) + t;
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) acc[ct][x] = mfma16x16x32<DT>(a, qf[ct][s], acc[ct][x]);
+        for (int ct = 0; ct < C; ++ct) acc[ct][x] = mfma16x16x32<DT>(a, qf[ct][s], acc[ct][x]);
       }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      uint2 sb = make_uint2(0u, 0u);
-      if constexpr (KB != 0) sb = ent[2 * (8 * g + e)];
+      f32x4 k = f32x4{0.f, 0.f, 0.f, 0.f};
+      if constexpr (KB != 0) k = kent[e];
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        sv[ct][e] = acc[ct][e >> 2][e & 3];
-        if constexpr (KB != 0) {
-          float x = lo_f(sb.x) * sv[ct][e];
-          x = __builtin_fmaf(hi_f(sb.x), acc[ct][2 + (e >> 2)][e & 3], x);
-          x = __builtin_fmaf(lo_f(sb.y), q0[ct], x);
-          sv[ct][e] = __builtin_fmaf(hi_f(sb.y), q1[ct], x);
+      for (int ct = 0; ct < C; ++ct) {
+        if constexpr (KB == 0) {
+          sv[ct][e] = acc[ct][e >> 2][e & 3];
+        } else {
+          float x = __builtin_fmaf(k[3], q1[ct], -base[ct]);
+          x = __builtin_fmaf(k[2], q0[ct], x);
+          x = __builtin_fmaf(k[1], acc[ct][2 + (e >> 2)][e & 3], x);
+          sv[ct][e] = __builtin_fmaf(k[0], acc[ct][e >> 2][e & 3], x);
         }
       }
     }
     if (place >= pt.full) {
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
+      for (int ct = 0; ct < C; ++ct) {
         const uint32_t mask =
             seen_tokens(s_seen, s_from, min(col0 + 16 * ct + n, cols - 1) >> r.lg, r.P, 32 * pt.unit(place) + 8 * g);
 #pragma unroll
@@ -600,10 +616,10 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
       }
     }
     // the largest scores, and one branch for all columns' references
-    float mx[CT];
+    float mx[C];
     bool raise = false;
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
+    for (int ct = 0; ct < C; ++ct) {
       mx[ct] = sv[ct][0];
 #pragma unroll
       for (int e = 1; e < 8; ++e) mx[ct] = fmaxf(mx[ct], sv[ct][e]);
@@ -611,12 +627,19 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
     }
     if (__any(raise)) {
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        const float top = fmaxf(m[ct], max_over_groups(mx[ct]) * sc);
-        const float f = top == m[ct] ? 1.0f : __builtin_amdgcn_exp2f(m[ct] - top);
+      for (int ct = 0; ct < C; ++ct) {
+        const float most = max_over_groups(mx[ct]), was = base[ct];
+        const float top = fmaxf(m[ct], KB ? was + most : most * sc);
+        const bool same = top == m[ct];
+        const float f = same ? 1.0f : __builtin_amdgcn_exp2f(m[ct] - top);
         m[ct] = top;
         base[ct] = (top == -INFINITY ? 0.0f : top) - kLift;
-        limit[ct] = (top + kTreeSlack) / sc;
+        limit[ct] = KB ? (top == -INFINITY ? top : kTreeSlack) : (top + kTreeSlack) / sc;
+        if constexpr (KB != 0) {
+          const float less = same ? 0.0f : was - base[ct];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sv[ct][e] += less;
+        }
         l[ct] *= f;
         if constexpr (KB != 0) {
           ob0[ct] *= f;
@@ -628,28 +651,29 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
     }
     // the weights, as operands' two parts; affine caches: times the value scales,
     // o_d = sum_t (p_t vs_j) c_td + sum_t p_t vb_j for group j of 64 dims
-    u32x4 hi[CT][KB ? 2 : 1], lo[CT][KB ? 2 : 1];
-    [[maybe_unused]] float w0[CT][KB ? 8 : 1], w1[CT][KB ? 8 : 1];
+    u32x4 hi[C][KB ? 2 : 1], lo[C][KB ? 2 : 1];
+    [[maybe_unused]] float w0[C][KB ? 8 : 1], w1[C][KB ? 8 : 1];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       uint2 sb = make_uint2(0u, 0u);
-      if constexpr (KB != 0) sb = ent[2 * (8 * g + e) + 1];
+      if constexpr (KB != 0) sb = vent[e];
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[ct][e], sc, -base[ct]));
+      for (int ct = 0; ct < C; ++ct) {
+        const float p = __builtin_amdgcn_exp2f(KB ? sv[ct][e] : __builtin_fmaf(sv[ct][e], sc, -base[ct]));
         if constexpr (KB == 0) {
           sv[ct][e] = p;
         } else {
           l[ct][0] += p;
-          w0[ct][e] = p * lo_f(sb.x);
-          w1[ct][e] = p * hi_f(sb.x);
+          // (a multiplication with a 16-bit operand is an addition of 0 as well)
+          w0[ct][e] = __builtin_fmaf(p, lo_f(sb.x), 0.0f);
+          w1[ct][e] = __builtin_fmaf(p, hi_f(sb.x), 0.0f);
           ob0[ct] = __builtin_fmaf(p, lo_f(sb.y), ob0[ct]);
           ob1[ct] = __builtin_fmaf(p, hi_f(sb.y), ob1[ct]);
         }
       }
     }
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
+    for (int ct = 0; ct < C; ++ct) {
       if constexpr (CONV) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) hi[ct][0][j] = cvt_pk<0>(sv[ct][2 * j], sv[ct][2 * j + 1]);
@@ -674,14 +698,17 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
         for (int dt = 0; dt < 8; ++dt) {
           const u32x4 v = in[(8 + dt) * 64];
 #pragma unroll
-          for (int ct = 0; ct < CT; ++ct) o[ct][dt] = mfma16x16x32<0>(v, hi[ct][0], o[ct][dt]);
+          for (int ct = 0; ct < C; ++ct) o[ct][dt] = mfma16x16x32<0>(v, hi[ct][0], o[ct][dt]);
         }
       }
+      // (a branch of its own: as the other one's else the sums would change registers
+      // in every unit)
+      asm volatile("" : "+s"(raw));
       if (raw != 0) {
         // (the unit's other tiles back to bf16, exactly where they are not below 2^-14)
-        u32x4 bl[CT];
+        u32x4 bl[C];
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) tree_split<1>(sv[ct], one, hi[ct][0], bl[ct]);
+        for (int ct = 0; ct < C; ++ct) tree_split<1>(sv[ct], one, hi[ct][0], bl[ct]);
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt) {
           u32x4 v = in[(8 + dt) * 64];
@@ -689,9 +716,9 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[j] = cvt_pk<1>(lo_f(v[j]), hi_f(v[j]));
 #pragma unroll
-          for (int ct = 0; ct < CT; ++ct) o[ct][dt] = mfma16x16x32<1>(v, hi[ct][0], o[ct][dt]);
+          for (int ct = 0; ct < C; ++ct) o[ct][dt] = mfma16x16x32<1>(v, hi[ct][0], o[ct][dt]);
 #pragma unroll
-          for (int ct = 0; ct < CT; ++ct) o[ct][dt] = mfma16x16x32<1>(v, bl[ct], o[ct][dt]);
+          for (int ct = 0; ct < C; ++ct) o[ct][dt] = mfma16x16x32<1>(v, bl[ct], o[ct][dt]);
         }
       }
       return;
@@ -701,31 +728,33 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
       const u32x4 v = in[(8 + dt) * 64];
       constexpr int HALF = KB ? 4 : 8;
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) o[ct][dt] = mfma16x16x32<PT>(v, hi[ct][dt / HALF], o[ct][dt]);
+      for (int ct = 0; ct < C; ++ct) o[ct][dt] = mfma16x16x32<PT>(v, hi[ct][dt / HALF], o[ct][dt]);
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) o[ct][dt] = mfma16x16x32<PT>(v, lo[ct][dt / HALF], o[ct][dt]);
+      for (int ct = 0; ct < C; ++ct) o[ct][dt] = mfma16x16x32<PT>(v, lo[ct][dt / HALF], o[ct][dt]);
     }
   };
 
   __syncthreads();
-  stage(0, 0);
-  load(2);
-  sync();
+  auto run = [&](auto count) __attribute__((always_inline)) {
 #pragma unroll 1
-  for (int s = 0; s < steps; ++s) {
-    const int slot = SLOTS == 1 ? 0 : s & 1;
-    if (col0 < cols)
+    for (int s = 0; s < steps; ++s) {
+      const int slot = SLOTS == 1 ? 0 : s & 1;
+      stage(s, slot);
+      load(s + 2);
+      sync();
+      if constexpr (decltype(count)::value > 0)
 #pragma unroll 1
-      for (int u = 0; u < UB; ++u) {
-        const int place = STEP * s + TW * u + tw;
-        if (place < pt.places) compute(place, slot * STEP + TW * u + tw);
-      }
-    if (s + 1 == steps) break;
-    if constexpr (SLOTS == 1) sync();
-    stage(s + 1, SLOTS == 1 ? 0 : slot ^ 1);
-    load(s + 3);
-    sync();
-  }
+        for (int u = 0; u < UB; ++u) {
+          const int place = STEP * s + TW * u + tw;
+          if (place < pt.places) compute(count, place, slot * STEP + TW * u + tw);
+        }
+      if constexpr (SLOTS == 1) sync();
+    }
+  };
+  // (a wave's barriers are those of its own loop: all waves reach as many)
+  if (CW == 1 || own == CT) run(std::integral_constant<int, CT>{});
+  else if (own == 1) run(std::integral_constant<int, 1>{});
+  else run(std::integral_constant<int, 0>{});
   __syncthreads();
   tree_odd<DT, KB, CT>(geo, r, seq, h, s_odd[tw], s_seen, s_from, col0, cols, o);
 
@@ -733,7 +762,8 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
   float (*s_o)[COLS][kHeadDim + 4] = (float (*)[COLS][kHeadDim + 4])s_mem;
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
-    const int c = 16 * (CT * cw + ct) + n;
+    if (ct >= own) break;
+    const int c = 16 * (tile0 + ct) + n;
     const float lc = KB ? sum_over_groups(l[ct][0]) : l[ct][0];
     if (g == 0) {
       s_m[tw][c] = m[ct] == -INFINITY ? m[ct] : base[ct];
