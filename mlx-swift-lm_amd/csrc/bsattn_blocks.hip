@@ -172,7 +172,7 @@ template <int TB>
 __device__ __forceinline__ PackedBlock packed_block(const Geometry& geo, const StepRows& sr) {
   const int lane = threadIdx.x & 63, x = blockIdx.x;
   const int at = min(lane, sr.n - 1);
-  const int taken = lane < sr.n ? sr.taken[at] : 0, end = sr.ends[at];
+  const int taken = lane < sr.n ? sr.taken[at] : 0, end = sr.ends[at], start = sr.starts[at];
   if (x == 0 && blockIdx.y == 0 && (int)threadIdx.x < sr.n && taken > 0) geo.meta[sr.ids[at]] = end;
   const int blocks = taken > 0 ? (end - 1) / TB - (end - taken) / TB + 1 : 0;
   const int upto = wave_scan_incl(blocks);
@@ -185,7 +185,7 @@ __device__ __forceinline__ PackedBlock packed_block(const Geometry& geo, const S
   b.end = __builtin_amdgcn_readlane(end, i);
   b.old = b.end - __builtin_amdgcn_readlane(taken, i);
   b.blk = b.old / TB + x - __builtin_amdgcn_readlane(upto - blocks, i);
-  b.row0 = (int64_t)uniform(sr.starts[i]) - b.old;
+  b.row0 = (int64_t)__builtin_amdgcn_readlane(start, i) - b.old;
   const int64_t row = b.row0 + max(b.blk * TB, b.old);
   const int slot = row >= 0 && row < sr.rows ? uniform(sr.slots[row]) : -1;
   const int page = slot / TB;

@@ -147,12 +147,14 @@ __global__ __launch_bounds__(256) void k_keep(Geometry geo, StepRows sr, const i
   __shared__ u32x4 s_blk[KB == 0 ? 64 : TB * KB / 16][16];  // a block's keys, or their code tile
   __shared__ u32x4 s_sb[KB ? TB : 1];
   const int h = blockIdx.x, i = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
-  const int taken = min(sr.taken[i], kMaxNodes);
+  // (everything that does not depend on another load is asked for at once)
+  const int taken = min(sr.taken[i], kMaxNodes), start = sr.starts[i], seq = sr.ids[i], P = sr.ends[i] - taken;
+  const int list = kept[(size_t)i * width + min(lane, width - 1)], many = n_kept[i];
+  asm volatile("" ::"v"(list), "s"(many), "s"(start), "s"(P));
   if (taken <= 0) return;
-  const int start = sr.starts[i], seq = sr.ids[i], P = sr.ends[i] - taken;
   // the list, up to the first entry that does not ascend or is no node
-  const int want = min(min(max(n_kept[i], 0), width), taken);
-  const int from = lane < want ? kept[(size_t)i * width + lane] : -1;
+  const int want = min(min(max(many, 0), width), taken);
+  const int from = lane < want ? list : -1;
   const int before = __shfl_up(from, 1, 64);
   const uint64_t bad = __ballot(lane >= want || from < 0 || from >= taken || (lane > 0 && from <= before));
   const int m = bad ? __ffsll((unsigned long long)bad) - 1 : 64;
@@ -197,24 +199,26 @@ __global__ __launch_bounds__(256) void k_keep(Geometry geo, StepRows sr, const i
     const int grp = g0 + 2 * x + (tid >> 7), d = tid & 127;
     if (grp > g1) continue;
     T piece = *v_at(s_slot[max(8 * grp, P) - P], d);
+    uint32_t part[8];  // (all eight are on their way before the first is needed)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int slot = s_slot[s_from[min(max(8 * grp + e - P, 0), m - 1)]];
+      if constexpr (KB == 0) {
+        part[e] = *((const uint16_t*)(slab(slot) + geo.v_off) + v_elem(TB, slot % TB, d));
+      } else {
+        const uint8_t* at = slab(slot) + geo.v_off + vq_byte(KB, TB, slot % TB, d, &sh);
+        part[e] = ((uint32_t)*at >> sh) & ((1u << KB) - 1);
+      }
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int j = 8 * grp + e - P;
-      if (j < 0 || j >= m) continue;
-      const int slot = s_slot[s_from[j]];
-      if constexpr (KB == 0) {
-        const uint32_t w = *((const uint16_t*)(slab(slot) + geo.v_off) + v_elem(TB, slot % TB, d));
-        piece[e >> 1] = (e & 1) ? (piece[e >> 1] & 0x0000FFFFu) | (w << 16) : (piece[e >> 1] & 0xFFFF0000u) | w;
-      } else {
-        const uint8_t* at = slab(slot) + geo.v_off + vq_byte(KB, TB, slot % TB, d, &sh);
-        const uint32_t w = ((uint32_t)*at >> sh) & ((1u << KB) - 1);
-        if constexpr (KB == 4) {
-          piece = (piece & ~(0xFu << (4 * q_nib(e)))) | (w << (4 * q_nib(e)));
-        } else {
-          uint32_t& p = e < 4 ? piece.x : piece.y;
-          p = (p & ~(0xFFu << (8 * (e & 3)))) | (w << (8 * (e & 3)));
-        }
-      }
+      const bool in = j >= 0 && j < m;
+      auto with = [&](uint32_t word, int at, uint32_t mask) { return in ? (word & ~(mask << at)) | (part[e] << at) : word; };
+      if constexpr (KB == 0) piece[e >> 1] = with(piece[e >> 1], 16 * (e & 1), 0xFFFFu);
+      else if constexpr (KB == 4) piece = with(piece, 4 * q_nib(e), 0xFu);
+      else if (e < 4) piece.x = with(piece.x, 8 * e, 0xFFu);
+      else piece.y = with(piece.y, 8 * (e - 4), 0xFFu);
     }
     vp[x] = piece;
   }
