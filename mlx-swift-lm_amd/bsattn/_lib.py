@@ -64,7 +64,7 @@ EXPORTS = (
 )
 
 KERNEL_SCORE, KERNEL_TOPK, KERNEL_ATTEND, KERNEL_COMBINE, KERNEL_APPEND, KERNEL_SUMMARY, KERNEL_PREFILL, \
-    KERNEL_ROTATE, KERNEL_DENSE, KERNEL_FORK = range(10)
+    KERNEL_ROTATE, KERNEL_DENSE, KERNEL_FORK, KERNEL_MAP, KERNEL_TREE, KERNEL_KEEP = range(13)
 
 
 class BsattnError(RuntimeError):
