@@ -57,7 +57,7 @@ class Step:
         torch.cuda.current_stream(self.device).synchronize()
         self._most, self._n = most, 0
         self.starts, self.taken, self.ends = self._starts[:1], self._taken[:0], self._ends[:0].view(len(caches), 0)
-        self._handles = (ctypes.c_void_p * len(caches))()
+        self._handles, self._held = (ctypes.c_void_p * len(caches))(), None
         self._c = _lib.Step(n_caches=len(caches), rows=self.rows, max_tokens=self.maxTokens, n_seqs=0,
                             starts=self._starts.data_ptr(), taken=self._taken.data_ptr(),
                             requests=self.requests.data_ptr(), positions=self.positions.data_ptr(),
@@ -83,10 +83,12 @@ class Step:
             raise ValueError(f"counts must hold 1 to {self._most} requests, got {tuple(counts.shape)}")
         at = self._check_ints(counts, "counts", (n,))
         up = None if parents is None else self._check_ints(parents, "parents", (self.rows,))
-        for i, c in enumerate(self.caches):
-            if c._h is None:
+        held = [c._h for c in self.caches]
+        if held != self._held:
+            if None in held:
                 raise ValueError("a cache of the step is closed")
-            self._handles[i] = c._h
+            self._handles[:] = [h.value for h in held]
+            self._held = held
         check(lib().bsattn_step_map(self._handles, self._ref, at, up, _row_ids(seq_ids, n), n, _stream(self.device)))
         if n != self._n:
             self._n = n

@@ -92,13 +92,17 @@ int bsattn_step_map(bsattn_cache* const* caches, bsattn_step* st, const int32_t*
     return fail(BSATTN_ERR_INVALID, "a tree has at most %d nodes (max_tokens is %d)", kMaxNodes, st->max_tokens);
   std::vector<int32_t> seqs;
   bool synced = true;
+  int32_t least = 0;  // sequences of the smallest cache so far
   for (int l = 0; l < st->n_caches; ++l) {
     const bsattn_cache* c = caches[l];
     if (!c) return fail(BSATTN_ERR_INVALID, "null cache");
     if (c->d.device != caches[0]->d.device) return fail(BSATTN_ERR_INVALID, "the step's caches are on different GPUs");
     for (int k = 0; k < l; ++k)
       if (caches[k] == c) return fail(BSATTN_ERR_INVALID, "a cache is listed twice");
-    if (int rc = seq_list(c, seq_ids, n_seqs, seqs)) return rc;
+    // (what the smallest cache takes the others do)
+    if (l == 0 || c->d.max_seqs < least)
+      if (int rc = seq_list(c, seq_ids, n_seqs, seqs)) return rc;
+    least = l == 0 ? c->d.max_seqs : std::min(least, c->d.max_seqs);
     if (c->num_pages * c->d.block_size > INT32_MAX)
       return fail(BSATTN_ERR_RANGE, "a pool of %lld tokens: slots are 32-bit", (long long)(c->num_pages * c->d.block_size));
     synced = synced && !c->stale;

@@ -13,6 +13,14 @@
 // enters as two 16-bit parts, for 16 (bf16) or 22 (fp16) bits.  Affine codes enter
 // as 1024 + c (K, fp16) and c (V, bf16), exactly; scales and biases act on scores
 // and weights.
+//
+// What bounds it: 16 columns and fewer the reads; from 64 on the issue of a SIMD,
+// which products (16 cycles each) and VALU work share nearly one after the other.
+// A wave's unit of 32 tokens by 32 columns is 34 products for bf16 (V as fp16, see
+// CONV), 52 for fp16, 48 for codes, beside 16 exponentials and 50 to 210 other VALU
+// instructions.  Whole launches: 64 columns over 8 x 32k bf16 tokens 183 us (1074
+// MB: 5.9 TB/s, a plain streaming read 154 us), 256 350 (786 TFLOP/s; 63% of a
+// large product's rate), 100 over 4 x 131k int4 499, 96 over 4 x 262k int8 466.
 #include <hip/hip_ext.h>
 #include <hip/hip_runtime.h>
 #include <stdint.h>

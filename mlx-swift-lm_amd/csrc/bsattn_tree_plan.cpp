@@ -16,7 +16,11 @@ int64_t tree_plan(const Geometry& g, TreeBatch& tb) {
     all += tb.units[i];
     most = std::max(most, tb.units[i]);
   }
-  // one round of workgroups
+  // One round of workgroups: eight waves of 256 registers fill a CU, of four two fit.
+  // Two rounds cost starts, ends and partials: 64 columns over 8 x 32k bf16 tokens 188
+  // us in one, 200 in two, 220 in three; 256 350, 369, 448; 100 over 4 x 131k int4 499,
+  // 512, 523; 192 in windows of ragged trees 160, 187, 223.  (Ragged lengths would gain
+  // from two, 96 columns over 32 requests: the step 541 and 524.)
   const int64_t want = (tb.tiles > 2 ? 1 : 2) * (int64_t)std::max(g.cus, 1), each = (int64_t)g.hkv * tb.groups;
   auto parts = [&](int i, int cu) { return std::max(1, (tb.units[i] + cu - 1) / cu); };
   auto fits = [&](int cu) {
