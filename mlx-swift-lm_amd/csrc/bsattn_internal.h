@@ -360,6 +360,7 @@ hipError_t launch_keep(const Geometry& g, const StepRows& sr, const int32_t* kep
 struct TreeBatch {
   int32_t n, max_tokens, cu, window;
   int32_t tiles, groups;  // column tiles of 16 in a workgroup, workgroups for a request's columns
+  bool narrow;            // waves of one column tile each
   float sl2;
   const float* sinks;  // [hq], or null
   const int32_t* starts;
@@ -368,7 +369,7 @@ struct TreeBatch {
   int64_t qr, qh;      // elements between rows and heads of q
   int32_t ids[kMaxBatch], units[kMaxBatch], row0[kMaxBatch], part0[kMaxBatch + 1];
 };
-// sets cu, tiles, groups, row0 and part0 from units (the most of each request);
+// sets cu, tiles, groups, narrow, row0 and part0 from units (the most of each request);
 // the rows of the workspace (0: none is needed)
 int64_t tree_plan(const Geometry& g, TreeBatch& tb);
 hipError_t launch_tree(const Geometry& g, const TreeBatch& tb, const void* q, void* out, float* ws, hipEvent_t done,

@@ -156,8 +156,9 @@ __device__ __forceinline__ TreePlace tree_place(const TreeBatch& tb) {
   const int lane = threadIdx.x & 63, at = blockIdx.x;
   p.h = blockIdx.y;
   p.group = blockIdx.z;
-  const uint64_t held = __ballot(lane < tb.n && tb.part0[min(lane, tb.n - 1)] <= at);
-  p.i = at < tb.part0[tb.n] ? uniform(__popcll(held) - 1) : -1;
+  int last = 0;
+  if (tb.n > 1) last = uniform(__popcll(__ballot(lane < tb.n && tb.part0[min(lane, tb.n - 1)] <= at)) - 1);
+  p.i = at < tb.part0[tb.n] ? last : -1;
   p.part = at - tb.part0[max(p.i, 0)];
   return p;
 }
@@ -761,7 +762,7 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
   };
   // (a wave's barriers are those of its own loop: all waves reach as many)
   if (CW == 1 || own == CT) run(std::integral_constant<int, CT>{});
-  else if (own == 1) run(std::integral_constant<int, 1>{});
+  else if (CT > 1 && own == 1) run(std::integral_constant<int, 1>{});
   else run(std::integral_constant<int, 0>{});
   __syncthreads();
   tree_odd<DT, KB, CT>(geo, r, seq, h, s_odd[tw], s_seen, s_from, col0, cols, o);
@@ -806,17 +807,19 @@ __global__ __launch_bounds__(256) void k_tree_join(Geometry geo, TreeBatch tb, c
   const int hq = blockIdx.x, which = blockIdx.y * (8 / ROWS) + slot / ROWS;
   const int i = min(which / tb.max_tokens, tb.n - 1), node = which - i * tb.max_tokens;
   const TreeRange r = tree_range(geo, tb, ROWS == 8 ? uniform(i) : i);
-  // (requests of one part: the launch before wrote the output)
-  const bool there = which < tb.n * tb.max_tokens && node < r.N && tb.part0[i + 1] - tb.part0[i] > 1;
+  // (requests of one part: the launch before wrote the output, and they have no
+  // partials.  The loads go by the parts of the launch and do not wait for the lengths)
+  const int cut = tb.part0[i + 1] - tb.part0[i], most = which < tb.n * tb.max_tokens && cut > 1 ? cut : 0;
+  const bool there = most > 0 && node < r.N;
   float M = -INFINITY, L = 0.f;
   f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
   const int parts = there ? (r.units + r.cu - 1) / r.cu : 0;
-  for (int p0 = y; p0 < parts; p0 += 4 * ROWS) {
+  for (int p0 = y; p0 < most; p0 += 4 * ROWS) {
     f32x4 x[4];
     float m[4], l[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int p = min(p0 + j * ROWS, parts - 1);
+      const int p = min(p0 + j * ROWS, most - 1);
       const float2* part = (const float2*)(ws + ((int64_t)(tb.row0[i] + p * tb.max_tokens + node) * geo.hq + hq) * kPartial);
       const float2 xa = part[2 * c], xb = part[2 * c + 1], ml = part[kHeadDim / 2];
       x[j] = f32x4{xa.x, xa.y, xb.x, xb.y};
@@ -879,8 +882,8 @@ static void tree_dispatch(const Geometry& g, const TreeBatch& tb, const uint16_t
   auto go = [&](auto kernel, int threads) { launch(kernel, grid, dim3(threads), 0, s, prof, kProfTree, g, tb, q, out, ws); };
   if (tb.tiles == 1) go(k_tree<DT, KB, 1, 1>, 256);
   else if (tb.tiles == 2) go(k_tree<DT, KB, 2, 1>, 256);
-  else if (tb.tiles == 4) go(k_tree<DT, KB, 2, 2>, 512);
-  else if (tb.tiles == 8) go(k_tree<DT, KB, 2, 4>, 512);
+  else if (tb.tiles == 4) tb.narrow ? go(k_tree<DT, KB, 1, 4>, 512) : go(k_tree<DT, KB, 2, 2>, 512);
+  else if (tb.tiles == 8) tb.narrow ? go(k_tree<DT, KB, 1, 8>, 512) : go(k_tree<DT, KB, 2, 4>, 512);
   else go(k_tree<DT, KB, 2, 8>, 512);
 }
 

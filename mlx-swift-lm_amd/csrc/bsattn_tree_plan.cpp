@@ -41,6 +41,12 @@ int64_t tree_plan(const Geometry& g, TreeBatch& tb) {
   }
   const bool even = 4 * lo <= 32 || 2 * (int64_t)4 * lo * want <= 3 * all * each;
   tb.cu = !fits(4 * lo) ? cut(want) : even ? 4 * lo : cut(3 * want);
+  // With few units a workgroup's time is its ends: waves of one column tile leave half
+  // as many teams' sums to join.  One request, 64 columns over 4k bf16 tokens (4 units
+  // a workgroup) 18.4 us, 20.0 with waves of two, 8k (8) 19.6 and 21.2, 16k (16) 25.4
+  // and 25.9, 32k 34.2 and 34.0; 128 columns over 8k 25.5 and 26.5, 16k 33.3 and 32.6,
+  // 64k 74.5 and 66.5.
+  tb.narrow = (tb.tiles == 4 || tb.tiles == 8) && tb.cu <= 8;
   // (it ends: a request of one part has no partials)
   while (true) {
     int64_t n = 0, blocks = 0;
