@@ -146,6 +146,21 @@ struct Piece<4> {
   typedef uint32_t T;
 };
 
+// dims 2c, 2c + 1 of a full block's summary: the sums and roundings of fold_block,
+// two dims a thread (a kept path that fills a block: 10.2 us with eight, 8.2 so)
+template <int DT, int TB>
+__device__ __forceinline__ uint32_t fold_pair(const uint32_t* blk, int c) {
+  float a = 0.f, b = 0.f;
+#pragma unroll 16
+  for (int t = 0; t < TB; ++t) {
+    const uint32_t w = blk[64 * t + c];
+    const float x = DT == 0 ? lo_f(w) : __uint_as_float(w << 16), y = DT == 0 ? hi_f(w) : __uint_as_float(w & 0xFFFF0000u);
+    a = t == 0 ? x : __fadd_rn(a, x);
+    b = t == 0 ? y : __fadd_rn(b, y);
+  }
+  return pack2<DT>(__fmul_rn(a, 1.0f / TB), __fmul_rn(b, 1.0f / TB));
+}
+
 template <int DT, int KB, int TB>
 __global__ __launch_bounds__(256) void k_keep(Geometry geo, StepRows sr, const int32_t* __restrict__ kept, int width,
                                               const int32_t* __restrict__ n_kept) {
@@ -260,7 +275,7 @@ __global__ __launch_bounds__(256) void k_keep(Geometry geo, StepRows sr, const i
     }
     __syncthreads();
     if constexpr (KB == 0) {
-      if (tid < 16) *(u32x4*)(summary_row(geo, seq, h, blk) + 8 * tid) = fold_block<DT>(s_blk, TB, tid);
+      if (tid < 64) ((uint32_t*)summary_row(geo, seq, h, blk))[tid] = fold_pair<DT, TB>((const uint32_t*)s_blk, tid);
     } else {
       if (tid < kHeadDim)
         summary_row(geo, seq, h, blk)[tid] = fold_block_q<KB ? KB : 4>((const uint8_t*)s_blk, (const uint16_t*)s_sb, TB, tid);

@@ -46,7 +46,7 @@ int64_t tree_plan(const Geometry& g, TreeBatch& tb) {
   // a workgroup) 18.4 us, 20.0 with waves of two, 8k (8) 19.6 and 21.2, 16k (16) 25.4
   // and 25.9, 32k 34.2 and 34.0; 128 columns over 8k 25.5 and 26.5, 16k 33.3 and 32.6,
   // 64k 74.5 and 66.5.
-  tb.narrow = (tb.tiles == 4 || tb.tiles == 8) && tb.cu <= 8;
+  tb.narrow = (tb.tiles == 4 || tb.tiles == 8) && tb.cu <= 12;
   // (it ends: a request of one part has no partials)
   while (true) {
     int64_t n = 0, blocks = 0;

@@ -160,6 +160,15 @@ static void refusals() {
   refused(bsattn_step_map(same, &s.st, counts, nullptr, nullptr, 3, nullptr), BSATTN_ERR_INVALID, "twice");
   bsattn_cache* longer[] = {a, other};
   refused(bsattn_step_map(longer, &s.st, counts, nullptr, nullptr, 3, nullptr), BSATTN_ERR_INVALID, "holds 40 tokens");
+  bsattn_cache* small = cache(2, 8, 40);
+  for (auto list : {std::vector<bsattn_cache*>{a, small}, {small, a}}) {  // (whichever comes first)
+    refused(bsattn_step_map(list.data(), &s.st, counts, nullptr, nullptr, 3, nullptr), BSATTN_ERR_RANGE, "max_seqs 2");
+    const int32_t ends[2] = {0, 2};
+    refused(bsattn_step_map(list.data(), &s.st, counts, nullptr, ends, 2, nullptr), BSATTN_ERR_RANGE, "out of range");
+    CHECK(bsattn_step_map(list.data(), &s.st, counts, nullptr, nullptr, 2, nullptr) == BSATTN_OK);
+  }
+  bsattn_cache_destroy(small);
+  s.st.stamp = 0;
   bsattn_cache* none[] = {a, nullptr};
   refused(bsattn_step_map(none, &s.st, counts, nullptr, nullptr, 3, nullptr), BSATTN_ERR_INVALID, "null cache");
   // what comes before a map
