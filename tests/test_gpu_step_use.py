@@ -514,3 +514,43 @@ def test_kernel_times(gpu):
     for kind in (_lib.KERNEL_MAP, _lib.KERNEL_TREE, _lib.KERNEL_KEEP, _lib.KERNEL_APPEND):
         ms, n = c.profileRead(kind)
         assert n == 1 and 0 < ms < 50
+
+
+# ---------------------------------------------------------------------------
+# random shapes
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("seed", range(40))
+def test_random_rounds(gpu, seed):
+    """Two rounds of seeded random caches, layouts, lengths, counts, trees, windows, sinks, sequence orders and kept
+    paths: attention against the formula, states against caches that were given the kept tokens."""
+    import random
+    import torch
+    r = random.Random(seed)
+    dtype, bits = r.choice(KINDS)
+    Tb, (Hq, Hkv) = r.choice([32, 64]), r.choice([(8, 8), (4, 1), (32, 8), (16, 1), (8, 2), (16, 2), (64, 4), (2, 2)])
+    B, most = r.randint(1, 9), r.choice([1, 4, 9, 16, 33, 64])
+    lens = [r.choice([0, 1, 31, 32, 63, 64, r.randint(2, 300), r.randint(300, 6000)]) for _ in range(B)]
+    log(f"[random {seed}] {dtype} bits={bits} Tb={Tb} {Hq}/{Hkv} most={most} {lens}")
+    c, ref = (_cache(lens, Hq, Hkv, Tb, dtype, bits, spare=2 * 64) for _ in range(2))
+    salient = r.random() < 0.5
+    for x in (c, ref):
+        _fill(gpu, x, lens, 1000 + seed, salient=salient)
+    for turn in range(2):
+        ids = r.sample(range(B), r.randint(1, B))
+        counts = [r.choice([0, 1, r.randint(1, most), most]) for _ in ids]
+        trees = None if r.random() < 0.25 else [_tree(10 * seed + i, n, r.choice([0, 0.1])) for i, n in enumerate(counts)]
+        window = r.choice([None, None, 1, 50, 700])
+        sinks = _randn(gpu, seed, (Hq,), "f16").float() if r.random() < 0.4 else None
+        step = _verify(gpu, c, [lens[b] for b in ids], counts, trees, 50 * seed + turn, f"{seed} {turn}", ids=ids,
+                       window=window, sinks=sinks, rows=max(1, sum(counts)) + r.randint(0, 3), fused=r.random() < 0.5)
+        _, k, v = _rows(gpu, c, 50 * seed + turn, step.rows)
+        kept = [sorted(r.sample(range(n), r.randint(0, min(n, 12)))) for n in counts]
+        width = max(1, max(len(p) for p in kept))
+        c.keep(step, _ints(gpu, [p + [0] * (width - len(p)) for p in kept]), _ints(gpu, [len(p) for p in kept]))
+        c.sync()
+        for i, (b, p) in enumerate(zip(ids, kept)):
+            at = torch.tensor([sum(counts[:i]) + j for j in p], dtype=torch.long, device=gpu)
+            _plain_append(ref, k[at], v[at], b)
+            lens[b] += len(p)
+        assert [c.seqLen(b) for b in range(B)] == lens
+        assert _same(_state(c, range(B)), _state(ref, range(B))), turn
