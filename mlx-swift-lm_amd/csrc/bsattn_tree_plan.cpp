@@ -1,6 +1,7 @@
 // bsattn_tree_plan.cpp -- how a tree attention's tokens are cut into the parts
 // that its workgroups take (bsattn_tree.hip), and where their partials lie.
 #include <algorithm>
+#include <cstdint>
 
 #include "bsattn_internal.h"
 
@@ -16,31 +17,48 @@ int64_t tree_plan(const Geometry& g, TreeBatch& tb) {
     all += tb.units[i];
     most = std::max(most, tb.units[i]);
   }
-  // One round of workgroups: eight waves of 256 registers fill a CU, of four two fit.
-  // Two rounds cost starts, ends and partials: 64 columns over 8 x 32k bf16 tokens 188
-  // us in one, 200 in two, 220 in three; 256 350, 369, 448; 100 over 4 x 131k int4 499,
-  // 512, 523; 192 in windows of ragged trees 160, 187, 223.  (Ragged lengths would gain
-  // from two, 96 columns over 32 requests: the step 541 and 524.)
+  // Workgroups of one round: eight waves of 256 registers fill a CU, of four two fit.
+  // Further rounds cost starts, ends and partials, about the time of 12 units a
+  // workgroup: 64 columns over 8 x 32k bf16 tokens 188 us in one round, 200 in two, 220
+  // in three; 256 350, 369, 448; 100 over 4 x 131k int4 499, 512, 523; 192 in windows
+  // of ragged trees 160, 187, 223.  Where the longest request's part would outlast the
+  // others by far, more are shorter all the same: 96 columns over 32 requests of 300 to
+  // 20000 tokens, bf16 304 us in two or three rounds, int4 341 in three, 383 in two; 64
+  // over 40 x 9k bf16 tokens 344 with a part each, one round and a quarter, 298 in four.
+  // By little they are not (what the others leave of the memory's rate falls to the
+  // longest): 64 over 9 x 13k tokens, a seventh more units in the longest part, 97 us,
+  // cut for two rounds 105.
   const int64_t want = (tb.tiles > 2 ? 1 : 2) * (int64_t)std::max(g.cus, 1), each = (int64_t)g.hkv * tb.groups;
+  constexpr int64_t kEnds = 12;
   auto parts = [&](int i, int cu) { return std::max(1, (tb.units[i] + cu - 1) / cu); };
-  auto fits = [&](int cu) {
+  auto workgroups = [&](int cu) {
     int64_t n = 0;
     for (int i = 0; i < tb.n; ++i) n += parts(i, cu);
-    return n * each <= want;
+    return n * each;
   };
-  auto cut = [&](int64_t workgroups) {
-    const int64_t cu = std::max<int64_t>(4, (all * each + workgroups - 1) / workgroups);
-    return ((int)std::min<int64_t>(cu, most) + 3) & ~3;
+  // (in units: all rounds as long as the longest part, or the work spread evenly and a part)
+  auto time = [&](int cu) {
+    const int64_t n = workgroups(cu), part = cu + kEnds;
+    return std::min((n + want - 1) / want * part, (all * each + n * kEnds) / want + part);
   };
-  tb.cu = cut(want);
-  int lo = tb.cu / 4, hi = (most + 3) / 4;  // in fours: the smallest that fits
-  while (lo < hi) {
-    const int mid = lo + (hi - lo) / 2;
-    if (fits(4 * mid)) hi = mid;
-    else lo = mid + 1;
+  const int64_t least = (tb.n * each + want - 1) / want, bound = all * each / want + kEnds;
+  int64_t best = INT64_MAX;
+  for (int64_t more : {0, 2, 3}) {
+    if (best <= bound + bound / 8) break;
+    const int64_t rounds = least + more;
+    // in fours: the smallest that fits
+    int lo = (int)std::max<int64_t>(1, all * each / (4 * rounds * want)), hi = std::max(lo, (most + 3) / 4);
+    while (lo < hi) {
+      const int mid = lo + (hi - lo) / 2;
+      if (workgroups(4 * mid) <= rounds * want) hi = mid;
+      else lo = mid + 1;
+    }
+    const int64_t t = time(4 * lo);
+    if (best == INT64_MAX || t < best - best / 8) {
+      best = t;
+      tb.cu = 4 * lo;
+    }
   }
-  const bool even = 4 * lo <= 32 || 2 * (int64_t)4 * lo * want <= 3 * all * each;
-  tb.cu = !fits(4 * lo) ? cut(want) : even ? 4 * lo : cut(3 * want);
   // With few units a workgroup's time is its ends: waves of one column tile leave half
   // as many teams' sums to join.  One request, 64 columns over 4k bf16 tokens (4 units
   // a workgroup) 18.4 us, 20.0 with waves of two, 8k (8) 19.6 and 21.2, 16k (16) 25.4
