@@ -366,12 +366,12 @@ int bsattn_append_packed(bsattn_cache* cache, const bsattn_step* step, const voi
 
 /* Dense attention of the step's rows, q [rows, Hq, D] (strides as above) ->
  * out [rows, Hq, D] (dense, 16-byte aligned), after their append and before a
- * bsattn_keep of them: a node sees the tokens its
- * request held before the step and its own ancestors, or with a window those
- * of them at the last `window` positions (0: all).  sinks: as in
- * bsattn_decode_dense.  Absent nodes give zeros; rows of no request are left
- * as they were.  max_tokens is at most BSATTN_TREE_NODES.  Workspaces, split
- * sequences and infinite attended values as in bsattn_decode_dense. */
+ * bsattn_keep of them: a node sees the tokens its request held before the step
+ * and its own ancestors, or with a window those of them at the last `window`
+ * positions (0: all).  sinks: as in bsattn_decode_dense.  Absent nodes give
+ * zeros; rows of no request are left as they were.  max_tokens is at most
+ * BSATTN_TREE_NODES.  Workspaces, split sequences and infinite attended values
+ * as in bsattn_decode_dense. */
 int bsattn_attend_tree(bsattn_cache* cache, const bsattn_step* step, const void* q,
                        const int64_t* q_strides, int32_t window, const float* sinks, float scale,
                        void* out, void* stream);

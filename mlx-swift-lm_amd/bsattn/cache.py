@@ -570,10 +570,10 @@ class BlockSparseKVCache:
     def attendTree(self, queries: torch.Tensor, step, scale: float, window: Optional[int] = None,
                    sinks: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Dense attention of a step's rows after appendPacked and before keep,
-        queries [rows, Hq, D] (a view will do): each sees what its request held before and its ancestors in the
-        tree, or those of them at the last `window` positions.  sinks as in
-        decodeDense.  Rows of no request are left as they are in out [rows, Hq,
-        D]."""
+        queries [rows, Hq, D] (a view will do): each sees what its request held
+        before and its ancestors in the tree, or those of them at the last
+        `window` positions.  sinks as in decodeDense.  Rows of no request are
+        left as they are in out [rows, Hq, D]."""
         qs = self._check_packed(queries, "queries", self._hq, step.rows)
         window, logits = self._check_window(window), self._check_sinks(sinks)
         if out is None:
