@@ -315,7 +315,11 @@ int bsattn_sync(bsattn_cache* cache, void* stream);
  *
  * The caller owns the arrays (device memory) and keeps them and the struct
  * while calls or graphs that use them are pending; a step is used with one
- * stream at a time, and with the caches that it was last mapped for. */
+ * stream at a time, and with the caches that it was last mapped for.  Calls out
+ * of order, or after the host has changed a cache's sequences, are refused where
+ * the library can know: it does not see replays, so a step whose map was
+ * captured, and any step of a cache whose packed append was, are taken as they
+ * come. */
 #define BSATTN_STEP_SEQS 64    /* most requests of a step */
 #define BSATTN_STEP_CACHES 128 /* most caches of a step */
 #define BSATTN_TREE_NODES 64   /* most tokens of a request whose tree can be attended or kept */

@@ -32,13 +32,22 @@ int check_sizes(const bsattn_step& st) {
 }
 
 // the step's last map is the last that the cache was mapped for, and the
-// cache's sequences are as they were then
-int check_step(const bsattn_cache* c, const bsattn_step* st) {
+// cache's sequences are as they were then; or it was captured, and holds at its
+// replays.  layer: the cache's place among the step's; ordered: whether the host
+// knows the last call with it
+int check_step(const bsattn_cache* c, const bsattn_step* st, int& layer, bool& ordered) {
   if (!c || !st) return fail(BSATTN_ERR_INVALID, "null argument");
   if (int rc = check_sizes(*st)) return rc;
-  if (st->stamp == 0 || c->step != st->stamp)
+  layer = st->stamp != 0 && c->step == st->stamp ? c->step_layer : -1;
+  ordered = !c->captured_append;
+  for (const auto& m : c->captured_maps)
+    if (m.first == st->stamp) {
+      layer = m.second;
+      ordered = false;
+    }
+  if (layer < 0)
     return fail(BSATTN_ERR_INVALID, "the cache was not mapped for this step, or has changed since: call bsattn_step_map");
-  if (st->n_seqs < 1 || st->n_seqs > std::min(kMaxBatch, c->d.max_seqs) || c->step_layer >= st->n_caches)
+  if (st->n_seqs < 1 || st->n_seqs > std::min(kMaxBatch, c->d.max_seqs) || layer >= st->n_caches)
     return fail(BSATTN_ERR_INVALID, "the step has changed since its map");
   for (int i = 0; i < st->n_seqs; ++i)
     if (st->ids[i] < 0 || st->ids[i] >= c->d.max_seqs) return fail(BSATTN_ERR_INVALID, "the step has changed since its map");
@@ -52,7 +61,7 @@ int check_tree(const bsattn_step* st) {
   return BSATTN_OK;
 }
 
-StepRows step_rows(const bsattn_cache* c, const bsattn_step& st) {
+StepRows step_rows(const bsattn_cache* c, const bsattn_step& st, int layer) {
   StepRows sr{};
   sr.n = st.n_seqs;
   sr.rows = st.rows;
@@ -60,8 +69,8 @@ StepRows step_rows(const bsattn_cache* c, const bsattn_step& st) {
   sr.pages = c->num_pages;
   sr.starts = st.starts;
   sr.taken = st.taken;
-  sr.slots = st.slots + (size_t)c->step_layer * st.rows;
-  sr.ends = st.ends + (size_t)c->step_layer * st.n_seqs;
+  sr.slots = st.slots + (size_t)layer * st.rows;
+  sr.ends = st.ends + (size_t)layer * st.n_seqs;
   std::copy(st.ids, st.ids + st.n_seqs, sr.ids);
   return sr;
 }
@@ -136,11 +145,15 @@ int bsattn_step_map(bsattn_cache* const* caches, bsattn_step* st, const int32_t*
     const Geometry& g = caches[l]->geo;
     sm.cache[l] = StepCache{g.meta, g.bt_off, g.cap_off, g.mbps, g.tb};
   }
+  const bool captured = capturing(s);
+  if (captured)  // (nothing below throws)
+    for (int l = 0; l < st->n_caches; ++l) caches[l]->captured_maps.reserve(caches[l]->captured_maps.size() + 1);
   Timing tm[kProfKinds];
   Timing* prof = prof_slots(caches[0], s, tm);
   const hipError_t e = launch_step_map(sm, s, prof);
   prof_collect(caches[0], prof);
   if (e != hipSuccess) return hip_fail(e, "step map launch");
+  const uint64_t before = st->stamp;  // (what was captured under it is this step's no more)
   st->n_seqs = n_seqs;
   std::copy(seqs.begin(), seqs.end(), st->ids);
   st->stamp = ++g_steps;
@@ -148,6 +161,11 @@ int bsattn_step_map(bsattn_cache* const* caches, bsattn_step* st, const int32_t*
     caches[l]->step = st->stamp;
     caches[l]->step_layer = l;
     caches[l]->step_state = bsattn_cache::kMapped;
+    if (!captured) continue;
+    auto& maps = caches[l]->captured_maps;
+    auto old = std::find_if(maps.begin(), maps.end(), [&](const auto& m) { return m.first == before; });
+    if (old != maps.end()) *old = {st->stamp, l};
+    else maps.emplace_back(st->stamp, l);
   }
   return BSATTN_OK;
 } catch (...) {
@@ -156,7 +174,9 @@ int bsattn_step_map(bsattn_cache* const* caches, bsattn_step* st, const int32_t*
 
 int bsattn_append_packed(bsattn_cache* c, const bsattn_step* st, const void* k, const int64_t* k_strides,
                          const void* v, const int64_t* v_strides, void* stream) try {
-  if (int rc = check_step(c, st)) return rc;
+  int layer;
+  bool ordered;
+  if (int rc = check_step(c, st, layer, ordered)) return rc;
   int64_t ks[2], vs[2];
   if (int rc = packed_strides("k", k, k_strides, c->geo.hkv, ks)) return rc;
   if (int rc = packed_strides("v", v, v_strides, c->geo.hkv, vs)) return rc;
@@ -166,11 +186,12 @@ int bsattn_append_packed(bsattn_cache* c, const bsattn_step* st, const void* k, 
   if (int rc = send_unsent(c, s)) return rc;
   Timing tm[kProfKinds];
   Timing* prof = prof_slots(c, s, tm);
-  const hipError_t e = launch_append_packed(c->geo, step_rows(c, *st), k, ks[0], ks[1], v, vs[0], vs[1], s, prof);
+  const hipError_t e = launch_append_packed(c->geo, step_rows(c, *st, layer), k, ks[0], ks[1], v, vs[0], vs[1], s, prof);
   prof_collect(c, prof);
   if (e != hipSuccess) return hip_fail(e, "packed append launch");
   c->stale = true;
   c->step_state = bsattn_cache::kAppended;
+  if (capturing(s)) c->captured_append = true;
   return BSATTN_OK;
 } catch (...) {
   return on_exception();
@@ -178,9 +199,11 @@ int bsattn_append_packed(bsattn_cache* c, const bsattn_step* st, const void* k, 
 
 int bsattn_attend_tree(bsattn_cache* c, const bsattn_step* st, const void* q, const int64_t* q_strides, int32_t window,
                        const float* sinks, float scale, void* out, void* stream) try {
-  if (int rc = check_step(c, st)) return rc;
+  int layer;
+  bool ordered;
+  if (int rc = check_step(c, st, layer, ordered)) return rc;
   if (int rc = check_tree(st)) return rc;
-  if (c->step_state != bsattn_cache::kAppended)
+  if (ordered && c->step_state != bsattn_cache::kAppended)
     return fail(BSATTN_ERR_INVALID, c->step_state == bsattn_cache::kKept
                                         ? "the step's tokens have moved (bsattn_keep)"
                                         : "the step's tokens are not in the cache: call bsattn_append_packed");
@@ -234,9 +257,11 @@ int bsattn_attend_tree(bsattn_cache* c, const bsattn_step* st, const void* q, co
 
 int bsattn_keep(bsattn_cache* c, const bsattn_step* st, const int32_t* kept, int32_t width, const int32_t* n_kept,
                 void* stream) try {
-  if (int rc = check_step(c, st)) return rc;
+  int layer;
+  bool ordered;
+  if (int rc = check_step(c, st, layer, ordered)) return rc;
   if (int rc = check_tree(st)) return rc;
-  if (c->step_state == bsattn_cache::kMapped)
+  if (ordered && c->step_state == bsattn_cache::kMapped)
     return fail(BSATTN_ERR_INVALID, "the step's tokens are not in the cache: call bsattn_append_packed");
   if (!kept || !n_kept) return fail(BSATTN_ERR_INVALID, "null argument");
   if (width < 1) return fail(BSATTN_ERR_INVALID, "width must be >= 1 (got %d)", width);
@@ -246,7 +271,7 @@ int bsattn_keep(bsattn_cache* c, const bsattn_step* st, const int32_t* kept, int
   if (int rc = send_unsent(c, s)) return rc;
   Timing tm[kProfKinds];
   Timing* prof = prof_slots(c, s, tm);
-  const hipError_t e = launch_keep(c->geo, step_rows(c, *st), kept, width, n_kept, s, prof);
+  const hipError_t e = launch_keep(c->geo, step_rows(c, *st, layer), kept, width, n_kept, s, prof);
   prof_collect(c, prof);
   if (e != hipSuccess) return hip_fail(e, "keep launch");
   c->stale = true;

@@ -281,6 +281,60 @@ static void failures() {
   bsattn_cache_destroy(a);
 }
 
+// what was captured replays unseen: its step is taken at any time, others' rules stay
+static void captures() {
+  bsattn_cache *a = cache(2, 8, 40), *b = cache(2, 8, 40);
+  CHECK(bsattn_reserve(a, nullptr, 2, 32, nullptr) == BSATTN_OK && bsattn_reserve(b, nullptr, 2, 32, nullptr) == BSATTN_OK);
+  Arrays s(2, 16, 8), t(1, 16, 8), u(2, 16, 8);
+  bsattn_cache *both[] = {a, b}, *swapped[] = {b, a};
+  const int32_t counts[2] = {3, 5}, kept[2] = {0, 0}, one[2] = {1, 1};
+  auto map = [&](bsattn_cache** l, Arrays& st) { return bsattn_step_map(l, &st.st, counts, nullptr, nullptr, 2, nullptr); };
+  auto append = [&](bsattn_cache* c, Arrays& st) { return bsattn_append_packed(c, &st.st, x, nullptr, x, nullptr, nullptr); };
+  auto attend = [&](bsattn_cache* c, Arrays& st) {
+    return bsattn_attend_tree(c, &st.st, x, nullptr, 0, nullptr, 1.f, x, nullptr);
+  };
+  auto keep = [&](bsattn_cache* c, Arrays& st) { return bsattn_keep(c, &st.st, kept, 1, one, nullptr); };
+  // a captured map: the host's appends do not end its step, nor do other steps' maps
+  stub::capture = hipStreamCaptureStatusActive;
+  CHECK(map(both, s) == BSATTN_OK && map(swapped, u) == BSATTN_OK);
+  stub::capture = hipStreamCaptureStatusNone;
+  CHECK(bsattn_append(a, x, x, nullptr, 2, 1, nullptr) == BSATTN_OK && bsattn_append(b, x, x, nullptr, 2, 1, nullptr) == BSATTN_OK);
+  CHECK(keep(b, s) == BSATTN_OK && stub::last_rows.slots == s.slots.data() + 16 && attend(b, s) == BSATTN_OK);
+  CHECK(append(b, u) == BSATTN_OK && stub::last_rows.slots == u.slots.data() && append(a, s) == BSATTN_OK);
+  CHECK(stub::last_rows.slots == s.slots.data());
+  CHECK(bsattn_sync(a, nullptr) == BSATTN_OK && bsattn_sync(b, nullptr) == BSATTN_OK);
+  CHECK(bsattn_reset(a, nullptr, 2, nullptr) == BSATTN_OK && bsattn_append(a, x, x, nullptr, 2, 40, nullptr) == BSATTN_OK &&
+        bsattn_reserve(a, nullptr, 2, 32, nullptr) == BSATTN_OK);
+  // captured again: the earlier one's place, not one more
+  CHECK(bsattn_reset(b, nullptr, 2, nullptr) == BSATTN_OK && bsattn_append(b, x, x, nullptr, 2, 40, nullptr) == BSATTN_OK &&
+        bsattn_reserve(b, nullptr, 2, 32, nullptr) == BSATTN_OK);
+  stub::capture = hipStreamCaptureStatusActive;
+  const uint64_t before = s.st.stamp;
+  CHECK(map(swapped, s) == BSATTN_OK && s.st.stamp != before && append(a, s) == BSATTN_OK);
+  CHECK(stub::last_rows.slots == s.slots.data() + 16);
+  stub::capture = hipStreamCaptureStatusNone;
+  s.st.stamp = before;
+  refused(append(a, s), BSATTN_ERR_INVALID, "not mapped");
+  CHECK(bsattn_sync(a, nullptr) == BSATTN_OK);
+  bsattn_cache_destroy(a);
+  a = both[0] = cache(2, 8, 40);
+  CHECK(bsattn_reserve(a, nullptr, 2, 32, nullptr) == BSATTN_OK);
+  // a step mapped eagerly keeps its rules
+  CHECK(map(both, t) == BSATTN_OK);
+  refused(attend(a, t), BSATTN_ERR_INVALID, "bsattn_append_packed");
+  refused(attend(b, t), BSATTN_ERR_INVALID, "not mapped");
+  // until its append is captured
+  stub::capture = hipStreamCaptureStatusActive;
+  CHECK(append(a, t) == BSATTN_OK && attend(a, t) == BSATTN_OK);
+  stub::capture = hipStreamCaptureStatusNone;
+  CHECK(bsattn_sync(a, nullptr) == BSATTN_OK && map(both, t) == BSATTN_OK);
+  CHECK(keep(a, t) == BSATTN_OK && attend(a, t) == BSATTN_OK && bsattn_sync(a, nullptr) == BSATTN_OK);
+  CHECK(bsattn_append(a, x, x, nullptr, 2, 1, nullptr) == BSATTN_OK);
+  refused(keep(a, t), BSATTN_ERR_INVALID, "has changed since");
+  bsattn_cache_destroy(a);
+  bsattn_cache_destroy(b);
+}
+
 // the workspace: none for short requests, the cache's own for few partials, the
 // streams' for more (with the event that lets the next user in), one of the
 // cache's for captures, and one part a request where there is none
@@ -329,6 +383,7 @@ static void workspaces() {
 int main() {
   refusals();
   failures();
+  captures();
   workspaces();
   std::puts("ok");
   return 0;

@@ -143,6 +143,72 @@ def test_captured_rounds(gpu, dtype, bits, N):
         assert _same(_state(a, range(B)), _state(b, range(B)))
 
 
+@pytest.mark.parametrize("what", ["append", "map"])
+def test_captured_parts_of_rounds(gpu, what):
+    """The append and attention captured, with or without the map, and the rest of each round eager, host calls between
+    the rounds: states of a cache that was given the kept tokens."""
+    import bsattn
+    import torch
+    log(f"[captured parts] {what}")
+    B, N = 2, 9
+    c, ref = (_cache([600] * B, 8, 2, 32, "bf16") for _ in range(2))
+    for x in (c, ref):
+        _fill(gpu, x, [50, 333], 3)
+    c.reserve(64)
+    step = bsattn.Step([c], rows=B * N, maxTokens=N)
+    counts, kept, many = _ints(gpu, [N, N]), _ints(gpu, [[0, 2, 5]] * B), _ints(gpu, [0, 0])
+    q, k, v = _rows(gpu, c, 1, B * N, fused=False)
+    out = torch.zeros_like(q)
+
+    def first():
+        c.appendPacked(k, v, step)
+        c.attendTree(q, step, SCALE, out=out)
+
+    step.map(counts)
+    first()
+    c.keep(step, kept, many)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    if what == "append":
+        step.map(counts)
+    with torch.cuda.graph(g):
+        if what == "map":
+            step.map(counts)
+        first()
+    for turn in range(6):
+        n = [(3 * turn + i) % (N + 1) for i in range(B)]
+        counts.copy_(_ints(gpu, n))
+        many.copy_(_ints(gpu, [min(3, x // 2) for x in n]))
+        for x, y in zip((q, k, v), _rows(gpu, c, 20 + turn, B * N, fused=False)):
+            x.copy_(y)
+        c.sync()
+        if turn in (2, 4):  # (the host's calls between the rounds)
+            more = [_randn(gpu, 70 + turn + x, (B, 2, 3, D), "bf16") for x in (0, 1)]
+            for x in (c, ref):
+                x.append(*more)
+                x.trim(1)
+            c.reserve(64)
+        lens = [c.seqLen(b) for b in range(B)]
+        if what == "append":
+            step.map(counts)
+        out.fill_(7)
+        g.replay()
+        c.sync()
+        assert [c.seqLen(b) for b in range(B)] == [x + y for x, y in zip(lens, n)]
+        held = sum(n)
+        if held:
+            _check(out[:held, :, None], _tree_reference(c, q, step, lens, n, None)[:held], "bf16", f"turn {turn}")
+        assert (out[held:] == 7).all()
+        c.keep(step, kept, many)
+        c.sync()
+        for b in range(B):
+            path = [0, 2, 5][:min(3, n[b] // 2)]
+            at = torch.tensor([sum(n[:b]) + x for x in path], dtype=torch.long, device=gpu)
+            _plain_append(ref, k[at], v[at], b)
+            assert c.seqLen(b) == lens[b] + len(path)
+        assert _same(_state(c, range(B)), _state(ref, range(B))), turn
+
+
 def test_two_graphs_of_a_cache(gpu):
     """Two captured attentions of one cache, replayed in turn on a stream, share its workspace: each replay is right."""
     import torch
