@@ -317,8 +317,9 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
   // units of a team, and of the workgroup, in a step.  16-bit caches: four, however
   // many teams there are (256 columns over 8 x 32k bf16 tokens, 1 and 4: 394 and 377
   // us); affine ones one per team, since their units' pieces and entries then stay in
-  // fewer registers (132 columns over 8 x 16k int8 tokens, 1 and 4: 336 and 365 us for
-  // the round, 100 over 4 x 131k int4 ones, 1 and 2: 552 and 566)
+  // fewer registers (132 columns over 8 x 16k int8 tokens, 1 and 4: 280 and 328 us for
+  // the step; 1 and 2, 96 over 4 x 262k int8 487 and 518, 100 over 4 x 131k int4 503
+  // and 508)
   constexpr int UB = KB == 0 && CW > 2 ? CW / 2 : 1, STEP = TW * UB;
   constexpr int F = 8 / CW;  // K, and V, operand fragments of a unit that a wave brings: cw + CW x
   static_assert(4 % STEP == 0, "parts are cut in fours");
