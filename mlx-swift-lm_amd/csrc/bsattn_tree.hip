@@ -300,8 +300,8 @@ struct Raw<4> {
 };
 
 // ---------------------------------------------------------------------------
-// CW waves hold 16 CT columns each and take the same units; TW such teams take
-// different ones, a unit each per step.  A unit passes through LDS, as 16-bit
+// CW waves hold up to CT column tiles each and take the same units; TW such teams
+// take different ones, UB each per step.  A unit passes through LDS, as 16-bit
 // operands: each wave of the team brings its share of the fragments, loaded a
 // step before.  So K and V are read, and affine codes converted, once for all of
 // the columns (each wave on its own with its own loads: 64 columns 208, 256 485 us

@@ -423,9 +423,21 @@ def _values(gpu, kind, shape, seed):
 @pytest.mark.parametrize("N", [4, 8, 16, 40])
 def test_value_ranges(gpu, kind, N):
     """bf16 values that fp16 does not hold, or holds in part: columns of every width (16 heads of 2)."""
-    import torch
     log(f"[values] {kind} N={N}")
-    T, Hq, Hkv = 700, 16, 2
+    _check_values(gpu, kind, N, 700, 16, 2)
+
+
+@pytest.mark.parametrize("kind", ["dims", "some huge", "zeros", "tokens"])
+@pytest.mark.parametrize("N", [16, 32])
+def test_value_ranges_of_long_sequences(gpu, kind, N):
+    """The same where workgroups have many units (64 and 128 columns in waves of two column tiles)."""
+    log(f"[values, long] {kind} N={N}")
+    _check_values(gpu, kind, N, 20000, 32, 8)
+
+
+def _check_values(gpu, kind, N, T, Hq, Hkv):
+    import torch
+    G = Hq // Hkv
     c = _cache([T], Hq, Hkv, 64, "bf16", spare=64)
     c.append(_randn(gpu, 3, (1, Hkv, T, D), "bf16"), _values(gpu, kind, (1, Hkv, T, D), 4))
     step = _step(gpu, [c], [N], [_tree(3, N)])
@@ -444,9 +456,9 @@ def test_value_ranges(gpu, kind, N):
     for h in range(Hkv):
         for j, path in enumerate(paths):
             on = list(range(T)) + [T + a for a in path]
-            p = torch.softmax(q[j, 8 * h:8 * h + 8].double() @ keys[h][on].t() * SCALE, -1)
-            reach[j, 8 * h:8 * h + 8] = p @ vals[h][on].abs()
-    top = vals.abs().amax(1).repeat_interleave(8, 0)[None]  # [1, Hq, D]
+            p = torch.softmax(q[j, G * h:G * h + G].double() @ keys[h][on].t() * SCALE, -1)
+            reach[j, G * h:G * h + G] = p @ vals[h][on].abs()
+    top = vals.abs().amax(1).repeat_interleave(G, 0)[None]  # [1, Hq, D]
     tol = HALF_STEP["bf16"] * want.abs() + 2.0 ** -11 * reach + torch.where(top >= 2.0 ** -10, 2.0 ** -25, 0.0)
     worst = ((out - want).abs() / tol.clamp_min(1e-300)).max().item()
     assert worst <= 1, worst
