@@ -10,17 +10,21 @@
 //   O^T[dim][col]  += V^T[dim][token] . P^T  (A = V^T,    B = P^T)
 // with MFMA 16x16x32.  A lane (column n, group g) holds column n's share of tokens
 // 8g .. 8g + 7 in both, so P goes from one to the other without a shuffle.  P
-// enters as two 16-bit parts, for 16 (bf16) or 22 (fp16) bits.  Affine codes enter
+// enters as two 16-bit parts, for 16 (bf16) or 22 (fp16) bits, whatever the columns
+// (bf16 values as fp16 where that holds their size, and P as one fp16 number, took
+// half of those products, 361 for 414 us with 256 columns over 8 x 32k tokens; but
+// weights had 11 bits, and a value of 2^-20 with all the weight, beside an unattended
+// one of 1, was off by several of bf16's half steps).  Affine codes enter
 // as 1024 + c (K, fp16) and c (V, bf16), exactly; scales and biases act on scores
 // and weights.
 //
 // What bounds it: 16 columns and fewer the reads; from 64 on the issue of a SIMD,
 // which products (16 cycles each) and VALU work share nearly one after the other.
-// A wave's unit of 32 tokens by 32 columns is 34 products for bf16 (V as fp16, see
-// CONV), 52 for fp16, 48 for codes, beside 16 exponentials and 50 to 210 other VALU
-// instructions.  Whole launches: 64 columns over 8 x 32k bf16 tokens 183 us (1074
-// MB: 5.9 TB/s, a plain streaming read 154 us), 256 350 (786 TFLOP/s; 63% of a
-// large product's rate), 100 over 4 x 131k int4 499, 96 over 4 x 262k int8 466.
+// A wave's unit of 32 tokens by 32 columns is 52 products, 48 for codes, beside 16
+// exponentials and 50 to 210 other VALU instructions.  Passes: 64 columns over 8 x
+// 32k bf16 tokens 200 us (1074 MB: 5.4 TB/s, a plain streaming read 154 us), 256 414
+// (664 TFLOP/s; 51% of a large product's rate), 100 over 4 x 131k int4 499, 96 over
+// 4 x 262k int8 469.
 #include <hip/hip_ext.h>
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -40,8 +44,6 @@ constexpr float kTreeSlack = 6.0f;
 constexpr float kTreeTop = 14.0f;
 
 // What a request brings to a launch, and the units of its part
-typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-
 struct TreeRange {
   int T, N, P, lo, u0, units, cu;
   int lg;  // log2 of the heads of a group
@@ -323,12 +325,8 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
   constexpr int UB = KB == 0 && CW > 2 ? CW / 2 : 1, STEP = TW * UB;
   constexpr int F = 8 / CW;  // K, and V, operand fragments of a unit that a wave brings: cw + CW x
   static_assert(4 % STEP == 0, "parts are cut in fours");
-  // P's type.  Weights times scales need bf16's range, and codes are exact in it.
-  // bf16 caches: V is brought as fp16 where that takes it as it is, fragment by
-  // fragment, and P then enters once, rounded to fp16's 11 bits (a sixteenth of the
-  // output's half step): half of PV's products and most of the work on P
-  constexpr bool CONV = KB == 0 && DT == 1 && CW >= 2;
-  constexpr int PT = KB ? 1 : CONV ? 0 : DT;
+  // P's type.  Weights times scales need bf16's range, and codes are exact in it
+  constexpr int PT = KB ? 1 : DT;
   // fp16 weights are lifted to at most 2^14, so that small ones keep their bits
   constexpr float kLift = PT == 0 ? kTreeTop - kTreeSlack : 0.0f;
   constexpr int COLS = 16 * CT * CW;
@@ -340,7 +338,6 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
   // (affine) the tokens' scales and biases: K's in 32 bits, times the scores' scale
   __shared__ f32x4 s_kent[KB ? SLOTS * STEP : 1][KB ? 32 : 1];
   __shared__ uint2 s_vent[KB ? SLOTS * STEP : 1][KB ? 32 : 1];
-  __shared__ uint8_t s_raw[SLOTS * STEP][8];  // (CONV) per wave of a team: which dim tiles of V are bf16
   __shared__ uint64_t s_seen[kMaxNodes];
   __shared__ int s_from[kMaxNodes];
   __shared__ uint2 s_odd[TW][8];  // units with values that are infinite or no numbers, and their tokens
@@ -459,7 +456,7 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
         const int f = cw + CW * x;
         if constexpr (KB == 0) {
           to[f * 64] = rk[u][x];
-          if constexpr (!CONV) to[(8 + f) * 64] = rv[u][x];
+          to[(8 + f) * 64] = rv[u][x];
         } else if constexpr (KB == 4) {
           to[f * 64] = nib_to_f16_dec(rk[u][x], code_base);
           to[(8 + f) * 64] = nib_to_bf16(rv[u][x]);
@@ -467,32 +464,6 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
           to[f * 64] = byte_to_f16(rk[u][x].x, rk[u][x].y);
           to[(8 + f) * 64] = byte_to_bf16(rv[u][x].x, rv[u][x].y);
         }
-      }
-      if constexpr (CONV) {
-        // fp16 takes a tile whose values are below 65536, with one at 2^-10 or more in
-        // each dim's eight tokens (values below 2^-14 are off by up to 2^-25 then, a
-        // 2^-15th of it at most); units with tokens that are not seen stay as they are
-        uint32_t raw = 0;
-#pragma unroll
-        for (int x = 0; x < F; ++x) {
-          const int f = cw + CW * x;
-          u16x2 big = {0, 0};
-          u32x4 v;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t w = rv[u][x][j], mag = w & 0x7FFF7FFFu;
-            big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2, mag));
-            v[j] = cvt_pk<0>(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
-          }
-          const uint32_t top = max((uint32_t)big[0], (uint32_t)big[1]);
-          const bool ok = place < pt.full && __all(top - 0x3A80u < 0x4780u - 0x3A80u);
-          if (!ok) {
-            raw |= 1u << f;
-            v = rv[u][x];
-          }
-          to[(8 + f) * 64] = v;
-        }
-        if (lane == 0) s_raw[at][cw] = (uint8_t)raw;
       }
       if (place >= pt.full) {
         // Some columns do not see all of the unit.  Values of tokens that none sees
@@ -684,11 +655,7 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
     }
 #pragma unroll
     for (int ct = 0; ct < C; ++ct) {
-      if constexpr (CONV) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) hi[ct][0][j] = cvt_pk<0>(sv[ct][2 * j], sv[ct][2 * j + 1]);
-        l[ct] = mfma16x16x32<0>(ones, hi[ct][0], l[ct]);
-      } else if constexpr (KB == 0) {
+      if constexpr (KB == 0) {
         tree_split<PT>(sv[ct], one, hi[ct][0], lo[ct][0]);
         l[ct] = mfma16x16x32<PT>(ones, hi[ct][0], l[ct]);
         l[ct] = mfma16x16x32<PT>(ones, lo[ct][0], l[ct]);
@@ -696,42 +663,6 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
         tree_split<1>(w0[ct], one, hi[ct][0], lo[ct][0]);
         tree_split<1>(w1[ct], one, hi[ct][1], lo[ct][1]);
       }
-    }
-    if constexpr (CONV) {
-      uint32_t raw = 0;
-      const uint2 each = *(const uint2*)s_raw[at];
-#pragma unroll
-      for (int x = 0; x < CW; ++x) raw |= (x < 4 ? each.x : each.y) >> (8 * (x & 3)) & 0xFFu;
-      raw = (uint32_t)uniform((int)raw);
-      if (raw == 0) {
-#pragma unroll
-        for (int dt = 0; dt < 8; ++dt) {
-          const u32x4 v = in[(8 + dt) * 64];
-#pragma unroll
-          for (int ct = 0; ct < C; ++ct) o[ct][dt] = mfma16x16x32<0>(v, hi[ct][0], o[ct][dt]);
-        }
-      }
-      // (a branch of its own: as the other one's else the sums would change registers
-      // in every unit)
-      asm volatile("" : "+s"(raw));
-      if (raw != 0) {
-        // (the unit's other tiles back to bf16, exactly where they are not below 2^-14)
-        u32x4 bl[C];
-#pragma unroll
-        for (int ct = 0; ct < C; ++ct) tree_split<1>(sv[ct], one, hi[ct][0], bl[ct]);
-#pragma unroll
-        for (int dt = 0; dt < 8; ++dt) {
-          u32x4 v = in[(8 + dt) * 64];
-          if (!(raw >> dt & 1))
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = cvt_pk<1>(lo_f(v[j]), hi_f(v[j]));
-#pragma unroll
-          for (int ct = 0; ct < C; ++ct) o[ct][dt] = mfma16x16x32<1>(v, hi[ct][0], o[ct][dt]);
-#pragma unroll
-          for (int ct = 0; ct < C; ++ct) o[ct][dt] = mfma16x16x32<1>(v, bl[ct], o[ct][dt]);
-        }
-      }
-      return;
     }
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) {
