@@ -153,7 +153,7 @@ int bsattn_step_map(bsattn_cache* const* caches, bsattn_step* st, const int32_t*
   const hipError_t e = launch_step_map(sm, s, prof);
   prof_collect(caches[0], prof);
   if (e != hipSuccess) return hip_fail(e, "step map launch");
-  const uint64_t before = st->stamp;  // (what was captured under it is this step's no more)
+  const uint64_t before = st->stamp;  // (what was captured under it goes by the new one)
   st->n_seqs = n_seqs;
   std::copy(seqs.begin(), seqs.end(), st->ids);
   st->stamp = ++g_steps;
@@ -161,11 +161,11 @@ int bsattn_step_map(bsattn_cache* const* caches, bsattn_step* st, const int32_t*
     caches[l]->step = st->stamp;
     caches[l]->step_layer = l;
     caches[l]->step_state = bsattn_cache::kMapped;
-    if (!captured) continue;
+    // (a step that was captured stays so: its graph may replay after any map)
     auto& maps = caches[l]->captured_maps;
     auto old = std::find_if(maps.begin(), maps.end(), [&](const auto& m) { return m.first == before; });
     if (old != maps.end()) *old = {st->stamp, l};
-    else maps.emplace_back(st->stamp, l);
+    else if (captured) maps.emplace_back(st->stamp, l);
   }
   return BSATTN_OK;
 } catch (...) {

@@ -1,0 +1,69 @@
+// step_rules.cpp -- which calls with a step are taken and which are refused,
+// around captures and around host calls for other sequences.  The launches'
+// stand-ins and the helpers are steps.cpp's.
+#include "../../mlx-swift-lm_amd/csrc/bsattn_host.h"
+
+#define main steps_main
+#include "steps.cpp"
+#undef main
+
+struct Rig {
+  bsattn_cache *a, *b;
+  bsattn_cache* both[2];
+  const int32_t counts[3] = {3, 5, 2}, kept[3] = {0, 0, 0}, one[3] = {1, 1, 1};
+  explicit Rig(int seqs = 2) : a(cache(seqs, 16, 40)), b(cache(seqs, 16, 40)), both{a, b} { reserve(); }
+  ~Rig() {
+    bsattn_cache_destroy(a);
+    bsattn_cache_destroy(b);
+  }
+  void sync() {
+    for (bsattn_cache* c : both) CHECK(bsattn_sync(c, nullptr) == BSATTN_OK);
+  }
+  void reserve() {
+    for (bsattn_cache* c : both) CHECK(bsattn_reserve(c, nullptr, c->d.max_seqs, 32, nullptr) == BSATTN_OK);
+  }
+  // a host call for every sequence
+  void more() {
+    sync();
+    for (bsattn_cache* c : both) CHECK(bsattn_append(c, x, x, nullptr, c->d.max_seqs, 1, nullptr) == BSATTN_OK);
+    reserve();
+  }
+  int map(Arrays& s, int n = 2, const int32_t* ids = nullptr, bool swap = false) {
+    bsattn_cache* swapped[2] = {b, a};
+    return bsattn_step_map(swap ? swapped : both, &s.st, counts, nullptr, ids, n, nullptr);
+  }
+  int append(bsattn_cache* c, Arrays& s) { return bsattn_append_packed(c, &s.st, x, nullptr, x, nullptr, nullptr); }
+  int attend(bsattn_cache* c, Arrays& s) {
+    return bsattn_attend_tree(c, &s.st, x, nullptr, 0, nullptr, 1.f, x, nullptr);
+  }
+  int keep(bsattn_cache* c, Arrays& s) { return bsattn_keep(c, &s.st, kept, 1, one, nullptr); }
+  template <typename F>
+  void captured(F calls) {
+    stub::capture = hipStreamCaptureStatusActive;
+    calls();
+    stub::capture = hipStreamCaptureStatusNone;
+  }
+};
+
+// an eager map of a step whose map was captured: the graph may still replay
+static void eager_map_of_a_captured_step() {
+  Rig r;
+  Arrays s(2, 16, 8);
+  r.captured([&] { CHECK(r.map(s) == BSATTN_OK); });
+  CHECK(r.map(s) == BSATTN_OK);
+  r.more();
+  // (here the graph replays)
+  for (bsattn_cache* c : r.both) CHECK(r.append(c, s) == BSATTN_OK && r.attend(c, s) == BSATTN_OK && r.keep(c, s) == BSATTN_OK);
+  for (int turn = 0; turn < 5; ++turn) {
+    r.captured([&] { CHECK(r.map(s) == BSATTN_OK); });
+    CHECK(r.map(s) == BSATTN_OK);
+    r.more();
+    CHECK(r.keep(r.b, s) == BSATTN_OK && stub::last_rows.slots == s.slots.data() + 16);
+  }
+}
+
+int main() {
+  eager_map_of_a_captured_step();
+  std::puts("ok");
+  return 0;
+}
