@@ -108,10 +108,14 @@ struct bsattn_cache {
   uint64_t step = 0;
   int32_t step_layer = 0;
   enum { kMapped, kAppended, kKept } step_state = kMapped;  // the last call with it
-  // maps that were captured, with the cache's place in each, and whether an append
-  // was: the host does not see their replays
-  std::vector<std::pair<uint64_t, int32_t>> captured_maps;
-  bool captured_append = false;
+  // steps of which the map or this cache's append was captured: the host does not
+  // see their replays
+  struct CapturedStep {
+    uint64_t stamp;     // of the step's last map
+    int32_t layer;      // the cache's place in it
+    bool map, append;   // which of them
+  };
+  std::vector<CapturedStep> captured_steps;
   // opt-in per-kernel timing (bsattn_profile_*)
   bool profiling = false;
   std::vector<hipEvent_t> event_pool;

@@ -31,20 +31,26 @@ int check_sizes(const bsattn_step& st) {
   return BSATTN_OK;
 }
 
+using CapturedStep = bsattn_cache::CapturedStep;
+
+// what was captured of a step (null: nothing)
+CapturedStep* captured_step(bsattn_cache* c, uint64_t stamp) {
+  for (CapturedStep& x : c->captured_steps)
+    if (x.stamp == stamp) return &x;
+  return nullptr;
+}
+
 // the step's last map is the last that the cache was mapped for, and the
 // cache's sequences are as they were then; or it was captured, and holds at its
 // replays.  layer: the cache's place among the step's; ordered: whether the host
 // knows the last call with it
-int check_step(const bsattn_cache* c, const bsattn_step* st, int& layer, bool& ordered) {
+int check_step(bsattn_cache* c, const bsattn_step* st, int& layer, bool& ordered) {
   if (!c || !st) return fail(BSATTN_ERR_INVALID, "null argument");
   if (int rc = check_sizes(*st)) return rc;
   layer = st->stamp != 0 && c->step == st->stamp ? c->step_layer : -1;
-  ordered = !c->captured_append;
-  for (const auto& m : c->captured_maps)
-    if (m.first == st->stamp) {
-      layer = m.second;
-      ordered = false;
-    }
+  const CapturedStep* was = captured_step(c, st->stamp);
+  if (was && was->map) layer = was->layer;
+  ordered = !was;
   if (layer < 0)
     return fail(BSATTN_ERR_INVALID, "the cache was not mapped for this step, or has changed since: call bsattn_step_map");
   if (st->n_seqs < 1 || st->n_seqs > std::min(kMaxBatch, c->d.max_seqs) || layer >= st->n_caches)
@@ -147,7 +153,7 @@ int bsattn_step_map(bsattn_cache* const* caches, bsattn_step* st, const int32_t*
   }
   const bool captured = capturing(s);
   if (captured)  // (nothing below throws)
-    for (int l = 0; l < st->n_caches; ++l) caches[l]->captured_maps.reserve(caches[l]->captured_maps.size() + 1);
+    for (int l = 0; l < st->n_caches; ++l) caches[l]->captured_steps.reserve(caches[l]->captured_steps.size() + 1);
   Timing tm[kProfKinds];
   Timing* prof = prof_slots(caches[0], s, tm);
   const hipError_t e = launch_step_map(sm, s, prof);
@@ -162,10 +168,8 @@ int bsattn_step_map(bsattn_cache* const* caches, bsattn_step* st, const int32_t*
     caches[l]->step_layer = l;
     caches[l]->step_state = bsattn_cache::kMapped;
     // (a step that was captured stays so: its graph may replay after any map)
-    auto& maps = caches[l]->captured_maps;
-    auto old = std::find_if(maps.begin(), maps.end(), [&](const auto& m) { return m.first == before; });
-    if (old != maps.end()) *old = {st->stamp, l};
-    else if (captured) maps.emplace_back(st->stamp, l);
+    if (CapturedStep* was = captured_step(caches[l], before)) *was = {st->stamp, l, was->map || captured, was->append};
+    else if (captured) caches[l]->captured_steps.push_back({st->stamp, l, true, false});
   }
   return BSATTN_OK;
 } catch (...) {
@@ -184,6 +188,8 @@ int bsattn_append_packed(bsattn_cache* c, const bsattn_step* st, const void* k, 
   if (!dg.ok) return fail(BSATTN_ERR_HIP, "hipSetDevice(%d) failed", c->d.device);
   hipStream_t s = (hipStream_t)stream;
   if (int rc = send_unsent(c, s)) return rc;
+  const bool captured = capturing(s);
+  if (captured) c->captured_steps.reserve(c->captured_steps.size() + 1);  // (nothing below throws)
   Timing tm[kProfKinds];
   Timing* prof = prof_slots(c, s, tm);
   const hipError_t e = launch_append_packed(c->geo, step_rows(c, *st, layer), k, ks[0], ks[1], v, vs[0], vs[1], s, prof);
@@ -191,7 +197,10 @@ int bsattn_append_packed(bsattn_cache* c, const bsattn_step* st, const void* k, 
   if (e != hipSuccess) return hip_fail(e, "packed append launch");
   c->stale = true;
   c->step_state = bsattn_cache::kAppended;
-  if (capturing(s)) c->captured_append = true;
+  if (captured) {
+    if (CapturedStep* was = captured_step(c, st->stamp)) was->append = true;
+    else c->captured_steps.push_back({st->stamp, layer, false, true});
+  }
   return BSATTN_OK;
 } catch (...) {
   return on_exception();

@@ -62,8 +62,33 @@ static void eager_map_of_a_captured_step() {
   }
 }
 
+// a captured append takes the order checks from its own step only
+static void captured_append_of_another_step() {
+  Rig r;
+  Arrays s(2, 16, 8), t(2, 16, 8);
+  CHECK(r.map(s) == BSATTN_OK);
+  r.captured([&] { CHECK(r.append(r.a, s) == BSATTN_OK); });
+  CHECK(r.keep(r.a, s) == BSATTN_OK && r.append(r.b, s) == BSATTN_OK && r.keep(r.b, s) == BSATTN_OK);
+  for (int turn = 0; turn < 2; ++turn) {
+    CHECK(r.map(t) == BSATTN_OK);
+    for (bsattn_cache* c : r.both) {
+      refused(r.attend(c, t), BSATTN_ERR_INVALID, "bsattn_append_packed");
+      refused(r.keep(c, t), BSATTN_ERR_INVALID, "bsattn_append_packed");
+      CHECK(r.append(c, t) == BSATTN_OK && r.attend(c, t) == BSATTN_OK && r.keep(c, t) == BSATTN_OK);
+      refused(r.attend(c, t), BSATTN_ERR_INVALID, "moved");
+    }
+    // its own: taken as it comes after a map, in that cache
+    CHECK(r.map(s) == BSATTN_OK && r.attend(r.a, s) == BSATTN_OK && r.keep(r.a, s) == BSATTN_OK && r.attend(r.a, s) == BSATTN_OK);
+    refused(r.attend(r.b, s), BSATTN_ERR_INVALID, "bsattn_append_packed");
+    CHECK(r.append(r.b, s) == BSATTN_OK && r.keep(r.b, s) == BSATTN_OK);
+    r.more();
+    refused(r.keep(r.a, s), BSATTN_ERR_INVALID, "has changed since");
+  }
+}
+
 int main() {
   eager_map_of_a_captured_step();
+  captured_append_of_another_step();
   std::puts("ok");
   return 0;
 }
