@@ -40,6 +40,12 @@ CapturedStep* captured_step(bsattn_cache* c, uint64_t stamp) {
   return nullptr;
 }
 
+// the last call with the step that the cache is mapped for; a call that is only
+// recorded moves nothing yet
+void step_moves(bsattn_cache* c, const bsattn_step* st, bool captured, decltype(bsattn_cache::step_state) to) {
+  if (!captured && c->step == st->stamp) c->step_state = to;
+}
+
 // the step's last map is the last that the cache was mapped for, and the
 // cache's sequences are as they were then; or it was captured, and holds at its
 // replays.  layer: the cache's place among the step's; ordered: whether the host
@@ -164,9 +170,11 @@ int bsattn_step_map(bsattn_cache* const* caches, bsattn_step* st, const int32_t*
   std::copy(seqs.begin(), seqs.end(), st->ids);
   st->stamp = ++g_steps;
   for (int l = 0; l < st->n_caches; ++l) {
-    caches[l]->step = st->stamp;
-    caches[l]->step_layer = l;
-    caches[l]->step_state = bsattn_cache::kMapped;
+    if (!captured) {  // (recorded: another step that is under way stays so)
+      caches[l]->step = st->stamp;
+      caches[l]->step_layer = l;
+      caches[l]->step_state = bsattn_cache::kMapped;
+    }
     // (a step that was captured stays so: its graph may replay after any map)
     if (CapturedStep* was = captured_step(caches[l], before)) *was = {st->stamp, l, was->map || captured, was->append};
     else if (captured) caches[l]->captured_steps.push_back({st->stamp, l, true, false});
@@ -196,7 +204,7 @@ int bsattn_append_packed(bsattn_cache* c, const bsattn_step* st, const void* k, 
   prof_collect(c, prof);
   if (e != hipSuccess) return hip_fail(e, "packed append launch");
   c->stale = true;
-  c->step_state = bsattn_cache::kAppended;
+  step_moves(c, st, captured, bsattn_cache::kAppended);
   if (captured) {
     if (CapturedStep* was = captured_step(c, st->stamp)) was->append = true;
     else c->captured_steps.push_back({st->stamp, layer, false, true});
@@ -284,7 +292,7 @@ int bsattn_keep(bsattn_cache* c, const bsattn_step* st, const int32_t* kept, int
   prof_collect(c, prof);
   if (e != hipSuccess) return hip_fail(e, "keep launch");
   c->stale = true;
-  c->step_state = bsattn_cache::kKept;
+  step_moves(c, st, capturing(s), bsattn_cache::kKept);
   return BSATTN_OK;
 } catch (...) {
   return on_exception();

@@ -86,9 +86,29 @@ static void captured_append_of_another_step() {
   }
 }
 
+// what is recorded moves nothing: a step that is under way stays where it is
+static void captures_beside_a_step() {
+  Rig r;
+  Arrays s(2, 16, 8), t(2, 16, 8);
+  CHECK(r.map(t) == BSATTN_OK && r.append(r.a, t) == BSATTN_OK);
+  r.captured([&] {
+    CHECK(r.map(s) == BSATTN_OK && r.append(r.a, s) == BSATTN_OK && r.attend(r.a, s) == BSATTN_OK && r.keep(r.a, s) == BSATTN_OK);
+  });
+  CHECK(r.attend(r.a, t) == BSATTN_OK);
+  // nor do calls with another step that was captured
+  CHECK(r.append(r.b, s) == BSATTN_OK);
+  refused(r.attend(r.b, t), BSATTN_ERR_INVALID, "bsattn_append_packed");
+  CHECK(r.append(r.b, t) == BSATTN_OK && r.attend(r.b, t) == BSATTN_OK);
+  // a captured keep
+  r.captured([&] { CHECK(r.keep(r.a, t) == BSATTN_OK); });
+  CHECK(r.attend(r.a, t) == BSATTN_OK && r.keep(r.a, t) == BSATTN_OK);
+  refused(r.attend(r.a, t), BSATTN_ERR_INVALID, "moved");
+}
+
 int main() {
   eager_map_of_a_captured_step();
   captured_append_of_another_step();
+  captures_beside_a_step();
   std::puts("ok");
   return 0;
 }
