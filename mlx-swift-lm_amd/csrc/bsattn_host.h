@@ -16,6 +16,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <memory>
 #include <mutex>
 #include <new>
 #include <stdexcept>
@@ -114,6 +115,12 @@ struct bsattn_cache {
     uint64_t stamp;     // of the step's last map
     int32_t layer;      // the cache's place in it
     bool map, append;   // which of them
+    // requests of the captured map, its rows and the cache's place in it; whether
+    // another captured one was for others, and whether the last map is, or was
+    // captured itself
+    std::shared_ptr<const std::vector<int32_t>> ids;
+    int32_t rows, place;
+    bool several, other, recorded;
   };
   std::vector<CapturedStep> captured_steps;
   // opt-in per-kernel timing (bsattn_profile_*)

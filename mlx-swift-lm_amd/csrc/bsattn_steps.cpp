@@ -50,7 +50,7 @@ void step_moves(bsattn_cache* c, const bsattn_step* st, bool captured, decltype(
 // cache's sequences are as they were then; or it was captured, and holds at its
 // replays.  layer: the cache's place among the step's; ordered: whether the host
 // knows the last call with it
-int check_step(bsattn_cache* c, const bsattn_step* st, int& layer, bool& ordered) {
+int check_step(bsattn_cache* c, const bsattn_step* st, void* stream, int& layer, bool& ordered) {
   if (!c || !st) return fail(BSATTN_ERR_INVALID, "null argument");
   if (int rc = check_sizes(*st)) return rc;
   layer = st->stamp != 0 && c->step == st->stamp ? c->step_layer : -1;
@@ -59,6 +59,10 @@ int check_step(bsattn_cache* c, const bsattn_step* st, int& layer, bool& ordered
   ordered = !was;
   if (layer < 0)
     return fail(BSATTN_ERR_INVALID, "the cache was not mapped for this step, or has changed since: call bsattn_step_map");
+  // (which map ran last, the host's or a replay's, it cannot tell: the arrays are
+  // laid out for that one's requests)
+  if (was && was->map && was->other && !(was->recorded && capturing((hipStream_t)stream)))
+    return fail(BSATTN_ERR_INVALID, "the step's map was captured for other requests: use another step for these");
   if (st->n_seqs < 1 || st->n_seqs > std::min(kMaxBatch, c->d.max_seqs) || layer >= st->n_caches)
     return fail(BSATTN_ERR_INVALID, "the step has changed since its map");
   for (int i = 0; i < st->n_seqs; ++i)
@@ -158,8 +162,11 @@ int bsattn_step_map(bsattn_cache* const* caches, bsattn_step* st, const int32_t*
     sm.cache[l] = StepCache{g.meta, g.bt_off, g.cap_off, g.mbps, g.tb};
   }
   const bool captured = capturing(s);
-  if (captured)  // (nothing below throws)
+  std::shared_ptr<const std::vector<int32_t>> ids;
+  if (captured) {  // (nothing below throws)
+    ids = std::make_shared<const std::vector<int32_t>>(seqs);
     for (int l = 0; l < st->n_caches; ++l) caches[l]->captured_steps.reserve(caches[l]->captured_steps.size() + 1);
+  }
   Timing tm[kProfKinds];
   Timing* prof = prof_slots(caches[0], s, tm);
   const hipError_t e = launch_step_map(sm, s, prof);
@@ -176,8 +183,19 @@ int bsattn_step_map(bsattn_cache* const* caches, bsattn_step* st, const int32_t*
       caches[l]->step_state = bsattn_cache::kMapped;
     }
     // (a step that was captured stays so: its graph may replay after any map)
-    if (CapturedStep* was = captured_step(caches[l], before)) *was = {st->stamp, l, was->map || captured, was->append};
-    else if (captured) caches[l]->captured_steps.push_back({st->stamp, l, true, false});
+    CapturedStep* was = captured_step(caches[l], before);
+    if (!was) {
+      if (captured) caches[l]->captured_steps.push_back({st->stamp, l, true, false, ids, st->rows, l, false, false, true});
+      continue;
+    }
+    const bool other = was->map && (was->place != l || was->rows != st->rows || *was->ids != seqs);
+    if (captured && !was->map) was->ids = ids, was->rows = st->rows, was->place = l;
+    was->stamp = st->stamp;
+    was->layer = l;
+    was->map |= captured;
+    was->several |= captured && other;
+    was->other = other || was->several;
+    was->recorded = captured;
   }
   return BSATTN_OK;
 } catch (...) {
@@ -188,7 +206,7 @@ int bsattn_append_packed(bsattn_cache* c, const bsattn_step* st, const void* k, 
                          const void* v, const int64_t* v_strides, void* stream) try {
   int layer;
   bool ordered;
-  if (int rc = check_step(c, st, layer, ordered)) return rc;
+  if (int rc = check_step(c, st, stream, layer, ordered)) return rc;
   int64_t ks[2], vs[2];
   if (int rc = packed_strides("k", k, k_strides, c->geo.hkv, ks)) return rc;
   if (int rc = packed_strides("v", v, v_strides, c->geo.hkv, vs)) return rc;
@@ -207,7 +225,7 @@ int bsattn_append_packed(bsattn_cache* c, const bsattn_step* st, const void* k, 
   step_moves(c, st, captured, bsattn_cache::kAppended);
   if (captured) {
     if (CapturedStep* was = captured_step(c, st->stamp)) was->append = true;
-    else c->captured_steps.push_back({st->stamp, layer, false, true});
+    else c->captured_steps.push_back({st->stamp, layer, false, true, nullptr, 0, 0, false, false, false});
   }
   return BSATTN_OK;
 } catch (...) {
@@ -218,7 +236,7 @@ int bsattn_attend_tree(bsattn_cache* c, const bsattn_step* st, const void* q, co
                        const float* sinks, float scale, void* out, void* stream) try {
   int layer;
   bool ordered;
-  if (int rc = check_step(c, st, layer, ordered)) return rc;
+  if (int rc = check_step(c, st, stream, layer, ordered)) return rc;
   if (int rc = check_tree(st)) return rc;
   if (ordered && c->step_state != bsattn_cache::kAppended)
     return fail(BSATTN_ERR_INVALID, c->step_state == bsattn_cache::kKept
@@ -276,7 +294,7 @@ int bsattn_keep(bsattn_cache* c, const bsattn_step* st, const int32_t* kept, int
                 void* stream) try {
   int layer;
   bool ordered;
-  if (int rc = check_step(c, st, layer, ordered)) return rc;
+  if (int rc = check_step(c, st, stream, layer, ordered)) return rc;
   if (int rc = check_tree(st)) return rc;
   if (ordered && c->step_state == bsattn_cache::kMapped)
     return fail(BSATTN_ERR_INVALID, "the step's tokens are not in the cache: call bsattn_append_packed");

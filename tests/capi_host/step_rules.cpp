@@ -105,10 +105,47 @@ static void captures_beside_a_step() {
   refused(r.attend(r.a, t), BSATTN_ERR_INVALID, "moved");
 }
 
+// a captured map and eager ones for other requests: the arrays may be either's
+static void other_requests() {
+  Rig r(3);
+  const char* text = "captured for other requests";
+  const int32_t back[2] = {1, 0}, far[2] = {0, 2};
+  Arrays s(2, 16, 8);
+  r.captured([&] { CHECK(r.map(s) == BSATTN_OK); });
+  CHECK(r.append(r.a, s) == BSATTN_OK && r.append(r.b, s) == BSATTN_OK && r.keep(r.a, s) == BSATTN_OK);
+  for (int how = 0; how < 5; ++how) {
+    if (how == 0) CHECK(r.map(s, 1) == BSATTN_OK);
+    if (how == 1) CHECK(r.map(s, 3) == BSATTN_OK);
+    if (how == 2) CHECK(r.map(s, 2, back) == BSATTN_OK);
+    if (how == 3) CHECK(r.map(s, 2, far) == BSATTN_OK);
+    if (how == 4) CHECK(r.map(s, 2, nullptr, true) == BSATTN_OK);
+    // (here the graph may have replayed)
+    for (bsattn_cache* c : r.both)
+      for (int rc : {r.append(c, s), r.attend(c, s), r.keep(c, s)}) refused(rc, BSATTN_ERR_INVALID, text);
+    // nor into a graph of its own, where the map is not
+    r.captured([&] { refused(r.append(r.a, s), BSATTN_ERR_INVALID, text); });
+    // mapped as it was captured
+    CHECK(r.map(s) == BSATTN_OK && r.append(r.b, s) == BSATTN_OK && r.keep(r.a, s) == BSATTN_OK);
+  }
+  // captured for two lists: within each capture they are known
+  r.captured([&] {
+    CHECK(r.map(s, 2, far) == BSATTN_OK && r.append(r.a, s) == BSATTN_OK && r.attend(r.a, s) == BSATTN_OK && r.keep(r.a, s) == BSATTN_OK);
+  });
+  for (const int32_t* ids : {(const int32_t*)nullptr, far}) {
+    refused(r.keep(r.a, s), BSATTN_ERR_INVALID, text);
+    CHECK(r.map(s, 2, ids) == BSATTN_OK);
+  }
+  refused(r.keep(r.a, s), BSATTN_ERR_INVALID, text);
+  // another step for these
+  Arrays t(2, 16, 8);
+  CHECK(r.map(t, 2, far) == BSATTN_OK && r.append(r.a, t) == BSATTN_OK && r.attend(r.a, t) == BSATTN_OK && r.keep(r.a, t) == BSATTN_OK);
+}
+
 int main() {
   eager_map_of_a_captured_step();
   captured_append_of_another_step();
   captures_beside_a_step();
+  other_requests();
   std::puts("ok");
   return 0;
 }
