@@ -316,8 +316,9 @@ int bsattn_sync(bsattn_cache* cache, void* stream);
  * The caller owns the arrays (device memory) and keeps them and the struct
  * while calls or graphs that use them are pending; a step is used with one
  * stream at a time, and with the caches that it was last mapped for.  Calls out
- * of order, or after the host has changed a cache's sequences, are refused where
- * the library can know: it does not see replays, so a step whose map, or whose
+ * of order, or after the host has changed one of the step's sequences (an append
+ * to it, trim, reset, a fork from or to it; other sequences may change), are
+ * refused where the library can know: it does not see replays, so a step whose map, or whose
  * packed append to a cache, was captured is taken as it comes.  A graph keeps
  * the requests (n_seqs, seq_ids) of its capture.  A step whose map was captured
  * and that is now mapped for others, or with its caches in another order, is
@@ -365,8 +366,8 @@ int bsattn_step_map(bsattn_cache* const* caches, bsattn_step* step, const int32_
  * summaries of the blocks they fill, and sets the device-side lengths to
  * `ends`.  strides: elements between rows and between heads, multiples of 8
  * (null: dense); the dims are contiguous, 16-byte aligned.  A step can be
- * appended again (the rows are overwritten) until the host changes the
- * cache's sequences.  As after bsattn_append_step the host's view is behind
+ * appended again (the rows are overwritten) until the host changes one of its
+ * sequences.  As after bsattn_append_step the host's view is behind
  * until bsattn_sync. */
 int bsattn_append_packed(bsattn_cache* cache, const bsattn_step* step, const void* k,
                          const int64_t* k_strides, const void* v, const int64_t* v_strides,

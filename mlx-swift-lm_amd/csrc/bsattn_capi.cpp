@@ -200,6 +200,8 @@ int bsattn_cache_create(const bsattn_desc* desc, bsattn_cache** out) try {
     c->pages.assign(d.max_seqs, {});
     c->free_pages.resize(c->num_pages);
     c->sharers.assign(c->num_pages, 0);
+    c->in_step.assign(d.max_seqs, 0);
+    c->step_seqs.reserve(kMaxBatch);
   } catch (...) {
     delete c;
     throw;
@@ -372,7 +374,7 @@ int bsattn_append_step(bsattn_cache* c, const void* k, const void* v, const int3
     if (e != hipSuccess) return hip_fail(e, "append step launch");
   }
   c->stale = true;
-  c->step = 0;
+  end_step(c, seqs);
   return BSATTN_OK;
 } catch (...) {
   return on_exception();
@@ -456,7 +458,7 @@ int append_impl(bsattn_cache* c, const int32_t* seq_ids, int32_t n_seqs, int32_t
     if (e != hipSuccess) return hip_fail(e, "append launch");
   }
   ap.sent();
-  c->step = 0;
+  end_step(c, seqs);
   for (int s_ : seqs) c->len[s_] += n_tokens;
   return BSATTN_OK;
 }
@@ -778,7 +780,7 @@ int bsattn_append_decode(bsattn_cache* c, const void* k, const void* v, const vo
   prof_collect(c, prof);
   if (e != hipSuccess) return hip_fail(e, "append-decode launch");
   patches.sent();
-  c->step = 0;
+  end_step(c, seqs);
   for (int sq : seqs) c->len[sq] += 1;
   return BSATTN_OK;
 } catch (...) {
@@ -927,7 +929,7 @@ int bsattn_trim(bsattn_cache* c, const int32_t* seq_ids, int32_t n_seqs, int32_t
   UnsharedTails tails;
   rc = unshare_tails(c, seqs, n_tokens, (hipStream_t)stream, tails);
   if (rc) return rc;
-  c->step = 0;
+  end_step(c, seqs);
   c->free_pages.resize(c->free_pages.size() - tails.from_free);
   for (int i = 0; i < n_seqs; ++i) {
     const int sq = seqs[i];
@@ -962,7 +964,7 @@ int bsattn_reset(bsattn_cache* c, const int32_t* seq_ids, int32_t n_seqs, void* 
   if (rc) return rc;
   Patches patches;
   patches.reserve(2 * seqs.size());  // the loop below then cannot throw
-  c->step = 0;
+  end_step(c, seqs);
   for (int sq : seqs) {
     c->len[sq] = 0;
     release_pages(c, sq, 0, patches);

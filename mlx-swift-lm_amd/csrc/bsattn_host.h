@@ -105,9 +105,12 @@ struct bsattn_cache {
   // the host): sent before the next call's own (send_unsent)
   bsattn::Patches unsent;
   // the step that the cache was last mapped for (0: none, or the host has
-  // changed its sequences since), and its place among the step's caches
+  // changed one of its sequences since), its place among the step's caches, and
+  // the step's sequences, also as a mark on each of the cache's
   uint64_t step = 0;
   int32_t step_layer = 0;
+  std::vector<int32_t> step_seqs;
+  std::vector<char> in_step;
   enum { kMapped, kAppended, kKept } step_state = kMapped;  // the last call with it
   // steps of which the map or this cache's append was captured: the host does not
   // see their replays
@@ -401,6 +404,13 @@ hipError_t with_partials(bsattn_cache* c, int64_t rows, hipStream_t s, F launch)
   if (capturing(s)) return launch(graph_workspace(c, rows), nullptr);
   PrefillSpaces* spaces = PrefillSpaces::of(c->d.device);
   return spaces ? spaces->with(s, launch) : launch(nullptr, nullptr);
+}
+
+// The host has changed seqs: a step that is under way with one of them ends
+inline void end_step(bsattn_cache* c, const std::vector<int32_t>& seqs) {
+  if (c->step == 0) return;
+  for (int s : seqs)
+    if (c->in_step[s]) c->step = 0;
 }
 
 // Calls that need the exact token counts refuse while device-side appends

@@ -305,7 +305,10 @@ int bsattn_fork(bsattn_cache* c, const int32_t* src_ids, const int32_t* dst_ids,
     c->pages[dst[i]].swap(rows[i]);
     c->len[dst[i]] = tokens[i];
   }
-  c->step = 0;
+  // (a step's own tokens may lie in pages that its sequence shares now)
+  end_step(c, dst);
+  for (int i = 0; i < n; ++i)
+    if (c->in_step[src_ids[i]]) c->step = 0;
   return BSATTN_OK;
 } catch (...) {
   return on_exception();

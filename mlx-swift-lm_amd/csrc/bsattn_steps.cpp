@@ -181,6 +181,9 @@ int bsattn_step_map(bsattn_cache* const* caches, bsattn_step* st, const int32_t*
       caches[l]->step = st->stamp;
       caches[l]->step_layer = l;
       caches[l]->step_state = bsattn_cache::kMapped;
+      for (int sq : caches[l]->step_seqs) caches[l]->in_step[sq] = 0;
+      caches[l]->step_seqs.assign(seqs.begin(), seqs.end());  // (within what create reserved)
+      for (int sq : seqs) caches[l]->in_step[sq] = 1;
     }
     // (a step that was captured stays so: its graph may replay after any map)
     CapturedStep* was = captured_step(caches[l], before);

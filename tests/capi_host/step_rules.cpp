@@ -141,11 +141,68 @@ static void other_requests() {
   CHECK(r.map(t, 2, far) == BSATTN_OK && r.append(r.a, t) == BSATTN_OK && r.attend(r.a, t) == BSATTN_OK && r.keep(r.a, t) == BSATTN_OK);
 }
 
+// host calls for other sequences leave a step under way; those for one of its own end it
+static void other_sequences() {
+  Rig r(6);
+  bsattn_cache* c = r.a;
+  const int32_t ids[2] = {4, 1}, free_one = 2, other = 0, own = 4, second = 1;
+  CHECK(bsattn_reset(c, &free_one, 1, nullptr) == BSATTN_OK);
+  Arrays s(1, 16, 8);
+  auto begin = [&] {
+    CHECK(bsattn_sync(c, nullptr) == BSATTN_OK && r.map(s, 2, ids) == BSATTN_OK && r.append(c, s) == BSATTN_OK &&
+          r.attend(c, s) == BSATTN_OK && bsattn_sync(c, nullptr) == BSATTN_OK);
+  };
+  int32_t got = 0;
+  auto calls = [&](int how, const int32_t* id) {
+    switch (how) {
+      case 0: return bsattn_append(c, x, x, id, 1, 3, nullptr);
+      case 1: return bsattn_append_decode(c, x, x, x, id, 1, 1.f, x, nullptr, nullptr);
+      case 2: return bsattn_append_step(c, x, x, id, 1, nullptr);
+      case 3: return bsattn_trim(c, id, 1, 1, &got, nullptr);
+      default: return bsattn_reset(c, id, 1, nullptr);
+    }
+  };
+  for (int how = 0; how < 5; ++how) {
+    begin();
+    CHECK(calls(how, &other) == BSATTN_OK);
+    CHECK(r.attend(c, s) == BSATTN_OK && r.keep(c, s) == BSATTN_OK);
+    for (const int32_t* id : {&own, &second}) {
+      begin();
+      CHECK(calls(how, id) == BSATTN_OK);
+      for (int rc : {r.append(c, s), r.attend(c, s), r.keep(c, s)}) refused(rc, BSATTN_ERR_INVALID, "has changed since");
+      CHECK(bsattn_sync(c, nullptr) == BSATTN_OK);
+      if (how == 4)
+        CHECK(bsattn_append(c, x, x, id, 1, 40, nullptr) == BSATTN_OK && bsattn_reserve(c, id, 1, 32, nullptr) == BSATTN_OK);
+    }
+    CHECK(bsattn_reset(c, &other, 1, nullptr) == BSATTN_OK && bsattn_append(c, x, x, &other, 1, 40, nullptr) == BSATTN_OK);
+    CHECK(bsattn_reserve(c, nullptr, 6, 32, nullptr) == BSATTN_OK && bsattn_reset(c, &free_one, 1, nullptr) == BSATTN_OK);
+  }
+  // a fork between others, from the step's, to the step's
+  begin();
+  CHECK(bsattn_fork(c, &other, &free_one, 1, nullptr, nullptr) == BSATTN_OK && r.keep(c, s) == BSATTN_OK);
+  begin();
+  CHECK(bsattn_reset(c, &free_one, 1, nullptr) == BSATTN_OK && r.attend(c, s) == BSATTN_OK);
+  CHECK(bsattn_fork(c, &own, &free_one, 1, nullptr, nullptr) == BSATTN_OK);
+  refused(r.keep(c, s), BSATTN_ERR_INVALID, "has changed since");
+  CHECK(bsattn_reset(c, &own, 1, nullptr) == BSATTN_OK);
+  begin();
+  CHECK(s.taken[0] == 0);  // (it holds no pages)
+  CHECK(bsattn_fork(c, &other, &own, 1, nullptr, nullptr) == BSATTN_OK);
+  refused(r.keep(c, s), BSATTN_ERR_INVALID, "has changed since");
+  // the marks are the last map's
+  const int32_t two[2] = {0, 3};
+  CHECK(r.map(s, 2, two) == BSATTN_OK && r.append(c, s) == BSATTN_OK && bsattn_sync(c, nullptr) == BSATTN_OK);
+  CHECK(bsattn_trim(c, ids, 2, 1, nullptr, nullptr) == BSATTN_OK && r.keep(c, s) == BSATTN_OK && bsattn_sync(c, nullptr) == BSATTN_OK);
+  CHECK(bsattn_trim(c, two + 1, 1, 1, nullptr, nullptr) == BSATTN_OK);
+  refused(r.keep(c, s), BSATTN_ERR_INVALID, "has changed since");
+}
+
 int main() {
   eager_map_of_a_captured_step();
   captured_append_of_another_step();
   captures_beside_a_step();
   other_requests();
+  other_sequences();
   std::puts("ok");
   return 0;
 }
