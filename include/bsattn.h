@@ -313,8 +313,8 @@ int bsattn_sync(bsattn_cache* cache, void* stream);
  * captured.  Its generalisation of SpeculativeTokenIterator.speculateRound
  * (Evaluate.swift:841-931), which verifies one chain of drafts and trims.
  *
- * The caller owns the arrays (device memory) and keeps them and the struct
- * while calls or graphs that use them are pending; a step is used with one
+ * The caller owns the arrays (device memory) and keeps them and the struct,
+ * where it is, while calls or graphs that use them are pending; a step is used with one
  * stream at a time, and with the caches that it was last mapped for.  Calls out
  * of order, or after the host has changed one of the step's sequences (an append
  * to it, trim, reset, a fork from or to it; other sequences may change), are
@@ -344,7 +344,7 @@ typedef struct bsattn_step {
   int32_t* slots;      /* [n_caches, rows]: page * block_size + place in it, -1: none */
   int32_t* ends;       /* [n_caches, n_seqs]: the request's length with its new tokens */
   int32_t ids[BSATTN_STEP_SEQS]; /* the requests' sequences */
-  uint64_t stamp;      /* names the map to the caches */
+  uint64_t stamp;      /* names the map to the caches (0 before the first one) */
 } bsattn_step;
 
 /* Where the new tokens of a step lie: builds the step's arrays on the device.

@@ -124,6 +124,7 @@ struct bsattn_cache {
     std::shared_ptr<const std::vector<int32_t>> ids;
     int32_t rows, place;
     bool several, other, recorded;
+    const bsattn_step* at;  // where the step lay then: another one there has taken its place
   };
   std::vector<CapturedStep> captured_steps;
   // opt-in per-kernel timing (bsattn_profile_*)

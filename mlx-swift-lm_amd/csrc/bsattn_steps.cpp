@@ -40,6 +40,18 @@ CapturedStep* captured_step(bsattn_cache* c, uint64_t stamp) {
   return nullptr;
 }
 
+// the stamp that a step's entry goes by before its map (0: it has none): its last
+// one, or an earlier one where it was mapped for other caches since.  A step
+// without a stamp is new, whatever lay there before.
+uint64_t captured_before(const std::vector<CapturedStep>& steps, const bsattn_step* st, uint64_t before) {
+  uint64_t own = 0;
+  for (const CapturedStep& x : steps) {
+    if (before != 0 && x.stamp == before) return before;
+    if (before != 0 && x.at == st) own = x.stamp;
+  }
+  return own;
+}
+
 // the last call with the step that the cache is mapped for; a call that is only
 // recorded moves nothing yet
 void step_moves(bsattn_cache* c, const bsattn_step* st, bool captured, decltype(bsattn_cache::step_state) to) {
@@ -185,10 +197,16 @@ int bsattn_step_map(bsattn_cache* const* caches, bsattn_step* st, const int32_t*
       caches[l]->step_seqs.assign(seqs.begin(), seqs.end());  // (within what create reserved)
       for (int sq : seqs) caches[l]->in_step[sq] = 1;
     }
+    // (entries of steps whose memory this one has now have served)
+    auto& steps = caches[l]->captured_steps;
+    const uint64_t own = captured_before(steps, st, before);
+    steps.erase(std::remove_if(steps.begin(), steps.end(),
+                               [&](const CapturedStep& x) { return x.at == st && x.stamp != own; }),
+                steps.end());
     // (a step that was captured stays so: its graph may replay after any map)
-    CapturedStep* was = captured_step(caches[l], before);
+    CapturedStep* was = captured_step(caches[l], own);
     if (!was) {
-      if (captured) caches[l]->captured_steps.push_back({st->stamp, l, true, false, ids, st->rows, l, false, false, true});
+      if (captured) steps.push_back({st->stamp, l, true, false, ids, st->rows, l, false, false, true, st});
       continue;
     }
     const bool other = was->map && (was->place != l || was->rows != st->rows || *was->ids != seqs);
@@ -199,6 +217,7 @@ int bsattn_step_map(bsattn_cache* const* caches, bsattn_step* st, const int32_t*
     was->several |= captured && other;
     was->other = other || was->several;
     was->recorded = captured;
+    was->at = st;
   }
   return BSATTN_OK;
 } catch (...) {
@@ -228,7 +247,7 @@ int bsattn_append_packed(bsattn_cache* c, const bsattn_step* st, const void* k, 
   step_moves(c, st, captured, bsattn_cache::kAppended);
   if (captured) {
     if (CapturedStep* was = captured_step(c, st->stamp)) was->append = true;
-    else c->captured_steps.push_back({st->stamp, layer, false, true, nullptr, 0, 0, false, false, false});
+    else c->captured_steps.push_back({st->stamp, layer, false, true, nullptr, 0, 0, false, false, false, st});
   }
   return BSATTN_OK;
 } catch (...) {

@@ -197,12 +197,43 @@ static void other_sequences() {
   refused(r.keep(c, s), BSATTN_ERR_INVALID, "has changed since");
 }
 
+// steps that come and go, each captured: what is kept of them does not grow with their number
+static void many_captured_steps() {
+  Rig r;
+  Arrays s(2, 16, 8), t(2, 16, 8);
+  r.captured([&] { CHECK(r.map(t) == BSATTN_OK && r.append(r.a, t) == BSATTN_OK); });
+  const bsattn_step fresh = Arrays(2, 16, 8).st;
+  for (int turn = 0; turn < 100; ++turn) {
+    const bsattn_step was = s.st;
+    s.st = fresh;  // (a new struct in the old one's memory, with the old arrays)
+    s.st.starts = was.starts, s.st.taken = was.taken, s.st.requests = was.requests, s.st.positions = was.positions;
+    s.st.ancestors = was.ancestors, s.st.slots = was.slots, s.st.ends = was.ends;
+    if (turn % 3 == 0) CHECK(r.map(s) == BSATTN_OK);
+    r.captured([&] { CHECK((turn % 3 == 0 || r.map(s) == BSATTN_OK) && r.append(r.a, s) == BSATTN_OK); });
+    CHECK(r.a->captured_steps.size() <= 2 && r.b->captured_steps.size() <= 2);
+  }
+  // the others are as they were
+  CHECK(r.attend(r.a, t) == BSATTN_OK && r.append(r.b, t) == BSATTN_OK && r.keep(r.a, s) == BSATTN_OK);
+  // one that was mapped for other caches in between has not changed
+  Arrays u(2, 16, 8);
+  r.captured([&] { CHECK(r.map(u) == BSATTN_OK); });
+  bsattn_cache* alone = cache(2, 16, 40);
+  u.st.n_caches = 1;
+  CHECK(bsattn_step_map(&alone, &u.st, r.counts, nullptr, nullptr, 2, nullptr) == BSATTN_OK);
+  refused(r.keep(r.a, u), BSATTN_ERR_INVALID, "not mapped");
+  u.st.n_caches = 2;
+  CHECK(r.map(u) == BSATTN_OK && r.keep(r.a, u) == BSATTN_OK && r.map(u, 1) == BSATTN_OK);
+  refused(r.keep(r.a, u), BSATTN_ERR_INVALID, "captured for other requests");
+  bsattn_cache_destroy(alone);
+}
+
 int main() {
   eager_map_of_a_captured_step();
   captured_append_of_another_step();
   captures_beside_a_step();
   other_requests();
   other_sequences();
+  many_captured_steps();
   std::puts("ok");
   return 0;
 }
