@@ -18,7 +18,8 @@ public final class BlockSparseStep {
     /// the first n (+ 1), n and caches * n entries of the per-request ones hold.
     public let starts, taken, requests, positions, slots, ends: MLXArray
     public let ancestors: MLXArray?
-    var step: bsattn_step = .init()
+    /// One place for the object's life: the library knows a captured step by it.
+    let step = UnsafeMutablePointer<bsattn_step>.allocate(capacity: 1)
 
     public init(caches: [BlockSparseKVCache], rows: Int, maxTokens: Int) {
         precondition(caches.count >= 1 && caches.count <= Int(BSATTN_STEP_CACHES) && rows >= 1 && maxTokens >= 1,
@@ -37,17 +38,20 @@ public final class BlockSparseStep {
         ends = new([caches.count * most])
         ancestors = maxTokens <= Int(BSATTN_TREE_NODES) ? device.empty([rows], dtype: .uint64) : nil
         func at(_ x: MLXArray) -> UnsafeMutablePointer<Int32> { device.pointer(x).assumingMemoryBound(to: Int32.self) }
-        step.n_caches = Int32(caches.count)
-        step.rows = Int32(rows)
-        step.max_tokens = Int32(maxTokens)
-        step.starts = at(starts)
-        step.taken = at(taken)
-        step.requests = at(requests)
-        step.positions = at(positions)
-        step.ancestors = ancestors.map { device.pointer($0).assumingMemoryBound(to: UInt64.self) }
-        step.slots = at(slots)
-        step.ends = at(ends)
+        step.initialize(to: bsattn_step())
+        step.pointee.n_caches = Int32(caches.count)
+        step.pointee.rows = Int32(rows)
+        step.pointee.max_tokens = Int32(maxTokens)
+        step.pointee.starts = at(starts)
+        step.pointee.taken = at(taken)
+        step.pointee.requests = at(requests)
+        step.pointee.positions = at(positions)
+        step.pointee.ancestors = ancestors.map { device.pointer($0).assumingMemoryBound(to: UInt64.self) }
+        step.pointee.slots = at(slots)
+        step.pointee.ends = at(ends)
     }
+
+    deinit { step.deallocate() }
 
     /// counts [n] int32: tokens of each request, whose pages are held already
     /// (reserve); parents [rows] int32: each node's parent among its request's
@@ -63,7 +67,7 @@ public final class BlockSparseStep {
         let (c, p) = (at(counts), parents.map(at))
         withSeqIds(seqIds, rows: counts.dim(0)) { ids in
             handles.withUnsafeBufferPointer { h in
-                bsCheck(bsattn_step_map(h.baseAddress, &step, c, p, ids, Int32(counts.dim(0)), caches[0].stream),
+                bsCheck(bsattn_step_map(h.baseAddress, step, c, p, ids, Int32(counts.dim(0)), caches[0].stream),
                         "bsattn_step_map")
             }
         }
@@ -93,7 +97,7 @@ extension BlockSparseKVCache {
     public func appendPacked(keys: MLXArray, values: MLXArray, step: BlockSparseStep) {
         checkPacked(keys, step, heads: kvHeads)
         checkPacked(values, step, heads: kvHeads)
-        bsCheck(bsattn_append_packed(handle, &step.step, device.pointer(keys), nil, device.pointer(values), nil, stream),
+        bsCheck(bsattn_append_packed(handle, step.step, device.pointer(keys), nil, device.pointer(values), nil, stream),
                 "bsattn_append_packed")
     }
 
@@ -110,7 +114,7 @@ extension BlockSparseKVCache {
                      "sinks must be [Hq] float32")
         let out = device.empty(queries.shape, dtype: dtype)
         let sp = sinks.map { UnsafePointer(device.pointer($0).assumingMemoryBound(to: Float.self)) }
-        bsCheck(bsattn_attend_tree(handle, &step.step, device.pointer(queries), nil, Int32(window ?? 0), sp, scale,
+        bsCheck(bsattn_attend_tree(handle, step.step, device.pointer(queries), nil, Int32(window ?? 0), sp, scale,
                                    device.pointer(out), stream), "bsattn_attend_tree")
         return out
     }
@@ -120,11 +124,11 @@ extension BlockSparseKVCache {
     /// behind what it held before.
     public func keep(step: BlockSparseStep, kept: MLXArray, nKept: MLXArray) {
         precondition(kept.ndim == 2 && kept.dim(1) >= 1 && kept.dtype == .int32 && nKept.shape == [kept.dim(0)]
-                         && nKept.dtype == .int32 && kept.dim(0) == Int(step.step.n_seqs),
+                         && nKept.dtype == .int32 && kept.dim(0) == Int(step.step.pointee.n_seqs),
                      "kept must be [n, width] and nKept [n], int32")
         func at(_ x: MLXArray) -> UnsafePointer<Int32> {
             UnsafePointer(device.pointer(x).assumingMemoryBound(to: Int32.self))
         }
-        bsCheck(bsattn_keep(handle, &step.step, at(kept), Int32(kept.dim(1)), at(nKept), stream), "bsattn_keep")
+        bsCheck(bsattn_keep(handle, step.step, at(kept), Int32(kept.dim(1)), at(nKept), stream), "bsattn_keep")
     }
 }
