@@ -38,7 +38,7 @@ public final class BlockSparseStep {
         ends = new([caches.count * most])
         ancestors = maxTokens <= Int(BSATTN_TREE_NODES) ? device.empty([rows], dtype: .uint64) : nil
         func at(_ x: MLXArray) -> UnsafeMutablePointer<Int32> { device.pointer(x).assumingMemoryBound(to: Int32.self) }
-        step.initialize(to: bsattn_step())
+        step.initialize(to: .init())
         step.pointee.n_caches = Int32(caches.count)
         step.pointee.rows = Int32(rows)
         step.pointee.max_tokens = Int32(maxTokens)
