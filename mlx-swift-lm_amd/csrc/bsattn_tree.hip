@@ -35,6 +35,7 @@
 #include "bsattn_append.h"
 #include "bsattn_codes.h"
 #include "bsattn_device.h"
+#include "bsattn_tree_parts.h"
 
 namespace bsattn {
 
@@ -43,28 +44,8 @@ constexpr float kTreeLog2e = 1.4426950408889634f;
 constexpr float kTreeSlack = 6.0f;
 constexpr float kTreeTop = 14.0f;
 
-// What a request brings to a launch, and the units of its part
-struct TreeRange {
-  int T, N, P, lo, u0, units, cu;
-  int lg;  // log2 of the heads of a group
-};
 __device__ __forceinline__ TreeRange tree_range(const Geometry& geo, const TreeBatch& tb, int i) {
-  TreeRange r;
-  r.T = geo.meta[tb.ids[i]];
-  r.N = min(min(tb.taken[i], tb.max_tokens), r.T);
-  r.P = r.T - r.N;
-  r.lg = __builtin_ctz((unsigned)geo.group);
-  r.lo = tb.window > 0 ? max(0, r.P - tb.window + 1) : 0;  // the first token that a root sees
-  r.u0 = r.lo >> 5;
-  r.units = r.N > 0 ? ((r.T - 1) >> 5) - r.u0 + 1 : 0;
-  // (more tokens than the launch was cut for, as when a graph replays after
-  // further reservations: as many parts, of more units each)
-  r.cu = tb.cu;
-  if (r.units > tb.units[i]) {
-    const int most = max(1, tb.part0[i + 1] - tb.part0[i]);
-    r.cu = max(r.cu, ((r.units + most - 1) / most + 3) & ~3);
-  }
-  return r;
+  return tree_range(tb, i, geo.meta[tb.ids[i]], tb.taken[i], geo.group);
 }
 
 // slabs of the units that a wave takes, the block table read through the scalar cache
@@ -147,9 +128,8 @@ __device__ __forceinline__ uint32_t seen_tokens(const uint64_t* s_seen, const in
   return (cached | tree) & 0xFFu;
 }
 
-// What a workgroup takes of the launch: grid (parts, kv heads, column groups),
-// the parts padded so that the groups of a (part, head) lie a multiple of 8
-// workgroups apart, on one XCD, whose L2 then holds the K and V they share
+// What a workgroup takes of the launch: grid (tree_grid's parts, kv heads, column
+// groups)
 struct TreePlace {
   int i, h, group, part;  // i: -1 where there is nothing
 };
@@ -177,25 +157,6 @@ __device__ __forceinline__ void tree_nodes(const TreeBatch& tb, const TreeRange&
     for (int k = depth + 1; k > tb.window; --k) seen &= seen - 1;  // (the furthest come first)
   s_seen[j] = seen;
 }
-
-// The units of a part: those that every column sees whole (from fa on, `full` of
-// them), then the others, in front of them and behind (at most 7 in all)
-struct TreePart {
-  int ua, fa, full, places;
-  __device__ __forceinline__ TreePart(const TreeBatch& tb, const TreeRange& r, int part) {
-    ua = r.u0 + part * r.cu;
-    const int ub = min(ua + r.cu, r.u0 + r.units);
-    const int whole0 = tb.window > 0 ? (max(0, r.P + r.N - tb.window) + 31) >> 5 : 0, whole1 = r.P >> 5;
-    fa = min(max(ua, whole0), ub);
-    full = max(min(ub, whole1) - fa, 0);
-    places = ub - ua;
-  }
-  // (places past the part's: its last one)
-  __device__ __forceinline__ int unit(int at) const {
-    const int p = min(at, places - 1), k = ua + p - full;
-    return p < full ? fa + p : k < fa ? k : k + full;
-  }
-};
 
 // What was noted: a value that is infinite or no number is so in the output of
 // every column that sees its token, whatever its weight
@@ -279,7 +240,7 @@ __device__ __forceinline__ void tree_write(const Geometry& geo, const TreeBatch&
       *(uint2*)(out + ((int64_t)(start + node) * geo.hq + hq) * kHeadDim + d) =
           make_uint2(pack2<DT>(a[0], a[1]), pack2<DT>(a[2], a[3]));
     } else {
-      float* pp = partials + ((int64_t)(tb.row0[i] + part * tb.max_tokens + node) * geo.hq + hq) * kPartial;
+      float* pp = partials + ((int64_t)tree_row(tb, i, part, node) * geo.hq + hq) * kPartial;
       // (partials are 130 floats apart)
       *(float2*)(pp + d) = make_float2(a[0], a[1]);
       *(float2*)(pp + d + 2) = make_float2(a[2], a[3]);
@@ -351,7 +312,7 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
   const TreeRange r = tree_range(geo, tb, i);
   const int first = at.group * COLS, cols = r.N << r.lg;
   if (first >= cols || part * r.cu >= r.units) return;
-  const bool direct = tb.part0[i + 1] - tb.part0[i] <= 1;
+  const bool direct = tree_direct(tb, i);
   const int start = uniform(tb.starts[i]), seq = tb.ids[i];
   const TreePart pt(tb, r, part);
   // the wave's column tiles, spread evenly over the team; waves w and w + 4 share a
@@ -745,14 +706,14 @@ __global__ __launch_bounds__(256) void k_tree_join(Geometry geo, TreeBatch tb, c
   const bool there = most > 0 && node < r.N;
   float M = -INFINITY, L = 0.f;
   f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int parts = there ? (r.units + r.cu - 1) / r.cu : 0;
+  const int parts = there ? tree_parts(r) : 0;
   for (int p0 = y; p0 < most; p0 += 4 * ROWS) {
     f32x4 x[4];
     float m[4], l[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int p = min(p0 + j * ROWS, most - 1);
-      const float2* part = (const float2*)(ws + ((int64_t)(tb.row0[i] + p * tb.max_tokens + node) * geo.hq + hq) * kPartial);
+      const float2* part = (const float2*)(ws + ((int64_t)tree_row(tb, i, p, node) * geo.hq + hq) * kPartial);
       const float2 xa = part[2 * c], xb = part[2 * c + 1], ml = part[kHeadDim / 2];
       x[j] = f32x4{xa.x, xa.y, xb.x, xb.y};
       // (without a token that is seen: no reference, and a sum of 0, or NaN)
@@ -809,8 +770,7 @@ __global__ __launch_bounds__(256) void k_tree_join(Geometry geo, TreeBatch tb, c
 template <int DT, int KB>
 static void tree_dispatch(const Geometry& g, const TreeBatch& tb, const uint16_t* q, uint16_t* out, float* ws,
                           hipStream_t s, Timing* prof) {
-  const int parts = tb.groups > 1 ? (tb.part0[tb.n] + 7) & ~7 : tb.part0[tb.n];
-  const dim3 grid(parts, g.hkv, tb.groups);
+  const dim3 grid(tree_grid(tb), g.hkv, tb.groups);
   auto go = [&](auto kernel, int threads) { launch(kernel, grid, dim3(threads), 0, s, prof, kProfTree, g, tb, q, out, ws); };
   if (tb.tiles == 1) go(k_tree<DT, KB, 1, 1>, 256);
   else if (tb.tiles == 2) go(k_tree<DT, KB, 2, 1>, 256);
