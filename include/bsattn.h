@@ -380,7 +380,7 @@ int bsattn_append_packed(bsattn_cache* cache, const bsattn_step* step, const voi
  * positions (0: all).  sinks: as in bsattn_decode_dense.  Absent nodes give
  * zeros; rows of no request are left as they were.  max_tokens is at most
  * BSATTN_TREE_NODES.  Workspaces, split sequences and infinite attended values
- * as in bsattn_decode_dense. */
+ * as in bsattn_decode_dense; blocks that forks share are read for each of them. */
 int bsattn_attend_tree(bsattn_cache* cache, const bsattn_step* step, const void* q,
                        const int64_t* q_strides, int32_t window, const float* sinks, float scale,
                        void* out, void* stream);
@@ -391,7 +391,10 @@ int bsattn_attend_tree(bsattn_cache* cache, const bsattn_step* step, const void*
  * that is not, or that is no node), moved together behind what it held before;
  * its device-side length is that and the kept ones.  Blocks that are full then
  * get their summary.  With no node kept the step is taken back (also after
- * another bsattn_keep of it).  max_tokens is at most BSATTN_TREE_NODES. */
+ * another bsattn_keep of it).  After one that moved nodes another one that keeps
+ * some finds other nodes' keys and values in their places, and the library does
+ * not see it: append the rows again first.  max_tokens is at most
+ * BSATTN_TREE_NODES. */
 int bsattn_keep(bsattn_cache* cache, const bsattn_step* step, const int32_t* kept, int32_t width,
                 const int32_t* n_kept, void* stream);
 

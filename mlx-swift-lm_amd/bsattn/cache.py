@@ -590,7 +590,8 @@ class BlockSparseKVCache:
     def keep(self, step, kept: torch.Tensor, nKept: torch.Tensor) -> None:
         """Of the tokens that the step appended, request i keeps its nodes
         kept[i, :nKept[i]] (int32 [n, width] and [n], ascending), moved together
-        behind what it held before; the others are dropped."""
+        behind what it held before; the others are dropped.  Once nodes have
+        moved, only a keep of none (or appendPacked again) finds the step's."""
         n = step._n
         if kept.dim() != 2 or kept.shape[1] < 1:
             raise ValueError(f"kept must be [{n}, width], got {tuple(kept.shape)}")

@@ -18,13 +18,17 @@
 // as 1024 + c (K, fp16) and c (V, bf16), exactly; scales and biases act on scores
 // and weights.
 //
-// What bounds it: 16 columns and fewer the reads; from 64 on the issue of a SIMD,
-// which products (16 cycles each) and VALU work share nearly one after the other.
-// A wave's unit of 32 tokens by 32 columns is 52 products, 48 for codes, beside 16
-// exponentials and 50 to 210 other VALU instructions.  Passes: 64 columns over 8 x
+// What bounds it: 64 columns and fewer the reads; above, the order within a wave:
+// a unit's scores, its softmax and its products follow each other, and the two
+// waves of a SIMD hide only a part of that.  A wave's unit of 32 tokens by 32
+// columns is 52 products (of 16 cycles) beside 92 VALU instructions (256 columns,
+// bf16; 105 with 64), 48 beside 296 for int8 and 307 for int4, exponentials (16)
+// and the codes' conversion included (counted over whole launches).  The matrix
+// cores are busy for 50% of the SIMDs' time with 256 bf16 columns and 28% with
+// affine caches; waves wait for 30 to 34% of theirs.  Passes: 64 columns over 8 x
 // 32k bf16 tokens 200 us (1074 MB: 5.4 TB/s, a plain streaming read 154 us), 256 414
-// (664 TFLOP/s; 51% of a large product's rate), 100 over 4 x 131k int4 499, 96 over
-// 4 x 262k int8 469.
+// (664 TFLOP/s; 51% of a large product's rate), 100 over 4 x 131k int4 502, 96 over
+// 4 x 262k int8 477.
 #include <hip/hip_ext.h>
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -278,7 +282,7 @@ __global__ __launch_bounds__(CW == 1 ? 256 : 512, 2) void k_tree(Geometry geo, T
   static_assert(KB == 0 || DT == 0, "affine caches: fp16");
   constexpr int W = CW == 1 ? 4 : 8, TW = W / CW, SLOTS = CW == 1 ? 1 : 2;
   // units of a team, and of the workgroup, in a step.  16-bit caches: four, however
-  // many teams there are (256 columns over 8 x 32k bf16 tokens, 1 and 4: 394 and 377
+  // many teams there are (256 columns over 8 x 32k bf16 tokens, 1 and 4: 418 and 403
   // us); affine ones one per team, since their units' pieces and entries then stay in
   // fewer registers (132 columns over 8 x 16k int8 tokens, 1 and 4: 280 and 328 us for
   // the step; 1 and 2, 96 over 4 x 262k int8 487 and 518, 100 over 4 x 131k int4 503

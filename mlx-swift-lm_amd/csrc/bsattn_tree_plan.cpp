@@ -19,15 +19,17 @@ int64_t tree_plan(const Geometry& g, TreeBatch& tb) {
   }
   // Workgroups of one round: eight waves of 256 registers fill a CU, of four two fit.
   // Further rounds cost starts, ends and partials, about the time of 12 units a
-  // workgroup: 64 columns over 8 x 32k bf16 tokens 188 us in one round, 200 in two, 220
-  // in three; 256 350, 369, 448; 100 over 4 x 131k int4 499, 512, 523; 192 in windows
-  // of ragged trees 160, 187, 223.  Where the longest request's part would outlast the
+  // workgroup: 64 columns over 8 x 32k bf16 tokens 188 us in one round, 201 in two, 224
+  // in three; 256 403, 428, 507; 100 over 4 x 131k int4 497, 511, 526; 192 in windows
+  // of ragged trees 160, 190, 226.  Where the longest request's part would outlast the
   // others by far, more are shorter all the same: 96 columns over 32 requests of 300 to
-  // 20000 tokens, bf16 304 us in two or three rounds, int4 341 in three, 383 in two; 64
-  // over 40 x 9k bf16 tokens 344 with a part each, one round and a quarter, 298 in four.
+  // 20000 tokens, bf16 300 us in two or three rounds, int4 342 in three, 382 in two; 64
+  // over 40 x 9k bf16 tokens 334 with a part each, one round and a quarter, 296 in four.
   // By little they are not (what the others leave of the memory's rate falls to the
-  // longest): 64 over 9 x 13k tokens, a seventh more units in the longest part, 97 us,
-  // cut for two rounds 105.
+  // longest): 64 over 9 x 13k tokens, a seventh more units in the longest part, 96 us,
+  // cut for two rounds 107.  One round more is not among the tries: it is at once good
+  // enough for what three leave behind it (those int4 requests 382 for 342 us, 40 x 9k
+  // int4 tokens 273 for 259) and gains 4% elsewhere at most.
   const int64_t want = (tb.tiles > 2 ? 1 : 2) * (int64_t)std::max(g.cus, 1), each = (int64_t)g.hkv * tb.groups;
   constexpr int64_t kEnds = 12;
   auto parts = [&](int i, int cu) { return std::max(1, (tb.units[i] + cu - 1) / cu); };
@@ -61,9 +63,9 @@ int64_t tree_plan(const Geometry& g, TreeBatch& tb) {
   }
   // With few units a workgroup's time is its ends: waves of one column tile leave half
   // as many teams' sums to join.  One request, 64 columns over 4k bf16 tokens (4 units
-  // a workgroup) 18.4 us, 20.0 with waves of two, 8k (8) 19.6 and 21.2, 16k (16) 25.4
-  // and 25.9, 32k 34.2 and 34.0; 128 columns over 8k 25.5 and 26.5, 16k 33.3 and 32.6,
-  // 64k 74.5 and 66.5.
+  // a workgroup) 17.8 us, 19.3 with waves of two, 8k (8) 19.1 and 20.7, 16k (16) 24.4
+  // and 25.2, 32k 33.0 and 33.5; 128 columns over 8k 25.9 and 26.1, 16k 33.9 and 32.4,
+  // 64k 75.4 and 69.7.
   tb.narrow = (tb.tiles == 4 || tb.tiles == 8) && tb.cu <= 12;
   // (it ends: a request of one part has no partials)
   while (true) {

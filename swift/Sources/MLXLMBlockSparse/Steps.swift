@@ -121,7 +121,8 @@ extension BlockSparseKVCache {
 
     /// Of the tokens that the step appended, request i keeps its nodes kept[i,
     /// ..< nKept[i]] (int32 [n, width] and [n], ascending), moved together
-    /// behind what it held before.
+    /// behind what it held before.  Once nodes have moved, only a keep of none
+    /// (or `appendPacked` again) finds the step's.
     public func keep(step: BlockSparseStep, kept: MLXArray, nKept: MLXArray) {
         precondition(kept.ndim == 2 && kept.dim(1) >= 1 && kept.dtype == .int32 && nKept.shape == [kept.dim(0)]
                          && nKept.dtype == .int32 && kept.dim(0) == Int(step.step.pointee.n_seqs),
