@@ -314,13 +314,13 @@ int bsattn_sync(bsattn_cache* cache, void* stream);
  * (Evaluate.swift:841-931), which verifies one chain of drafts and trims.
  *
  * The caller owns the arrays (device memory) and keeps them and the struct,
- * where it is, while calls or graphs that use them are pending; a step is used with one
- * stream at a time, and with the caches that it was last mapped for.  Calls out
- * of order, or after the host has changed one of the step's sequences (an append
- * to it, trim, reset, a fork from or to it; other sequences may change), are
- * refused where the library can know: it does not see replays, so a step whose map, or whose
- * packed append to a cache, was captured is taken as it comes.  A graph keeps
- * the requests (n_seqs, seq_ids) of its capture.  A step whose map was captured
+ * where it is, while calls or graphs that use them are pending; a step is used
+ * with one stream at a time, and with the caches that it was last mapped for.
+ * Calls out of order, or after one of the step's sequences has changed (an
+ * append to it, trim, reset, a fork from or to it, an append or a kept path of
+ * another step; other sequences may change), are refused where the library can
+ * know: it does not see replays, so a step whose map, or whose packed append to
+ * a cache, was captured is taken as it comes.  A graph keeps the requests (n_seqs, seq_ids) of its capture.  A step whose map was captured
  * and that is now mapped for others, or with its caches in another order, is
  * refused by the calls outside a graph, which could not tell whose arrays they
  * find; and a graph that holds calls with a step without its map may replay

@@ -52,10 +52,20 @@ uint64_t captured_before(const std::vector<CapturedStep>& steps, const bsattn_st
   return own;
 }
 
-// the last call with the step that the cache is mapped for; a call that is only
-// recorded moves nothing yet
+// the last call with the step that the cache is mapped for; one with another step
+// (a captured one) changes its sequences under it.  A call that is only recorded
+// moves nothing yet
 void step_moves(bsattn_cache* c, const bsattn_step* st, bool captured, decltype(bsattn_cache::step_state) to) {
-  if (!captured && c->step == st->stamp) c->step_state = to;
+  if (captured || c->step == 0) return;
+  if (c->step == st->stamp) {
+    c->step_state = to;
+    return;
+  }
+  for (int i = 0; i < st->n_seqs; ++i)
+    if (c->in_step[st->ids[i]]) {
+      c->step = 0;
+      return;
+    }
 }
 
 // the step's last map is the last that the cache was mapped for, and the

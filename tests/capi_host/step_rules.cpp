@@ -95,10 +95,6 @@ static void captures_beside_a_step() {
     CHECK(r.map(s) == BSATTN_OK && r.append(r.a, s) == BSATTN_OK && r.attend(r.a, s) == BSATTN_OK && r.keep(r.a, s) == BSATTN_OK);
   });
   CHECK(r.attend(r.a, t) == BSATTN_OK);
-  // nor do calls with another step that was captured
-  CHECK(r.append(r.b, s) == BSATTN_OK);
-  refused(r.attend(r.b, t), BSATTN_ERR_INVALID, "bsattn_append_packed");
-  CHECK(r.append(r.b, t) == BSATTN_OK && r.attend(r.b, t) == BSATTN_OK);
   // a captured keep
   r.captured([&] { CHECK(r.keep(r.a, t) == BSATTN_OK); });
   CHECK(r.attend(r.a, t) == BSATTN_OK && r.keep(r.a, t) == BSATTN_OK);
@@ -227,6 +223,27 @@ static void many_captured_steps() {
   bsattn_cache_destroy(alone);
 }
 
+// what runs of a captured step changes its sequences: another step of theirs ends, one of others does not
+static void captured_step_beside_a_step() {
+  const int32_t mine[2] = {0, 1}, theirs[2] = {2, 1}, apart[2] = {2, 3};
+  for (bool keeps : {false, true})
+    for (const int32_t* ids : {theirs, apart}) {
+      Rig r(4);
+      Arrays s(2, 16, 8), t(2, 16, 8);
+      CHECK(r.map(s, 2, ids) == BSATTN_OK);  // (so that its arrays hold something)
+      r.captured([&] { CHECK(r.map(s, 2, ids) == BSATTN_OK); });
+      CHECK(r.map(t, 2, mine) == BSATTN_OK);
+      for (bsattn_cache* c : r.both) {
+        CHECK(r.append(c, t) == BSATTN_OK && r.attend(c, t) == BSATTN_OK && r.attend(c, s) == BSATTN_OK);
+        CHECK(r.attend(c, t) == BSATTN_OK);  // (attention changes nothing)
+        CHECK((keeps ? r.keep(c, s) : r.append(c, s)) == BSATTN_OK);
+        if (ids == apart) CHECK(r.attend(c, t) == BSATTN_OK && r.keep(c, t) == BSATTN_OK);
+        else
+          for (int rc : {r.append(c, t), r.attend(c, t), r.keep(c, t)}) refused(rc, BSATTN_ERR_INVALID, "has changed since");
+      }
+    }
+}
+
 int main() {
   eager_map_of_a_captured_step();
   captured_append_of_another_step();
@@ -234,6 +251,7 @@ int main() {
   other_requests();
   other_sequences();
   many_captured_steps();
+  captured_step_beside_a_step();
   std::puts("ok");
   return 0;
 }
