@@ -320,11 +320,12 @@ int bsattn_sync(bsattn_cache* cache, void* stream);
  * append to it, trim, reset, a fork from or to it, an append or a kept path of
  * another step; other sequences may change), are refused where the library can
  * know: it does not see replays, so a step whose map, or whose packed append to
- * a cache, was captured is taken as it comes.  A graph keeps the requests (n_seqs, seq_ids) of its capture.  A step whose map was captured
- * and that is now mapped for others, or with its caches in another order, is
- * refused by the calls outside a graph, which could not tell whose arrays they
- * find; and a graph that holds calls with a step without its map may replay
- * only while the step is mapped for the requests of the capture. */
+ * a cache, was captured is taken as it comes.  A graph keeps the requests
+ * (n_seqs, seq_ids) of its capture.  A step whose map was captured and that is
+ * now mapped for others, or with its caches in another order, is refused by the
+ * calls outside a graph, which could not tell whose arrays they find; and a
+ * graph that holds calls with a step without its map may replay only while the
+ * step is mapped for the requests of the capture. */
 #define BSATTN_STEP_SEQS 64    /* most requests of a step */
 #define BSATTN_STEP_CACHES 128 /* most caches of a step */
 #define BSATTN_TREE_NODES 64   /* most tokens of a request whose tree can be attended or kept */

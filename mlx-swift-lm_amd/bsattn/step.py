@@ -27,7 +27,9 @@ class Step:
     most 64 where they form trees).  Packed tensors are [rows, heads, D];
     request i's tokens are its rows starts[i] .. starts[i] + taken[i] - 1, and
     rows behind the last request's are nobody's.  One stream at a time; keep the
-    object while calls or graphs that use it are pending.
+    object while calls or graphs that use it are pending.  A graph keeps the
+    requests of its capture: once a captured step is mapped for others, its calls
+    outside graphs are refused (another Step takes them).
 
     map() writes, on the device: starts [n + 1], taken [n] (0: the request does
     not fit), requests [rows] (-1: none), positions [rows] (what rotary
